@@ -459,6 +459,132 @@ typedef struct {
 size_t mla_weight_grad_workspace_bytes(const mla_weight_grad_args* a);
 int mla_weight_grad(const mla_weight_grad_args* a, void* stream);
 
+/* --------------------------------------------------------- linear layers --
+ * Activations of the entry points below: none, z < 0 ? 0 : z, z / (1 + e^-z), and the tanh form
+ * 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))). */
+#define MLA_ACT_NONE 0
+#define MLA_ACT_RELU 1
+#define MLA_ACT_SILU 2
+#define MLA_ACT_GELU_TANH 3
+
+/* Bytes of the buffer `saved` for one [M, N] pre-activation: whole 32 x 32 blocks of 24-bit values in an order of the
+ * kernels' own (mla_linear_act writes it for mla_act_grad, mla_gated_linear twice as many for mla_gated_linear_bwd). */
+size_t mla_linear_saved_size(int64_t M, int64_t N);
+
+/* A linear layer with its epilogue:
+ *   z[m][n] = sum_k x[m][k] W[n][k] + bias[n],   y[m][n] = bf16(act(z[m][n]) + residual[m][n])
+ * fp32 sums and epilogue, one rounding.  x [M, K], W [N, K] (an nn.Linear weight), residual and y [M, N]: bf16 rows with row
+ * strides; bias bf16 [N] or NULL, residual or NULL (it may be y itself).  saved: NULL, or mla_linear_saved_size(M, N) bytes
+ * that receive z for mla_act_grad.  N and K multiples of 8; all pointers 16-byte aligned (bias 8), strides multiples of 8
+ * that cover a row (residual's may also be 0: one row for all).  The workspace (mla_linear_act_workspace_bytes, 256-byte
+ * aligned) holds fp32 partials where a product is cut along k.  Deterministic.
+ *
+ * Replaces: o_proj with the block's residual sum (transformer.py:300, :348) and the feed-forward's second product with
+ *           its own (:125, :351).
+ */
+typedef struct {
+  const void *x, *w, *bias, *residual;
+  void *y, *saved;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t M, N, K, x_stride, w_stride, residual_stride, y_stride;
+  int32_t activation;
+} mla_linear_act_args;
+size_t mla_linear_act_workspace_bytes(const mla_linear_act_args* a);
+int mla_linear_act(const mla_linear_act_args* a, void* stream);
+
+/* The first half of a gated feed-forward block:
+ *   g[m][n] = sum_k x[m][k] W_gate[n][k],  u[m][n] = sum_k x[m][k] W_up[n][k],  h[m][n] = bf16(act(g) u)
+ * both products of a tile in one pass over x.  x [M, K], weights [N, K], h [M, N] as in mla_linear_act; saved: NULL, or
+ * 2 mla_linear_saved_size(M, N) bytes that receive g and u for mla_gated_linear_bwd.  activation: not MLA_ACT_NONE.
+ *
+ * Replaces: silu(w1 x) * w3 x (transformer.py:117-125).
+ */
+typedef struct {
+  const void *x, *w_gate, *w_up;
+  void *h, *saved;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t M, N, K, x_stride, w_gate_stride, w_up_stride, h_stride;
+  int32_t activation;
+} mla_gated_linear_args;
+size_t mla_gated_linear_workspace_bytes(const mla_gated_linear_args* a);
+int mla_gated_linear(const mla_gated_linear_args* a, void* stream);
+
+/* Its gradient through the second product: with dh[m][n] = sum_k dy[m][k] W_down[k][n] (fp32, never stored),
+ *   dgu[m][n] = bf16(dh u act'(g)),   dgu[m][N + n] = bf16(dh act(g))
+ * dy [M, K], W_down [K, N] (the second product's nn.Linear weight), dgu [M, 2 N] (row stride dgu_stride), saved as
+ * mla_gated_linear wrote it.
+ *
+ * Replaces: autograd of transformer.py:125 up to the two first products.
+ */
+typedef struct {
+  const void *dy, *w_down, *saved;
+  void* dgu;
+  int64_t M, N, K, dy_stride, w_stride, dgu_stride;
+  int32_t activation;
+} mla_gated_linear_bwd_args;
+int mla_gated_linear_bwd(const mla_gated_linear_bwd_args* a, void* stream);
+
+/* The input gradient of one linear layer, or of two over the same input:
+ *   dx[m][k] = bf16(sum_n dy[m][n] W0[n][k] + sum_n dy[m][N + n] W1[n][k])     (the second sum where w1 is not NULL)
+ * dy [M, N] or [M, 2 N], weights [N, K], dx [M, K]; fp32 sums over both.  N and K multiples of 8.
+ *
+ * Replaces: autograd of the products above with respect to x.
+ */
+typedef struct {
+  const void *dy, *w0, *w1;
+  void* dx;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t M, N, K, dy_stride, w0_stride, w1_stride, dx_stride;
+} mla_linear_dx_args;
+size_t mla_linear_dx_workspace_bytes(const mla_linear_dx_args* a);
+int mla_linear_dx(const mla_linear_dx_args* a, void* stream);
+
+/* The epilogue's gradient: dz[m][n] = bf16(dy[m][n] act'(z[m][n])) with z as mla_linear_act saved it, and
+ * db[n] = sum_m dy act'(z) in fp32, rounded once to db_dtype.  MLA_ACT_NONE: dz = dy is not written and saved not read.
+ * db may be NULL, dz too for MLA_ACT_NONE.  dy, dz [M, N] bf16 rows.  The sums run in a fixed order through the workspace.
+ *
+ * Replaces: autograd of a layer's bias and activation.
+ */
+typedef struct {
+  const void *dy, *saved;
+  void *dz, *db;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t M, N, dy_stride, dz_stride;
+  int32_t activation, db_dtype;
+} mla_act_grad_args;
+size_t mla_act_grad_workspace_bytes(const mla_act_grad_args* a);
+int mla_act_grad(const mla_act_grad_args* a, void* stream);
+
+/* ----------------------------------------------------- gradient clipping --
+ * Norm of many tensors taken together, and their scaling by it:
+ *   norm = sqrt(sum over all elements of all tensors of g^2), or max |g| where norm_is_max      (a NaN anywhere: NaN)
+ *   factor = min(1, max_norm / (norm + 1e-6)),   g <- g factor          (mla_grad_clip; fp32, one rounding to g's type)
+ * ptrs, numels, dtypes: host arrays of n_tensors entries (device pointers; counts; MLA_DTYPE_*), read before the call returns;
+ * a tensor is numel elements in a row, aligned to its element, and does not overlap another one.  norm: one fp32 on the device.
+ * Squares are summed in fp64 in a fixed order, so no finite gradient overflows and results repeat bit for bit.
+ * Workspace: mla_grad_norm_workspace_bytes(a) bytes (by n_tensors alone), 16-byte aligned.
+ *
+ * Replaces: torch.nn.utils.clip_grad_norm_ at train.py:454.
+ */
+typedef struct {
+  void* const* ptrs;
+  const int64_t* numels;
+  const int32_t* dtypes;
+  int64_t n_tensors;
+  float* norm;
+  void* workspace;
+  size_t workspace_bytes;
+  float max_norm;
+  int32_t norm_is_max;
+} mla_grad_norm_args;
+size_t mla_grad_norm_workspace_bytes(const mla_grad_norm_args* a);
+int mla_grad_norm(const mla_grad_norm_args* a, void* stream);
+int mla_grad_clip(const mla_grad_norm_args* a, void* stream);
+
 /* ---------------------------------------------------- chunked linear CE --
  * One vocabulary chunk of the exact softmax cross-entropy over tied output weights, given
  * that chunk's logits [N, Vc] (row stride ld) = x . W[v0 : v0 + Vc]^T of `dtype`
@@ -496,7 +622,7 @@ int mla_ce_chunk(const mla_ce_chunk_args* a, void* stream);
  * mla_args_size: sizeof() of the argument structs, for binding checks
  *   (0 rope, 1 prefill_fwd, 2 prefill_bwd, 3 decode, 4 rmsnorm, 5 rmsnorm_bwd, 6 decode_out,
  *    7 rope_append, 8 absorb_q, 9 ce_chunk, 10 linear_rows, 11 prefill_cached, 12 norm_linear,
- *    13 weight_grad).
+ *    13 weight_grad, 14 linear_act, 15 gated_linear, 16 gated_linear_bwd, 17 linear_dx, 18 act_grad, 19 grad_norm).
  */
 const char* mla_last_error(void);
 int mla_abi_version(void);

@@ -21,6 +21,7 @@ MLA_ERR_LAUNCH = -4
 MLA_DTYPE_BF16 = 0
 MLA_DTYPE_F32 = 1
 MLA_DECODE_STATIC_SCRATCH_BYTES = 12 << 20
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3}  # MLA_ACT_*
 ABI_VERSION = 3
 
 
@@ -174,9 +175,63 @@ class WeightGradArgs(ctypes.Structure):
     ]
 
 
+class LinearActArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p), ("w", c_void_p), ("bias", c_void_p), ("residual", c_void_p), ("y", c_void_p), ("saved", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("M", c_int64), ("N", c_int64), ("K", c_int64), ("x_stride", c_int64), ("w_stride", c_int64),
+        ("residual_stride", c_int64), ("y_stride", c_int64), ("activation", c_int32),
+    ]
+
+
+class GatedLinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p), ("w_gate", c_void_p), ("w_up", c_void_p), ("h", c_void_p), ("saved", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("M", c_int64), ("N", c_int64), ("K", c_int64), ("x_stride", c_int64), ("w_gate_stride", c_int64),
+        ("w_up_stride", c_int64), ("h_stride", c_int64), ("activation", c_int32),
+    ]
+
+
+class GatedLinearBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("dy", c_void_p), ("w_down", c_void_p), ("saved", c_void_p), ("dgu", c_void_p),
+        ("M", c_int64), ("N", c_int64), ("K", c_int64), ("dy_stride", c_int64), ("w_stride", c_int64),
+        ("dgu_stride", c_int64), ("activation", c_int32),
+    ]
+
+
+class LinearDxArgs(ctypes.Structure):
+    _fields_ = [
+        ("dy", c_void_p), ("w0", c_void_p), ("w1", c_void_p), ("dx", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("M", c_int64), ("N", c_int64), ("K", c_int64), ("dy_stride", c_int64), ("w0_stride", c_int64),
+        ("w1_stride", c_int64), ("dx_stride", c_int64),
+    ]
+
+
+class ActGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("dy", c_void_p), ("saved", c_void_p), ("dz", c_void_p), ("db", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("M", c_int64), ("N", c_int64), ("dy_stride", c_int64), ("dz_stride", c_int64),
+        ("activation", c_int32), ("db_dtype", c_int32),
+    ]
+
+
+class GradNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("ptrs", c_void_p), ("numels", c_void_p), ("dtypes", c_void_p),  # host arrays
+        ("n_tensors", c_int64),
+        ("norm", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("max_norm", c_float), ("norm_is_max", c_int32),
+    ]
+
+
 ARGS_STRUCTS = {0: RopeArgs, 1: PrefillFwdArgs, 2: PrefillBwdArgs, 3: DecodeArgs, 4: RmsNormArgs,
                 5: RmsNormBwdArgs, 6: DecodeOutArgs, 7: RopeAppendArgs, 8: AbsorbQArgs, 9: CeChunkArgs,
-                10: LinearRowsArgs, 11: PrefillCachedArgs, 12: NormLinearArgs, 13: WeightGradArgs}
+                10: LinearRowsArgs, 11: PrefillCachedArgs, 12: NormLinearArgs, 13: WeightGradArgs, 14: LinearActArgs,
+                15: GatedLinearArgs, 16: GatedLinearBwdArgs, 17: LinearDxArgs, 18: ActGradArgs, 19: GradNormArgs}
 
 # exported symbol -> (restype, argtypes)
 SIGNATURES = {
@@ -204,6 +259,19 @@ SIGNATURES = {
     "mla_rmsnorm": (c_int, [POINTER(RmsNormArgs), c_void_p]),
     "mla_rmsnorm_bwd_workspace_bytes": (c_size_t, [POINTER(RmsNormBwdArgs)]),
     "mla_rmsnorm_bwd": (c_int, [POINTER(RmsNormBwdArgs), c_void_p]),
+    "mla_linear_saved_size": (c_size_t, [c_int64, c_int64]),
+    "mla_linear_act_workspace_bytes": (c_size_t, [POINTER(LinearActArgs)]),
+    "mla_linear_act": (c_int, [POINTER(LinearActArgs), c_void_p]),
+    "mla_gated_linear_workspace_bytes": (c_size_t, [POINTER(GatedLinearArgs)]),
+    "mla_gated_linear": (c_int, [POINTER(GatedLinearArgs), c_void_p]),
+    "mla_gated_linear_bwd": (c_int, [POINTER(GatedLinearBwdArgs), c_void_p]),
+    "mla_linear_dx_workspace_bytes": (c_size_t, [POINTER(LinearDxArgs)]),
+    "mla_linear_dx": (c_int, [POINTER(LinearDxArgs), c_void_p]),
+    "mla_act_grad_workspace_bytes": (c_size_t, [POINTER(ActGradArgs)]),
+    "mla_act_grad": (c_int, [POINTER(ActGradArgs), c_void_p]),
+    "mla_grad_norm_workspace_bytes": (c_size_t, [POINTER(GradNormArgs)]),
+    "mla_grad_norm": (c_int, [POINTER(GradNormArgs), c_void_p]),
+    "mla_grad_clip": (c_int, [POINTER(GradNormArgs), c_void_p]),
     "mla_last_error": (ctypes.c_char_p, []),
     "mla_abi_version": (c_int, []),
     "mla_args_size": (c_size_t, [c_int]),

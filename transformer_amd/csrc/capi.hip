@@ -66,6 +66,12 @@ extern "C" size_t mla_args_size(int which) {
     case 11: return sizeof(mla_prefill_cached_args);
     case 12: return sizeof(mla_norm_linear_args);
     case 13: return sizeof(mla_weight_grad_args);
+    case 14: return sizeof(mla_linear_act_args);
+    case 15: return sizeof(mla_gated_linear_args);
+    case 16: return sizeof(mla_gated_linear_bwd_args);
+    case 17: return sizeof(mla_linear_dx_args);
+    case 18: return sizeof(mla_act_grad_args);
+    case 19: return sizeof(mla_grad_norm_args);
     default: return 0;
   }
 }

@@ -1,0 +1,177 @@
+// The first half of a gated feed-forward block (gfx950): h = bf16(act(x Wg^T) o (x Wu^T)), both products of a tile in one
+// pass over x, and its gradient through the second product: dh = dy Wd stays in the accumulators, where the saved g and u turn
+// it into dg and du.  The products are gemm_core.h's tiles.
+#include "gemm_epilogue.h"
+#include "linear_checks.h"
+
+namespace mla {
+
+struct GatedParams {
+  GemmArgs g;
+  bf16* out;             // h [M][N], or dgu [M][2 N]
+  unsigned char* saved;  // g and u: blocks of 32 x 32, g's then u's of each
+  int64_t os;
+};
+
+__device__ __forceinline__ unsigned char* gated_saved_at(const GatedParams& p, int m, int n) {
+  return p.saved + ((int64_t)(m >> 5) * ((p.g.N + 31) >> 5) + (n >> 5)) * (2 * kSavedBlock);
+}
+
+// A tile covers T / 2 columns of both weights, a wave's first blocks the gate's and the others the same columns of the up
+// projection, so that a lane holds g and u of one output in the same registers of two blocks.
+template <class C, int ACT>
+__global__ __launch_bounds__(C::THREADS, 2) void gated_linear_kernel(GatedParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
+  const WavePos<C> at;
+  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1) {
+    const StagedRows<C, C::TN> st{s0, s1};
+    constexpr int HB = C::NB / 2;
+    const int mv = min(C::T, p.g.M - m0), nv = min(C::TN, p.g.N - n0);
+#pragma unroll
+    for (int j = 0; j < C::XJ; ++j)
+#pragma unroll
+      for (int i = 0; i < HB; ++i) {
+        const f32x16 &g = acc.a[i][j], &u = acc.a[HB + i][j];
+        const int mb = 32 * (C::XJ * at.wm + j), nb = 32 * (at.wn * HB + i);
+        if (p.saved && mb < mv && nb < nv) {
+          unsigned char* to = gated_saved_at(p, m0 + mb, n0 + nb);
+          saved_store(to, at.lane, g);
+          saved_store(to + kSavedBlock, at.lane, u);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(g[4 * q + e]) * u[4 * q + e];
+          sts8(st.at(mb + at.l32, nb / 8 + q) + 8 * at.hk, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+        }
+      }
+    __syncthreads();
+    store_rows<C>(st, C::T, p.out + (int64_t)m0 * p.os + n0, p.os, mv, nv, [](int r) { return r; });
+    __syncthreads();
+  });
+}
+
+template <class C, int ACT>
+__global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
+  const WavePos<C> at;
+  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1) {
+    const StagedRows<C, C::T> st{s0, s1};
+    const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
+    const int sr = 32 * at.wm + at.l32;
+    bf16* out = p.out + (int64_t)m0 * p.os + n0;
+#pragma unroll
+    for (int j = 0; j < C::XJ; ++j) {
+      const int mb = 32 * (C::XJ * at.wm + j);
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) {
+        const int nb = 32 * (at.wn * C::NB + i);
+        if (mb >= mv || nb >= nv) continue;  // (wave-uniform) no output of the block is stored
+        const unsigned char* from = gated_saved_at(p, m0 + mb, n0 + nb);
+        const SavedRegs g = saved_load(from, at.lane), u = saved_load(from + kSavedBlock, at.lane);
+        f32x16& dh = acc.a[i][j];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float dg[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float value, slope;
+            act_both<ACT>(saved_value(g, 4 * q + e), value, slope);
+            dg[e] = dh[4 * q + e] * saved_value(u, 4 * q + e) * slope;
+            dh[4 * q + e] *= value;  // du
+          }
+          sts8(st.at(sr, nb / 8 + q) + 8 * at.hk, u32x2{pack_bf16x2(dg[0], dg[1]), pack_bf16x2(dg[2], dg[3])});
+        }
+      }
+      __syncthreads();
+      store_rows<C>(st, 32 * C::WM, out, p.os, mv, nv, [&](int r) { return pass_row<C>(r, j); });
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& du = acc.a[i][j];
+          sts8(st.at(sr, 4 * (at.wn * C::NB + i) + q) + 8 * at.hk,
+               u32x2{pack_bf16x2(du[4 * q], du[4 * q + 1]), pack_bf16x2(du[4 * q + 2], du[4 * q + 3])});
+        }
+      __syncthreads();
+      store_rows<C>(st, 32 * C::WM, out + p.g.N, p.os, mv, nv, [&](int r) { return pass_row<C>(r, j); });
+      __syncthreads();
+    }
+  });
+}
+
+template <class C, bool BWD, int ACT>
+static void gated_go(const GatedParams& p, hipStream_t s) {
+  if (BWD) gated_linear_bwd_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+  else gated_linear_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+}
+
+template <class C, bool BWD>
+static void gated_launch(GatedParams& p, int act, hipStream_t s) {
+  gemm_tile_counts<C>(p.g);
+  if (act == MLA_ACT_RELU) gated_go<C, BWD, MLA_ACT_RELU>(p, s);
+  else if (act == MLA_ACT_SILU) gated_go<C, BWD, MLA_ACT_SILU>(p, s);
+  else gated_go<C, BWD, MLA_ACT_GELU_TANH>(p, s);
+}
+
+static int check_gate(const char* op, int act) {
+  MLA_CHECK(act > MLA_ACT_NONE && act <= MLA_ACT_GELU_TANH, MLA_ERR_UNSUPPORTED, "%s: activation %d", op, act);
+  return MLA_OK;
+}
+
+}  // namespace mla
+
+using namespace mla;
+
+extern "C" size_t mla_gated_linear_workspace_bytes(const mla_gated_linear_args* a) {
+  (void)a;
+  return 0;
+}
+
+extern "C" int mla_gated_linear(const mla_gated_linear_args* a, void* stream) {
+  const char* op = "mla_gated_linear";
+  MLA_CHECK(a, MLA_ERR_INVALID_ARG, "%s: null args", op);
+  MLA_TRY(check_linear_sizes(op, a->M, a->N, a->K));
+  MLA_TRY(check_gate(op, a->activation));
+  if (a->M == 0) return MLA_OK;
+  MLA_TRY(check_rows(op, "x", a->x, a->K, a->x_stride));
+  MLA_TRY(check_rows(op, "w_gate", a->w_gate, a->K, a->w_gate_stride));
+  MLA_TRY(check_rows(op, "w_up", a->w_up, a->K, a->w_up_stride));
+  MLA_TRY(check_rows(op, "h", a->h, a->N, a->h_stride));
+  MLA_CHECK(((uintptr_t)a->saved & 15) == 0, MLA_ERR_INVALID_ARG, "%s: saved must be 16-byte aligned", op);
+  GatedParams p{};
+  p.g = GemmArgs{(const bf16*)a->x, (const bf16*)a->w_gate, (const bf16*)a->w_up, a->x_stride, a->w_gate_stride, a->w_up_stride,
+                 (int)a->M, (int)a->N, (int)a->K, 1};
+  p.out = (bf16*)a->h;
+  p.saved = (unsigned char*)a->saved;
+  p.os = a->h_stride;
+  hipStream_t s = (hipStream_t)stream;
+  if (gemm_plan(a->M, 2 * a->N, a->K, 1).large) gated_launch<GemmCfg<256, 2, 4, false, true>, false>(p, a->activation, s);
+  else gated_launch<GemmCfg<128, 2, 2, false, true>, false>(p, a->activation, s);
+  return launch_status(op);
+}
+
+extern "C" int mla_gated_linear_bwd(const mla_gated_linear_bwd_args* a, void* stream) {
+  const char* op = "mla_gated_linear_bwd";
+  MLA_CHECK(a, MLA_ERR_INVALID_ARG, "%s: null args", op);
+  MLA_TRY(check_linear_sizes(op, a->M, a->N, a->K));
+  MLA_TRY(check_gate(op, a->activation));
+  if (a->M == 0) return MLA_OK;
+  MLA_TRY(check_rows(op, "dy", a->dy, a->K, a->dy_stride));
+  MLA_TRY(check_rows(op, "w_down", a->w_down, a->N, a->w_stride));
+  MLA_TRY(check_weight_reach(op, "w_down", a->K, a->w_stride));
+  MLA_TRY(check_rows(op, "dgu", a->dgu, 2 * a->N, a->dgu_stride));
+  MLA_CHECK(a->saved && ((uintptr_t)a->saved & 15) == 0, MLA_ERR_INVALID_ARG, "%s: saved must be given, 16-byte aligned", op);
+  GatedParams p{};
+  p.g = GemmArgs{(const bf16*)a->dy, (const bf16*)a->w_down, nullptr, a->dy_stride, a->w_stride, 0, (int)a->M, (int)a->N,
+                 (int)a->K, 1};
+  p.out = (bf16*)a->dgu;
+  p.saved = (unsigned char*)const_cast<void*>(a->saved);
+  p.os = a->dgu_stride;
+  hipStream_t s = (hipStream_t)stream;
+  if (gemm_plan(a->M, a->N, a->K, 1).large) gated_launch<GemmCfg<256, 2, 4, true, false>, true>(p, a->activation, s);
+  else gated_launch<GemmCfg<128, 2, 2, true, false>, true>(p, a->activation, s);
+  return launch_status(op);
+}

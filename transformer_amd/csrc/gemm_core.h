@@ -1,0 +1,317 @@
+// The tile product that the linear layers' kernels share (linear_act.hip): C^T [n][m] = W . x^T over k, bf16 operands, fp32
+// sums, on v_mfma_f32_32x32x16_bf16.  x [M][K] has k contiguous; W either has too (rows of a layer's weight: y = x W^T) or has
+// n contiguous (the same weight read from its other side: dx = dy W), in which case its fragments come by transpose reads.
+//
+// A workgroup of WN x WM waves computes tiles of T x T outputs, one after the other, k in stages of 64.  A stage is two
+// slots of T rows x 64 k, x's and W's, in a ring of five that direct-to-LDS loads fill: when the products of a stage have read
+// their two slots, W of the stage after next and x of the one behind it go there.  The loads run on across the end of a tile, so
+// that the next tile's first stage lands under this tile's last products and its epilogue, which has the two slots last read
+// for its own use.  Loads past the last tile have empty descriptors.
+//
+// A staged row of 64 k (128 bytes: pieces of 64 bytes reach half the rate, 60 against 95-130 bytes/ns per CU measured) holds
+// its chunk c of 16 bytes at c ^ ((row / 2) mod 8), so that 16 rows x one chunk are free of bank conflicts; a staged k row of T n
+// holds chunk c at c ^ 4 (row mod 4), so that the four rows of a half-wave's transpose read fall on four different 64-byte bank
+// groups.  The one barrier of a stage lies before its last 16-wide step: that step's products run under the next stage's
+// first reads, the others under the reads of the step after them.
+#pragma once
+
+#include "mla_common.h"
+
+namespace mla {
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+
+// T x T outputs of WN x WM waves; KMAJOR: W is [k][n]; PAIR: a tile's W rows come from two weights of N columns each, T / 2
+// of each, a wave's first NB / 2 blocks from w0, the rest from w1 at the same columns
+template <int T_, int WN_, int WM_, bool KMAJOR_, bool PAIR_>
+struct GemmCfg {
+  static constexpr int T = T_, WN = WN_, WM = WM_, BK = 64, HS = BK / 16;
+  static constexpr bool KMAJOR = KMAJOR_, PAIR = PAIR_;
+  static constexpr int WAVES = WN * WM, THREADS = 64 * WAVES;
+  static constexpr int NB = T / WN / 32, XJ = T / WM / 32;  // 32 x 32 blocks per wave
+  static constexpr int TN = PAIR ? T / 2 : T;               // columns of the weights that a tile covers
+  static constexpr int SLOT = T * BK * 2;                   // T rows of 64 k, or 64 k rows of T
+  static constexpr int RING = 5;
+  static constexpr int LOADS = SLOT / 1024 / WAVES;         // of a wave per slot
+  static constexpr int LDS = RING * SLOT;
+  static_assert(SLOT % (1024 * WAVES) == 0 && LDS <= 160 * 1024, "the ring fits the LDS");
+};
+
+// y (a tile's outputs, as an epilogue defines them) over rows m of x, columns n of W; k runs over `parts` segments of K each:
+// x's columns p K .. (p + 1) K with w0, then w1
+struct GemmArgs {
+  const bf16* x;   // [M][parts K], row stride xs
+  const bf16* w0;  // [N][K] row stride ws0, or KMAJOR [K][N]
+  const bf16* w1;  // PAIR: the second weight; parts == 2: that of the second part
+  int64_t xs, ws0, ws1;
+  int M, N, K, parts;
+  int n_mt, n_nt;  // tiles
+  int gm;          // m tiles of a block of tiles (see gemm_tile_at)
+};
+
+template <int N>
+__device__ __forceinline__ void gemm_wait_vmem() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ int gemm_swz(int row) { return (row >> 1) & 7; }
+
+template <class C>
+struct GemmAcc {
+  f32x16 a[C::NB][C::XJ];
+};
+
+// Tile `id` of n_mt x n_nt: consecutive logical ids run on one XCD (the hardware places workgroup id on XCD id % 8) and walk
+// blocks of gm m tiles x all n tiles, m fastest, so that the tiles an XCD runs at once share their rows in its L2.
+__device__ __forceinline__ void gemm_tile_at(const GemmArgs& a, int id, int& mt, int& nt) {
+  const int n_wg = a.n_mt * a.n_nt;
+  const int q = n_wg >> 3, r = n_wg & 7, xcd = id & 7;
+  id = xcd * q + min(xcd, r) + (id >> 3);
+  const int per = a.gm * a.n_nt, grp = id / per, in = id - grp * per;
+  const int rows = min(a.gm, a.n_mt - grp * a.gm);
+  mt = grp * a.gm + in % rows;
+  nt = in / rows;
+}
+
+// Runs the tiles blockIdx.x, blockIdx.x + gridDim.x, ...: for each, epi(acc, m0, n0, stage0, stage1), where the two stages are
+// SLOT bytes each that the epilogue may use until its last barrier (every wave must have passed it before it returns).
+template <class C, class Epi>
+__device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds, Epi&& epi) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = w % C::WN, wm = w / C::WN;
+  const int l32 = lane & 31, hk = lane >> 5;
+  const int n_tiles = p.n_mt * p.n_nt;
+  const int n_st = (p.K + C::BK - 1) / C::BK;
+  const int tail = p.K - (n_st - 1) * C::BK;  // k of a part's last stage, a multiple of 8
+
+  // ---- loads: a cursor for x and one for W, each (tile, part, stage) with the descriptors of its tile and part, which end at
+  // the last valid row; lanes past them load nothing, and the outputs that such rows reach are not stored
+  const uint32_t lds0 = lds_addr(lds);
+  uint32_t xoff[C::LOADS], woff[C::LOADS];  // this lane's bytes in each of the wave's loads, at k = 0
+  bool second[C::LOADS];                    // PAIR (wave-uniform): the load is of w1's rows
+#pragma unroll
+  for (int j = 0; j < C::LOADS; ++j) {
+    const int i = w + C::WAVES * j, row = 8 * i + (lane >> 3);
+    xoff[j] = (uint32_t)(row * p.xs * 2) + (uint32_t)(((lane & 7) ^ gemm_swz(row)) * 16);
+    second[j] = false;
+    if (C::KMAJOR) {
+      const int at = i * 1024 + lane * 16, kr = at / (C::T * 2), pos = (at % (C::T * 2)) >> 4;
+      woff[j] = (uint32_t)(kr * p.ws0 * 2) + (uint32_t)((pos ^ (4 * (kr & 3))) * 16);
+    } else {
+      int src = row;
+      if (C::PAIR) {
+        const int b = (8 * i) / 32, per = C::NB / 2;  // block b of the tile, b % NB of its wave
+        second[j] = b % C::NB >= per;
+        src = (b / C::NB * per + b % per) * 32 + (row & 31);
+      }
+      woff[j] = (uint32_t)(src * (C::PAIR && second[j] ? p.ws1 : p.ws0) * 2) + (uint32_t)(((lane & 7) ^ gemm_swz(row)) * 16);
+    }
+  }
+  struct Cursor {
+    int tile, part, st;
+  };
+  Cursor cx{(int)blockIdx.x, 0, 0}, cw = cx;
+  buf_rsrc rx, rw0, rw1;
+  auto point_x = [&]() {
+    int mt, nt;
+    gemm_tile_at(p, min(cx.tile, n_tiles - 1), mt, nt);
+    const int m0 = mt * C::T;
+    rx = make_rsrc(p.x + (int64_t)m0 * p.xs + (int64_t)cx.part * p.K,
+                   cx.tile < n_tiles ? rows_bytes(min(C::T, p.M - m0), p.xs, p.K * 2) : 0u);
+  };
+  auto point_w = [&]() {
+    int mt, nt;
+    gemm_tile_at(p, min(cw.tile, n_tiles - 1), mt, nt);
+    const int n0 = nt * C::TN, nv = min(C::TN, p.N - n0);
+    const bool live = cw.tile < n_tiles;
+    const bf16* wp = !C::PAIR && cw.part ? p.w1 : p.w0;
+    if (C::KMAJOR) {
+      rw0 = make_rsrc(wp + n0, live ? rows_bytes(p.K, p.ws0, nv * 2) : 0u);
+    } else {
+      rw0 = make_rsrc(wp + (int64_t)n0 * p.ws0, live ? rows_bytes(nv, p.ws0, p.K * 2) : 0u);
+      if (C::PAIR) rw1 = make_rsrc(p.w1 + (int64_t)n0 * p.ws1, live ? rows_bytes(nv, p.ws1, p.K * 2) : 0u);
+    }
+  };
+  auto advance = [&](Cursor& c) -> bool {  // whether the descriptors change
+    if (++c.st < n_st) return false;
+    c.st = 0;
+    if (++c.part == p.parts) {
+      c.part = 0;
+      c.tile = c.tile < n_tiles ? c.tile + (int)gridDim.x : c.tile;
+    }
+    return true;
+  };
+  auto load_x = [&](int slot, int j) {
+    dma16(rx, xoff[j] + (uint32_t)(cx.st * C::BK * 2), lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
+  };
+  auto done_x = [&]() {
+    if (advance(cx)) point_x();
+  };
+  auto issue_x = [&](int slot) {
+#pragma unroll
+    for (int j = 0; j < C::LOADS; ++j) load_x(slot, j);
+    done_x();
+  };
+  const uint32_t wstep = C::KMAJOR ? (uint32_t)(C::BK * p.ws0 * 2) : (uint32_t)(C::BK * 2);
+  auto load_w = [&](int slot, int j) {
+    dma16(C::PAIR && second[j] ? rw1 : rw0, woff[j] + (uint32_t)cw.st * wstep,
+          lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
+  };
+  auto done_w = [&]() {
+    if (advance(cw)) point_w();
+  };
+  auto issue_w = [&](int slot) {
+#pragma unroll
+    for (int j = 0; j < C::LOADS; ++j) load_w(slot, j);
+    done_w();
+  };
+
+  // ---- fragment reads: lane (l32, hk) takes row l32 of a block and k = 16 h + 8 hk + [0, 8).  Transpose reads: lane
+  // (hk, l16) addresses 4 columns of row 8 hk + l16 / 4 (+ 4, + 16 h); 32-column block b of a row sits at 64 (b ^ (row mod 4))
+  // within its 256 bytes.
+  int offw[C::KMAJOR ? C::NB : C::HS], offx[C::HS];
+  if (C::KMAJOR) {
+    const int l16 = lane & 15, r2 = l16 >> 2;
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i) {
+      const int b = wn * C::NB + i;
+      offw[i] = (8 * hk + r2) * (C::T * 2) + 256 * (b >> 2) + 64 * ((b & 3) ^ r2) + 32 * ((lane >> 4) & 1) + 8 * (l16 & 3);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < C::HS; ++h) {
+    const int rw_ = 32 * C::NB * wn + l32;  // the block's row within the tile is + 32 i (the swizzle unchanged)
+    if (!C::KMAJOR) offw[h] = rw_ * 128 + (((2 * h + hk) ^ gemm_swz(rw_)) * 16);
+    const int rx_ = 32 * C::XJ * wm + l32;
+    offx[h] = rx_ * 128 + (((2 * h + hk) ^ gemm_swz(rx_)) * 16);
+  }
+  bf16x8 fx[C::HS][C::XJ], fw[2][C::NB];  // x of a stage's four steps, W of this step and the next
+  auto read_x = [&](int slot, int h) {
+    const unsigned char* xt = lds + slot * C::SLOT;
+#pragma unroll
+    for (int j = 0; j < C::XJ; ++j) fx[h][j] = as_bf16x8(lds16(xt + offx[h] + j * 32 * 128));
+  };
+  auto read_w = [&](int slot, int h) {
+    const unsigned char* wt = lds + slot * C::SLOT;
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i) {
+      if (C::KMAJOR) {
+        const unsigned char* a = wt + offw[i] + 16 * h * (C::T * 2);
+        const s16x4_t lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)a);
+        const s16x4_t hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(a + 4 * (C::T * 2)));
+        const u32x2 l = __builtin_bit_cast(u32x2, lo4), hh = __builtin_bit_cast(u32x2, hi4);
+        fw[h & 1][i] = as_bf16x8(u32x4{l[0], l[1], hh[0], hh[1]});
+      } else {
+        fw[h & 1][i] = as_bf16x8(lds16(wt + offw[h] + i * 32 * 128));
+      }
+    }
+  };
+  GemmAcc<C> acc;
+  auto multiply = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i)
+#pragma unroll
+      for (int j = 0; j < C::XJ; ++j) acc.a[i][j] = mfma32(fw[h & 1][i], fx[h][j], acc.a[i][j]);
+  };
+  // the reads go out between the step's first products (left alone, the compiler moves them to their use)
+  auto interleave = [&]() {
+    constexpr int reads = C::XJ + (C::KMAJOR ? 2 : 1) * C::NB, products = C::NB * C::XJ;
+    constexpr int each = (reads + products - 1) / products;
+#pragma unroll
+    for (int n = 0; n < products; ++n) {
+      __builtin_amdgcn_sched_group_barrier(0x100, each, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // step h of a part's last stage: k past its end (whole chunks: the lane's 8 k are in or out together) becomes zero in both
+  auto cut = [&](int h) {
+    const bool in = 16 * h + 8 * hk < tail;
+    const u32x4 z{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < C::XJ; ++j) fx[h][j] = as_bf16x8(in ? as_u32x4(fx[h][j]) : z);
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i) fw[h & 1][i] = as_bf16x8(in ? as_u32x4(fw[h & 1][i]) : z);
+  };
+
+  if ((int)blockIdx.x >= n_tiles) return;
+  point_x();
+  point_w();
+  issue_x(0);
+  issue_w(1);
+  issue_x(2);
+  issue_w(3);
+  issue_x(4);
+  gemm_wait_vmem<3 * C::LOADS>();
+  __syncthreads();
+  int sx = 0, sw = 1;  // the slots of the stage being multiplied
+  auto next_slots = [&]() {
+    sx = sx >= 3 ? sx - 3 : sx + 2;
+    sw = sw >= 3 ? sw - 3 : sw + 2;
+  };
+  auto read_first = [&]() {  // what a stage's slots give before its first step's products
+    read_w(sw, 0);
+#pragma unroll
+    for (int h = 0; h + 1 < C::HS; ++h) read_x(sx, h);
+  };
+  read_first();
+  for (int tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i)
+#pragma unroll
+      for (int j = 0; j < C::XJ; ++j) acc.a[i][j] = f32x16{};
+    for (int part = 0; part < p.parts; ++part) {
+      for (int st = 0; st + 1 < n_st; ++st) {
+        read_x(sx, C::HS - 1);
+        read_w(sw, 1);
+        multiply(0);
+        interleave();
+        __syncthreads();  // every wave holds the stage's x in registers
+        issue_w(sx);
+#pragma unroll
+        for (int h = 1; h + 1 < C::HS; ++h) {
+          read_w(sw, h + 1);
+          multiply(h);
+          interleave();
+        }
+        // every wave holds the stage in registers and the next one has landed: all but the one behind it
+        gemm_wait_vmem<2 * C::LOADS>();
+        __syncthreads();
+        issue_x(sw);
+        next_slots();
+        __builtin_amdgcn_sched_barrier(0);
+        read_first();
+        multiply(C::HS - 1);
+        interleave();
+      }
+      read_x(sx, C::HS - 1);
+#pragma unroll
+      for (int h = 0; h + 1 < C::HS; ++h) {
+        read_w(sw, h + 1);
+        cut(h);
+        multiply(h);
+      }
+      cut(C::HS - 1);
+      gemm_wait_vmem<C::LOADS>();
+      __syncthreads();
+      const int s0 = sx, s1 = sw;
+      next_slots();
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(C::HS - 1);
+      if (part + 1 == p.parts) {
+        int mt, nt;
+        gemm_tile_at(p, tile, mt, nt);
+        epi(acc, mt * C::T, nt * C::TN, lds + s0 * C::SLOT, lds + s1 * C::SLOT);
+        gemm_wait_vmem<0>();  // (its stores share the counter that the stages' waits count down)
+      }
+      issue_w(s0);
+      issue_x(s1);
+      read_first();
+    }
+  }
+  gemm_wait_vmem<0>();  // no load is in flight into LDS when the workgroup ends
+}
+
+}  // namespace mla

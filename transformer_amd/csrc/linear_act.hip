@@ -1,0 +1,209 @@
+// Linear layers with their epilogue (gfx950): y = bf16(act(x W^T + bias) + residual), and the input gradient dx = dy W of one
+// layer or of two over the same input (one fp32 sum).  The products are gemm_core.h's tiles; the epilogue works on the fp32
+// accumulators, so bias, activation and residual cost no pass over y and no rounding of their own.
+#include <algorithm>
+
+#include "gemm_epilogue.h"
+#include "linear_checks.h"
+
+namespace mla {
+
+struct LinearParams {
+  GemmArgs g;
+  const bf16* bias;
+  const bf16* residual;
+  bf16* y;
+  unsigned char* saved;
+  int64_t rs, ys;
+};
+
+template <class C, int ACT>
+__global__ __launch_bounds__(C::THREADS, 2) void linear_act_kernel(LinearParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
+  const WavePos<C> at;
+  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1) {
+    const StagedRows<C, C::T> st{s0, s1};
+    constexpr int R = 32 * C::WM, CH = C::T / 8;
+    const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
+    const int sr = 32 * at.wm + at.l32;
+#pragma unroll
+    for (int j = 0; j < C::XJ; ++j) {
+      if (p.residual) {
+        const bf16* res = p.residual + (int64_t)m0 * p.rs + n0;
+#pragma unroll 4
+        for (int c = threadIdx.x; c < R * CH; c += C::THREADS) {
+          const int r = c / CH, ch = c % CH, m = pass_row<C>(r, j);
+          if (m < mv && 8 * ch < nv) sts16(st.at(r, ch), ldg16(res + m * p.rs + 8 * ch));
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) {
+        f32x16& a = acc.a[i][j];
+        const int nb = (at.wn * C::NB + i) * 32;  // the block's first column within the tile
+        if (p.bias) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int n = nb + 8 * q + 4 * at.hk;
+            if (n < nv) {
+              const u32x2 b = ldg8(p.bias + n0 + n);
+              a[4 * q] += lo_bf16(b[0]);
+              a[4 * q + 1] += hi_bf16(b[0]);
+              a[4 * q + 2] += lo_bf16(b[1]);
+              a[4 * q + 3] += hi_bf16(b[1]);
+            }
+          }
+        }
+        const int mb = 32 * (C::XJ * at.wm + j);
+        if (p.saved && mb < mv && nb < nv)
+          saved_store(p.saved + ((int64_t)((m0 + mb) >> 5) * ((p.g.N + 31) >> 5) + ((n0 + nb) >> 5)) * kSavedBlock, at.lane, a);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          unsigned char* to = st.at(sr, nb / 8 + q) + 8 * at.hk;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(a[4 * q + e]);
+          if (p.residual) {
+            const u32x2 b = lds8(to);
+            v[0] += lo_bf16(b[0]);
+            v[1] += hi_bf16(b[0]);
+            v[2] += lo_bf16(b[1]);
+            v[3] += hi_bf16(b[1]);
+          }
+          sts8(to, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+        }
+      }
+      __syncthreads();
+      store_rows<C>(st, R, p.y + (int64_t)m0 * p.ys + n0, p.ys, mv, nv, [&](int r) { return pass_row<C>(r, j); });
+      __syncthreads();
+    }
+  });
+}
+
+template <class C>
+__global__ __launch_bounds__(C::THREADS, 2) void linear_dx_kernel(LinearParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
+  const WavePos<C> at;
+  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1) {
+    const StagedRows<C, C::T> st{s0, s1};
+    const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
+#pragma unroll
+    for (int j = 0; j < C::XJ; ++j) {
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& a = acc.a[i][j];
+          sts8(st.at(32 * at.wm + at.l32, (at.wn * C::NB + i) * 4 + q) + 8 * at.hk,
+               u32x2{pack_bf16x2(a[4 * q], a[4 * q + 1]), pack_bf16x2(a[4 * q + 2], a[4 * q + 3])});
+        }
+      __syncthreads();
+      store_rows<C>(st, 32 * C::WM, p.y + (int64_t)m0 * p.ys + n0, p.ys, mv, nv, [&](int r) { return pass_row<C>(r, j); });
+      __syncthreads();
+    }
+  });
+}
+
+template <class C, int ACT>
+static void linear_act_go(const LinearParams& p, hipStream_t s) {
+  linear_act_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+}
+
+template <class C>
+static void linear_act_launch(LinearParams& p, int act, hipStream_t s) {
+  gemm_tile_counts<C>(p.g);
+  if (act == MLA_ACT_RELU) linear_act_go<C, MLA_ACT_RELU>(p, s);
+  else if (act == MLA_ACT_SILU) linear_act_go<C, MLA_ACT_SILU>(p, s);
+  else if (act == MLA_ACT_GELU_TANH) linear_act_go<C, MLA_ACT_GELU_TANH>(p, s);
+  else linear_act_go<C, MLA_ACT_NONE>(p, s);
+}
+
+template <class C>
+static void linear_dx_launch(LinearParams& p, hipStream_t s) {
+  gemm_tile_counts<C>(p.g);
+  linear_dx_kernel<C><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+}
+
+static int linear_act_check(const mla_linear_act_args* a) {
+  const char* op = "mla_linear_act";
+  MLA_CHECK(a, MLA_ERR_INVALID_ARG, "%s: null args", op);
+  MLA_TRY(check_linear_sizes(op, a->M, a->N, a->K));
+  MLA_CHECK(a->activation >= MLA_ACT_NONE && a->activation <= MLA_ACT_GELU_TANH, MLA_ERR_UNSUPPORTED,
+            "%s: activation %d", op, a->activation);
+  if (a->M == 0 || a->N == 0) return MLA_OK;
+  MLA_TRY(check_rows(op, "x", a->x, a->K, a->x_stride));
+  MLA_TRY(check_rows(op, "w", a->w, a->K, a->w_stride));
+  MLA_TRY(check_rows(op, "y", a->y, a->N, a->y_stride));
+  MLA_CHECK(((uintptr_t)a->bias & 7) == 0, MLA_ERR_INVALID_ARG, "%s: bias must be 8-byte aligned", op);
+  if (a->residual) MLA_TRY(check_rows(op, "residual", a->residual, a->residual_stride ? a->N : 0, a->residual_stride));
+  MLA_CHECK(((uintptr_t)a->saved & 15) == 0, MLA_ERR_INVALID_ARG, "%s: saved must be 16-byte aligned", op);
+  return MLA_OK;
+}
+
+static int linear_dx_check(const mla_linear_dx_args* a) {
+  const char* op = "mla_linear_dx";
+  MLA_CHECK(a, MLA_ERR_INVALID_ARG, "%s: null args", op);
+  MLA_TRY(check_linear_sizes(op, a->M, a->N, a->K));
+  if (a->M == 0 || a->K == 0) return MLA_OK;
+  const int64_t parts = a->w1 ? 2 : 1;
+  MLA_TRY(check_rows(op, "dy", a->dy, parts * a->N, a->dy_stride));
+  MLA_TRY(check_rows(op, "w0", a->w0, a->K, a->w0_stride));
+  MLA_TRY(check_rows(op, "dx", a->dx, a->K, a->dx_stride));
+  MLA_TRY(check_weight_reach(op, "w0", a->N, a->w0_stride));
+  if (a->w1) {
+    MLA_TRY(check_rows(op, "w1", a->w1, a->K, a->w1_stride));
+    MLA_TRY(check_weight_reach(op, "w1", a->N, a->w1_stride));
+  }
+  return MLA_OK;
+}
+
+}  // namespace mla
+
+using namespace mla;
+
+extern "C" size_t mla_linear_saved_size(int64_t M, int64_t N) {
+  if (M <= 0 || N <= 0 || M >= kLinearMaxM || N >= kLinearMaxN) return 0;
+  return (size_t)((M + 31) / 32) * (size_t)((N + 31) / 32) * kSavedBlock;
+}
+
+extern "C" size_t mla_linear_act_workspace_bytes(const mla_linear_act_args* a) {
+  (void)a;
+  return 0;
+}
+
+extern "C" int mla_linear_act(const mla_linear_act_args* a, void* stream) {
+  MLA_TRY(linear_act_check(a));
+  if (a->M == 0 || a->N == 0) return MLA_OK;
+  LinearParams p{};
+  p.g = GemmArgs{(const bf16*)a->x, (const bf16*)a->w, nullptr, a->x_stride, a->w_stride, 0, (int)a->M, (int)a->N, (int)a->K, 1};
+  p.bias = (const bf16*)a->bias;
+  p.residual = (const bf16*)a->residual;
+  p.y = (bf16*)a->y;
+  p.saved = (unsigned char*)a->saved;
+  p.rs = a->residual_stride;
+  p.ys = a->y_stride;
+  hipStream_t s = (hipStream_t)stream;
+  if (gemm_plan(a->M, a->N, a->K, 1).large) linear_act_launch<GemmCfg<256, 2, 4, false, false>>(p, a->activation, s);
+  else linear_act_launch<GemmCfg<128, 2, 2, false, false>>(p, a->activation, s);
+  return launch_status("mla_linear_act");
+}
+
+extern "C" size_t mla_linear_dx_workspace_bytes(const mla_linear_dx_args* a) {
+  (void)a;
+  return 0;
+}
+
+extern "C" int mla_linear_dx(const mla_linear_dx_args* a, void* stream) {
+  MLA_TRY(linear_dx_check(a));
+  if (a->M == 0 || a->K == 0) return MLA_OK;
+  const int parts = a->w1 ? 2 : 1;
+  LinearParams p{};
+  p.g = GemmArgs{(const bf16*)a->dy, (const bf16*)a->w0, (const bf16*)a->w1, a->dy_stride, a->w0_stride, a->w1_stride, (int)a->M,
+                 (int)a->K, (int)a->N, parts};
+  p.y = (bf16*)a->dx;
+  p.ys = a->dx_stride;
+  hipStream_t s = (hipStream_t)stream;
+  if (gemm_plan(a->M, a->K, a->N, parts).large) linear_dx_launch<GemmCfg<256, 2, 4, true, false>>(p, s);
+  else linear_dx_launch<GemmCfg<128, 2, 2, true, false>>(p, s);
+  return launch_status("mla_linear_dx");
+}

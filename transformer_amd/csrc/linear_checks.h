@@ -1,0 +1,53 @@
+// Host-side checks and launch shapes of the linear layers' entry points.
+#pragma once
+
+#include "gemm_core.h"
+
+namespace mla {
+
+constexpr int64_t kLinearMaxM = 1 << 30, kLinearMaxN = 1 << 20, kLinearMaxStride = 1 << 22;
+
+// Sizes of a product: rows of 16-byte chunks, 32-bit indexes of rows and tiles.  K = 0 (an empty sum) is refused.
+inline int check_linear_sizes(const char* op, int64_t M, int64_t N, int64_t K) {
+  MLA_CHECK(M >= 0 && N >= 0 && K >= 0 && M < kLinearMaxM && N < kLinearMaxN && K < kLinearMaxN, MLA_ERR_INVALID_ARG,
+            "%s: size out of range", op);
+  MLA_CHECK(N % 8 == 0 && K % 8 == 0 && N > 0 && K > 0, MLA_ERR_UNSUPPORTED,
+            "%s: N = %lld and K = %lld must be positive multiples of 8", op, (long long)N, (long long)K);
+  // tiles of 64 columns at least
+  MLA_CHECK((M / 128 + 1) * (N / 64 + 1) < (1ll << 30) && (M / 128 + 1) * (K / 64 + 1) < (1ll << 30), MLA_ERR_INVALID_ARG,
+            "%s: too many tiles", op);
+  return MLA_OK;
+}
+
+// bf16 rows of `width` columns: a tile's 256 rows are addressed with 32-bit offsets from its first
+inline int check_rows(const char* op, const char* name, const void* ptr, int64_t width, int64_t stride) {
+  MLA_CHECK(ptr, MLA_ERR_INVALID_ARG, "%s: %s is null", op, name);
+  MLA_CHECK(((uintptr_t)ptr & 15) == 0, MLA_ERR_INVALID_ARG, "%s: %s must be 16-byte aligned", op, name);
+  MLA_CHECK(stride >= width && stride % 8 == 0, MLA_ERR_INVALID_ARG,
+            "%s: %s's row stride %lld must cover a row and be a multiple of 8", op, name, (long long)stride);
+  MLA_CHECK(stride < kLinearMaxStride, MLA_ERR_UNSUPPORTED, "%s: %s's row stride %lld is too large", op, name,
+            (long long)stride);
+  return MLA_OK;
+}
+
+// a weight read along its rows' direction is addressed as a whole with 32-bit byte offsets
+inline int check_weight_reach(const char* op, const char* name, int64_t rows, int64_t stride) {
+  MLA_CHECK((rows + 64) * stride * 2 < (1ll << 31), MLA_ERR_UNSUPPORTED, "%s: %s of 2 GiB or more", op, name);
+  return MLA_OK;
+}
+
+template <class C>
+inline void gemm_tile_counts(GemmArgs& g) {
+  g.n_mt = (g.M + C::T - 1) / C::T;
+  g.n_nt = (g.N + C::TN - 1) / C::TN;
+  g.gm = 8;
+}
+
+// one workgroup of 256 x 256 tiles per CU, two of 128 x 128
+template <class C>
+inline unsigned gemm_grid(const GemmArgs& g) {
+  const int64_t tiles = (int64_t)g.n_mt * g.n_nt, most = C::LDS > 80 * 1024 ? 256 : 512;
+  return (unsigned)(tiles < most ? tiles : most);
+}
+
+}  // namespace mla

@@ -122,4 +122,19 @@ inline WgPlan wg_plan(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
+// ---- linear_act.hip's and gated_linear.hip's tiles (gemm_core.h)
+struct GemmPlan {
+  int large;  // tiles of 256 x 256, one workgroup per CU; else 128 x 128, two
+};
+
+// y [M, N] over parts x K
+inline GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int64_t parts) {
+  const double stages = (double)((K + 63) / 64 * parts);
+  const int64_t t256 = ((M + 255) / 256) * ((N + 255) / 256), t128 = ((M + 127) / 128) * ((N + 127) / 128);
+  const double large = (double)((t256 + 255) / 256) * (1.2 * stages + 10.0);
+  // up to one workgroup a CU runs faster than two that share it
+  const double small = t128 <= 256 ? 0.55 * stages + 4.0 : (double)((t128 + 511) / 512) * (0.85 * stages + 5.0);
+  return GemmPlan{large < small};
+}
+
 }  // namespace mla

@@ -1,0 +1,118 @@
+"""The norm of a training step's gradients and their clipping on the MI355X, with no host synchronisation.
+
+``clip_grad_norm_(parameters, max_norm)`` is a drop-in for ``torch.nn.utils.clip_grad_norm_`` as the reference's step calls it
+(train.py:454): two passes over all gradients, a HIP launch each for up to 128 tensors.  ``grad_norm(tensors)`` is the first
+pass alone.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Iterable, List, Union
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .kernels import _alloc_workspace
+from .linear_ops import _launch
+
+_CODES = {torch.float32: _lib.MLA_DTYPE_F32, torch.bfloat16: _lib.MLA_DTYPE_BF16}
+
+
+def _dense(t: Tensor) -> bool:
+    """Whether ``t``'s elements fill its memory without gaps, in any order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _check(op: str, tensors: List[Tensor], norm_type: float) -> bool:
+    """Whether the norm is the largest magnitude (else the 2-norm); refuses what the kernels do not take."""
+    norm_type = float(norm_type)
+    if norm_type not in (2.0, math.inf):
+        raise ValueError(f"{op}: norm_type {norm_type} is not built (2 or inf)")
+    device = None
+    for t in tensors:
+        if t.layout != torch.strided:
+            raise ValueError(f"{op}: sparse gradients are not built")
+        if not t.is_cuda:
+            raise RuntimeError(f"transformer_amd.{op} runs on a ROCm GPU only (no CPU path); got a tensor on {t.device}")
+        if t.dtype not in _CODES:
+            raise TypeError(f"{op}: gradients must be float32 or bfloat16, got {t.dtype}")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"{op}: gradients on {device} and {t.device}: one device is needed")
+    return norm_type == math.inf
+
+
+def _run(op: str, entry: str, tensors: List[Tensor], is_max: bool, max_norm: float) -> Tensor:
+    n = len(tensors)
+    like = tensors[0]
+    norm = torch.empty((), dtype=torch.float32, device=like.device)
+    # host tables, read before the entry point returns
+    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
+    numels = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
+    dtypes = (ctypes.c_int32 * n)(*[_CODES[t.dtype] for t in tensors])
+    args = _lib.GradNormArgs(
+        ptrs=ctypes.addressof(ptrs), numels=ctypes.addressof(numels), dtypes=ctypes.addressof(dtypes), n_tensors=n,
+        norm=norm.data_ptr(), workspace=None, workspace_bytes=0, max_norm=max_norm, norm_is_max=int(is_max))
+    nbytes = int(_lib.entry("mla_grad_norm_workspace_bytes")(ctypes.byref(args)))
+    ws = _alloc_workspace(nbytes, like.device)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    _launch(entry, args, like, op)
+    return norm
+
+
+def grad_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
+    """The norm (2, or inf: the largest magnitude) of all elements of ``tensors`` together, an fp32 scalar on their device.
+    Tensors are fp32 or bf16, of any layout, on one device; squares are summed in fp64.  A NaN anywhere gives NaN."""
+    tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
+    is_max = _check("grad_norm", tensors, norm_type)
+    if not tensors:
+        return torch.tensor(0.0)
+    with torch.no_grad():
+        return _run("grad_norm", "mla_grad_norm", [t if _dense(t) else t.contiguous() for t in tensors], is_max, 0.0)
+
+
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False, foreach: bool = None) -> Tensor:
+    """Scales the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))`` and returns their norm before
+    that, as ``torch.nn.utils.clip_grad_norm_`` does; parameters without a gradient are passed over.  ``norm_type``: 2 or inf.
+    ``error_if_nonfinite`` waits for the norm and raises before anything is scaled.  ``foreach`` is accepted and ignored.
+    Gradients are fp32 or bf16 on one device; two that share memory are refused."""
+    op = "clip_grad_norm_"
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"{op}: max_norm must be at least 0, got {max_norm}")
+    parameters = [parameters] if isinstance(parameters, Tensor) else parameters
+    grads = [p.grad for p in parameters if p.grad is not None]
+    is_max = _check(op, grads, norm_type)
+    if not grads:
+        return torch.tensor(0.0)
+    with torch.no_grad():
+        flat, back = [], []
+        for g in grads:
+            if _dense(g):
+                flat.append(g)
+                continue
+            if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+                raise ValueError(f"{op}: a gradient with strides {g.stride()} shares memory between its elements")
+            flat.append(g.contiguous())
+            back.append((g, flat[-1]))
+        if error_if_nonfinite:
+            norm = _run(op, "mla_grad_norm", flat, is_max, 0.0)
+            if not bool(torch.isfinite(norm)):
+                raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so "
+                                   "it cannot be clipped.")
+        norm = _run(op, "mla_grad_clip", flat, is_max, max_norm)
+        for g, c in back:
+            g.copy_(c)
+        torch.autograd.graph.increment_version(grads)
+    return norm
