@@ -3,6 +3,7 @@
 // it into dg and du.  The products are gemm_core.h's tiles.
 #include "gemm_epilogue.h"
 #include "linear_checks.h"
+#include "rows_core.h"
 
 namespace mla {
 
@@ -102,9 +103,36 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedPa
   });
 }
 
+template <int MB, int ACT>
+__global__ __launch_bounds__(64 * kRcWaves) void gated_linear_rows_kernel(GatedParams p, RowsArgs r) {
+  __shared__ f32x4 red[kRcWaves][2 * MB][64];
+  RowsProduct<MB, true> t;
+  t.run(r, red);
+  if (!t.mine) return;
+  const f32x4 g = t.sum[0], u = t.sum[1];
+  if (p.saved) {
+    unsigned char* to = gated_saved_at(p, t.m, t.n);
+    saved_store4(to, t.m, t.n, g);
+    saved_store4(to + kSavedBlock, t.m, t.n, u);
+  }
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(g[e]) * u[e];
+  stg8(p.out + t.m * p.os + t.n, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+}
+
+template <int ACT>
+static void gated_rows_go(const GatedParams& p, hipStream_t s) {
+  const RowsArgs r{p.g.x, p.g.w0, p.g.w1, p.g.xs, p.g.ws0, p.g.ws1, p.g.M, p.g.N, p.g.K, rows_columns(p.g.N)};
+  const dim3 grid((unsigned)((r.N + r.cg - 1) / r.cg)), wg(64 * kRcWaves);
+  if (r.M <= 16) gated_linear_rows_kernel<1, ACT><<<grid, wg, 0, s>>>(p, r);
+  else if (r.M <= 32) gated_linear_rows_kernel<2, ACT><<<grid, wg, 0, s>>>(p, r);
+  else gated_linear_rows_kernel<4, ACT><<<grid, wg, 0, s>>>(p, r);
+}
+
 template <class C, bool BWD, int ACT>
 static void gated_go(const GatedParams& p, hipStream_t s) {
-  if (BWD) gated_linear_bwd_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+  if constexpr (BWD) gated_linear_bwd_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
   else gated_linear_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
 }
 
@@ -148,7 +176,11 @@ extern "C" int mla_gated_linear(const mla_gated_linear_args* a, void* stream) {
   p.saved = (unsigned char*)a->saved;
   p.os = a->h_stride;
   hipStream_t s = (hipStream_t)stream;
-  if (gemm_plan(a->M, 2 * a->N, a->K, 1).large) gated_launch<GemmCfg<256, 2, 4, false, true>, false>(p, a->activation, s);
+  if (a->M <= kRcMaxRows) {
+    if (a->activation == MLA_ACT_RELU) gated_rows_go<MLA_ACT_RELU>(p, s);
+    else if (a->activation == MLA_ACT_SILU) gated_rows_go<MLA_ACT_SILU>(p, s);
+    else gated_rows_go<MLA_ACT_GELU_TANH>(p, s);
+  } else if (gemm_plan(a->M, 2 * a->N, a->K, 1).large) gated_launch<GemmCfg<256, 2, 4, false, true>, false>(p, a->activation, s);
   else gated_launch<GemmCfg<128, 2, 2, false, true>, false>(p, a->activation, s);
   return launch_status(op);
 }

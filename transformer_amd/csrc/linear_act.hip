@@ -5,6 +5,7 @@
 
 #include "gemm_epilogue.h"
 #include "linear_checks.h"
+#include "rows_core.h"
 
 namespace mla {
 
@@ -104,6 +105,36 @@ __global__ __launch_bounds__(C::THREADS, 2) void linear_dx_kernel(LinearParams p
   });
 }
 
+template <int MB, int ACT>
+__global__ __launch_bounds__(64 * kRcWaves) void linear_act_rows_kernel(LinearParams p, RowsArgs r) {
+  __shared__ f32x4 red[kRcWaves][MB][64];
+  RowsProduct<MB, false> t;
+  t.run(r, red);
+  if (!t.mine) return;
+  f32x4 v = t.sum[0];
+  if (p.bias) {
+    const u32x2 b = ldg8(p.bias + t.n);
+    v += f32x4{lo_bf16(b[0]), hi_bf16(b[0]), lo_bf16(b[1]), hi_bf16(b[1])};
+  }
+  if (p.saved) saved_store4(p.saved + ((int64_t)(t.m >> 5) * ((r.N + 31) >> 5) + (t.n >> 5)) * kSavedBlock, t.m, t.n, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(v[e]);
+  if (p.residual) {
+    const u32x2 b = ldg8(p.residual + t.m * p.rs + t.n);
+    v += f32x4{lo_bf16(b[0]), hi_bf16(b[0]), lo_bf16(b[1]), hi_bf16(b[1])};
+  }
+  stg8(p.y + t.m * p.ys + t.n, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+}
+
+template <int ACT>
+static void linear_act_rows_go(const LinearParams& p, hipStream_t s) {
+  const RowsArgs r{p.g.x, p.g.w0, nullptr, p.g.xs, p.g.ws0, 0, p.g.M, p.g.N, p.g.K, rows_columns(p.g.N)};
+  const dim3 grid((unsigned)((r.N + r.cg - 1) / r.cg)), wg(64 * kRcWaves);
+  if (r.M <= 16) linear_act_rows_kernel<1, ACT><<<grid, wg, 0, s>>>(p, r);
+  else if (r.M <= 32) linear_act_rows_kernel<2, ACT><<<grid, wg, 0, s>>>(p, r);
+  else linear_act_rows_kernel<4, ACT><<<grid, wg, 0, s>>>(p, r);
+}
+
 template <class C, int ACT>
 static void linear_act_go(const LinearParams& p, hipStream_t s) {
   linear_act_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
@@ -183,7 +214,12 @@ extern "C" int mla_linear_act(const mla_linear_act_args* a, void* stream) {
   p.rs = a->residual_stride;
   p.ys = a->y_stride;
   hipStream_t s = (hipStream_t)stream;
-  if (gemm_plan(a->M, a->N, a->K, 1).large) linear_act_launch<GemmCfg<256, 2, 4, false, false>>(p, a->activation, s);
+  if (a->M <= kRcMaxRows) {
+    if (a->activation == MLA_ACT_RELU) linear_act_rows_go<MLA_ACT_RELU>(p, s);
+    else if (a->activation == MLA_ACT_SILU) linear_act_rows_go<MLA_ACT_SILU>(p, s);
+    else if (a->activation == MLA_ACT_GELU_TANH) linear_act_rows_go<MLA_ACT_GELU_TANH>(p, s);
+    else linear_act_rows_go<MLA_ACT_NONE>(p, s);
+  } else if (gemm_plan(a->M, a->N, a->K, 1).large) linear_act_launch<GemmCfg<256, 2, 4, false, false>>(p, a->activation, s);
   else linear_act_launch<GemmCfg<128, 2, 2, false, false>>(p, a->activation, s);
   return launch_status("mla_linear_act");
 }

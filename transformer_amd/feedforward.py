@@ -18,8 +18,6 @@ from torch import Tensor
 
 from . import linear_ops, training
 
-ops = linear_ops.eager  # torch.ops.mla_mi355x, without the dispatcher where nothing needs it
-
 
 def _inputs(op: str, x: Tensor, residual):
     """(x as bf16, the residual that the kernel adds, the one that torch adds to its result)."""
@@ -35,15 +33,11 @@ def _inputs(op: str, x: Tensor, residual):
     return x, residual, None
 
 
-def _keeps(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 def linear_act(x: Tensor, weight: Tensor, bias: Tensor = None, residual: Tensor = None, activation: str = "none") -> Tensor:
     """``act(x W^T + bias) + residual`` for ``x [..., K]``, ``weight [N, K]``, ``bias [N]`` and ``residual [..., N]``, K and N
     multiples of 8; ``activation``: "none", "relu", "silu" or "gelu_tanh".  fp32 sums and epilogue, one rounding to bf16."""
     x, res, after = _inputs("linear_act", x, residual)
-    y, _ = ops.linear_act(x, weight, bias, res, activation, activation != "none" and _keeps(x, weight, bias))
+    y = linear_ops.linear(x, weight, bias, res, activation)
     return y if after is None else after + y
 
 
@@ -54,7 +48,7 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, residual:
     and the result are rounded to bf16 once each.  With gradients the block keeps the hidden layer (bf16) and both first
     products (24 bits each): 8 bytes per hidden value."""
     x, res, after = _inputs("gated_ffn", x, residual)
-    y, _, _ = ops.gated_ffn(x, w_gate, w_up, w_down, res, activation, _keeps(x, w_gate, w_up, w_down))
+    y = linear_ops.gated(x, w_gate, w_up, w_down, res, activation)
     return y if after is None else after + y
 
 

@@ -14,8 +14,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .kernels import _alloc_workspace
-from .linear_ops import _launch
+from .linear_ops import _fit_workspace, _launch
 
 _CODES = {torch.float32: _lib.MLA_DTYPE_F32, torch.bfloat16: _lib.MLA_DTYPE_BF16}
 
@@ -37,19 +36,22 @@ def _check(op: str, tensors: List[Tensor], norm_type: float) -> bool:
     norm_type = float(norm_type)
     if norm_type not in (2.0, math.inf):
         raise ValueError(f"{op}: norm_type {norm_type} is not built (2 or inf)")
-    device = None
-    for t in tensors:
-        if t.layout != torch.strided:
-            raise ValueError(f"{op}: sparse gradients are not built")
-        if not t.is_cuda:
-            raise RuntimeError(f"transformer_amd.{op} runs on a ROCm GPU only (no CPU path); got a tensor on {t.device}")
-        if t.dtype not in _CODES:
-            raise TypeError(f"{op}: gradients must be float32 or bfloat16, got {t.dtype}")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError(f"{op}: gradients on {device} and {t.device}: one device is needed")
+    if tensors:
+        dev = tensors[0].device
+        for t in tensors:
+            if t.device != dev or t.dtype not in _CODES or t.layout != torch.strided or not t.is_cuda:
+                _refuse(op, t, dev)
     return norm_type == math.inf
+
+
+def _refuse(op: str, t: Tensor, device: torch.device) -> None:
+    if t.layout != torch.strided:
+        raise ValueError(f"{op}: sparse gradients are not built")
+    if not t.is_cuda:
+        raise RuntimeError(f"transformer_amd.{op} runs on a ROCm GPU only (no CPU path); got a tensor on {t.device}")
+    if t.dtype not in _CODES:
+        raise TypeError(f"{op}: gradients must be float32 or bfloat16, got {t.dtype}")
+    raise ValueError(f"{op}: gradients on {device} and {t.device}: one device is needed")
 
 
 def _run(op: str, entry: str, tensors: List[Tensor], is_max: bool, max_norm: float) -> Tensor:
@@ -60,12 +62,9 @@ def _run(op: str, entry: str, tensors: List[Tensor], is_max: bool, max_norm: flo
     ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
     numels = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
     dtypes = (ctypes.c_int32 * n)(*[_CODES[t.dtype] for t in tensors])
-    args = _lib.GradNormArgs(
-        ptrs=ctypes.addressof(ptrs), numels=ctypes.addressof(numels), dtypes=ctypes.addressof(dtypes), n_tensors=n,
-        norm=norm.data_ptr(), workspace=None, workspace_bytes=0, max_norm=max_norm, norm_is_max=int(is_max))
-    nbytes = int(_lib.entry("mla_grad_norm_workspace_bytes")(ctypes.byref(args)))
-    ws = _alloc_workspace(nbytes, like.device)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    args = _lib.GradNormArgs(ctypes.addressof(ptrs), ctypes.addressof(numels), ctypes.addressof(dtypes), n, norm.data_ptr(), None,
+                             0, max_norm, int(is_max))
+    ws = _fit_workspace("mla_grad_norm_workspace_bytes", args, like)  # noqa: F841  (kept until the launch)
     _launch(entry, args, like, op)
     return norm
 
@@ -97,8 +96,10 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     if not grads:
         return torch.tensor(0.0)
     with torch.no_grad():
-        flat, back = [], []
-        for g in grads:
+        flat, back = grads, []
+        if not all(g.is_contiguous() for g in grads):
+            flat = []
+        for g in grads if flat is not grads else ():
             if _dense(g):
                 flat.append(g)
                 continue

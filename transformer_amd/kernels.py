@@ -1140,9 +1140,9 @@ class _EagerOps:
     directly when ``dispatcher_needed`` is false, its autograd formula as a plain autograd.Function
     when a gradient is all that is needed, else the registered operator."""
 
-    def __init__(self, names):
-        for name in names:
+    def __init__(self):
+        for name in _BODIES:
             setattr(self, name, _eager_call(name))
 
 
-eager = _EagerOps(_BODIES)
+eager = _EagerOps()

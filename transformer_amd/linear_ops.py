@@ -1,7 +1,8 @@
 """The linear layers' operators (``torch.ops.mla_mi355x.linear_act``, ``gated_ffn`` and their backwards).
 
-They are registered as those of ``kernels`` are; ``eager`` runs their bodies without the dispatcher where nothing needs it.
-There is no CPU path: a CPU tensor, or a missing library, raises.
+They are registered as those of ``kernels`` are.  ``linear`` and ``gated`` are what eager callers take: the same bodies without
+the dispatcher where nothing needs it, with an autograd.Function where a gradient is all that is needed.  There is no CPU path:
+a CPU tensor, or a missing library, raises.
 """
 from __future__ import annotations
 
@@ -11,22 +12,26 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
-from . import _lib
-from .kernels import (_alloc_workspace, _bf16, _dt_code, _EagerOps, _op, _ptr, _register_autograd, _require_gpu, _stream,
-                      batched_grad, weight_grad, weight_grad_or_none)
+from . import _lib, kernels
+from ._lib import ACTIVATIONS
+from .kernels import _alloc_workspace, _dt_code, _op, _register_autograd, weight_grad, weight_grad_or_none
 
 LINEAR_MAX_STRIDE = 1 << 22
+_BF16, _F32 = torch.bfloat16, torch.float32
 
+
+# ----------------------------------------------------------------- helpers
 
 def _launch(entry: str, args, like: Tensor, op: str) -> None:
     """Call a C entry point on ``like``'s device and its current stream, whichever device is the current one."""
     fn, dev = _lib.entry(entry), like.get_device()
     if dev == torch._C._cuda_getDevice():
-        rc = fn(ctypes.byref(args), _stream(like))
+        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(ctypes.byref(args), _stream(like))
-    _lib.check(rc, op)
+            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, op)
 
 
 def _fit_workspace(entry: str, args, like: Tensor) -> Optional[Tensor]:
@@ -42,14 +47,15 @@ def _fit_workspace(entry: str, args, like: Tensor) -> Optional[Tensor]:
 def _matrix(t: Tensor, K: int, one_row: bool = False) -> Tensor:
     """``t [..., K]`` as rows the linear kernels take: unit inner stride, 16-byte aligned, a row stride that is a multiple of
     8 and covers a row (``one_row``: or 0, the same row for all); copied where its layout is another."""
-    t = t.reshape(-1, K)
-    if t.size(0) <= 1:
-        ok = t.stride(1) == 1 or K == 1
-    else:
-        s = t.stride(0)
-        ok = t.stride(1) == 1 and s % 8 == 0 and s < LINEAR_MAX_STRIDE and (s >= K or (one_row and s == 0))
-    if ok and t.data_ptr() % 16 == 0:
-        return t
+    if t.dim() != 2:
+        t = t.reshape(-1, K)
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        if t.stride(1) == 1:
+            s = t.stride(0)
+            if t.size(0) <= 1 or (s % 8 == 0 and s < LINEAR_MAX_STRIDE and (s >= K or (one_row and s == 0))):
+                return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -58,47 +64,81 @@ def _row_stride(t: Tensor) -> int:
 
 
 def _weight_bf16(w: Tensor) -> Tensor:
-    return _matrix(w.detach().to(torch.bfloat16), w.size(1))
+    return _matrix(w if w.dtype == _BF16 else w.to(_BF16), w.size(1))
 
 
 def _activation(op: str, name: str, gate: bool = False) -> int:
-    code = _lib.ACTIVATIONS.get(name)
-    if code is None or (gate and name == "none"):
-        raise ValueError(f"{op}: activation {name!r} is not one of "
-                         f"{[a for a in _lib.ACTIVATIONS if not (gate and a == 'none')]}")
+    code = ACTIVATIONS.get(name)
+    if code is None or (gate and code == 0):
+        raise ValueError(f"{op}: activation {name!r} is not one of {[a for a in ACTIVATIONS if not (gate and a == 'none')]}")
     return code
 
 
-def _linear_check(op: str, x: Tensor, weights, residual: Optional[Tensor], n_out: int) -> None:
-    _require_gpu(op, x, residual, *weights.values())
-    _bf16(op, x=x)
-    for name, w in weights.items():
-        if w.dtype not in (torch.bfloat16, torch.float32):
-            raise TypeError(f"{op}: {name} must be bfloat16 or float32, got {w.dtype}")
-        if w.device != x.device:
-            raise ValueError(f"{op}: {name} is on {w.device}, x on {x.device}")
-        if w.dim() == 2 and (w.size(0) % 8 or w.size(1) % 8 or not w.numel()):
-            raise ValueError(f"{op}: {name} {tuple(w.shape)}: both sizes must be positive multiples of 8")
+def _check(op: str, x: Tensor, weights, names, residual: Optional[Tensor], n_out: int) -> None:
+    """Types, devices and sizes of the inputs (their shapes were compared already)."""
+    dev = x.get_device()
+    for t, name in zip(weights, names):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{op}: tensors must be on a ROCm GPU (got {t.device}); transformer_amd has no CPU implementation")
+        if t.dtype != _BF16 and t.dtype != _F32:
+            raise TypeError(f"{op}: {name} must be bfloat16 or float32, got {t.dtype}")
+        if t.get_device() != dev:
+            raise ValueError(f"{op}: {name} is on {t.device}, x on {x.device}")
+        if t.dim() == 2:
+            n, k = t.shape
+            if n % 8 or k % 8 or not n or not k:
+                raise ValueError(f"{op}: {name} {tuple(t.shape)}: both sizes must be positive multiples of 8")
+    kernels._require_gpu(op, x, residual)
+    if x.dtype != _BF16:
+        raise TypeError(f"{op}: x must be bfloat16, got {x.dtype}")
     if residual is not None:
-        _bf16(op, residual=residual)
-        if residual.shape != (*x.shape[:-1], n_out) or residual.device != x.device:
+        if residual.dtype != _BF16:
+            raise TypeError(f"{op}: residual must be bfloat16, got {residual.dtype}")
+        if residual.shape != (*x.shape[:-1], n_out) or residual.get_device() != dev:
             raise ValueError(f"{op}: residual must be {(*x.shape[:-1], n_out)} on {x.device}, got {tuple(residual.shape)} "
                              f"on {residual.device}")
 
 
-def _saved_buffer(M: int, N: int, blocks: int, like: Tensor) -> Tensor:
-    return torch.empty(blocks * int(_lib.entry("mla_linear_saved_size")(M, N)), dtype=torch.uint8, device=like.device)
+def _saved_size(M: int, N: int) -> int:
+    return 3072 * ((M + 31) // 32) * ((N + 31) // 32)  # mla_linear_saved_size
 
 
-def _linear_act_run(op, x2, w, bias, res2, code, saved, out):
-    """``out = act(x2 w^T + bias) + res2`` on bf16 matrices as :func:`_matrix` leaves them."""
-    (M, K), N = x2.shape, w.size(0)
+def _linear_run(op, x2, w, bias, res2, code, saved, y, M):
+    """``y = act(x2 w^T + bias) + res2`` on bf16 matrices as :func:`_matrix` leaves them."""
+    N, K = w.shape
     args = _lib.LinearActArgs(
-        x=x2.data_ptr(), w=w.data_ptr(), bias=_ptr(bias), residual=_ptr(res2), y=out.data_ptr(), saved=_ptr(saved),
-        workspace=None, workspace_bytes=0, M=M, N=N, K=K, x_stride=_row_stride(x2), w_stride=_row_stride(w),
-        residual_stride=0 if res2 is None else _row_stride(res2), y_stride=N, activation=code)
-    ws = _fit_workspace("mla_linear_act_workspace_bytes", args, out)  # noqa: F841  (kept until the launch)
-    _launch("mla_linear_act", args, out, op)
+        x2.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(), None if res2 is None else res2.data_ptr(),
+        y.data_ptr(), None if saved is None else saved.data_ptr(), None, 0, M, N, K, _row_stride(x2), _row_stride(w),
+        0 if res2 is None else _row_stride(res2), N, code)
+    _launch("mla_linear_act", args, y, op)
+
+
+# ----------------------------------------------------------------- linear layer with its epilogue
+
+def _linear_act(x, weight, bias, residual, activation, save):
+    """``(y, saved or None)``; see :func:`linear_act`."""
+    op = "mla_mi355x::linear_act"
+    code = _activation(op, activation)
+    if weight.dim() != 2 or x.dim() < 1 or x.size(-1) != weight.size(1) or (bias is not None
+                                                                            and bias.shape != (weight.size(0),)):
+        raise ValueError(f"{op}: expected x [..., K], weight [N, K], bias [N]; got {tuple(x.shape)}, {tuple(weight.shape)}, "
+                         f"{None if bias is None else tuple(bias.shape)}")
+    N, K = weight.shape
+    _check(op, x, (weight, bias), ("weight", "bias"), residual, N)
+    x2 = _matrix(x, K)
+    M = x2.size(0)
+    y = torch.empty((*x.shape[:-1], N), dtype=_BF16, device=x.device)
+    saved = torch.empty(_saved_size(M, N), dtype=torch.uint8, device=x.device) if save and code else None
+    if M:
+        b = bias
+        if b is not None:
+            b = b.to(_BF16).contiguous()
+            if b.data_ptr() % 8:
+                b = b.clone()
+        _linear_run(op, x2, _weight_bf16(weight), b, None if residual is None else _matrix(residual, N, True), code, saved, y, M)
+    return y, saved
 
 
 @_op("linear_act", mutates_args=())
@@ -108,30 +148,12 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Opti
     [N]``, ``residual [..., N]`` bf16: fp32 sums and epilogue, one rounding.  ``activation``: none, relu, silu, gelu_tanh.
     Returns ``y`` and, with ``save`` and an activation, what the backward keeps of the pre-activation (else an empty
     tensor).  K and N multiples of 8."""
-    op = "mla_mi355x::linear_act"
-    code = _activation(op, activation)
-    if weight.dim() != 2 or x.dim() < 1 or x.size(-1) != weight.size(1) or (bias is not None
-                                                                            and bias.shape != (weight.size(0),)):
-        raise ValueError(f"{op}: expected x [..., K], weight [N, K], bias [N]; got {tuple(x.shape)}, {tuple(weight.shape)}, "
-                         f"{None if bias is None else tuple(bias.shape)}")
-    N, K = weight.shape
-    _linear_check(op, x, {"weight": weight, **({} if bias is None else {"bias": bias})}, residual, N)
-    x2 = _matrix(x, K)
-    M = x2.size(0)
-    y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
-    saved = _saved_buffer(M if save and code else 0, N, 1, x)
-    if M:
-        b = None if bias is None else bias.detach().to(torch.bfloat16).contiguous()
-        if b is not None and b.data_ptr() % 8:
-            b = b.clone()
-        _linear_act_run(op, x2, _weight_bf16(weight), b, None if residual is None else _matrix(residual, N, True), code,
-                        saved if saved.numel() else None, y)
-    return y.view(*x.shape[:-1], N), saved
+    y, saved = _linear_act(x, weight, bias, residual, activation, save)
+    return y, x.new_empty(0, dtype=torch.uint8) if saved is None else saved
 
 
 def _saved_fake(x, K, N, blocks, wanted):
-    M = x.numel() // K
-    return x.new_empty(blocks * 3072 * ((M + 31) // 32) * ((N + 31) // 32) if wanted else 0, dtype=torch.uint8)
+    return x.new_empty(blocks * _saved_size(x.numel() // K, N) if wanted else 0, dtype=torch.uint8)
 
 
 @linear_act.register_fake
@@ -140,11 +162,11 @@ def _(x, weight, bias, residual, activation, save):
     return x.new_empty(*x.shape[:-1], N), _saved_fake(x, K, N, 1, save and activation != "none")
 
 
-def _weight_grad_rows_any(dy: Tensor, x: Tensor, dtype: torch.dtype) -> Tensor:
+def _weight_grad(dy: Tensor, x: Tensor, dtype: torch.dtype) -> Tensor:
     """``dy^T x`` in ``dtype`` for any number of rows: those beyond the kernel's 32-bit reach in several parts, added in fp32."""
     if dy.size(0) == 0:
         return torch.zeros(dy.size(1), x.size(1), dtype=dtype, device=dy.device)
-    dw = weight_grad_or_none(dy, x, dtype == torch.float32)
+    dw = weight_grad_or_none(dy, x, dtype == _F32)
     if dw is None:
         rows = (1 << 30) // max(_row_stride(dy), _row_stride(x)) - 257
         if rows < 32:
@@ -152,22 +174,44 @@ def _weight_grad_rows_any(dy: Tensor, x: Tensor, dtype: torch.dtype) -> Tensor:
         for r in range(0, dy.size(0), rows):
             part = weight_grad(dy[r:r + rows], x[r:r + rows], True)
             dw = part if dw is None else dw.add_(part)
-    return dw.to(dtype)
+    return dw if dw.dtype == dtype else dw.to(dtype)
 
 
 def _linear_dx(op: str, dy: Tensor, weights, shape) -> Tensor:
     """``sum_p dy_p W_p`` for bf16 rows ``dy [M, P N]`` and P = 1 or 2 weights ``[N, K]``, as ``shape``."""
-    w = [_weight_bf16(t) for t in weights]
-    (N, K), M = w[0].shape, dy.size(0)
-    dx = torch.empty(M, K, dtype=torch.bfloat16, device=dy.device)
+    w0, w1 = _weight_bf16(weights[0]), _weight_bf16(weights[1]) if len(weights) > 1 else None
+    (N, K), M = w0.shape, dy.size(0)
+    dx = torch.empty(shape, dtype=_BF16, device=dy.device)
     if M:
-        args = _lib.LinearDxArgs(
-            dy=dy.data_ptr(), w0=w[0].data_ptr(), w1=w[1].data_ptr() if len(w) > 1 else None, dx=dx.data_ptr(),
-            workspace=None, workspace_bytes=0, M=M, N=N, K=K, dy_stride=_row_stride(dy), w0_stride=_row_stride(w[0]),
-            w1_stride=_row_stride(w[1]) if len(w) > 1 else 0, dx_stride=K)
-        ws = _fit_workspace("mla_linear_dx_workspace_bytes", args, dx)  # noqa: F841
+        args = _lib.LinearDxArgs(dy.data_ptr(), w0.data_ptr(), None if w1 is None else w1.data_ptr(), dx.data_ptr(), None, 0,
+                                 M, N, K, _row_stride(dy), _row_stride(w0), 0 if w1 is None else _row_stride(w1), K)
         _launch("mla_linear_dx", args, dx, op)
-    return dx.view(shape)
+    return dx
+
+
+def _linear_act_bwd(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype):
+    """``(dx, dw, db)``, None where not needed; see :func:`linear_act_bwd`."""
+    op = "mla_mi355x::linear_act_bwd"
+    code = _activation(op, activation)
+    N, K = weight.shape
+    dy2, x2 = _matrix(dy if dy.dtype == _BF16 else dy.to(_BF16), N), _matrix(x, K)
+    M = x2.size(0)
+    if dy2.size(0) != M or (code and saved.numel() != _saved_size(M, N)):
+        raise ValueError(f"{op}: dy {tuple(dy.shape)} and saved do not belong to x {tuple(x.shape)} and weight "
+                         f"{tuple(weight.shape)}")
+    dz, db = dy2, None
+    if db_dtype is not None:
+        db = (torch.empty if M else torch.zeros)(N, dtype=db_dtype, device=x.device)
+    if M and (code or db is not None):
+        if code:
+            dz = torch.empty(M, N, dtype=_BF16, device=x.device)
+        args = _lib.ActGradArgs(dy2.data_ptr(), saved.data_ptr() if code else None, dz.data_ptr() if code else None,
+                                None if db is None else db.data_ptr(), None, 0, M, N, _row_stride(dy2), N, code,
+                                0 if db is None else _dt_code(db))
+        ws = None if db is None else _fit_workspace("mla_act_grad_workspace_bytes", args, dy2)  # noqa: F841
+        _launch("mla_act_grad", args, dy2, op)
+    return (_linear_dx(op, dz, (weight,), x.shape) if need_dx else None,
+            _weight_grad(dz, x2, weight.dtype) if need_dw else None, db)
 
 
 @_op("linear_act_bwd", mutates_args=())
@@ -175,39 +219,35 @@ def linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, saved: Tensor, activat
                    db_dtype: Optional[torch.dtype]) -> Tuple[Tensor, Tensor, Tensor]:
     """Gradients ``(dx, dw, db)`` of :func:`linear_act` from ``dy`` and what it saved; ``dw`` in the weight's dtype, ``db`` in
     ``db_dtype`` (None: no bias).  Empty tensors where a gradient is not needed."""
-    op = "mla_mi355x::linear_act_bwd"
-    code = _activation(op, activation)
-    _require_gpu(op, dy, x, weight, saved)
-    _bf16(op, x=x)
-    N, K = weight.shape
-    dy2, x2 = _matrix(dy.to(torch.bfloat16), N), _matrix(x, K)
-    M = x2.size(0)
-    if dy2.size(0) != M:
-        raise ValueError(f"{op}: dy {tuple(dy.shape)} does not match x {tuple(x.shape)}")
-    none = x.new_empty(0)
-    dz, db = dy2, none
-    if db_dtype is not None:
-        db = torch.zeros(N, dtype=db_dtype, device=x.device) if M == 0 else torch.empty(N, dtype=db_dtype, device=x.device)
-    if M and (code or db_dtype is not None):
-        if code:
-            if saved.numel() != int(_lib.entry("mla_linear_saved_size")(M, N)):
-                raise ValueError(f"{op}: saved does not belong to x {tuple(x.shape)} and weight {tuple(weight.shape)}")
-            dz = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
-        args = _lib.ActGradArgs(
-            dy=dy2.data_ptr(), saved=_ptr(saved) if code else None, dz=dz.data_ptr() if code else None,
-            db=db.data_ptr() if db_dtype is not None else None, workspace=None, workspace_bytes=0, M=M, N=N,
-            dy_stride=_row_stride(dy2), dz_stride=N, activation=code, db_dtype=_dt_code(db))
-        ws = _fit_workspace("mla_act_grad_workspace_bytes", args, dy2)  # noqa: F841
-        _launch("mla_act_grad", args, dy2, op)
-    dx = _linear_dx(op, dz, (weight,), x.shape) if need_dx else none
-    dw = _weight_grad_rows_any(dz, x2, weight.dtype) if need_dw else none
-    return dx, dw, db
+    kernels._require_gpu("mla_mi355x::linear_act_bwd", dy, x, weight, saved)
+    kernels._bf16("mla_mi355x::linear_act_bwd", x=x)
+    got = _linear_act_bwd(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype)
+    return tuple(x.new_empty(0) if t is None else t for t in got)
 
 
 @linear_act_bwd.register_fake
 def _(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype):
-    return (x.new_empty(x.shape if need_dx else 0), weight.new_empty(weight.shape if need_dw else 0),
+    return (x.new_empty(x.shape if need_dx else 0), weight.new_empty(weight.shape) if need_dw else x.new_empty(0),
             x.new_empty(0) if db_dtype is None else x.new_empty(weight.size(0), dtype=db_dtype))
+
+
+def _plain_backward(dy: Tensor) -> bool:
+    """Whether a backward may run the bodies: it is not itself differentiated, batched or under a dispatch mode."""
+    return not (torch.is_grad_enabled() or kernels.batched_grad(dy) or kernels._not_plain((dy,)))
+
+
+def _linear_act_grads(ctx, dy, need):
+    """The gradients for (x, weight, bias) from the saved tensors of either autograd path."""
+    x, weight, bias, saved = ctx.saved_tensors
+    plain = _plain_backward(dy)
+    if ctx.activation != "none" and (saved is None or not saved.numel()) and x.numel():  # not kept: the product again
+        saved = torch.ops.mla_mi355x.linear_act(x.detach(), weight.detach(), None if bias is None else bias.detach(), None,
+                                                ctx.activation, True)[1]
+    if saved is None:
+        saved = x.new_empty(0, dtype=torch.uint8)
+    run = _linear_act_bwd if plain else torch.ops.mla_mi355x.linear_act_bwd
+    got = run(dy, x, weight, saved, ctx.activation, need[0], need[1], bias.dtype if bias is not None and need[2] else None)
+    return tuple(g if n else None for g, n in zip(got, (need[0], need[1], bias is not None and need[2])))
 
 
 def _linear_act_setup(ctx, inputs, output):
@@ -218,23 +258,70 @@ def _linear_act_setup(ctx, inputs, output):
 
 
 def _linear_act_backward(ctx, dy, dsaved):
-    x, weight, bias, saved = ctx.saved_tensors
     need = ctx.needs_input_grad
-    ops = _ops_for(dy)
-    dx = dw = db = None
-    if any(need[:3]):
-        if ctx.activation != "none" and not saved.numel() and x.numel():  # not kept: the product again
-            saved = ops.linear_act(x, weight, bias, None, ctx.activation, True)[1]
-        dx, dw, db = ops.linear_act_bwd(dy, x, weight, saved, ctx.activation, need[0], need[1],
-                                        bias.dtype if bias is not None and need[2] else None)
-    return (dx if need[0] else None, dw if need[1] else None, db if bias is not None and need[2] else None,
-            dy if need[3] else None, None, None)
+    grads = _linear_act_grads(ctx, dy, need) if any(need[:3]) else (None,) * 3
+    return (*grads, dy if need[3] else None, None, None)
 
 
 _register_autograd(linear_act, "linear_act", _linear_act_setup, _linear_act_backward)
 
 
+class _LinearAct(torch.autograd.Function):
+    """The operator's body and formula without its dispatch (60 to 80 us of host time a call)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        with kernels.below_autograd():
+            y, saved = _linear_act(x, weight, bias, residual, activation, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, bias, saved)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        grads = _linear_act_grads(ctx, dy, need) if any(need[:3]) else (None,) * 3
+        return (*grads, dy if need[3] else None, None)
+
+
+def linear(x, weight, bias, residual, activation) -> Tensor:
+    """:func:`linear_act`'s ``y`` for eager callers."""
+    args = (x, weight, bias, residual)
+    if kernels._needs_grad(args):
+        if kernels.function_fits(args):
+            return _LinearAct.apply(x, weight, bias, residual, activation)
+        return torch.ops.mla_mi355x.linear_act(x, weight, bias, residual, activation, True)[0]
+    if kernels._not_plain(args):
+        return torch.ops.mla_mi355x.linear_act(x, weight, bias, residual, activation, False)[0]
+    return _linear_act(x, weight, bias, residual, activation, False)[0]
+
+
 # ----------------------------------------------------------------- gated feed-forward block
+
+def _gated_ffn(x, w_gate, w_up, w_down, residual, activation, save):
+    """``(y, h, saved or None)``; see :func:`gated_ffn`."""
+    op = "mla_mi355x::gated_ffn"
+    code = _activation(op, activation, gate=True)
+    if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1] or x.dim() < 1 \
+            or x.size(-1) != w_gate.size(1):
+        raise ValueError(f"{op}: expected x [..., D], w_gate and w_up [H, D], w_down [D, H]; got {tuple(x.shape)}, "
+                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
+    H, D = w_gate.shape
+    _check(op, x, (w_gate, w_up, w_down), ("w_gate", "w_up", "w_down"), residual, D)
+    x2 = _matrix(x, D)
+    M = x2.size(0)
+    y = torch.empty(x.shape, dtype=_BF16, device=x.device)
+    h = torch.empty((M, H), dtype=_BF16, device=x.device)
+    saved = torch.empty(2 * _saved_size(M, H), dtype=torch.uint8, device=x.device) if save else None
+    if M:
+        wg, wu = _weight_bf16(w_gate), _weight_bf16(w_up)
+        args = _lib.GatedLinearArgs(
+            x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), None if saved is None else saved.data_ptr(), None, 0, M, H,
+            D, _row_stride(x2), _row_stride(wg), _row_stride(wu), H, code)
+        _launch("mla_gated_linear", args, h, op)
+        _linear_run(op, h, _weight_bf16(w_down), None, None if residual is None else _matrix(residual, D, True), 0, None, y, M)
+    return y, h, saved
+
 
 @_op("gated_ffn", mutates_args=())
 def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, residual: Optional[Tensor], activation: str,
@@ -243,29 +330,8 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, residual:
     H]`` (bf16, or fp32 read as bf16): silu(w1 x) * w3 x through w2 (transformer.py:117-125).  ``activation``: relu, silu,
     gelu_tanh.  The hidden layer is rounded to bf16 once, between the products.  Returns ``y`` and, with ``save``, the
     hidden layer and what the backward keeps of the two products (else empty tensors).  D and H multiples of 8."""
-    op = "mla_mi355x::gated_ffn"
-    code = _activation(op, activation, gate=True)
-    if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1] or x.dim() < 1 \
-            or x.size(-1) != w_gate.size(1):
-        raise ValueError(f"{op}: expected x [..., D], w_gate and w_up [H, D], w_down [D, H]; got {tuple(x.shape)}, "
-                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
-    H, D = w_gate.shape
-    _linear_check(op, x, {"w_gate": w_gate, "w_up": w_up, "w_down": w_down}, residual, D)
-    x2 = _matrix(x, D)
-    M = x2.size(0)
-    y = torch.empty(M, D, dtype=torch.bfloat16, device=x.device)
-    h = torch.empty(M, H, dtype=torch.bfloat16, device=x.device)
-    saved = _saved_buffer(M if save else 0, H, 2, x)
-    if M:
-        wg, wu = _weight_bf16(w_gate), _weight_bf16(w_up)
-        args = _lib.GatedLinearArgs(
-            x=x2.data_ptr(), w_gate=wg.data_ptr(), w_up=wu.data_ptr(), h=h.data_ptr(),
-            saved=saved.data_ptr() if save else None, workspace=None, workspace_bytes=0, M=M, N=H, K=D,
-            x_stride=_row_stride(x2), w_gate_stride=_row_stride(wg), w_up_stride=_row_stride(wu), h_stride=H, activation=code)
-        ws = _fit_workspace("mla_gated_linear_workspace_bytes", args, h)  # noqa: F841
-        _launch("mla_gated_linear", args, h, op)
-        _linear_act_run(op, h, _weight_bf16(w_down), None, None if residual is None else _matrix(residual, D, True), 0, None, y)
-    return y.view(x.shape), h if save else h.new_empty(0), saved
+    y, h, saved = _gated_ffn(x, w_gate, w_up, w_down, residual, activation, save)
+    return (y, h, saved) if save else (y, x.new_empty(0), x.new_empty(0, dtype=torch.uint8))
 
 
 @gated_ffn.register_fake
@@ -274,49 +340,64 @@ def _(x, w_gate, w_up, w_down, residual, activation, save):
     return (x.new_empty(x.shape), x.new_empty((x.numel() // D, H) if save else 0), _saved_fake(x, D, H, 2, save))
 
 
+def _gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, need_gate, need_up, need_down):
+    """``(dx, dw_gate, dw_up, dw_down)``, None where not needed; see :func:`gated_ffn_bwd`."""
+    op = "mla_mi355x::gated_ffn_bwd"
+    code = _activation(op, activation, gate=True)
+    H, D = w_gate.shape
+    dy2, x2 = _matrix(dy if dy.dtype == _BF16 else dy.to(_BF16), D), _matrix(x, D)
+    M = x2.size(0)
+    if dy2.size(0) != M or tuple(h.shape) != (M, H) or not h.is_contiguous() or saved.numel() != 2 * _saved_size(M, H):
+        raise ValueError(f"{op}: dy {tuple(dy.shape)}, h {tuple(h.shape)} and saved do not belong to x {tuple(x.shape)}")
+    dx = dwg = dwu = None
+    dwd = _weight_grad(dy2, h, w_down.dtype) if need_down else None
+    if need_dx or need_gate or need_up:
+        dgu = torch.empty((M, 2 * H), dtype=_BF16, device=x.device)
+        if M:
+            wd = _weight_bf16(w_down)
+            args = _lib.GatedLinearBwdArgs(dy2.data_ptr(), wd.data_ptr(), saved.data_ptr(), dgu.data_ptr(), M, H, D,
+                                           _row_stride(dy2), _row_stride(wd), 2 * H, code)
+            _launch("mla_gated_linear_bwd", args, dgu, op)
+        if need_dx:
+            dx = _linear_dx(op, dgu, (w_gate, w_up), x.shape)
+        if need_gate and need_up and w_gate.dtype == w_up.dtype:  # one product, its rows the two gradients
+            dwg, dwu = _weight_grad(dgu, x2, w_gate.dtype).split(H)
+        else:
+            dwg = _weight_grad(dgu[:, :H], x2, w_gate.dtype) if need_gate else None
+            dwu = _weight_grad(dgu[:, H:], x2, w_up.dtype) if need_up else None
+    return dx, dwg, dwu, dwd
+
+
 @_op("gated_ffn_bwd", mutates_args=())
 def gated_ffn_bwd(dy: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, h: Tensor, saved: Tensor,
                   activation: str, need_dx: bool, need_gate: bool, need_up: bool,
                   need_down: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
     """Gradients ``(dx, dw_gate, dw_up, dw_down)`` of :func:`gated_ffn` from ``dy`` and what it saved, the weights' in their
     dtypes.  Empty tensors where a gradient is not needed."""
-    op = "mla_mi355x::gated_ffn_bwd"
-    code = _activation(op, activation, gate=True)
-    _require_gpu(op, dy, x, w_gate, w_up, w_down, h, saved)
-    _bf16(op, x=x, h=h)
-    H, D = w_gate.shape
-    dy2, x2 = _matrix(dy.to(torch.bfloat16), D), _matrix(x, D)
-    M = x2.size(0)
-    if dy2.size(0) != M or tuple(h.shape) != (M, H) or not h.is_contiguous() \
-            or saved.numel() != 2 * int(_lib.entry("mla_linear_saved_size")(M, H)):
-        raise ValueError(f"{op}: dy {tuple(dy.shape)}, h {tuple(h.shape)} and saved do not belong to x {tuple(x.shape)}")
-    none = x.new_empty(0)
-    dx, dwg, dwu, dwd = none, none, none, none
-    if need_down:
-        dwd = _weight_grad_rows_any(dy2, h, w_down.dtype)
-    if need_dx or need_gate or need_up:
-        dgu = torch.empty(M, 2 * H, dtype=torch.bfloat16, device=x.device)
-        if M:
-            wd = _weight_bf16(w_down)
-            args = _lib.GatedLinearBwdArgs(
-                dy=dy2.data_ptr(), w_down=wd.data_ptr(), saved=saved.data_ptr(), dgu=dgu.data_ptr(), M=M, N=H, K=D,
-                dy_stride=_row_stride(dy2), w_stride=_row_stride(wd), dgu_stride=2 * H, activation=code)
-            _launch("mla_gated_linear_bwd", args, dgu, op)
-        if need_dx:
-            dx = _linear_dx(op, dgu, (w_gate, w_up), x.shape)
-        if need_gate and need_up and w_gate.dtype == w_up.dtype:  # one product, its rows the two gradients
-            dwg, dwu = _weight_grad_rows_any(dgu, x2, w_gate.dtype).split(H)
-            dwu = dwu.clone()  # (an operator's outputs share no memory)
-        else:
-            dwg = _weight_grad_rows_any(dgu[:, :H], x2, w_gate.dtype) if need_gate else none
-            dwu = _weight_grad_rows_any(dgu[:, H:], x2, w_up.dtype) if need_up else none
-    return dx, dwg, dwu, dwd
+    kernels._require_gpu("mla_mi355x::gated_ffn_bwd", dy, x, w_gate, w_up, w_down, h, saved)
+    kernels._bf16("mla_mi355x::gated_ffn_bwd", x=x, h=h)
+    dx, dwg, dwu, dwd = _gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, need_gate, need_up, need_down)
+    if dwg is not None and dwu is not None and dwu.untyped_storage().data_ptr() == dwg.untyped_storage().data_ptr():
+        dwu = dwu.clone()  # (an operator's outputs share no memory)
+    return tuple(x.new_empty(0) if t is None else t for t in (dx, dwg, dwu, dwd))
 
 
 @gated_ffn_bwd.register_fake
 def _(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, need_gate, need_up, need_down):
-    return (x.new_empty(x.shape if need_dx else 0), w_gate.new_empty(w_gate.shape if need_gate else 0),
-            w_up.new_empty(w_up.shape if need_up else 0), w_down.new_empty(w_down.shape if need_down else 0))
+    return tuple(t.new_empty(t.shape) if n else x.new_empty(0)
+                 for t, n in ((x, need_dx), (w_gate, need_gate), (w_up, need_up), (w_down, need_down)))
+
+
+def _gated_ffn_grads(ctx, dy, need):
+    """The gradients for (x, w_gate, w_up, w_down) from the saved tensors of either autograd path."""
+    x, w_gate, w_up, w_down, h, saved = ctx.saved_tensors
+    plain = _plain_backward(dy)
+    if not saved.numel() and x.numel():  # not kept: the first half again
+        _, h, saved = torch.ops.mla_mi355x.gated_ffn(x.detach(), w_gate.detach(), w_up.detach(), w_down.detach(), None,
+                                                     ctx.activation, True)
+    run = _gated_ffn_bwd if plain else torch.ops.mla_mi355x.gated_ffn_bwd
+    got = run(dy, x, w_gate, w_up, w_down, h, saved, ctx.activation, *need[:4])
+    return tuple(g if n else None for g, n in zip(got, need))
 
 
 def _gated_ffn_setup(ctx, inputs, output):
@@ -327,23 +408,41 @@ def _gated_ffn_setup(ctx, inputs, output):
 
 
 def _gated_ffn_backward(ctx, dy, dh, dsaved):
-    x, w_gate, w_up, w_down, h, saved = ctx.saved_tensors
     need = ctx.needs_input_grad
-    ops = _ops_for(dy)
-    grads = [None] * 4
-    if any(need[:4]):
-        if not saved.numel() and x.numel():  # not kept: the first half again
-            _, h, saved = ops.gated_ffn(x, w_gate, w_up, w_down, None, ctx.activation, True)
-        grads = ops.gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, ctx.activation, *need[:4])
-    return (*(g if n else None for g, n in zip(grads, need)), dy if need[4] else None, None, None)
+    grads = _gated_ffn_grads(ctx, dy, need) if any(need[:4]) else (None,) * 4
+    return (*grads, dy if need[4] else None, None, None)
 
 
 _register_autograd(gated_ffn, "gated_ffn", _gated_ffn_setup, _gated_ffn_backward)
 
 
-eager = _EagerOps(("linear_act", "linear_act_bwd", "gated_ffn", "gated_ffn_bwd"))
+class _GatedFfn(torch.autograd.Function):
+    """The operator's body and formula without its dispatch."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, residual, activation):
+        save = any(ctx.needs_input_grad[:4])
+        with kernels.below_autograd():
+            y, h, saved = _gated_ffn(x, w_gate, w_up, w_down, residual, activation, save)
+        if save:
+            ctx.save_for_backward(x, w_gate, w_up, w_down, h, saved)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        grads = _gated_ffn_grads(ctx, dy, need) if any(need[:4]) else (None,) * 4
+        return (*grads, dy if need[4] else None, None)
 
 
-def _ops_for(grad: Tensor):
-    """The operators that a backward formula runs on ``grad``."""
-    return torch.ops.mla_mi355x if batched_grad(grad) else eager
+def gated(x, w_gate, w_up, w_down, residual, activation) -> Tensor:
+    """:func:`gated_ffn`'s ``y`` for eager callers."""
+    args = (x, w_gate, w_up, w_down, residual)
+    if kernels._needs_grad(args):
+        if kernels.function_fits(args):
+            return _GatedFfn.apply(x, w_gate, w_up, w_down, residual, activation)
+        return torch.ops.mla_mi355x.gated_ffn(x, w_gate, w_up, w_down, residual, activation, True)[0]
+    if kernels._not_plain(args):
+        return torch.ops.mla_mi355x.gated_ffn(x, w_gate, w_up, w_down, residual, activation, False)[0]
+    return _gated_ffn(x, w_gate, w_up, w_down, residual, activation, False)[0]
