@@ -503,12 +503,9 @@ int mla_linear_act(const mla_linear_act_args* a, void* stream);
 typedef struct {
   const void *x, *w_gate, *w_up;
   void *h, *saved;
-  void* workspace;
-  size_t workspace_bytes;
   int64_t M, N, K, x_stride, w_gate_stride, w_up_stride, h_stride;
   int32_t activation;
 } mla_gated_linear_args;
-size_t mla_gated_linear_workspace_bytes(const mla_gated_linear_args* a);
 int mla_gated_linear(const mla_gated_linear_args* a, void* stream);
 
 /* Its gradient through the second product: with dh[m][n] = sum_k dy[m][k] W_down[k][n] (fp32, never stored),
@@ -528,7 +525,8 @@ int mla_gated_linear_bwd(const mla_gated_linear_bwd_args* a, void* stream);
 
 /* The input gradient of one linear layer, or of two over the same input:
  *   dx[m][k] = bf16(sum_n dy[m][n] W0[n][k] + sum_n dy[m][N + n] W1[n][k])     (the second sum where w1 is not NULL)
- * dy [M, N] or [M, 2 N], weights [N, K], dx [M, K]; fp32 sums over both.  N and K multiples of 8.
+ * dy [M, N] or [M, 2 N], weights [N, K], dx [M, K]; fp32 sums over both.  N and K multiples of 8;
+ * w0_stride and w1_stride the same.
  *
  * Replaces: autograd of the products above with respect to x.
  */

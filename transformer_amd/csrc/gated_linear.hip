@@ -23,8 +23,8 @@ __device__ __forceinline__ unsigned char* gated_saved_at(const GatedParams& p, i
 template <class C, int ACT>
 __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_kernel(GatedParams p) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
-  const WavePos<C> at;
-  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1) {
+  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1, int, int) {
+    const WavePos<C> at;
     const StagedRows<C, C::TN> st{s0, s1};
     constexpr int HB = C::NB / 2;
     const int mv = min(C::T, p.g.M - m0), nv = min(C::TN, p.g.N - n0);
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_kernel(GatedParams
         }
       }
     __syncthreads();
-    store_rows<C>(st, C::T, p.out + (int64_t)m0 * p.os + n0, p.os, mv, nv, [](int r) { return r; });
+    store_rows<C>(st, at.tid, C::T, p.out + (int64_t)m0 * p.os + n0, p.os, mv, nv, [](int r) { return r; });
     __syncthreads();
   });
 }
@@ -56,8 +56,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_kernel(GatedParams
 template <class C, int ACT>
 __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedParams p) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
-  const WavePos<C> at;
-  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1) {
+  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1, int, int) {
+    const WavePos<C> at;
     const StagedRows<C, C::T> st{s0, s1};
     const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
     const int sr = 32 * at.wm + at.l32;
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedPa
         }
       }
       __syncthreads();
-      store_rows<C>(st, 32 * C::WM, out, p.os, mv, nv, [&](int r) { return pass_row<C>(r, j); });
+      store_rows<C>(st, at.tid, 32 * C::WM, out, p.os, mv, nv, [&](int r) { return pass_row<C>(r, j); });
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < C::NB; ++i)
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedPa
                u32x2{pack_bf16x2(du[4 * q], du[4 * q + 1]), pack_bf16x2(du[4 * q + 2], du[4 * q + 3])});
         }
       __syncthreads();
-      store_rows<C>(st, 32 * C::WM, out + p.g.N, p.os, mv, nv, [&](int r) { return pass_row<C>(r, j); });
+      store_rows<C>(st, at.tid, 32 * C::WM, out + p.g.N, p.os, mv, nv, [&](int r) { return pass_row<C>(r, j); });
       __syncthreads();
     }
   });
@@ -137,8 +137,7 @@ static void gated_go(const GatedParams& p, hipStream_t s) {
 }
 
 template <class C, bool BWD>
-static void gated_launch(GatedParams& p, int act, hipStream_t s) {
-  gemm_tile_counts<C>(p.g);
+static void gated_launch(const GatedParams& p, int act, hipStream_t s) {
   if (act == MLA_ACT_RELU) gated_go<C, BWD, MLA_ACT_RELU>(p, s);
   else if (act == MLA_ACT_SILU) gated_go<C, BWD, MLA_ACT_SILU>(p, s);
   else gated_go<C, BWD, MLA_ACT_GELU_TANH>(p, s);
@@ -153,11 +152,6 @@ static int check_gate(const char* op, int act) {
 
 using namespace mla;
 
-extern "C" size_t mla_gated_linear_workspace_bytes(const mla_gated_linear_args* a) {
-  (void)a;
-  return 0;
-}
-
 extern "C" int mla_gated_linear(const mla_gated_linear_args* a, void* stream) {
   const char* op = "mla_gated_linear";
   MLA_CHECK(a, MLA_ERR_INVALID_ARG, "%s: null args", op);
@@ -170,8 +164,9 @@ extern "C" int mla_gated_linear(const mla_gated_linear_args* a, void* stream) {
   MLA_TRY(check_rows(op, "h", a->h, a->N, a->h_stride));
   MLA_CHECK(((uintptr_t)a->saved & 15) == 0, MLA_ERR_INVALID_ARG, "%s: saved must be 16-byte aligned", op);
   GatedParams p{};
-  p.g = GemmArgs{(const bf16*)a->x, (const bf16*)a->w_gate, (const bf16*)a->w_up, a->x_stride, a->w_gate_stride, a->w_up_stride,
-                 (int)a->M, (int)a->N, (int)a->K, 1};
+  p.g.x = (const bf16*)a->x, p.g.w0 = (const bf16*)a->w_gate, p.g.w1 = (const bf16*)a->w_up;
+  p.g.xs = a->x_stride, p.g.ws0 = a->w_gate_stride, p.g.ws1 = a->w_up_stride;
+  p.g.M = (int)a->M, p.g.N = (int)a->N, p.g.K = (int)a->K, p.g.parts = 1;
   p.out = (bf16*)a->h;
   p.saved = (unsigned char*)a->saved;
   p.os = a->h_stride;
@@ -180,7 +175,11 @@ extern "C" int mla_gated_linear(const mla_gated_linear_args* a, void* stream) {
     if (a->activation == MLA_ACT_RELU) gated_rows_go<MLA_ACT_RELU>(p, s);
     else if (a->activation == MLA_ACT_SILU) gated_rows_go<MLA_ACT_SILU>(p, s);
     else gated_rows_go<MLA_ACT_GELU_TANH>(p, s);
-  } else if (gemm_plan(a->M, 2 * a->N, a->K, 1).large) gated_launch<GemmCfg<256, 2, 4, false, true>, false>(p, a->activation, s);
+    return launch_status(op);
+  }
+  const GemmPlan pl = gemm_plan(a->M, 2 * a->N, a->K, 1, false);
+  MLA_TRY(gemm_apply(op, p.g, pl, nullptr, 0, 2));
+  if (pl.large) gated_launch<GemmCfg<256, 2, 4, false, true>, false>(p, a->activation, s);
   else gated_launch<GemmCfg<128, 2, 2, false, true>, false>(p, a->activation, s);
   return launch_status(op);
 }
@@ -197,13 +196,16 @@ extern "C" int mla_gated_linear_bwd(const mla_gated_linear_bwd_args* a, void* st
   MLA_TRY(check_rows(op, "dgu", a->dgu, 2 * a->N, a->dgu_stride));
   MLA_CHECK(a->saved && ((uintptr_t)a->saved & 15) == 0, MLA_ERR_INVALID_ARG, "%s: saved must be given, 16-byte aligned", op);
   GatedParams p{};
-  p.g = GemmArgs{(const bf16*)a->dy, (const bf16*)a->w_down, nullptr, a->dy_stride, a->w_stride, 0, (int)a->M, (int)a->N,
-                 (int)a->K, 1};
+  p.g.x = (const bf16*)a->dy, p.g.w0 = (const bf16*)a->w_down;
+  p.g.xs = a->dy_stride, p.g.ws0 = a->w_stride;
+  p.g.M = (int)a->M, p.g.N = (int)a->N, p.g.K = (int)a->K, p.g.parts = 1;
   p.out = (bf16*)a->dgu;
   p.saved = (unsigned char*)const_cast<void*>(a->saved);
   p.os = a->dgu_stride;
   hipStream_t s = (hipStream_t)stream;
-  if (gemm_plan(a->M, a->N, a->K, 1).large) gated_launch<GemmCfg<256, 2, 4, true, false>, true>(p, a->activation, s);
-  else gated_launch<GemmCfg<128, 2, 2, true, false>, true>(p, a->activation, s);
+  // (the saved values' loads and the two outputs' stores of one workgroup run under the products of the CU's other one:
+  // 12288 x 4608 over 1792 284 us, 331 with 256 x 256 tiles)
+  MLA_TRY(gemm_apply(op, p.g, GemmPlan{0, 1, 0, 0}, nullptr, 0));
+  gated_launch<GemmCfg<128, 2, 2, true, false>, true>(p, a->activation, s);
   return launch_status(op);
 }

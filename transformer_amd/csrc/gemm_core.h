@@ -48,6 +48,10 @@ struct GemmArgs {
   int M, N, K, parts;
   int n_mt, n_nt;  // tiles
   int gm;          // m tiles of a block of tiles (see gemm_tile_at)
+  // The first `full` tiles are whole; each of the others is cut along k into S pieces of `per` stages, whose fp32 sums go to
+  // `part` ([piece][tile][wave][block][quad][lane]) for gemm_finish.
+  int full, S, per;
+  float* part;
 };
 
 template <int N>
@@ -74,8 +78,19 @@ __device__ __forceinline__ void gemm_tile_at(const GemmArgs& a, int id, int& mt,
   nt = in / rows;
 }
 
-// Runs the tiles blockIdx.x, blockIdx.x + gridDim.x, ...: for each, epi(acc, m0, n0, stage0, stage1), where the two stages are
-// SLOT bytes each that the epilogue may use until its last barrier (every wave must have passed it before it returns).
+// An item of work: a tile, or a piece of one, as stages [beg, end) of all its parts' stages.
+struct GemmItem {
+  int tile, beg, end;
+};
+__device__ __forceinline__ GemmItem gemm_item(const GemmArgs& a, int id, int n_all) {
+  if (id < a.full) return GemmItem{id, 0, n_all};
+  const int rest = a.n_mt * a.n_nt - a.full, e = id - a.full, piece = e / rest;
+  return GemmItem{a.full + e - piece * rest, piece * a.per, min(n_all, (piece + 1) * a.per)};
+}
+
+// Runs the items blockIdx.x, blockIdx.x + gridDim.x, ...: for each whole tile epi(acc, m0, n0, stage0, stage1, 0, XJ), where
+// the two stages are SLOT bytes each that the epilogue may use until its last barrier (every wave must have passed it before
+// it returns), and the last two arguments the range of 32-row blocks j of each wave to be stored.
 template <class C, class Epi>
 __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds, Epi&& epi) {
   const int tid = threadIdx.x, lane = tid & 63;
@@ -83,8 +98,9 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   const int wn = w % C::WN, wm = w / C::WN;
   const int l32 = lane & 31, hk = lane >> 5;
   const int n_tiles = p.n_mt * p.n_nt;
-  const int n_st = (p.K + C::BK - 1) / C::BK;
-  const int tail = p.K - (n_st - 1) * C::BK;  // k of a part's last stage, a multiple of 8
+  const int n_st = (p.K + C::BK - 1) / C::BK, n_all = n_st * p.parts;
+  const int n_items = p.full + (n_tiles - p.full) * p.S;
+  const int last_k = p.K - (n_st - 1) * C::BK;  // k of a part's last stage, a multiple of 8
 
   // ---- loads: a cursor for x and one for W, each (tile, part, stage) with the descriptors of its tile and part, which end at
   // the last valid row; lanes past them load nothing, and the outputs that such rows reach are not stored
@@ -110,44 +126,53 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
     }
   }
   struct Cursor {
-    int tile, part, st;
+    int item, part, st, left;  // left: stages of the item from this one on
   };
-  Cursor cx{(int)blockIdx.x, 0, 0}, cw = cx;
+  auto enter = [&](Cursor& c) {
+    const GemmItem t = gemm_item(p, min(c.item, n_items - 1), n_all);
+    c.part = t.beg >= n_st;  // (at most two parts)
+    c.st = t.beg - c.part * n_st;
+    c.left = t.end - t.beg;
+  };
+  auto advance = [&](Cursor& c) -> bool {  // whether the descriptors change
+    if (--c.left == 0) {
+      c.item = c.item < n_items ? c.item + (int)gridDim.x : c.item;
+      enter(c);
+      return true;
+    }
+    if (++c.st < n_st) return false;
+    c.st = 0;
+    ++c.part;
+    return true;
+  };
   buf_rsrc rx, rw0, rw1;
-  auto point_x = [&]() {
+  auto point_x = [&](const Cursor& c) {
     int mt, nt;
-    gemm_tile_at(p, min(cx.tile, n_tiles - 1), mt, nt);
+    gemm_tile_at(p, gemm_item(p, min(c.item, n_items - 1), n_all).tile, mt, nt);
     const int m0 = mt * C::T;
-    rx = make_rsrc(p.x + (int64_t)m0 * p.xs + (int64_t)cx.part * p.K,
-                   cx.tile < n_tiles ? rows_bytes(min(C::T, p.M - m0), p.xs, p.K * 2) : 0u);
+    rx = make_rsrc(p.x + (int64_t)m0 * p.xs + (int64_t)c.part * p.K,
+                   c.item < n_items ? rows_bytes(min(C::T, p.M - m0), p.xs, p.K * 2) : 0u);
   };
-  auto point_w = [&]() {
+  auto point_w = [&](const Cursor& c) {
     int mt, nt;
-    gemm_tile_at(p, min(cw.tile, n_tiles - 1), mt, nt);
+    gemm_tile_at(p, gemm_item(p, min(c.item, n_items - 1), n_all).tile, mt, nt);
     const int n0 = nt * C::TN, nv = min(C::TN, p.N - n0);
-    const bool live = cw.tile < n_tiles;
-    const bf16* wp = !C::PAIR && cw.part ? p.w1 : p.w0;
+    const bool live = c.item < n_items;
+    const bf16* wp = !C::PAIR && c.part ? p.w1 : p.w0;
+    const int64_t ws = !C::PAIR && c.part ? p.ws1 : p.ws0;
     if (C::KMAJOR) {
-      rw0 = make_rsrc(wp + n0, live ? rows_bytes(p.K, p.ws0, nv * 2) : 0u);
+      rw0 = make_rsrc(wp + n0, live ? rows_bytes(p.K, ws, nv * 2) : 0u);
     } else {
-      rw0 = make_rsrc(wp + (int64_t)n0 * p.ws0, live ? rows_bytes(nv, p.ws0, p.K * 2) : 0u);
+      rw0 = make_rsrc(wp + (int64_t)n0 * ws, live ? rows_bytes(nv, ws, p.K * 2) : 0u);
       if (C::PAIR) rw1 = make_rsrc(p.w1 + (int64_t)n0 * p.ws1, live ? rows_bytes(nv, p.ws1, p.K * 2) : 0u);
     }
   };
-  auto advance = [&](Cursor& c) -> bool {  // whether the descriptors change
-    if (++c.st < n_st) return false;
-    c.st = 0;
-    if (++c.part == p.parts) {
-      c.part = 0;
-      c.tile = c.tile < n_tiles ? c.tile + (int)gridDim.x : c.tile;
-    }
-    return true;
-  };
+  Cursor cx{(int)blockIdx.x, 0, 0, 0}, cw;
   auto load_x = [&](int slot, int j) {
     dma16(rx, xoff[j] + (uint32_t)(cx.st * C::BK * 2), lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
   };
   auto done_x = [&]() {
-    if (advance(cx)) point_x();
+    if (advance(cx)) point_x(cx);
   };
   auto issue_x = [&](int slot) {
 #pragma unroll
@@ -160,7 +185,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
           lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
   };
   auto done_w = [&]() {
-    if (advance(cw)) point_w();
+    if (advance(cw)) point_w(cw);
   };
   auto issue_w = [&](int slot) {
 #pragma unroll
@@ -227,7 +252,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
     __builtin_amdgcn_sched_barrier(0);
   };
   // step h of a part's last stage: k past its end (whole chunks: the lane's 8 k are in or out together) becomes zero in both
-  auto cut = [&](int h) {
+  auto cut = [&](int h, int tail) {
     const bool in = 16 * h + 8 * hk < tail;
     const u32x4 z{0u, 0u, 0u, 0u};
 #pragma unroll
@@ -236,9 +261,11 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
     for (int i = 0; i < C::NB; ++i) fw[h & 1][i] = as_bf16x8(in ? as_u32x4(fw[h & 1][i]) : z);
   };
 
-  if ((int)blockIdx.x >= n_tiles) return;
-  point_x();
-  point_w();
+  if ((int)blockIdx.x >= n_items) return;
+  enter(cx);
+  cw = cx;
+  point_x(cx);
+  point_w(cw);
   issue_x(0);
   issue_w(1);
   issue_x(2);
@@ -257,13 +284,16 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
     for (int h = 0; h + 1 < C::HS; ++h) read_x(sx, h);
   };
   read_first();
-  for (int tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
+  for (int id = blockIdx.x; id < n_items; id += gridDim.x) {
+    const GemmItem item = gemm_item(p, id, n_all);
 #pragma unroll
     for (int i = 0; i < C::NB; ++i)
 #pragma unroll
       for (int j = 0; j < C::XJ; ++j) acc.a[i][j] = f32x16{};
-    for (int part = 0; part < p.parts; ++part) {
-      for (int st = 0; st + 1 < n_st; ++st) {
+    for (int g = item.beg; g < item.end;) {
+      const int part_end = g < n_st ? n_st : n_all, stop = min(item.end, part_end);
+      const int tail = stop == part_end ? last_k : C::BK;
+      for (; g + 1 < stop; ++g) {
         read_x(sx, C::HS - 1);
         read_w(sw, 1);
         multiply(0);
@@ -290,20 +320,37 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
 #pragma unroll
       for (int h = 0; h + 1 < C::HS; ++h) {
         read_w(sw, h + 1);
-        cut(h);
+        cut(h, tail);
         multiply(h);
       }
-      cut(C::HS - 1);
+      cut(C::HS - 1, tail);
       gemm_wait_vmem<C::LOADS>();
       __syncthreads();
       const int s0 = sx, s1 = sw;
       next_slots();
       __builtin_amdgcn_sched_barrier(0);
       multiply(C::HS - 1);
-      if (part + 1 == p.parts) {
-        int mt, nt;
-        gemm_tile_at(p, tile, mt, nt);
-        epi(acc, mt * C::T, nt * C::TN, lds + s0 * C::SLOT, lds + s1 * C::SLOT);
+      ++g;
+      if (g == item.end) {
+        if (id >= p.full && p.S > 1) {
+          int ln = lane;
+          asm volatile("" : "+v"(ln));  // (addresses formed here, not kept through the products)
+          f32x4* const dst = reinterpret_cast<f32x4*>(p.part) + (int64_t)(id - p.full) * (C::T * C::T / 4) +
+                             w * (C::NB * C::XJ * 256) + ln;
+#pragma unroll
+          for (int i = 0; i < C::NB; ++i)
+#pragma unroll
+            for (int j = 0; j < C::XJ; ++j)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const f32x16& a = acc.a[i][j];
+                dst[((i * C::XJ + j) * 4 + q) * 64] = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+              }
+        } else {
+          int mt, nt;
+          gemm_tile_at(p, item.tile, mt, nt);
+          epi(acc, mt * C::T, nt * C::TN, lds + s0 * C::SLOT, lds + s1 * C::SLOT, 0, C::XJ);
+        }
         gemm_wait_vmem<0>();  // (its stores share the counter that the stages' waits count down)
       }
       issue_w(s0);
@@ -312,6 +359,35 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
     }
   }
   gemm_wait_vmem<0>();  // no load is in flight into LDS when the workgroup ends
+}
+
+// The tiles that were cut: workgroup (tile, j) adds the pieces' sums of block row j in order and runs the epilogue on it.
+// Bound by reading the pieces, once.  lds: 2 SLOT bytes.
+template <class C, class Epi>
+__device__ __forceinline__ void gemm_finish(const GemmArgs& p, unsigned char* lds, Epi&& epi) {
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rest = p.n_mt * p.n_nt - p.full, t = blockIdx.x / C::XJ, jj = blockIdx.x % C::XJ;
+  const f32x4* src = reinterpret_cast<const f32x4*>(p.part) + (int64_t)t * (C::T * C::T / 4) + w * (C::NB * C::XJ * 256) + lane;
+  const int64_t step = (int64_t)rest * (C::T * C::T / 4);
+  GemmAcc<C> acc;
+#pragma unroll
+  for (int i = 0; i < C::NB; ++i)
+#pragma unroll
+    for (int j = 0; j < C::XJ; ++j) {
+      acc.a[i][j] = f32x16{};
+      if (j != jj) continue;
+      for (int s = 0; s < p.S; ++s) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 v = src[s * step + ((i * C::XJ + j) * 4 + q) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc.a[i][j][4 * q + e] += v[e];
+        }
+      }
+    }
+  int mt, nt;
+  gemm_tile_at(p, p.full + t, mt, nt);
+  epi(acc, mt * C::T, nt * C::TN, lds, lds + C::SLOT, jj, jj + 1);
 }
 
 }  // namespace mla

@@ -11,6 +11,23 @@
 
 namespace mla {
 
+// A thread's place in the workgroup, made anew for each epilogue: what derives from it would otherwise be formed before the
+// loop over tiles and kept in registers that the products need.
+template <class C>
+struct WavePos {
+  int tid, lane, wn, wm, l32, hk;
+  __device__ __forceinline__ WavePos() {
+    tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    wn = w % C::WN;
+    wm = w / C::WN;
+    l32 = lane & 31;
+    hk = lane >> 5;
+  }
+};
+
 template <class C, int COLS>
 struct StagedRows {
   static constexpr int RB = COLS * 2, CH = COLS / 8, PER = C::SLOT / RB;  // bytes and chunks of a row, rows of a slot
@@ -29,27 +46,14 @@ __device__ __forceinline__ int pass_row(int r, int j) {
 
 // The staged rows [0, R) to out (at the tile's first row and column): rows below mv, columns below nv (a multiple of 8)
 template <class C, int COLS, class RowOf>
-__device__ __forceinline__ void store_rows(const StagedRows<C, COLS>& st, int R, bf16* out, int64_t stride, int mv, int nv,
+__device__ __forceinline__ void store_rows(const StagedRows<C, COLS>& st, int tid, int R, bf16* out, int64_t stride, int mv, int nv,
                                            RowOf&& row_of) {
   constexpr int CH = COLS / 8;
 #pragma unroll 4
-  for (int c = threadIdx.x; c < R * CH; c += C::THREADS) {
+  for (int c = tid; c < R * CH; c += C::THREADS) {
     const int r = c / CH, ch = c % CH, m = row_of(r);
     if (m < mv && 8 * ch < nv) stg16(out + m * stride + 8 * ch, lds16(st.at(r, ch)));
   }
 }
-
-template <class C>
-struct WavePos {
-  int lane, wn, wm, l32, hk;
-  __device__ __forceinline__ WavePos() {
-    lane = threadIdx.x & 63;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    wn = w % C::WN;
-    wm = w / C::WN;
-    l32 = lane & 31;
-    hk = lane >> 5;
-  }
-};
 
 }  // namespace mla

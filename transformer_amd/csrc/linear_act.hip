@@ -18,90 +18,79 @@ struct LinearParams {
   int64_t rs, ys;
 };
 
+// The epilogue of the blocks [j0, j1) of each wave
+template <class C, int ACT>
+__device__ __forceinline__ void linear_epilogue(const LinearParams& p, GemmAcc<C>& acc, int m0, int n0,
+                                                unsigned char* s0, unsigned char* s1, int j0, int j1) {
+  const WavePos<C> at;
+  const StagedRows<C, C::T> st{s0, s1};
+  constexpr int R = 32 * C::WM, CH = C::T / 8;
+  const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
+  const int sr = 32 * at.wm + at.l32;
+#pragma unroll
+  for (int j = 0; j < C::XJ; ++j) {
+    if (j < j0 || j >= j1) continue;
+    if (p.residual) {
+      const bf16* res = p.residual + (int64_t)m0 * p.rs + n0;
+#pragma unroll 4
+      for (int c = at.tid; c < R * CH; c += C::THREADS) {
+        const int r = c / CH, ch = c % CH, m = pass_row<C>(r, j);
+        if (m < mv && 8 * ch < nv) sts16(st.at(r, ch), ldg16(res + m * p.rs + 8 * ch));
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i) {
+      f32x16 a = acc.a[i][j];
+      const int nb = (at.wn * C::NB + i) * 32;  // the block's first column within the tile
+      if (p.bias) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const u32x2 b = ldg8(p.bias + n0 + min(nb + 8 * q + 4 * at.hk, nv - 4));  // (columns past the last are not stored)
+          a[4 * q] += lo_bf16(b[0]);
+          a[4 * q + 1] += hi_bf16(b[0]);
+          a[4 * q + 2] += lo_bf16(b[1]);
+          a[4 * q + 3] += hi_bf16(b[1]);
+        }
+      }
+      const int mb = 32 * (C::XJ * at.wm + j);
+      if (p.saved && mb < mv && nb < nv)
+        saved_store(p.saved + ((int64_t)((m0 + mb) >> 5) * ((p.g.N + 31) >> 5) + ((n0 + nb) >> 5)) * kSavedBlock, at.lane, a);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        unsigned char* to = st.at(sr, nb / 8 + q) + 8 * at.hk;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(a[4 * q + e]);
+        if (p.residual) {
+          const u32x2 b = lds8(to);
+          v[0] += lo_bf16(b[0]);
+          v[1] += hi_bf16(b[0]);
+          v[2] += lo_bf16(b[1]);
+          v[3] += hi_bf16(b[1]);
+        }
+        sts8(to, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+      }
+    }
+    __syncthreads();
+    store_rows<C>(st, at.tid, R, p.y + (int64_t)m0 * p.ys + n0, p.ys, mv, nv, [&](int r) { return pass_row<C>(r, j); });
+    __syncthreads();
+  }
+}
+
 template <class C, int ACT>
 __global__ __launch_bounds__(C::THREADS, 2) void linear_act_kernel(LinearParams p) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
-  const WavePos<C> at;
-  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1) {
-    const StagedRows<C, C::T> st{s0, s1};
-    constexpr int R = 32 * C::WM, CH = C::T / 8;
-    const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
-    const int sr = 32 * at.wm + at.l32;
-#pragma unroll
-    for (int j = 0; j < C::XJ; ++j) {
-      if (p.residual) {
-        const bf16* res = p.residual + (int64_t)m0 * p.rs + n0;
-#pragma unroll 4
-        for (int c = threadIdx.x; c < R * CH; c += C::THREADS) {
-          const int r = c / CH, ch = c % CH, m = pass_row<C>(r, j);
-          if (m < mv && 8 * ch < nv) sts16(st.at(r, ch), ldg16(res + m * p.rs + 8 * ch));
-        }
-        __syncthreads();
-      }
-#pragma unroll
-      for (int i = 0; i < C::NB; ++i) {
-        f32x16& a = acc.a[i][j];
-        const int nb = (at.wn * C::NB + i) * 32;  // the block's first column within the tile
-        if (p.bias) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int n = nb + 8 * q + 4 * at.hk;
-            if (n < nv) {
-              const u32x2 b = ldg8(p.bias + n0 + n);
-              a[4 * q] += lo_bf16(b[0]);
-              a[4 * q + 1] += hi_bf16(b[0]);
-              a[4 * q + 2] += lo_bf16(b[1]);
-              a[4 * q + 3] += hi_bf16(b[1]);
-            }
-          }
-        }
-        const int mb = 32 * (C::XJ * at.wm + j);
-        if (p.saved && mb < mv && nb < nv)
-          saved_store(p.saved + ((int64_t)((m0 + mb) >> 5) * ((p.g.N + 31) >> 5) + ((n0 + nb) >> 5)) * kSavedBlock, at.lane, a);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          unsigned char* to = st.at(sr, nb / 8 + q) + 8 * at.hk;
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(a[4 * q + e]);
-          if (p.residual) {
-            const u32x2 b = lds8(to);
-            v[0] += lo_bf16(b[0]);
-            v[1] += hi_bf16(b[0]);
-            v[2] += lo_bf16(b[1]);
-            v[3] += hi_bf16(b[1]);
-          }
-          sts8(to, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
-        }
-      }
-      __syncthreads();
-      store_rows<C>(st, R, p.y + (int64_t)m0 * p.ys + n0, p.ys, mv, nv, [&](int r) { return pass_row<C>(r, j); });
-      __syncthreads();
-    }
+  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1, int j0, int j1) {
+    linear_epilogue<C, ACT>(p, acc, m0, n0, s0, s1, j0, j1);
   });
 }
 
-template <class C>
-__global__ __launch_bounds__(C::THREADS, 2) void linear_dx_kernel(LinearParams p) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
-  const WavePos<C> at;
-  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1) {
-    const StagedRows<C, C::T> st{s0, s1};
-    const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
-#pragma unroll
-    for (int j = 0; j < C::XJ; ++j) {
-#pragma unroll
-      for (int i = 0; i < C::NB; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x16& a = acc.a[i][j];
-          sts8(st.at(32 * at.wm + at.l32, (at.wn * C::NB + i) * 4 + q) + 8 * at.hk,
-               u32x2{pack_bf16x2(a[4 * q], a[4 * q + 1]), pack_bf16x2(a[4 * q + 2], a[4 * q + 3])});
-        }
-      __syncthreads();
-      store_rows<C>(st, 32 * C::WM, p.y + (int64_t)m0 * p.ys + n0, p.ys, mv, nv, [&](int r) { return pass_row<C>(r, j); });
-      __syncthreads();
-    }
+template <class C, int ACT>
+__global__ __launch_bounds__(C::THREADS, 1) void linear_act_finish_kernel(LinearParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * C::SLOT];
+  gemm_finish<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1, int j0, int j1) {
+    linear_epilogue<C, ACT>(p, acc, m0, n0, s0, s1, j0, j1);
   });
 }
 
@@ -138,21 +127,27 @@ static void linear_act_rows_go(const LinearParams& p, hipStream_t s) {
 template <class C, int ACT>
 static void linear_act_go(const LinearParams& p, hipStream_t s) {
   linear_act_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+  if (p.g.S > 1) linear_act_finish_kernel<C, ACT><<<dim3(gemm_finish_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
 }
 
+// dx is a product without an epilogue of its own
 template <class C>
-static void linear_act_launch(LinearParams& p, int act, hipStream_t s) {
-  gemm_tile_counts<C>(p.g);
-  if (act == MLA_ACT_RELU) linear_act_go<C, MLA_ACT_RELU>(p, s);
-  else if (act == MLA_ACT_SILU) linear_act_go<C, MLA_ACT_SILU>(p, s);
-  else if (act == MLA_ACT_GELU_TANH) linear_act_go<C, MLA_ACT_GELU_TANH>(p, s);
-  else linear_act_go<C, MLA_ACT_NONE>(p, s);
+static void linear_act_launch(const LinearParams& p, int act, hipStream_t s) {
+  if constexpr (!C::KMAJOR) {
+    if (act == MLA_ACT_RELU) return linear_act_go<C, MLA_ACT_RELU>(p, s);
+    if (act == MLA_ACT_SILU) return linear_act_go<C, MLA_ACT_SILU>(p, s);
+    if (act == MLA_ACT_GELU_TANH) return linear_act_go<C, MLA_ACT_GELU_TANH>(p, s);
+  }
+  linear_act_go<C, MLA_ACT_NONE>(p, s);
 }
 
-template <class C>
-static void linear_dx_launch(LinearParams& p, hipStream_t s) {
-  gemm_tile_counts<C>(p.g);
-  linear_dx_kernel<C><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+template <bool KMAJOR>
+static int linear_tiles(const char* op, LinearParams& p, int act, void* workspace, size_t bytes, hipStream_t s) {
+  const GemmPlan pl = gemm_plan(p.g.M, p.g.N, p.g.K, p.g.parts, true);
+  MLA_TRY(gemm_apply(op, p.g, pl, workspace, bytes));
+  if (pl.large) linear_act_launch<GemmCfg<256, 2, 4, KMAJOR, false>>(p, act, s);
+  else linear_act_launch<GemmCfg<128, 2, 2, KMAJOR, false>>(p, act, s);
+  return launch_status(op);
 }
 
 static int linear_act_check(const mla_linear_act_args* a) {
@@ -183,7 +178,7 @@ static int linear_dx_check(const mla_linear_dx_args* a) {
   MLA_TRY(check_weight_reach(op, "w0", a->N, a->w0_stride));
   if (a->w1) {
     MLA_TRY(check_rows(op, "w1", a->w1, a->K, a->w1_stride));
-    MLA_TRY(check_weight_reach(op, "w1", a->N, a->w1_stride));
+    MLA_CHECK(a->w1_stride == a->w0_stride, MLA_ERR_UNSUPPORTED, "%s: the weights' row strides must be the same", op);
   }
   return MLA_OK;
 }
@@ -198,15 +193,19 @@ extern "C" size_t mla_linear_saved_size(int64_t M, int64_t N) {
 }
 
 extern "C" size_t mla_linear_act_workspace_bytes(const mla_linear_act_args* a) {
-  (void)a;
-  return 0;
+  // 0 for the sizes mla_linear_act rejects
+  if (!a || check_linear_sizes("mla_linear_act", a->M, a->N, a->K) != MLA_OK || a->M <= kRcMaxRows) return 0;
+  return (size_t)gemm_plan(a->M, a->N, a->K, 1, true).part_bytes;
 }
 
 extern "C" int mla_linear_act(const mla_linear_act_args* a, void* stream) {
+  const char* op = "mla_linear_act";
   MLA_TRY(linear_act_check(a));
   if (a->M == 0 || a->N == 0) return MLA_OK;
   LinearParams p{};
-  p.g = GemmArgs{(const bf16*)a->x, (const bf16*)a->w, nullptr, a->x_stride, a->w_stride, 0, (int)a->M, (int)a->N, (int)a->K, 1};
+  p.g.x = (const bf16*)a->x, p.g.w0 = (const bf16*)a->w;
+  p.g.xs = a->x_stride, p.g.ws0 = a->w_stride;
+  p.g.M = (int)a->M, p.g.N = (int)a->N, p.g.K = (int)a->K, p.g.parts = 1;
   p.bias = (const bf16*)a->bias;
   p.residual = (const bf16*)a->residual;
   p.y = (bf16*)a->y;
@@ -214,32 +213,28 @@ extern "C" int mla_linear_act(const mla_linear_act_args* a, void* stream) {
   p.rs = a->residual_stride;
   p.ys = a->y_stride;
   hipStream_t s = (hipStream_t)stream;
-  if (a->M <= kRcMaxRows) {
-    if (a->activation == MLA_ACT_RELU) linear_act_rows_go<MLA_ACT_RELU>(p, s);
-    else if (a->activation == MLA_ACT_SILU) linear_act_rows_go<MLA_ACT_SILU>(p, s);
-    else if (a->activation == MLA_ACT_GELU_TANH) linear_act_rows_go<MLA_ACT_GELU_TANH>(p, s);
-    else linear_act_rows_go<MLA_ACT_NONE>(p, s);
-  } else if (gemm_plan(a->M, a->N, a->K, 1).large) linear_act_launch<GemmCfg<256, 2, 4, false, false>>(p, a->activation, s);
-  else linear_act_launch<GemmCfg<128, 2, 2, false, false>>(p, a->activation, s);
-  return launch_status("mla_linear_act");
+  if (a->M > kRcMaxRows) return linear_tiles<false>(op, p, a->activation, a->workspace, a->workspace_bytes, s);
+  if (a->activation == MLA_ACT_RELU) linear_act_rows_go<MLA_ACT_RELU>(p, s);
+  else if (a->activation == MLA_ACT_SILU) linear_act_rows_go<MLA_ACT_SILU>(p, s);
+  else if (a->activation == MLA_ACT_GELU_TANH) linear_act_rows_go<MLA_ACT_GELU_TANH>(p, s);
+  else linear_act_rows_go<MLA_ACT_NONE>(p, s);
+  return launch_status(op);
 }
 
 extern "C" size_t mla_linear_dx_workspace_bytes(const mla_linear_dx_args* a) {
-  (void)a;
-  return 0;
+  // 0 for the sizes mla_linear_dx rejects
+  if (!a || check_linear_sizes("mla_linear_dx", a->M, a->N, a->K) != MLA_OK) return 0;
+  return (size_t)gemm_plan(a->M, a->K, a->N, a->w1 ? 2 : 1, true).part_bytes;
 }
 
 extern "C" int mla_linear_dx(const mla_linear_dx_args* a, void* stream) {
   MLA_TRY(linear_dx_check(a));
-  if (a->M == 0 || a->K == 0) return MLA_OK;
-  const int parts = a->w1 ? 2 : 1;
+  if (a->M == 0) return MLA_OK;
   LinearParams p{};
-  p.g = GemmArgs{(const bf16*)a->dy, (const bf16*)a->w0, (const bf16*)a->w1, a->dy_stride, a->w0_stride, a->w1_stride, (int)a->M,
-                 (int)a->K, (int)a->N, parts};
+  p.g.x = (const bf16*)a->dy, p.g.w0 = (const bf16*)a->w0, p.g.w1 = (const bf16*)a->w1;
+  p.g.xs = a->dy_stride, p.g.ws0 = a->w0_stride, p.g.ws1 = a->w1_stride;
+  p.g.M = (int)a->M, p.g.N = (int)a->K, p.g.K = (int)a->N, p.g.parts = a->w1 ? 2 : 1;
   p.y = (bf16*)a->dx;
   p.ys = a->dx_stride;
-  hipStream_t s = (hipStream_t)stream;
-  if (gemm_plan(a->M, a->K, a->N, parts).large) linear_dx_launch<GemmCfg<256, 2, 4, true, false>>(p, s);
-  else linear_dx_launch<GemmCfg<128, 2, 2, true, false>>(p, s);
-  return launch_status("mla_linear_dx");
+  return linear_tiles<true>("mla_linear_dx", p, MLA_ACT_NONE, a->workspace, a->workspace_bytes, (hipStream_t)stream);
 }

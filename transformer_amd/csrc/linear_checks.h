@@ -36,18 +36,34 @@ inline int check_weight_reach(const char* op, const char* name, int64_t rows, in
   return MLA_OK;
 }
 
-template <class C>
-inline void gemm_tile_counts(GemmArgs& g) {
-  g.n_mt = (g.M + C::T - 1) / C::T;
-  g.n_nt = (g.N + C::TN - 1) / C::TN;
+// The plan's tiles and pieces; `cols` tile columns of an output column (2 for a pair of weights).  Without a workspace that
+// is large enough a plan that cuts tiles is refused.
+inline int gemm_apply(const char* op, GemmArgs& g, const GemmPlan& pl, void* workspace, size_t bytes, int cols = 1) {
+  const int T = pl.large ? 256 : 128;
+  g.n_mt = (g.M + T - 1) / T;
+  g.n_nt = (int)(((int64_t)g.N * cols + T - 1) / T);
   g.gm = 8;
+  const int tiles = g.n_mt * g.n_nt, slots = pl.large ? 256 : 512;
+  g.S = pl.S;
+  g.per = pl.per;
+  g.full = pl.S > 1 ? tiles / slots * slots : tiles;
+  g.part = (float*)workspace;
+  MLA_CHECK(pl.part_bytes == 0 || (workspace && bytes >= (size_t)pl.part_bytes && ((uintptr_t)workspace & 255) == 0),
+            MLA_ERR_WORKSPACE, "%s: workspace of %lld bytes (256-byte aligned) needed, %zu given", op, (long long)pl.part_bytes,
+            bytes);
+  return MLA_OK;
 }
 
 // one workgroup of 256 x 256 tiles per CU, two of 128 x 128
 template <class C>
 inline unsigned gemm_grid(const GemmArgs& g) {
-  const int64_t tiles = (int64_t)g.n_mt * g.n_nt, most = C::LDS > 80 * 1024 ? 256 : 512;
-  return (unsigned)(tiles < most ? tiles : most);
+  const int64_t tiles = (int64_t)g.n_mt * g.n_nt, items = g.full + (tiles - g.full) * g.S;
+  const int64_t most = C::T == 256 ? 256 : 512;
+  return (unsigned)(items < most ? items : most);
+}
+template <class C>
+inline unsigned gemm_finish_grid(const GemmArgs& g) {
+  return (unsigned)((g.n_mt * g.n_nt - g.full) * C::XJ);
 }
 
 }  // namespace mla

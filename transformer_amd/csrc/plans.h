@@ -125,16 +125,42 @@ inline WgPlan wg_plan(int64_t M, int64_t N, int64_t K) {
 // ---- linear_act.hip's and gated_linear.hip's tiles (gemm_core.h)
 struct GemmPlan {
   int large;  // tiles of 256 x 256, one workgroup per CU; else 128 x 128, two
+  int S, per;  // the tiles of an unfilled last round are cut along k into S pieces of `per` stages (1: not cut)
+  int64_t part_bytes;
 };
 
-// y [M, N] over parts x K
-inline GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int64_t parts) {
-  const double stages = (double)((K + 63) / 64 * parts);
-  const int64_t t256 = ((M + 255) / 256) * ((N + 255) / 256), t128 = ((M + 127) / 128) * ((N + 127) / 128);
-  const double large = (double)((t256 + 255) / 256) * (1.2 * stages + 10.0);
-  // up to one workgroup a CU runs faster than two that share it
-  const double small = t128 <= 256 ? 0.55 * stages + 4.0 : (double)((t128 + 511) / 512) * (0.85 * stages + 5.0);
-  return GemmPlan{large < small};
+// The plan of least estimated time (us) for y [M, N] over parts x K, `cut` where tiles may be cut along k.  A whole round takes
+// its stages at the measured 1.3 us (large tiles: 144 stages took 194 us) or 0.85 us (small ones, two on a CU; 0.6 alone on it)
+// plus what a tile's start and stores take; pieces add the fp32 sums they leave, written and read at 2.5 TB/s together, and a
+// second kernel.
+inline GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int64_t parts, bool cut) {
+  GemmPlan best{};
+  double best_t = 1e300;
+  const int64_t n = (K + 63) / 64 * parts;
+  for (int large = 1; large >= 0; --large) {
+    const int64_t T = large ? 256 : 128, slots = large ? 256 : 512;
+    const int64_t tiles = ((M + T - 1) / T) * ((N + T - 1) / T), rest = tiles % slots;
+    const double ts = large ? 1.3 : 0.85, fixed = large ? 12.0 : 6.0, alone = large ? 1.2 : 0.6;
+    const double rounds = (double)(tiles / slots) * ((double)n * ts + fixed);
+    for (int64_t S = 1; S <= 16 && S * 2 <= n; ++S) {
+      if (S > 1 && (!cut || rest == 0 || rest * S > slots)) break;
+      const int64_t per = (n + S - 1) / S;
+      if ((n + per - 1) / per != S) continue;  // fewer pieces hold the same stages
+      double t = rounds;
+      if (rest) t += (double)per * (rest * S <= 256 ? alone : ts) + fixed;
+      const int64_t pb = S > 1 ? rest * S * T * T * 4 : 0;
+      if (S > 1) t += 5.0 + (double)pb / 2.5e6;
+      if (t < best_t) {
+        best_t = t;
+        best = GemmPlan{large, (int)S, (int)per, pb};
+      }
+    }
+    if (n < 2) {  // (one stage: nothing to cut)
+      const double t = (double)((tiles + slots - 1) / slots) * ((double)n * ts + fixed);
+      if (t < best_t) best_t = t, best = GemmPlan{large, 1, (int)n, 0};
+    }
+  }
+  return best;
 }
 
 }  // namespace mla

@@ -17,6 +17,7 @@ from ._lib import ACTIVATIONS
 from .kernels import _alloc_workspace, _dt_code, _op, _register_autograd, weight_grad, weight_grad_or_none
 
 LINEAR_MAX_STRIDE = 1 << 22
+ROWS_MAX = 64  # rows up to which mla_linear_act needs no workspace
 _BF16, _F32 = torch.bfloat16, torch.float32
 
 
@@ -112,6 +113,7 @@ def _linear_run(op, x2, w, bias, res2, code, saved, y, M):
         x2.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(), None if res2 is None else res2.data_ptr(),
         y.data_ptr(), None if saved is None else saved.data_ptr(), None, 0, M, N, K, _row_stride(x2), _row_stride(w),
         0 if res2 is None else _row_stride(res2), N, code)
+    ws = _fit_workspace("mla_linear_act_workspace_bytes", args, y) if M > ROWS_MAX else None  # noqa: F841  (kept until the launch)
     _launch("mla_linear_act", args, y, op)
 
 
@@ -180,11 +182,14 @@ def _weight_grad(dy: Tensor, x: Tensor, dtype: torch.dtype) -> Tensor:
 def _linear_dx(op: str, dy: Tensor, weights, shape) -> Tensor:
     """``sum_p dy_p W_p`` for bf16 rows ``dy [M, P N]`` and P = 1 or 2 weights ``[N, K]``, as ``shape``."""
     w0, w1 = _weight_bf16(weights[0]), _weight_bf16(weights[1]) if len(weights) > 1 else None
+    if w1 is not None and _row_stride(w1) != _row_stride(w0):
+        w0, w1 = w0.contiguous(), w1.contiguous()
     (N, K), M = w0.shape, dy.size(0)
     dx = torch.empty(shape, dtype=_BF16, device=dy.device)
     if M:
         args = _lib.LinearDxArgs(dy.data_ptr(), w0.data_ptr(), None if w1 is None else w1.data_ptr(), dx.data_ptr(), None, 0,
                                  M, N, K, _row_stride(dy), _row_stride(w0), 0 if w1 is None else _row_stride(w1), K)
+        ws = _fit_workspace("mla_linear_dx_workspace_bytes", args, dx)  # noqa: F841  (kept until the launch)
         _launch("mla_linear_dx", args, dx, op)
     return dx
 
@@ -316,8 +321,8 @@ def _gated_ffn(x, w_gate, w_up, w_down, residual, activation, save):
     if M:
         wg, wu = _weight_bf16(w_gate), _weight_bf16(w_up)
         args = _lib.GatedLinearArgs(
-            x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), None if saved is None else saved.data_ptr(), None, 0, M, H,
-            D, _row_stride(x2), _row_stride(wg), _row_stride(wu), H, code)
+            x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), None if saved is None else saved.data_ptr(), M, H, D,
+            _row_stride(x2), _row_stride(wg), _row_stride(wu), H, code)
         _launch("mla_gated_linear", args, h, op)
         _linear_run(op, h, _weight_bf16(w_down), None, None if residual is None else _matrix(residual, D, True), 0, None, y, M)
     return y, h, saved
