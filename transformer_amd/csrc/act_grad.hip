@@ -24,45 +24,69 @@ struct ActGradParams {
 
 constexpr int kAgCols = 128;  // columns of a workgroup, 32 a wave
 
+// dy arrives and dz leaves in rows of 256 bytes through an LDS tile of 32 rows (a lane's quads straight from memory would be
+// 16 bytes of each of 32 rows an instruction: 2.5 TB/s); chunk c of 16 bytes of row r lies at c ^ (r mod 16), which spreads a
+// quad's 32 rows over the banks.  The next tile's loads are in flight under this one's arithmetic.
 template <int ACT>
 __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p) {
-  const int lane = threadIdx.x & 63, l32 = lane & 31, hk = lane >> 5;
-  const int n0 = blockIdx.x * kAgCols + 32 * (int)(threadIdx.x >> 6);
-  if (n0 >= p.N) return;  // (no barrier follows)
+  __shared__ __attribute__((aligned(16))) unsigned char tile[32 * 256];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hk = lane >> 5, w = tid >> 6;
+  const int n0 = blockIdx.x * kAgCols, wn = n0 + 32 * w;
   const int64_t hb = (p.N + 31) >> 5;
   const int b0 = blockIdx.y * p.seg, b1 = min(b0 + p.seg, (p.M + 31) >> 5);
+  // this thread's two chunks of a tile: rows tid / 16 and 16 more, chunk tid % 16 (N is whole chunks)
+  const int cr = tid >> 4, cc = tid & 15;
+  const bool col = n0 + 8 * cc < p.N;
+  unsigned char* const mine[2] = {tile + cr * 256 + ((cc ^ cr) * 16), tile + (cr + 16) * 256 + ((cc ^ cr) * 16)};
+  const bool live = wn < p.N;  // (wave-uniform) the wave's columns exist
+  u32x4 d[2];
+  SavedRegs z{};
+  auto load = [&](int b) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int m = 32 * b + cr + 16 * e;
+      d[e] = col && m < p.M ? ldg16(p.dy + (int64_t)m * p.dys + n0 + 8 * cc) : u32x4{0u, 0u, 0u, 0u};
+    }
+    if (ACT != MLA_ACT_NONE && live) z = saved_load(p.saved + (b * hb + (wn >> 5)) * kSavedBlock, lane);
+  };
   float sum[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+  load(b0);
   for (int b = b0; b < b1; ++b) {
-    const int m = 32 * b + l32;
-    const bool row = m < p.M;
-    u32x2 d[4];
+    sts16(mine[0], d[0]);
+    sts16(mine[1], d[1]);
+    const SavedRegs zb = z;
+    __syncthreads();
+    if (b + 1 < b1) load(b + 1);
+    const bool row = 32 * b + l32 < p.M;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int n = n0 + 8 * q + 4 * hk;
-      d[q] = row && n < p.N ? ldg8(p.dy + (int64_t)m * p.dys + n) : u32x2{0u, 0u};
-    }
-    SavedRegs z{};
-    if (ACT != MLA_ACT_NONE) z = saved_load(p.saved + (b * hb + (n0 >> 5)) * kSavedBlock, lane);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float v[4] = {lo_bf16(d[q][0]), hi_bf16(d[q][0]), lo_bf16(d[q][1]), hi_bf16(d[q][1])};
+      unsigned char* at = tile + l32 * 256 + (((4 * w + q) ^ (l32 & 15)) * 16) + 8 * hk;
+      const u32x2 x = lds8(at);
+      float v[4] = {lo_bf16(x[0]), hi_bf16(x[0]), lo_bf16(x[1]), hi_bf16(x[1])};
       if (ACT != MLA_ACT_NONE) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float value, slope;
-          act_both<ACT>(saved_value(z, 4 * q + e), value, slope);
+          act_both<ACT>(saved_value(zb, 4 * q + e), value, slope);
           v[e] *= slope;
         }
-        const int n = n0 + 8 * q + 4 * hk;
-        if (row && n < p.N) stg8(p.dz + (int64_t)m * p.dzs + n, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+        sts8(at, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[4 * q + e] += row ? v[e] : 0.f;  // (what z holds past the last row may be NaN)
     }
+    __syncthreads();
+    if (ACT != MLA_ACT_NONE) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int m = 32 * b + cr + 16 * e;
+        if (col && m < p.M) stg16(p.dz + (int64_t)m * p.dzs + n0 + 8 * cc, lds16(mine[e]));
+      }
+    }
   }
-  if (!p.part) return;
+  if (!p.part || !live) return;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
 #pragma unroll
@@ -71,7 +95,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p) {
   if (l32 == 0) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int n = n0 + 8 * q + 4 * hk;
+      const int n = wn + 8 * q + 4 * hk;
       if (n < p.N) stg16(p.part + (int64_t)blockIdx.y * p.N + n,
                          __builtin_bit_cast(u32x4, f32x4{sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]}));
     }

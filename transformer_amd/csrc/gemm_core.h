@@ -26,6 +26,10 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 // of each, a wave's first NB / 2 blocks from w0, the rest from w1 at the same columns
 template <int T_, int WN_, int WM_, bool KMAJOR_, bool PAIR_>
 struct GemmCfg {
+  // The first LW waves issue the loads, the others store the outputs: loads and stores of one wave complete in order, so a
+  // wave that did both would wait for the stores of a tile before the second stage of the next.
+  static constexpr int LW = T_ == 256 ? WN_ * WM_ / 2 : WN_ * WM_;
+  static constexpr int SW0 = LW < WN_ * WM_ ? LW : 0, SW = WN_ * WM_ - SW0;  // the storing waves' first and number
   static constexpr int T = T_, WN = WN_, WM = WM_, BK = 64, HS = BK / 16;
   static constexpr bool KMAJOR = KMAJOR_, PAIR = PAIR_;
   static constexpr int WAVES = WN * WM, THREADS = 64 * WAVES;
@@ -33,9 +37,9 @@ struct GemmCfg {
   static constexpr int TN = PAIR ? T / 2 : T;               // columns of the weights that a tile covers
   static constexpr int SLOT = T * BK * 2;                   // T rows of 64 k, or 64 k rows of T
   static constexpr int RING = 5;
-  static constexpr int LOADS = SLOT / 1024 / WAVES;         // of a wave per slot
+  static constexpr int LOADS = SLOT / 1024 / LW;            // of a loading wave per slot
   static constexpr int LDS = RING * SLOT;
-  static_assert(SLOT % (1024 * WAVES) == 0 && LDS <= 160 * 1024, "the ring fits the LDS");
+  static_assert(SLOT % (1024 * LW) == 0 && LDS <= 160 * 1024, "the ring fits the LDS");
 };
 
 // y (a tile's outputs, as an epilogue defines them) over rows m of x, columns n of W; k runs over `parts` segments of K each:
@@ -60,6 +64,19 @@ __device__ __forceinline__ void gemm_wait_vmem() {
 }
 
 __device__ __forceinline__ int gemm_swz(int row) { return (row >> 1) & 7; }
+
+// What a descriptor is made of, the same in every lane; made where it is used, from scalar registers (the compiler does not see
+// that of values which a loop carries past a branch).
+struct GemmSpan {
+  uint64_t base;
+  uint32_t bytes;
+  __device__ __forceinline__ buf_rsrc rsrc() const {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)base);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(base >> 32));
+    return make_rsrc((const void*)(((uint64_t)hi << 32) | lo), (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
+  }
+};
+__device__ __forceinline__ GemmSpan gemm_span(const void* p, uint32_t bytes) { return GemmSpan{(uint64_t)(uintptr_t)p, bytes}; }
 
 template <class C>
 struct GemmAcc {
@@ -105,11 +122,13 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   // ---- loads: a cursor for x and one for W, each (tile, part, stage) with the descriptors of its tile and part, which end at
   // the last valid row; lanes past them load nothing, and the outputs that such rows reach are not stored
   const uint32_t lds0 = lds_addr(lds);
+  const bool loads = w < C::LW;
+  const int lw = loads ? w : w - C::LW;
   uint32_t xoff[C::LOADS], woff[C::LOADS];  // this lane's bytes in each of the wave's loads, at k = 0
   bool second[C::LOADS];                    // PAIR (wave-uniform): the load is of w1's rows
 #pragma unroll
   for (int j = 0; j < C::LOADS; ++j) {
-    const int i = w + C::WAVES * j, row = 8 * i + (lane >> 3);
+    const int i = lw + C::LW * j, row = 8 * i + (lane >> 3);
     xoff[j] = (uint32_t)(row * p.xs * 2) + (uint32_t)(((lane & 7) ^ gemm_swz(row)) * 16);
     second[j] = false;
     if (C::KMAJOR) {
@@ -145,12 +164,12 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
     ++c.part;
     return true;
   };
-  buf_rsrc rx, rw0, rw1;
+  GemmSpan rx, rw0, rw1;
   auto point_x = [&](const Cursor& c) {
     int mt, nt;
     gemm_tile_at(p, gemm_item(p, min(c.item, n_items - 1), n_all).tile, mt, nt);
     const int m0 = mt * C::T;
-    rx = make_rsrc(p.x + (int64_t)m0 * p.xs + (int64_t)c.part * p.K,
+    rx = gemm_span(p.x + (int64_t)m0 * p.xs + (int64_t)c.part * p.K,
                    c.item < n_items ? rows_bytes(min(C::T, p.M - m0), p.xs, p.K * 2) : 0u);
   };
   auto point_w = [&](const Cursor& c) {
@@ -161,35 +180,37 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
     const bf16* wp = !C::PAIR && c.part ? p.w1 : p.w0;
     const int64_t ws = !C::PAIR && c.part ? p.ws1 : p.ws0;
     if (C::KMAJOR) {
-      rw0 = make_rsrc(wp + n0, live ? rows_bytes(p.K, ws, nv * 2) : 0u);
+      rw0 = gemm_span(wp + n0, live ? rows_bytes(p.K, ws, nv * 2) : 0u);
     } else {
-      rw0 = make_rsrc(wp + (int64_t)n0 * ws, live ? rows_bytes(nv, ws, p.K * 2) : 0u);
-      if (C::PAIR) rw1 = make_rsrc(p.w1 + (int64_t)n0 * p.ws1, live ? rows_bytes(nv, p.ws1, p.K * 2) : 0u);
+      rw0 = gemm_span(wp + (int64_t)n0 * ws, live ? rows_bytes(nv, ws, p.K * 2) : 0u);
+      if (C::PAIR) rw1 = gemm_span(p.w1 + (int64_t)n0 * p.ws1, live ? rows_bytes(nv, p.ws1, p.K * 2) : 0u);
     }
   };
   Cursor cx{(int)blockIdx.x, 0, 0, 0}, cw;
-  auto load_x = [&](int slot, int j) {
-    dma16(rx, xoff[j] + (uint32_t)(cx.st * C::BK * 2), lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
-  };
   auto done_x = [&]() {
     if (advance(cx)) point_x(cx);
   };
   auto issue_x = [&](int slot) {
+    if (loads) {
+      const buf_rsrc r = rx.rsrc();
 #pragma unroll
-    for (int j = 0; j < C::LOADS; ++j) load_x(slot, j);
+      for (int j = 0; j < C::LOADS; ++j)
+        dma16(r, xoff[j] + (uint32_t)(cx.st * C::BK * 2), lds0 + (uint32_t)(slot * C::SLOT + (lw + C::LW * j) * 1024));
+    }
     done_x();
   };
   const uint32_t wstep = C::KMAJOR ? (uint32_t)(C::BK * p.ws0 * 2) : (uint32_t)(C::BK * 2);
-  auto load_w = [&](int slot, int j) {
-    dma16(C::PAIR && second[j] ? rw1 : rw0, woff[j] + (uint32_t)cw.st * wstep,
-          lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
-  };
   auto done_w = [&]() {
     if (advance(cw)) point_w(cw);
   };
   auto issue_w = [&](int slot) {
+    if (loads) {
+      const buf_rsrc r0 = rw0.rsrc(), r1 = C::PAIR ? rw1.rsrc() : r0;
 #pragma unroll
-    for (int j = 0; j < C::LOADS; ++j) load_w(slot, j);
+      for (int j = 0; j < C::LOADS; ++j)
+        dma16(C::PAIR && second[j] ? r1 : r0, woff[j] + (uint32_t)cw.st * wstep,
+              lds0 + (uint32_t)(slot * C::SLOT + (lw + C::LW * j) * 1024));
+    }
     done_w();
   };
 
@@ -271,7 +292,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   issue_x(2);
   issue_w(3);
   issue_x(4);
-  gemm_wait_vmem<3 * C::LOADS>();
+  if (loads) gemm_wait_vmem<3 * C::LOADS>();
   __syncthreads();
   int sx = 0, sw = 1;  // the slots of the stage being multiplied
   auto next_slots = [&]() {
@@ -307,7 +328,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
           interleave();
         }
         // every wave holds the stage in registers and the next one has landed: all but the one behind it
-        gemm_wait_vmem<2 * C::LOADS>();
+        if (loads) gemm_wait_vmem<2 * C::LOADS>();
         __syncthreads();
         issue_x(sw);
         next_slots();
@@ -324,7 +345,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
         multiply(h);
       }
       cut(C::HS - 1, tail);
-      gemm_wait_vmem<C::LOADS>();
+      if (loads) gemm_wait_vmem<C::LOADS>();
       __syncthreads();
       const int s0 = sx, s1 = sw;
       next_slots();
@@ -351,7 +372,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
           gemm_tile_at(p, item.tile, mt, nt);
           epi(acc, mt * C::T, nt * C::TN, lds + s0 * C::SLOT, lds + s1 * C::SLOT, 0, C::XJ);
         }
-        gemm_wait_vmem<0>();  // (its stores share the counter that the stages' waits count down)
+        if (loads) gemm_wait_vmem<0>();  // (where loading waves store too, their stores share the counter)
       }
       issue_w(s0);
       issue_x(s1);
