@@ -60,8 +60,8 @@ def near(got, ref, what, tol=NORM):
 
 SIZES = [(1, 8, 8), (1, 1000, 520), (2, 24, 40), (31, 264, 72), (33, 8, 640), (64, 256, 64), (65, 264, 128), (127, 136, 1000),
          (129, 392, 200), (300, 1000, 64), (1000, 264, 1800)]
-# 256 x 256 tiles, whole and ragged, with a k tail (tests/test_gemm_plan.py asserts that these sizes take them)
-LARGE = [(4096, 4096, 256), (4090, 4072, 328), (4090, 328, 4072)]
+# 256 x 256 tiles, whole, ragged and cut along k, with a k tail (tests/test_gemm_plan.py asserts that these sizes take them)
+LARGE = [(4096, 4096, 256), (4090, 4072, 328), (4090, 328, 4072), (1250, 4104, 3248), (4750, 3496, 3144)]
 
 
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu_tanh"])

@@ -56,16 +56,18 @@ __device__ __forceinline__ void saved_store(unsigned char* block, int lane, cons
     const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(v[4 * k + 3]), __float_as_uint(v[4 * k + 2]), 0x0c0c0501u);
     lo[k] = a | (b << 16);
   }
-  stg16(block + lane * 16, hi[0]);
-  stg16(block + 1024 + lane * 16, hi[1]);
-  stg16(block + 2048 + lane * 16, lo);
+  __builtin_nontemporal_store(hi[0], (u32x4*)(block + lane * 16));
+  __builtin_nontemporal_store(hi[1], (u32x4*)(block + 1024 + lane * 16));
+  __builtin_nontemporal_store(lo, (u32x4*)(block + 2048 + lane * 16));
 }
 
 struct SavedRegs {
   u32x4 hi[2], lo;
 };
 __device__ __forceinline__ SavedRegs saved_load(const unsigned char* block, int lane) {
-  return SavedRegs{{ldg16(block + lane * 16), ldg16(block + 1024 + lane * 16)}, ldg16(block + 2048 + lane * 16)};
+  return SavedRegs{{__builtin_nontemporal_load((const u32x4*)(block + lane * 16)),
+                    __builtin_nontemporal_load((const u32x4*)(block + 1024 + lane * 16))},
+                   __builtin_nontemporal_load((const u32x4*)(block + 2048 + lane * 16))};
 }
 __device__ __forceinline__ float saved_value(const SavedRegs& r, int e) {
   const uint32_t h = r.hi[e >> 3][(e >> 1) & 3], l = r.lo[e >> 2];

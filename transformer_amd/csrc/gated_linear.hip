@@ -53,6 +53,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_kernel(GatedParams
   });
 }
 
+// Small tiles at any size: the saved values' loads and the two outputs' stores of one workgroup run under the products of the
+// CU's other one (12288 x 4608 over 1792 270-280 us; 331 with 256 x 256 tiles).
 template <class C, int ACT>
 __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedParams p) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
@@ -62,15 +64,23 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedPa
     const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
     const int sr = 32 * at.wm + at.l32;
     bf16* out = p.out + (int64_t)m0 * p.os + n0;
-#pragma unroll
-    for (int j = 0; j < C::XJ; ++j) {
-      const int mb = 32 * (C::XJ * at.wm + j);
+    // g and u of a pass's blocks, read together and, for the second pass, under the first one's stores (a block without
+    // outputs to store reads another one's)
+    SavedRegs g[C::NB], u[C::NB];
+    auto fetch = [&](int j) {
 #pragma unroll
       for (int i = 0; i < C::NB; ++i) {
-        const int nb = 32 * (at.wn * C::NB + i);
-        if (mb >= mv || nb >= nv) continue;  // (wave-uniform) no output of the block is stored
-        const unsigned char* from = gated_saved_at(p, m0 + mb, n0 + nb);
-        const SavedRegs g = saved_load(from, at.lane), u = saved_load(from + kSavedBlock, at.lane);
+        const int mb = 32 * (C::XJ * at.wm + j), nb = 32 * (at.wn * C::NB + i);
+        const unsigned char* from = gated_saved_at(p, m0 + (mb < mv ? mb : 0), n0 + (nb < nv ? nb : 0));
+        g[i] = saved_load(from, at.lane);
+        u[i] = saved_load(from + kSavedBlock, at.lane);
+      }
+    };
+    fetch(0);
+#pragma unroll
+    for (int j = 0; j < C::XJ; ++j) {
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) {
         f32x16& dh = acc.a[i][j];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -78,13 +88,15 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedPa
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float value, slope;
-            act_both<ACT>(saved_value(g, 4 * q + e), value, slope);
-            dg[e] = dh[4 * q + e] * saved_value(u, 4 * q + e) * slope;
+            act_both<ACT>(saved_value(g[i], 4 * q + e), value, slope);
+            dg[e] = dh[4 * q + e] * saved_value(u[i], 4 * q + e) * slope;
             dh[4 * q + e] *= value;  // du
           }
-          sts8(st.at(sr, nb / 8 + q) + 8 * at.hk, u32x2{pack_bf16x2(dg[0], dg[1]), pack_bf16x2(dg[2], dg[3])});
+          sts8(st.at(sr, 4 * (at.wn * C::NB + i) + q) + 8 * at.hk,
+               u32x2{pack_bf16x2(dg[0], dg[1]), pack_bf16x2(dg[2], dg[3])});
         }
       }
+      if (j + 1 < C::XJ) fetch(j + 1);
       __syncthreads();
       store_rows<C>(st, at.tid, 32 * C::WM, out, p.os, mv, nv, [&](int r) { return pass_row<C>(r, j); });
       __syncthreads();
@@ -203,8 +215,6 @@ extern "C" int mla_gated_linear_bwd(const mla_gated_linear_bwd_args* a, void* st
   p.saved = (unsigned char*)const_cast<void*>(a->saved);
   p.os = a->dgu_stride;
   hipStream_t s = (hipStream_t)stream;
-  // (the saved values' loads and the two outputs' stores of one workgroup run under the products of the CU's other one:
-  // 12288 x 4608 over 1792 284 us, 331 with 256 x 256 tiles)
   MLA_TRY(gemm_apply(op, p.g, GemmPlan{0, 1, 0, 0}, nullptr, 0));
   gated_launch<GemmCfg<128, 2, 2, true, false>, true>(p, a->activation, s);
   return launch_status(op);

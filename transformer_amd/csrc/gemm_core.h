@@ -3,16 +3,15 @@
 // n contiguous (the same weight read from its other side: dx = dy W), in which case its fragments come by transpose reads.
 //
 // A workgroup of WN x WM waves computes tiles of T x T outputs, one after the other, k in stages of 64.  A stage is two
-// slots of T rows x 64 k, x's and W's, in a ring of five that direct-to-LDS loads fill: when the products of a stage have read
-// their two slots, W of the stage after next and x of the one behind it go there.  The loads run on across the end of a tile, so
-// that the next tile's first stage lands under this tile's last products and its epilogue, which has the two slots last read
-// for its own use.  Loads past the last tile have empty descriptors.
+// slots of T rows x 64 k, x's and W's, in a ring of five that direct-to-LDS loads fill: when the first step of a stage has
+// read the rest of its x, that slot takes W of the stage after next, and W's, read at the end, x of the one behind it.  The
+// loads run on across the end of a tile, so that the next tile's first stage lands under this tile's last products and its
+// epilogue, which has the two slots last read for its own use.  Loads past the last tile have empty descriptors.
 //
 // A staged row of 64 k (128 bytes: pieces of 64 bytes reach half the rate, 60 against 95-130 bytes/ns per CU measured) holds
 // its chunk c of 16 bytes at c ^ ((row / 2) mod 8), so that 16 rows x one chunk are free of bank conflicts; a staged k row of T n
 // holds chunk c at c ^ 4 (row mod 4), so that the four rows of a half-wave's transpose read fall on four different 64-byte bank
-// groups.  The one barrier of a stage lies before its last 16-wide step: that step's products run under the next stage's
-// first reads, the others under the reads of the step after them.
+// groups.  A step's products run under the reads of the next one, the last step's under the next stage's first.
 #pragma once
 
 #include "mla_common.h"
@@ -26,10 +25,6 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 // of each, a wave's first NB / 2 blocks from w0, the rest from w1 at the same columns
 template <int T_, int WN_, int WM_, bool KMAJOR_, bool PAIR_>
 struct GemmCfg {
-  // The first LW waves issue the loads, the others store the outputs: loads and stores of one wave complete in order, so a
-  // wave that did both would wait for the stores of a tile before the second stage of the next.
-  static constexpr int LW = T_ == 256 ? WN_ * WM_ / 2 : WN_ * WM_;
-  static constexpr int SW0 = LW < WN_ * WM_ ? LW : 0, SW = WN_ * WM_ - SW0;  // the storing waves' first and number
   static constexpr int T = T_, WN = WN_, WM = WM_, BK = 64, HS = BK / 16;
   static constexpr bool KMAJOR = KMAJOR_, PAIR = PAIR_;
   static constexpr int WAVES = WN * WM, THREADS = 64 * WAVES;
@@ -37,9 +32,9 @@ struct GemmCfg {
   static constexpr int TN = PAIR ? T / 2 : T;               // columns of the weights that a tile covers
   static constexpr int SLOT = T * BK * 2;                   // T rows of 64 k, or 64 k rows of T
   static constexpr int RING = 5;
-  static constexpr int LOADS = SLOT / 1024 / LW;            // of a loading wave per slot
+  static constexpr int LOADS = SLOT / 1024 / WAVES;         // of a wave per slot
   static constexpr int LDS = RING * SLOT;
-  static_assert(SLOT % (1024 * LW) == 0 && LDS <= 160 * 1024, "the ring fits the LDS");
+  static_assert(SLOT % (1024 * WAVES) == 0 && LDS <= 160 * 1024, "the ring fits the LDS");
 };
 
 // y (a tile's outputs, as an epilogue defines them) over rows m of x, columns n of W; k runs over `parts` segments of K each:
@@ -122,13 +117,11 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   // ---- loads: a cursor for x and one for W, each (tile, part, stage) with the descriptors of its tile and part, which end at
   // the last valid row; lanes past them load nothing, and the outputs that such rows reach are not stored
   const uint32_t lds0 = lds_addr(lds);
-  const bool loads = w < C::LW;
-  const int lw = loads ? w : w - C::LW;
   uint32_t xoff[C::LOADS], woff[C::LOADS];  // this lane's bytes in each of the wave's loads, at k = 0
   bool second[C::LOADS];                    // PAIR (wave-uniform): the load is of w1's rows
 #pragma unroll
   for (int j = 0; j < C::LOADS; ++j) {
-    const int i = lw + C::LW * j, row = 8 * i + (lane >> 3);
+    const int i = w + C::WAVES * j, row = 8 * i + (lane >> 3);
     xoff[j] = (uint32_t)(row * p.xs * 2) + (uint32_t)(((lane & 7) ^ gemm_swz(row)) * 16);
     second[j] = false;
     if (C::KMAJOR) {
@@ -190,27 +183,27 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   auto done_x = [&]() {
     if (advance(cx)) point_x(cx);
   };
+  auto load_x = [&](const buf_rsrc& r, int slot, int j) {
+    dma16(r, xoff[j] + (uint32_t)(cx.st * C::BK * 2), lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
+  };
   auto issue_x = [&](int slot) {
-    if (loads) {
-      const buf_rsrc r = rx.rsrc();
+    const buf_rsrc r = rx.rsrc();
 #pragma unroll
-      for (int j = 0; j < C::LOADS; ++j)
-        dma16(r, xoff[j] + (uint32_t)(cx.st * C::BK * 2), lds0 + (uint32_t)(slot * C::SLOT + (lw + C::LW * j) * 1024));
-    }
+    for (int j = 0; j < C::LOADS; ++j) load_x(r, slot, j);
     done_x();
   };
   const uint32_t wstep = C::KMAJOR ? (uint32_t)(C::BK * p.ws0 * 2) : (uint32_t)(C::BK * 2);
   auto done_w = [&]() {
     if (advance(cw)) point_w(cw);
   };
+  auto load_w = [&](const buf_rsrc& r0, const buf_rsrc& r1, int slot, int j) {
+    dma16(C::PAIR && second[j] ? r1 : r0, woff[j] + (uint32_t)cw.st * wstep,
+          lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
+  };
   auto issue_w = [&](int slot) {
-    if (loads) {
-      const buf_rsrc r0 = rw0.rsrc(), r1 = C::PAIR ? rw1.rsrc() : r0;
+    const buf_rsrc r0 = rw0.rsrc(), r1 = C::PAIR ? rw1.rsrc() : r0;
 #pragma unroll
-      for (int j = 0; j < C::LOADS; ++j)
-        dma16(C::PAIR && second[j] ? r1 : r0, woff[j] + (uint32_t)cw.st * wstep,
-              lds0 + (uint32_t)(slot * C::SLOT + (lw + C::LW * j) * 1024));
-    }
+    for (int j = 0; j < C::LOADS; ++j) load_w(r0, r1, slot, j);
     done_w();
   };
 
@@ -261,6 +254,21 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
 #pragma unroll
       for (int j = 0; j < C::XJ; ++j) acc.a[i][j] = mfma32(fw[h & 1][i], fx[h][j], acc.a[i][j]);
   };
+  // A step's products with the wave's loads of one slot between them: one behind the other, the loads would wait for each other
+  // in the memory pipe, and the wave's next products for them.
+  auto multiply_loading = [&](int h, auto&& load) {
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i)
+#pragma unroll
+      for (int j = 0; j < C::XJ; ++j) {
+        constexpr int products = C::NB * C::XJ;
+        acc.a[i][j] = mfma32(fw[h & 1][i], fx[h][j], acc.a[i][j]);
+        const int n = i * C::XJ + j;
+#pragma unroll
+        for (int l = n * C::LOADS / products; l < (n + 1) * C::LOADS / products; ++l) load(l);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
   // the reads go out between the step's first products (left alone, the compiler moves them to their use)
   auto interleave = [&]() {
     constexpr int reads = C::XJ + (C::KMAJOR ? 2 : 1) * C::NB, products = C::NB * C::XJ;
@@ -292,12 +300,12 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   issue_x(2);
   issue_w(3);
   issue_x(4);
-  if (loads) gemm_wait_vmem<3 * C::LOADS>();
+  gemm_wait_vmem<3 * C::LOADS>();
   __syncthreads();
   int sx = 0, sw = 1;  // the slots of the stage being multiplied
   auto next_slots = [&]() {
-    sx = sx >= 3 ? sx - 3 : sx + 2;
-    sw = sw >= 3 ? sw - 3 : sw + 2;
+    sx = sx >= C::RING - 2 ? sx - (C::RING - 2) : sx + 2;
+    sw = sw >= C::RING - 2 ? sw - (C::RING - 2) : sw + 2;
   };
   auto read_first = [&]() {  // what a stage's slots give before its first step's products
     read_w(sw, 0);
@@ -320,22 +328,24 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
         multiply(0);
         interleave();
         __syncthreads();  // every wave holds the stage's x in registers
-        issue_w(sx);
-#pragma unroll
-        for (int h = 1; h + 1 < C::HS; ++h) {
-          read_w(sw, h + 1);
-          multiply(h);
-          interleave();
-        }
-        // every wave holds the stage in registers and the next one has landed: all but the one behind it
-        if (loads) gemm_wait_vmem<2 * C::LOADS>();
-        __syncthreads();
-        issue_x(sw);
-        next_slots();
+        read_w(sw, 2);
         __builtin_amdgcn_sched_barrier(0);
-        read_first();
-        multiply(C::HS - 1);
+        const buf_rsrc r0 = rw0.rsrc(), r1 = C::PAIR ? rw1.rsrc() : r0;
+        multiply_loading(1, [&](int j) { load_w(r0, r1, sx, j); });
+        done_w();
+        read_w(sw, 3);
+        multiply(2);
         interleave();
+        // every wave holds the stage in registers and the next one has landed: all but the one behind it
+        gemm_wait_vmem<2 * C::LOADS>();
+        __syncthreads();
+        const int s1 = sw;
+        next_slots();
+        read_first();
+        __builtin_amdgcn_sched_barrier(0);
+        const buf_rsrc r = rx.rsrc();
+        multiply_loading(3, [&](int j) { load_x(r, s1, j); });
+        done_x();
       }
       read_x(sx, C::HS - 1);
 #pragma unroll
@@ -345,7 +355,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
         multiply(h);
       }
       cut(C::HS - 1, tail);
-      if (loads) gemm_wait_vmem<C::LOADS>();
+      gemm_wait_vmem<C::LOADS>();
       __syncthreads();
       const int s0 = sx, s1 = sw;
       next_slots();
@@ -372,7 +382,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
           gemm_tile_at(p, item.tile, mt, nt);
           epi(acc, mt * C::T, nt * C::TN, lds + s0 * C::SLOT, lds + s1 * C::SLOT, 0, C::XJ);
         }
-        if (loads) gemm_wait_vmem<0>();  // (where loading waves store too, their stores share the counter)
+        gemm_wait_vmem<0>();  // (its stores share the counter that the stages' waits count down)
       }
       issue_w(s0);
       issue_x(s1);
@@ -397,13 +407,18 @@ __device__ __forceinline__ void gemm_finish(const GemmArgs& p, unsigned char* ld
     for (int j = 0; j < C::XJ; ++j) {
       acc.a[i][j] = f32x16{};
       if (j != jj) continue;
-      for (int s = 0; s < p.S; ++s) {
+      for (int s0 = 0; s0 < p.S; s0 += 4) {  // four pieces' reads in flight
+        f32x4 v[4][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 v = src[s * step + ((i * C::XJ + j) * 4 + q) * 64];
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc.a[i][j][4 * q + e] += v[e];
-        }
+          for (int q = 0; q < 4; ++q) v[s][q] = src[min(s0 + s, p.S - 1) * step + ((i * C::XJ + j) * 4 + q) * 64];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc.a[i][j][4 * q + e] += s0 + s < p.S ? v[s][q][e] : 0.f;
       }
     }
   int mt, nt;

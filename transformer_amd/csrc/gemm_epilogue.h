@@ -44,14 +44,13 @@ __device__ __forceinline__ int pass_row(int r, int j) {
   return 32 * (C::XJ * (r >> 5) + j) + (r & 31);
 }
 
-// The storing waves' part: the staged rows [0, R) to out (at the tile's first row and column): rows below mv, columns below nv (a multiple of 8)
+// The staged rows [0, R) to out (at the tile's first row and column): rows below mv, columns below nv (a multiple of 8)
 template <class C, int COLS, class RowOf>
 __device__ __forceinline__ void store_rows(const StagedRows<C, COLS>& st, int tid, int R, bf16* out, int64_t stride, int mv, int nv,
                                            RowOf&& row_of) {
   constexpr int CH = COLS / 8;
-  if (tid < 64 * C::SW0) return;
 #pragma unroll 4
-  for (int c = tid - 64 * C::SW0; c < R * CH; c += 64 * C::SW) {
+  for (int c = tid; c < R * CH; c += C::THREADS) {
     const int r = c / CH, ch = c % CH, m = row_of(r);
     if (m < mv && 8 * ch < nv) stg16(out + m * stride + 8 * ch, lds16(st.at(r, ch)));
   }

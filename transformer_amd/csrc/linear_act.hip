@@ -32,12 +32,10 @@ __device__ __forceinline__ void linear_epilogue(const LinearParams& p, GemmAcc<C
     if (j < j0 || j >= j1) continue;
     if (p.residual) {
       const bf16* res = p.residual + (int64_t)m0 * p.rs + n0;
-      if (at.tid < 64 * C::LW) {
 #pragma unroll 4
-        for (int c = at.tid; c < R * CH; c += 64 * C::LW) {
-          const int r = c / CH, ch = c % CH, m = pass_row<C>(r, j);
-          if (m < mv && 8 * ch < nv) sts16(st.at(r, ch), ldg16(res + m * p.rs + 8 * ch));
-        }
+      for (int c = at.tid; c < R * CH; c += C::THREADS) {
+        const int r = c / CH, ch = c % CH, m = pass_row<C>(r, j);
+        if (m < mv && 8 * ch < nv) sts16(st.at(r, ch), ldg16(res + m * p.rs + 8 * ch));
       }
       __syncthreads();
     }

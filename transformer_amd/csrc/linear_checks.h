@@ -54,11 +54,11 @@ inline int gemm_apply(const char* op, GemmArgs& g, const GemmPlan& pl, void* wor
   return MLA_OK;
 }
 
-// one workgroup of 256 x 256 tiles per CU, two of 128 x 128
+// one workgroup per CU, or two that share one
 template <class C>
 inline unsigned gemm_grid(const GemmArgs& g) {
   const int64_t tiles = (int64_t)g.n_mt * g.n_nt, items = g.full + (tiles - g.full) * g.S;
-  const int64_t most = C::T == 256 ? 256 : 512;
+  const int64_t most = C::LDS > 80 * 1024 ? 256 : 512;
   return (unsigned)(items < most ? items : most);
 }
 template <class C>

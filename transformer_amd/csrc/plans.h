@@ -124,14 +124,17 @@ inline WgPlan wg_plan(int64_t M, int64_t N, int64_t K) {
 
 // ---- linear_act.hip's and gated_linear.hip's tiles (gemm_core.h)
 struct GemmPlan {
-  int large;  // tiles of 256 x 256, one workgroup per CU; else 128 x 128, two
+  int large;   // tiles of 256 x 256, one workgroup a CU; else 128 x 128, two
   int S, per;  // the tiles of an unfilled last round are cut along k into S pieces of `per` stages (1: not cut)
   int64_t part_bytes;
 };
 
-// The plan of least estimated time (us) for y [M, N] over parts x K, `cut` where tiles may be cut along k.  A whole round takes
-// its stages at the measured 1.3 us (large tiles: 144 stages took 194 us) or 0.85 us (small ones, two on a CU; 0.6 alone on it)
-// plus what a tile's start and stores take; pieces add the fp32 sums they leave, written and read at 2.5 TB/s together, and a
+// The plan of least estimated time (us) for y [M, N] over parts x K, `cut` where tiles may be cut along k.  A round of
+// workgroups takes its stages at a measured time plus what a tile's start and stores take:
+//   large tiles 1.3 us a stage (144 stages of 256 tiles 190 us: the rate that power allows) and 12; small ones, two on a CU, 0.85
+//   (12288 x 9216 over 28 stages: 13.5 rounds in 406 us, the loads' rate) and 6, up to 256 of them, alone on theirs, 0.45 + 0.25
+//   of the CUs in use (2500 x 1000: 160 tiles x 28 stages 19 us; 1999 x 2048: 256 x 72 56 us) and 5.
+// Pieces add the fp32 sums they leave, written and read at 1.5 TB/s together (63 MB took 46 us more), and a
 // second kernel.
 inline GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int64_t parts, bool cut) {
   GemmPlan best{};
@@ -139,25 +142,21 @@ inline GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int64_t parts, bool c
   const int64_t n = (K + 63) / 64 * parts;
   for (int large = 1; large >= 0; --large) {
     const int64_t T = large ? 256 : 128, slots = large ? 256 : 512;
+    const double stage = large ? 1.3 : 0.85, fixed = large ? 12.0 : 6.0;
     const int64_t tiles = ((M + T - 1) / T) * ((N + T - 1) / T), rest = tiles % slots;
-    const double ts = large ? 1.3 : 0.85, fixed = large ? 12.0 : 6.0, alone = large ? 1.2 : 0.6;
-    const double rounds = (double)(tiles / slots) * ((double)n * ts + fixed);
-    for (int64_t S = 1; S <= 16 && S * 2 <= n; ++S) {
-      if (S > 1 && (!cut || rest == 0 || rest * S > slots)) break;
-      const int64_t per = (n + S - 1) / S;
+    for (int64_t S = 1; S <= 16; ++S) {
+      if (S > 1 && (!cut || S * 2 > n || rest == 0 || rest * S > slots)) break;
+      const int64_t per = (n + S - 1) / S, items = rest * S;
       if ((n + per - 1) / per != S) continue;  // fewer pieces hold the same stages
-      double t = rounds;
-      if (rest) t += (double)per * (rest * S <= 256 ? alone : ts) + fixed;
-      const int64_t pb = S > 1 ? rest * S * T * T * 4 : 0;
-      if (S > 1) t += 5.0 + (double)pb / 2.5e6;
+      double t = (double)(tiles / slots) * ((double)n * stage + fixed);
+      if (items > 0 && !large && items <= 256) t += (double)per * (0.45 + 0.25 * (double)items / 256) + 5.0;
+      else if (items > 0) t += (double)per * stage + fixed;
+      const int64_t pb = S > 1 ? items * T * T * 4 : 0;
+      if (S > 1) t += 5.0 + (double)pb / 1.5e6;
       if (t < best_t) {
         best_t = t;
         best = GemmPlan{large, (int)S, (int)per, pb};
       }
-    }
-    if (n < 2) {  // (one stage: nothing to cut)
-      const double t = (double)((tiles + slots - 1) / slots) * ((double)n * ts + fixed);
-      if (t < best_t) best_t = t, best = GemmPlan{large, 1, (int)n, 0};
     }
   }
   return best;
