@@ -228,3 +228,18 @@ def test_a_training_step_of_a_block():
         assert (r.double() - f).norm() <= bound * f.norm()
         assert ((p.grad.double() - r.double() * (0.01 / (total.double() + 1e-6))).abs()
                 <= r.double().abs() * (0.01 / total.double()) * (4 * EPS32 + (EPS16 if r.dtype == torch.bfloat16 else 0))).all()
+
+
+def test_sparse_and_overlapping_layouts_are_refused_before_anything_is_scaled():
+    from transformer_amd import clip_grad_norm_
+    one = torch.ones(4, 4, device=DEV)
+    p = torch.nn.Parameter(torch.zeros(4, 4, device=DEV))
+    p.grad = torch.eye(4, device=DEV).to_sparse()
+    with pytest.raises(ValueError):
+        clip_grad_norm_([*params([one]), p], 1.0)
+    with pytest.raises(ValueError):
+        clip_grad_norm_(params([one, torch.ones(4, device=DEV).expand(3, 4)]), 1.0)
+    buf = torch.ones(6, device=DEV)
+    with pytest.raises(ValueError):  # rows that overlap
+        clip_grad_norm_(params([buf.as_strided((3, 4), (1, 1))]), 1.0)
+    assert torch.equal(one, torch.ones(4, 4, device=DEV))

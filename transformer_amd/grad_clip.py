@@ -6,8 +6,8 @@ pass alone.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 from typing import Iterable, List, Union
 
 import torch
@@ -31,39 +31,58 @@ def _dense(t: Tensor) -> bool:
     return True
 
 
-def _check(op: str, tensors: List[Tensor], norm_type: float) -> bool:
-    """Whether the norm is the largest magnitude (else the 2-norm); refuses what the kernels do not take."""
+def _shares(t: Tensor) -> bool:
+    """Whether elements of ``t`` may share memory (a stride shorter than what lies below it)."""
+    reach = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride < reach:
+            return t.numel() > 0
+        reach += stride * (size - 1)
+    return False
+
+
+def _is_max(op: str, norm_type: float) -> bool:
+    """Whether the norm is the largest magnitude (else the 2-norm)."""
     norm_type = float(norm_type)
     if norm_type not in (2.0, math.inf):
         raise ValueError(f"{op}: norm_type {norm_type} is not built (2 or inf)")
-    if tensors:
-        dev = tensors[0].device
-        for t in tensors:
-            if t.device != dev or t.dtype not in _CODES or t.layout != torch.strided or not t.is_cuda:
-                _refuse(op, t, dev)
     return norm_type == math.inf
 
 
-def _refuse(op: str, t: Tensor, device: torch.device) -> None:
-    if t.layout != torch.strided:
-        raise ValueError(f"{op}: sparse gradients are not built")
-    if not t.is_cuda:
-        raise RuntimeError(f"transformer_amd.{op} runs on a ROCm GPU only (no CPU path); got a tensor on {t.device}")
-    if t.dtype not in _CODES:
-        raise TypeError(f"{op}: gradients must be float32 or bfloat16, got {t.dtype}")
-    raise ValueError(f"{op}: gradients on {device} and {t.device}: one device is needed")
+def _refuse(op: str, tensors: List[Tensor]) -> None:
+    """The error of a list that the kernels do not take."""
+    for t in tensors:
+        if t.layout != torch.strided:
+            raise ValueError(f"{op}: sparse gradients are not built")
+        if not t.is_cuda:
+            raise RuntimeError(f"transformer_amd.{op} runs on a ROCm GPU only (no CPU path); got a tensor on {t.device}")
+        if t.dtype not in _CODES:
+            raise TypeError(f"{op}: gradients must be float32 or bfloat16, got {t.dtype}")
+    raise ValueError(f"{op}: gradients on {sorted({str(t.device) for t in tensors})}: one device is needed")
+
+
+def _laid_out(op: str, tensors: List[Tensor]) -> List[Tensor]:
+    """``tensors`` without gaps in memory: those with gaps copied.  (Few look-ups a tensor: they are the host's cost.)"""
+    try:
+        devices, whole = {t.get_device() for t in tensors}, [t.is_contiguous() for t in tensors]
+    except RuntimeError:  # (sparse)
+        _refuse(op, tensors)
+    if len(devices) != 1 or -1 in devices or not _CODES.keys() >= {t.dtype for t in tensors} \
+            or not all(t.layout == torch.strided for t in tensors):
+        _refuse(op, tensors)
+    if all(whole):
+        return tensors
+    return [t if w or _dense(t) else t.detach().contiguous() for t, w in zip(tensors, whole)]
 
 
 def _run(op: str, entry: str, tensors: List[Tensor], is_max: bool, max_norm: float) -> Tensor:
-    n = len(tensors)
-    like = tensors[0]
+    n, like = len(tensors), tensors[0]
     norm = torch.empty((), dtype=torch.float32, device=like.device)
     # host tables, read before the entry point returns
-    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
-    numels = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
-    dtypes = (ctypes.c_int32 * n)(*[_CODES[t.dtype] for t in tensors])
-    args = _lib.GradNormArgs(ctypes.addressof(ptrs), ctypes.addressof(numels), ctypes.addressof(dtypes), n, norm.data_ptr(), None,
-                             0, max_norm, int(is_max))
+    ptrs, numels = array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors])
+    codes = array("i", [_CODES[t.dtype] for t in tensors])
+    args = _lib.GradNormArgs(ptrs.buffer_info()[0], numels.buffer_info()[0], codes.buffer_info()[0], n, norm.data_ptr(), None, 0,
+                             max_norm, int(is_max))
     ws = _fit_workspace("mla_grad_norm_workspace_bytes", args, like)  # noqa: F841  (kept until the launch)
     _launch(entry, args, like, op)
     return norm
@@ -73,11 +92,10 @@ def grad_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) 
     """The norm (2, or inf: the largest magnitude) of all elements of ``tensors`` together, an fp32 scalar on their device.
     Tensors are fp32 or bf16, of any layout, on one device; squares are summed in fp64.  A NaN anywhere gives NaN."""
     tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
-    is_max = _check("grad_norm", tensors, norm_type)
+    is_max = _is_max("grad_norm", norm_type)
     if not tensors:
         return torch.tensor(0.0)
-    with torch.no_grad():
-        return _run("grad_norm", "mla_grad_norm", [t if _dense(t) else t.contiguous() for t in tensors], is_max, 0.0)
+    return _run("grad_norm", "mla_grad_norm", _laid_out("grad_norm", tensors), is_max, 0.0)
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -90,30 +108,26 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"{op}: max_norm must be at least 0, got {max_norm}")
+    is_max = _is_max(op, norm_type)
     parameters = [parameters] if isinstance(parameters, Tensor) else parameters
-    grads = [p.grad for p in parameters if p.grad is not None]
-    is_max = _check(op, grads, norm_type)
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    with torch.no_grad():
-        flat, back = grads, []
-        if not all(g.is_contiguous() for g in grads):
-            flat = []
-        for g in grads if flat is not grads else ():
-            if _dense(g):
-                flat.append(g)
-                continue
-            if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+    flat = _laid_out(op, grads)
+    if flat is not grads:
+        for g in grads:
+            if _shares(g):
                 raise ValueError(f"{op}: a gradient with strides {g.stride()} shares memory between its elements")
-            flat.append(g.contiguous())
-            back.append((g, flat[-1]))
-        if error_if_nonfinite:
-            norm = _run(op, "mla_grad_norm", flat, is_max, 0.0)
-            if not bool(torch.isfinite(norm)):
-                raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so "
-                                   "it cannot be clipped.")
-        norm = _run(op, "mla_grad_clip", flat, is_max, max_norm)
-        for g, c in back:
-            g.copy_(c)
-        torch.autograd.graph.increment_version(grads)
+    if error_if_nonfinite:
+        norm = _run(op, "mla_grad_norm", flat, is_max, 0.0)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it "
+                               "cannot be clipped.")
+    norm = _run(op, "mla_grad_clip", flat, is_max, max_norm)
+    if flat is not grads:
+        with torch.no_grad():
+            for g, c in zip(grads, flat):
+                if g is not c:
+                    g.copy_(c)
+    torch.autograd.graph.increment_version(grads)
     return norm
