@@ -115,11 +115,12 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedPa
   });
 }
 
-template <int MB, int ACT>
+template <int MB, int CG, int ACT>
 __global__ __launch_bounds__(64 * kRcWaves) void gated_linear_rows_kernel(GatedParams p, RowsArgs r) {
-  __shared__ f32x4 red[kRcWaves][2 * MB][64];
-  RowsProduct<MB, true> t;
-  t.run(r, red);
+  typedef RowsProduct<MB, CG, true> Product;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[Product::LDS];
+  Product t;
+  t.run(r, lds);
   if (!t.mine) return;
   const f32x4 g = t.sum[0], u = t.sum[1];
   if (p.saved) {
@@ -133,13 +134,18 @@ __global__ __launch_bounds__(64 * kRcWaves) void gated_linear_rows_kernel(GatedP
   stg8(p.out + t.m * p.os + t.n, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
 }
 
+template <int CG, int ACT>
+static void gated_rows_launch(const GatedParams& p, hipStream_t s) {
+  const RowsArgs r{p.g.x, p.g.w0, p.g.w1, p.g.xs, p.g.ws0, p.g.ws1, p.g.M, p.g.N, p.g.K};
+  const dim3 grid((unsigned)((r.N + CG - 1) / CG)), wg(64 * kRcWaves);
+  if (r.M <= 16) gated_linear_rows_kernel<1, CG, ACT><<<grid, wg, 0, s>>>(p, r);
+  else if (r.M <= 32) gated_linear_rows_kernel<2, CG, ACT><<<grid, wg, 0, s>>>(p, r);
+  else gated_linear_rows_kernel<4, CG, ACT><<<grid, wg, 0, s>>>(p, r);
+}
 template <int ACT>
 static void gated_rows_go(const GatedParams& p, hipStream_t s) {
-  const RowsArgs r{p.g.x, p.g.w0, p.g.w1, p.g.xs, p.g.ws0, p.g.ws1, p.g.M, p.g.N, p.g.K, rows_columns(p.g.N)};
-  const dim3 grid((unsigned)((r.N + r.cg - 1) / r.cg)), wg(64 * kRcWaves);
-  if (r.M <= 16) gated_linear_rows_kernel<1, ACT><<<grid, wg, 0, s>>>(p, r);
-  else if (r.M <= 32) gated_linear_rows_kernel<2, ACT><<<grid, wg, 0, s>>>(p, r);
-  else gated_linear_rows_kernel<4, ACT><<<grid, wg, 0, s>>>(p, r);
+  if (rows_columns(p.g.N) == 16) gated_rows_launch<16, ACT>(p, s);
+  else gated_rows_launch<32, ACT>(p, s);
 }
 
 template <class C, bool BWD, int ACT>

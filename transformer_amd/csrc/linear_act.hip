@@ -94,11 +94,12 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_act_finish_kernel(Linear
   });
 }
 
-template <int MB, int ACT>
+template <int MB, int CG, int ACT>
 __global__ __launch_bounds__(64 * kRcWaves) void linear_act_rows_kernel(LinearParams p, RowsArgs r) {
-  __shared__ f32x4 red[kRcWaves][MB][64];
-  RowsProduct<MB, false> t;
-  t.run(r, red);
+  typedef RowsProduct<MB, CG, false> Product;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[Product::LDS];
+  Product t;
+  t.run(r, lds);
   if (!t.mine) return;
   f32x4 v = t.sum[0];
   if (p.bias) {
@@ -115,13 +116,18 @@ __global__ __launch_bounds__(64 * kRcWaves) void linear_act_rows_kernel(LinearPa
   stg8(p.y + t.m * p.ys + t.n, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
 }
 
+template <int CG, int ACT>
+static void linear_act_rows_launch(const LinearParams& p, hipStream_t s) {
+  const RowsArgs r{p.g.x, p.g.w0, nullptr, p.g.xs, p.g.ws0, 0, p.g.M, p.g.N, p.g.K};
+  const dim3 grid((unsigned)((r.N + CG - 1) / CG)), wg(64 * kRcWaves);
+  if (r.M <= 16) linear_act_rows_kernel<1, CG, ACT><<<grid, wg, 0, s>>>(p, r);
+  else if (r.M <= 32) linear_act_rows_kernel<2, CG, ACT><<<grid, wg, 0, s>>>(p, r);
+  else linear_act_rows_kernel<4, CG, ACT><<<grid, wg, 0, s>>>(p, r);
+}
 template <int ACT>
 static void linear_act_rows_go(const LinearParams& p, hipStream_t s) {
-  const RowsArgs r{p.g.x, p.g.w0, nullptr, p.g.xs, p.g.ws0, 0, p.g.M, p.g.N, p.g.K, rows_columns(p.g.N)};
-  const dim3 grid((unsigned)((r.N + r.cg - 1) / r.cg)), wg(64 * kRcWaves);
-  if (r.M <= 16) linear_act_rows_kernel<1, ACT><<<grid, wg, 0, s>>>(p, r);
-  else if (r.M <= 32) linear_act_rows_kernel<2, ACT><<<grid, wg, 0, s>>>(p, r);
-  else linear_act_rows_kernel<4, ACT><<<grid, wg, 0, s>>>(p, r);
+  if (rows_columns(p.g.N) == 16) linear_act_rows_launch<16, ACT>(p, s);
+  else linear_act_rows_launch<32, ACT>(p, s);
 }
 
 template <class C, int ACT>

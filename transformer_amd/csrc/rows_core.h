@@ -1,111 +1,143 @@
 // A few rows of x against a weight (a token of each sequence of a batch): bound by reading the weight once.
 //
-// A workgroup of eight waves takes CG (16 or 8) columns, or CG of each of two weights, over all of k: wave w the steps of 64 k
-// w, w + 8, ..., so that the eight read 1 KiB of every weight row at a time.  Fragments go from memory straight into registers
-// (v_mfma_f32_16x16x32_bf16: lane l takes row l % 16 and chunk l / 16 of 8 k; the two halves of a step make whole 128-byte
-// lines), several steps ahead of their products: 64 to 128 KiB of a CU's reads are in flight.  The waves' sums are added
-// through LDS in wave order.
+// A workgroup of eight waves takes CG columns of the weight, or of each of two weights, over all of k, in chunks of 256.  A chunk
+// of the CG weight rows and of all x rows (512 contiguous bytes of each) comes by direct-to-LDS loads into a ring that keeps up to
+// 144 KiB of a CU's reads in flight; wave w multiplies k 32 w .. 32 w + 31 of it (v_mfma_f32_16x16x32_bf16), and the waves' sums
+// are added through LDS in wave order.  Calls in a row, us (fragments straight from memory, 16 rows x 64 bytes an
+// instruction, in brackets): one row against 2 x 4608 x 1792 7.6 (10.3), 4.4 TB/s; 32 against 2 x 4608 x 2048 9.4 (18.0), 4.0
+// TB/s; 64 against 2 x 4608 x 1792 10.7 (22); one against 1792 x 4608 7.0 (7.3), 32 against 2048 x 4608 9.2 (14.3): 112 and 128
+// workgroups, whose chunks follow each other at the latency of the ring.
+//
+// A staged row's chunk c of 16 bytes lies at c ^ (row mod 16): the 16 rows of a fragment fall on different banks.
 #pragma once
 
+#include <algorithm>
+
 #include "act.h"
+#include "gemm_core.h"
 
 namespace mla {
 
-constexpr int kRcWaves = 8, kRcMaxRows = 64;
+constexpr int kRcWaves = 8, kRcMaxRows = 64, kRcK = 256;
 
 struct RowsArgs {
   const bf16 *x, *w0, *w1;
   int64_t xs, ws0, ws1;
   int M, N, K;
-  int cg;  // columns of a workgroup
 };
 
-// MB blocks of 16 rows (M <= 16 MB).  On return wave i < MB holds rows 16 i + l % 16 of both products, columns
-// n0 + 4 (l / 16) + [0, 4), and `mine` says whether the lane's are to be stored; the other waves hold nothing.
-template <int MB, bool PAIR>
+// MB blocks of 16 rows (M <= 16 MB); CG columns: 16 or 32
+template <int MB, int CG, bool PAIR>
 struct RowsProduct {
-  static constexpr int NW = PAIR ? 2 : 1;
-  static constexpr int BATCH = MB <= 2 ? 4 : 2;  // steps whose fragments are loaded together
-  f32x4 sum[NW];
+  static constexpr int NW = PAIR ? 2 : 1, CB = CG / 16;           // weights; blocks of 16 of their columns
+  static constexpr int WROWS = NW * CG, ROWS = WROWS + 16 * MB;   // staged rows
+  static constexpr int SLOT = ROWS * 2 * kRcK;
+  static constexpr int FIT = 144 * 1024 / SLOT, RING = FIT < 8 ? FIT : 8;
+  static constexpr int LOADS = ROWS / 2 / kRcWaves;               // of a wave per chunk, two rows each: CB per weight, MB of x
+  static constexpr int BLOCKS = NW * CB * MB;                         // 16 x 16 products of a wave
+  static constexpr int RED = kRcWaves * BLOCKS * 1024;
+  static constexpr int LDS = RING * SLOT > RED ? RING * SLOT : RED;
+  static_assert(RING >= 2 && LDS <= 160 * 1024 && (RING - 1) * LOADS <= 63 && CB * MB <= kRcWaves, "a workgroup's shape");
+  f32x4 sum[NW];  // of rows m, columns n .. n + 3, where `mine`
   int m, n;
   bool mine;
 
-  __device__ __forceinline__ void run(const RowsArgs& p, f32x4 (*red)[MB * NW][64]) {
+  __device__ __forceinline__ void run(const RowsArgs& p, unsigned char* lds) {
     const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = blockIdx.x * p.cg, nv = min(p.cg, p.N - n0);
-    // rows past the last valid one read it again; k past the end reads past the descriptor, which gives zeros
-    const buf_rsrc rx = make_rsrc(p.x, rows_bytes(p.M, p.xs, p.K * 2));
-    const buf_rsrc r0 = make_rsrc(p.w0 + (int64_t)n0 * p.ws0, rows_bytes(nv, p.ws0, p.K * 2));
-    const buf_rsrc r1 = PAIR ? make_rsrc(p.w1 + (int64_t)n0 * p.ws1, rows_bytes(nv, p.ws1, p.K * 2)) : r0;
-    const int wr = min(l16 & (p.cg - 1), nv - 1);
-    const uint32_t wo0 = (uint32_t)(wr * p.ws0 * 2), wo1 = PAIR ? (uint32_t)(wr * p.ws1 * 2) : 0u;
-    uint32_t xo[MB];
+    const int n0 = blockIdx.x * CG, nv = min(CG, p.N - n0);
+    // rows past the last valid one and k past the end are not loaded (the descriptors are made in scalar registers: see GemmSpan)
+    const buf_rsrc rx = gemm_span(p.x, rows_bytes(p.M, p.xs, p.K * 2)).rsrc();
+    const buf_rsrc r0 = gemm_span(p.w0 + (int64_t)n0 * p.ws0, rows_bytes(nv, p.ws0, p.K * 2)).rsrc();
+    const buf_rsrc r1 = PAIR ? gemm_span(p.w1 + (int64_t)n0 * p.ws1, rows_bytes(nv, p.ws1, p.K * 2)).rsrc() : r0;
+    const uint32_t lds0 = lds_addr(lds);
+    const int chunks = (p.K + kRcK - 1) / kRcK;
+    uint32_t off[LOADS];  // this lane's bytes in each of the wave's loads, at k = 0
+    int at[LOADS];        // its chunk of 16 bytes within a row's 512
 #pragma unroll
-    for (int i = 0; i < MB; ++i) xo[i] = (uint32_t)(min(16 * i + l16, p.M - 1) * p.xs * 2);
-    struct Step {
-      u32x4 w[NW][2], x[MB][2];
-    };
-    auto load = [&](int t, Step& s) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = 8 * t + 4 * h + q;
-        const bool in = 8 * c < p.K;
-        const uint32_t at = 16u * (uint32_t)c, out = 0x80000000u;
-        s.w[0][h] = bld16(r0, in ? wo0 + at : out);
-        if (PAIR) s.w[NW - 1][h] = bld16(r1, in ? wo1 + at : out);
-#pragma unroll
-        for (int i = 0; i < MB; ++i) s.x[i][h] = bld16(rx, in ? xo[i] + at : out);
-      }
-    };
-    f32x4 acc[NW][MB];
-#pragma unroll
-    for (int a = 0; a < NW; ++a)
-#pragma unroll
-      for (int i = 0; i < MB; ++i) acc[a][i] = f32x4{};
-    const int steps = (p.K + 63) / 64;
-    Step s[2][BATCH];
-#pragma unroll
-    for (int b = 0; b < BATCH; ++b) load(w + kRcWaves * b, s[0][b]);  // (steps past the last load nothing and add zeros)
-    auto batch = [&](int t, Step (&now)[BATCH], Step (&next)[BATCH]) {
-      if (t + kRcWaves * BATCH < steps) {
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b) load(t + kRcWaves * (BATCH + b), next[b]);
-      }
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int a = 0; a < NW; ++a)
-#pragma unroll
-            for (int i = 0; i < MB; ++i) acc[a][i] = mfma16(as_bf16x8(now[b].w[a][h]), as_bf16x8(now[b].x[i][h]), acc[a][i]);
-    };
-    for (int t = w; t < steps; t += 2 * kRcWaves * BATCH) {
-      batch(t, s[0], s[1]);
-      if (t + kRcWaves * BATCH < steps) batch(t + kRcWaves * BATCH, s[1], s[0]);
+    for (int j = 0; j < LOADS; ++j) {  // load j of every wave has the same source: CB of w0, CB of w1, MB of x
+      const int row = 2 * (w + kRcWaves * j) + (lane >> 5), base = j < CB ? 0 : j < NW * CB ? CG : WROWS;
+      at[j] = (lane & 31) ^ (row & 15);
+      off[j] = (uint32_t)((row - base) * (j < CB ? p.ws0 : j < NW * CB ? p.ws1 : p.xs) * 2) + 16u * (uint32_t)at[j];
     }
+    auto issue = [&](int c, int slot) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j)
+        dma16(j < CB ? r0 : j < NW * CB ? r1 : rx, kRcK * c + 8 * at[j] < p.K ? off[j] + (uint32_t)(c * 2 * kRcK) : 0x80000000u,
+              (uint32_t)__builtin_amdgcn_readfirstlane((int)lds0 + slot * SLOT + (w + kRcWaves * j) * 1024));
+    };
+    f32x4 acc[NW][CB][MB];
 #pragma unroll
     for (int a = 0; a < NW; ++a)
 #pragma unroll
-      for (int i = 0; i < MB; ++i) red[w][a * MB + i][lane] = acc[a][i];
+      for (int b = 0; b < CB; ++b)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) acc[a][b][i] = f32x4{};
+#pragma unroll
+    for (int c = 0; c + 1 < RING; ++c) issue(c, c);
+    const int ch = 4 * w + q;  // this lane's chunk of a staged row
+    for (int c = 0, slot = 0; c < chunks; ++c) {
+      // chunk c has landed when only the RING - 2 behind it are in flight; past the barrier every wave has read chunk c - 1
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2) * LOADS) : "memory");
+      __syncthreads();
+      issue(c + RING - 1, slot == 0 ? RING - 1 : slot - 1);
+      const int k0 = kRcK * c + 32 * w;
+      if (k0 < p.K) {  // (wave-uniform)
+        const unsigned char* st = lds + slot * SLOT;
+        const bool in = k0 + 8 * q < p.K;  // k is whole chunks: the lane's 8 are in or out together
+        const u32x4 z{0u, 0u, 0u, 0u};
+        bf16x8 fw[NW][CB], fx[MB];
+#pragma unroll
+        for (int a = 0; a < NW; ++a)
+#pragma unroll
+          for (int b = 0; b < CB; ++b) {
+            const int row = a * CG + 16 * b + l16;
+            const u32x4 v = lds16(st + row * 512 + ((ch ^ (row & 15)) * 16));
+            fw[a][b] = as_bf16x8(in ? v : z);
+          }
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          const int row = WROWS + 16 * i + l16;
+          const u32x4 v = lds16(st + row * 512 + ((ch ^ (row & 15)) * 16));
+          fx[i] = as_bf16x8(in ? v : z);
+        }
+#pragma unroll
+        for (int a = 0; a < NW; ++a)
+#pragma unroll
+          for (int b = 0; b < CB; ++b)
+#pragma unroll
+            for (int i = 0; i < MB; ++i) acc[a][b][i] = mfma16(fw[a][b], fx[i], acc[a][b][i]);
+      }
+      slot = slot + 1 == RING ? 0 : slot + 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (no load lands in what follows)
+    __syncthreads();
+    f32x4* const red = reinterpret_cast<f32x4*>(lds) + lane;
+#pragma unroll
+    for (int a = 0; a < NW; ++a)
+#pragma unroll
+      for (int b = 0; b < CB; ++b)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) red[(w * BLOCKS + (a * CB + b) * MB + i) * 64] = acc[a][b][i];
     __syncthreads();
     mine = false;
-    if (w >= MB) return;
+    if (w >= CB * MB) return;
+    const int b = w / MB, i = w % MB;
 #pragma unroll
     for (int a = 0; a < NW; ++a) {
-      sum[a] = red[0][a * MB + w][lane];
+      sum[a] = red[((a * CB + b) * MB + i) * 64];
 #pragma unroll
-      for (int v = 1; v < kRcWaves; ++v) sum[a] += red[v][a * MB + w][lane];
+      for (int v = 1; v < kRcWaves; ++v) sum[a] += red[(v * BLOCKS + (a * CB + b) * MB + i) * 64];
     }
-    m = 16 * w + l16;
-    n = n0 + 4 * q;
-    mine = m < p.M && 4 * q < nv;
+    m = 16 * i + l16;
+    n = n0 + 16 * b + 4 * q;
+    mine = m < p.M && 16 * b + 4 * q < nv;
   }
 };
 
-// columns of a workgroup: 16, or 8 (half of the products go unused) where 16 would leave CUs without one
-inline int rows_columns(int64_t N) { return N / 16 < 200 ? 8 : 16; }
+// Columns of a workgroup: 16, or 32 where 16 would make a second round (a CU alone moves several times its share of the
+// memory's rate, and the wider workgroup reads x half as often).
+inline int rows_columns(int64_t N) { return N <= 16 * 256 ? 16 : 32; }
 
 // the 4 consecutive n that a lane holds, in the layout of act.h's blocks
 __device__ __forceinline__ void saved_store4(unsigned char* block, int m, int n, const f32x4& v) {
