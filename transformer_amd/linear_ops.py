@@ -14,11 +14,12 @@ from torch import Tensor
 
 from . import _lib, kernels
 from ._lib import ACTIVATIONS
-from .kernels import _alloc_workspace, _dt_code, _op, _register_autograd, weight_grad, weight_grad_or_none
+from .kernels import _alloc_workspace, _dt_code, _op, _register_autograd
 
 LINEAR_MAX_STRIDE = 1 << 22
 ROWS_MAX = 64  # rows up to which mla_linear_act needs no workspace
 _BF16, _F32 = torch.bfloat16, torch.float32
+_byref, _current_device, _raw_stream = ctypes.byref, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 # ----------------------------------------------------------------- helpers
@@ -26,18 +27,18 @@ _BF16, _F32 = torch.bfloat16, torch.float32
 def _launch(entry: str, args, like: Tensor, op: str) -> None:
     """Call a C entry point on ``like``'s device and its current stream, whichever device is the current one."""
     fn, dev = _lib.entry(entry), like.get_device()
-    if dev == torch._C._cuda_getDevice():
-        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(dev))
+    if dev == _current_device():
+        rc = fn(_byref(args), _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(dev))
+            rc = fn(_byref(args), _raw_stream(dev))
     if rc:
         _lib.check(rc, op)
 
 
 def _fit_workspace(entry: str, args, like: Tensor) -> Optional[Tensor]:
     """The workspace that ``entry`` (a ``*_workspace_bytes`` function) asks for, set in ``args``; keep it until the call."""
-    nbytes = int(_lib.entry(entry)(ctypes.byref(args)))
+    nbytes = _lib.entry(entry)(_byref(args))
     if not nbytes:
         return None
     ws = _alloc_workspace(nbytes, like.device)
@@ -77,29 +78,38 @@ def _activation(op: str, name: str, gate: bool = False) -> int:
 
 def _check(op: str, x: Tensor, weights, names, residual: Optional[Tensor], n_out: int) -> None:
     """Types, devices and sizes of the inputs (their shapes were compared already)."""
-    dev = x.get_device()
+    dev, ok = x.get_device(), x.dtype == _BF16 and x.is_cuda
+    for t in weights:
+        if t is not None:
+            ok = ok and (t.dtype == _BF16 or t.dtype == _F32) and t.get_device() == dev
+            if ok and t.dim() == 2:
+                n, k = t.shape
+                ok = not (n % 8 or k % 8) and n * k > 0
+    if residual is not None:
+        ok = ok and residual.dtype == _BF16 and residual.get_device() == dev \
+            and residual.shape[:-1] == x.shape[:-1] and residual.shape[-1:] == (n_out,)
+    if not ok:
+        _refuse(op, x, weights, names, residual, n_out)
+
+
+def _refuse(op: str, x: Tensor, weights, names, residual: Optional[Tensor], n_out: int) -> None:
+    """The error of inputs that :func:`_check` did not pass."""
+    kernels._require_gpu(op, x, residual, *weights)
+    if x.dtype != _BF16:
+        raise TypeError(f"{op}: x must be bfloat16, got {x.dtype}")
     for t, name in zip(weights, names):
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{op}: tensors must be on a ROCm GPU (got {t.device}); transformer_amd has no CPU implementation")
         if t.dtype != _BF16 and t.dtype != _F32:
             raise TypeError(f"{op}: {name} must be bfloat16 or float32, got {t.dtype}")
-        if t.get_device() != dev:
+        if t.device != x.device:
             raise ValueError(f"{op}: {name} is on {t.device}, x on {x.device}")
-        if t.dim() == 2:
-            n, k = t.shape
-            if n % 8 or k % 8 or not n or not k:
-                raise ValueError(f"{op}: {name} {tuple(t.shape)}: both sizes must be positive multiples of 8")
-    kernels._require_gpu(op, x, residual)
-    if x.dtype != _BF16:
-        raise TypeError(f"{op}: x must be bfloat16, got {x.dtype}")
-    if residual is not None:
-        if residual.dtype != _BF16:
-            raise TypeError(f"{op}: residual must be bfloat16, got {residual.dtype}")
-        if residual.shape != (*x.shape[:-1], n_out) or residual.get_device() != dev:
-            raise ValueError(f"{op}: residual must be {(*x.shape[:-1], n_out)} on {x.device}, got {tuple(residual.shape)} "
-                             f"on {residual.device}")
+        if t.dim() == 2 and (t.size(0) % 8 or t.size(1) % 8 or not t.numel()):
+            raise ValueError(f"{op}: {name} {tuple(t.shape)}: both sizes must be positive multiples of 8")
+    if residual.dtype != _BF16:
+        raise TypeError(f"{op}: residual must be bfloat16, got {residual.dtype}")
+    raise ValueError(f"{op}: residual must be {(*x.shape[:-1], n_out)} on {x.device}, got {tuple(residual.shape)} on "
+                     f"{residual.device}")
 
 
 def _saved_size(M: int, N: int) -> int:
@@ -165,18 +175,26 @@ def _(x, weight, bias, residual, activation, save):
 
 
 def _weight_grad(dy: Tensor, x: Tensor, dtype: torch.dtype) -> Tensor:
-    """``dy^T x`` in ``dtype`` for any number of rows: those beyond the kernel's 32-bit reach in several parts, added in fp32."""
-    if dy.size(0) == 0:
-        return torch.zeros(dy.size(1), x.size(1), dtype=dtype, device=dy.device)
-    dw = weight_grad_or_none(dy, x, dtype == _F32)
-    if dw is None:
-        rows = (1 << 30) // max(_row_stride(dy), _row_stride(x)) - 257
-        if rows < 32:
-            raise ValueError(f"mla_mi355x::weight_grad: rows of {dy.size(1)} and {x.size(1)} are too wide")
-        for r in range(0, dy.size(0), rows):
-            part = weight_grad(dy[r:r + rows], x[r:r + rows], True)
-            dw = part if dw is None else dw.add_(part)
-    return dw if dw.dtype == dtype else dw.to(dtype)
+    """``dy^T x`` in ``dtype`` for rows as :func:`_matrix` leaves them, any number of them: those beyond the kernel's 32-bit reach
+    in several parts, added in fp32."""
+    (M, N), K = dy.shape, x.size(1)
+    if M == 0:
+        return torch.zeros(N, K, dtype=dtype, device=dy.device)
+    sy, sx = _row_stride(dy), _row_stride(x)
+    if kernels.weight_grad_fits(M, N, K, sy, sx):
+        dw = torch.empty((N, K), dtype=dtype, device=dy.device)
+        args = _lib.WeightGradArgs(dy.data_ptr(), x.data_ptr(), dw.data_ptr(), None, 0, M, N, K, sy, sx, K, _dt_code(dw))
+        ws = _fit_workspace("mla_weight_grad_workspace_bytes", args, dw)  # noqa: F841  (kept until the launch)
+        _launch("mla_weight_grad", args, dw, "mla_mi355x::weight_grad")
+        return dw
+    rows = (1 << 30) // max(sy, sx) - 257
+    if rows < 32:
+        raise ValueError(f"mla_mi355x::weight_grad: rows of {N} and {K} are too wide")
+    dw = None
+    for r in range(0, M, rows):
+        part = kernels.weight_grad(dy[r:r + rows], x[r:r + rows], True)
+        dw = part if dw is None else dw.add_(part)
+    return dw.to(dtype)
 
 
 def _linear_dx(op: str, dy: Tensor, weights, shape) -> Tensor:
@@ -238,7 +256,8 @@ def _(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype):
 
 def _plain_backward(dy: Tensor) -> bool:
     """Whether a backward may run the bodies: it is not itself differentiated, batched or under a dispatch mode."""
-    return not (torch.is_grad_enabled() or kernels.batched_grad(dy) or kernels._not_plain((dy,)))
+    return not (torch.is_grad_enabled() or type(dy) is not Tensor or kernels.batched_grad(dy)
+                or torch._C._len_torch_dispatch_stack() > 0 or torch._C._functorch.peek_interpreter_stack() is not None)
 
 
 def _linear_act_grads(ctx, dy, need):
