@@ -27,7 +27,8 @@ __device__ __forceinline__ void act_both(float z, float& value, float& slope) {
     value = z * s;
     slope = s * (1.f + z * (1.f - s));
   } else if (ACT == MLA_ACT_GELU_TANH) {
-    const float z2 = z * z, s = sigmoid(kGelu2c * (z + kGeluCube * z * z2));
+    const float z2 = fminf(z * z, 1e30f);  // (the slope's 0 times an infinity would be a NaN)
+    const float s = sigmoid(kGelu2c * (z + kGeluCube * z * z2));
     value = z * s;
     slope = s + z * s * (1.f - s) * (kGelu2c * (1.f + 3.f * kGeluCube * z2));
   } else if (ACT == MLA_ACT_RELU) {
