@@ -496,16 +496,20 @@ int mla_linear_act(const mla_linear_act_args* a, void* stream);
 /* The first half of a gated feed-forward block:
  *   g[m][n] = sum_k x[m][k] W_gate[n][k],  u[m][n] = sum_k x[m][k] W_up[n][k],  h[m][n] = bf16(act(g) u)
  * both products of a tile in one pass over x.  x [M, K], weights [N, K], h [M, N] as in mla_linear_act; saved: NULL, or
- * 2 mla_linear_saved_size(M, N) bytes that receive g and u for mla_gated_linear_bwd.  activation: not MLA_ACT_NONE.
+ * 2 mla_linear_saved_size(M, N) bytes that receive g and u for mla_gated_linear_bwd.  activation: not MLA_ACT_NONE.  The
+ * workspace as mla_linear_act's.
  *
  * Replaces: silu(w1 x) * w3 x (transformer.py:117-125).
  */
 typedef struct {
   const void *x, *w_gate, *w_up;
   void *h, *saved;
+  void* workspace;
+  size_t workspace_bytes;
   int64_t M, N, K, x_stride, w_gate_stride, w_up_stride, h_stride;
   int32_t activation;
 } mla_gated_linear_args;
+size_t mla_gated_linear_workspace_bytes(const mla_gated_linear_args* a);
 int mla_gated_linear(const mla_gated_linear_args* a, void* stream);
 
 /* Its gradient through the second product: with dh[m][n] = sum_k dy[m][k] W_down[k][n] (fp32, never stored),

@@ -13,6 +13,19 @@ pytestmark = pytest.mark.gpu
 NAN = float("nan")
 
 
+# with test_gpu_feedforward's sizes: every tile of every product, whole and cut along k (tests/test_gemm_plan.py asserts it)
+TILES = [(5924, 328, 672), (5558, 176, 4744), (3338, 3808, 600)]
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_further_tiles(M, N, K):
+    for act in ("silu", "gelu_tanh"):
+        T.test_linear_act_forward(M, N, K, True, True, act)
+        T.test_gated_ffn_forward(M, N, K, True, act)
+        T.test_linear_act_gradients(M, N, K, act)
+        T.test_gated_ffn_gradients(M, N, K, act)
+
+
 def inside(t, rows=3, left=8, right=16):
     """A copy of ``t [M, N]`` as a window of a buffer of NaNs, and that buffer."""
     M, N = t.shape
@@ -30,7 +43,7 @@ def untouched(view, buf, rows=3, left=8):
     return bool(buf[out].isnan().all())
 
 
-SIZES = [(1, 24, 40), (33, 136, 72), (64, 264, 328), (65, 136, 200), (200, 264, 136), (300, 1000, 72), (4090, 328, 4072)]
+SIZES = [(1, 24, 40), (33, 136, 72), (64, 264, 328), (65, 136, 200), (200, 264, 136), (300, 1000, 72), (4090, 328, 4072), *TILES]
 
 
 @pytest.mark.parametrize("act", ["none", "silu"])
@@ -72,7 +85,7 @@ def test_what_lies_around_the_operands_is_neither_read_into_results_nor_written(
         if code:
             h = out(M, N)
             call("mla_gated_linear", _lib.GatedLinearArgs(xv.data_ptr(), wv.data_ptr(), w2v.data_ptr(), h.data_ptr(),
-                                                          saved.data_ptr(), M, N, K, xv.stride(0), wv.stride(0), w2v.stride(0),
+                                                          saved.data_ptr(), None, 0, M, N, K, xv.stride(0), wv.stride(0), w2v.stride(0),
                                                           h.stride(0), code), y)
             dgu = out(M, 2 * N)
             wd, _ = put(w.t().contiguous())

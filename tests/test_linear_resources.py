@@ -11,9 +11,9 @@ from transformer_amd import build as B
 
 BUDGETS = {
     # file: [(kernel name regex, max VGPR + AGPR per lane, kernels)]
-    "linear_act.hip": [(r"linear_act_kernel", 256, 10), (r"linear_act_finish_kernel", 512, 10),
+    "linear_act.hip": [(r"linear_act_kernel", 256, 15), (r"linear_act_finish_kernel", 256, 15),
                        (r"linear_act_rows_kernel", 256, 24)],
-    "gated_linear.hip": [(r"gated_linear_kernel", 256, 6), (r"gated_linear_bwd_kernel", 256, 3),
+    "gated_linear.hip": [(r"gated_linear_kernel", 256, 9), (r"gated_linear_finish_kernel", 256, 9), (r"gated_linear_bwd_kernel", 256, 3),
                          (r"gated_linear_rows_kernel", 256, 18)],
     "act_grad.hip": [(r"act_grad_kernel", 128, 4), (r"act_grad_sum_kernel", 128, 1)],
     "grad_norm.hip": [(r"grad_norm_kernel", 128, 2), (r"grad_scale_kernel", 128, 2)],

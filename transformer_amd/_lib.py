@@ -187,6 +187,7 @@ class LinearActArgs(ctypes.Structure):
 class GatedLinearArgs(ctypes.Structure):
     _fields_ = [
         ("x", c_void_p), ("w_gate", c_void_p), ("w_up", c_void_p), ("h", c_void_p), ("saved", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
         ("M", c_int64), ("N", c_int64), ("K", c_int64), ("x_stride", c_int64), ("w_gate_stride", c_int64),
         ("w_up_stride", c_int64), ("h_stride", c_int64), ("activation", c_int32),
     ]
@@ -261,6 +262,7 @@ SIGNATURES = {
     "mla_linear_saved_size": (c_size_t, [c_int64, c_int64]),
     "mla_linear_act_workspace_bytes": (c_size_t, [POINTER(LinearActArgs)]),
     "mla_linear_act": (c_int, [POINTER(LinearActArgs), c_void_p]),
+    "mla_gated_linear_workspace_bytes": (c_size_t, [POINTER(GatedLinearArgs)]),
     "mla_gated_linear": (c_int, [POINTER(GatedLinearArgs), c_void_p]),
     "mla_gated_linear_bwd": (c_int, [POINTER(GatedLinearBwdArgs), c_void_p]),
     "mla_linear_dx_workspace_bytes": (c_size_t, [POINTER(LinearDxArgs)]),

@@ -18,38 +18,57 @@ __device__ __forceinline__ unsigned char* gated_saved_at(const GatedParams& p, i
   return p.saved + ((int64_t)(m >> 5) * ((p.g.N + 31) >> 5) + (n >> 5)) * (2 * kSavedBlock);
 }
 
-// A tile covers T / 2 columns of both weights, a wave's first blocks the gate's and the others the same columns of the up
-// projection, so that a lane holds g and u of one output in the same registers of two blocks.
+// A tile covers TW / 2 columns of both weights, a wave's first blocks the gate's and the others the same columns of the up
+// projection, so that a lane holds g and u of one output in the same registers of two blocks.  The epilogue of the blocks
+// [j0, j1) of each wave: all of them at once, or (ALL false) one.
+template <class C, int ACT, bool ALL>
+__device__ __forceinline__ void gated_epilogue(const GatedParams& p, GemmAcc<C>& acc, int m0, int n0, unsigned char* s0,
+                                               unsigned char* s1, int j0, int j1) {
+  const WavePos<C> at;
+  const StagedRows<C, C::TN> st{s0, s1};
+  constexpr int HB = C::NB / 2;
+  const int mv = min(C::TM, p.g.M - m0), nv = min(C::TN, p.g.N - n0);
+#pragma unroll
+  for (int j = 0; j < C::XJ; ++j) {
+    if (j < j0 || j >= j1) continue;
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+      const f32x16 &g = acc.a[i][j], &u = acc.a[HB + i][j];
+      const int mb = 32 * (C::XJ * at.wm + j), nb = 32 * (at.wn * HB + i);
+      if (p.saved && mb < mv && nb < nv) {
+        unsigned char* to = gated_saved_at(p, m0 + mb, n0 + nb);
+        saved_store(to, at.lane, g);
+        saved_store(to + kSavedBlock, at.lane, u);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(g[4 * q + e]) * u[4 * q + e];
+        sts8(st.at((ALL ? mb : 32 * at.wm) + at.l32, nb / 8 + q) + 8 * at.hk,
+             u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+      }
+    }
+  }
+  __syncthreads();
+  store_rows<C>(st, at.tid, ALL ? C::TM : 32 * C::WM, p.out + (int64_t)m0 * p.os + n0, p.os, mv, nv,
+                [&](int r) { return ALL ? r : pass_row<C>(r, j0); });
+  __syncthreads();
+}
+
 template <class C, int ACT>
 __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_kernel(GatedParams p) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
-  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1, int, int) {
-    const WavePos<C> at;
-    const StagedRows<C, C::TN> st{s0, s1};
-    constexpr int HB = C::NB / 2;
-    const int mv = min(C::T, p.g.M - m0), nv = min(C::TN, p.g.N - n0);
-#pragma unroll
-    for (int j = 0; j < C::XJ; ++j)
-#pragma unroll
-      for (int i = 0; i < HB; ++i) {
-        const f32x16 &g = acc.a[i][j], &u = acc.a[HB + i][j];
-        const int mb = 32 * (C::XJ * at.wm + j), nb = 32 * (at.wn * HB + i);
-        if (p.saved && mb < mv && nb < nv) {
-          unsigned char* to = gated_saved_at(p, m0 + mb, n0 + nb);
-          saved_store(to, at.lane, g);
-          saved_store(to + kSavedBlock, at.lane, u);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(g[4 * q + e]) * u[4 * q + e];
-          sts8(st.at(mb + at.l32, nb / 8 + q) + 8 * at.hk, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
-        }
-      }
-    __syncthreads();
-    store_rows<C>(st, at.tid, C::T, p.out + (int64_t)m0 * p.os + n0, p.os, mv, nv, [](int r) { return r; });
-    __syncthreads();
+  gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1, int j0, int j1) {
+    gated_epilogue<C, ACT, true>(p, acc, m0, n0, s0, s1, j0, j1);
+  });
+}
+
+template <class C, int ACT>
+__global__ __launch_bounds__(C::THREADS, 1) void gated_linear_finish_kernel(GatedParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[C::XSLOT + C::WSLOT];
+  gemm_finish<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1, int j0, int j1) {
+    gated_epilogue<C, ACT, false>(p, acc, m0, n0, s0, s1, j0, j1);
   });
 }
 
@@ -60,8 +79,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void gated_linear_bwd_kernel(GatedPa
   __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
   gemm_tiles<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1, int, int) {
     const WavePos<C> at;
-    const StagedRows<C, C::T> st{s0, s1};
-    const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
+    const StagedRows<C, C::TW> st{s0, s1};
+    const int mv = min(C::TM, p.g.M - m0), nv = min(C::TW, p.g.N - n0);
     const int sr = 32 * at.wm + at.l32;
     bf16* out = p.out + (int64_t)m0 * p.os + n0;
     // g and u of a pass's blocks, read together and, for the second pass, under the first one's stores (a block without
@@ -150,8 +169,12 @@ static void gated_rows_go(const GatedParams& p, hipStream_t s) {
 
 template <class C, bool BWD, int ACT>
 static void gated_go(const GatedParams& p, hipStream_t s) {
-  if constexpr (BWD) gated_linear_bwd_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
-  else gated_linear_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+  if constexpr (BWD) {
+    gated_linear_bwd_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+  } else {
+    gated_linear_kernel<C, ACT><<<dim3(gemm_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+    if (p.g.S > 1) gated_linear_finish_kernel<C, ACT><<<dim3(gemm_finish_grid<C>(p.g)), dim3(C::THREADS), 0, s>>>(p);
+  }
 }
 
 template <class C, bool BWD>
@@ -169,6 +192,12 @@ static int check_gate(const char* op, int act) {
 }  // namespace mla
 
 using namespace mla;
+
+extern "C" size_t mla_gated_linear_workspace_bytes(const mla_gated_linear_args* a) {
+  // 0 for the sizes mla_gated_linear rejects
+  if (!a || check_linear_sizes("mla_gated_linear", a->M, a->N, a->K) != MLA_OK || a->M <= kRcMaxRows) return 0;
+  return (size_t)gemm_plan(a->M, 2 * a->N, a->K, 1).part_bytes;
+}
 
 extern "C" int mla_gated_linear(const mla_gated_linear_args* a, void* stream) {
   const char* op = "mla_gated_linear";
@@ -195,10 +224,11 @@ extern "C" int mla_gated_linear(const mla_gated_linear_args* a, void* stream) {
     else gated_rows_go<MLA_ACT_GELU_TANH>(p, s);
     return launch_status(op);
   }
-  const GemmPlan pl = gemm_plan(a->M, 2 * a->N, a->K, 1, false);
-  MLA_TRY(gemm_apply(op, p.g, pl, nullptr, 0, 2));
-  if (pl.large) gated_launch<GemmCfg<256, 2, 4, false, true>, false>(p, a->activation, s);
-  else gated_launch<GemmCfg<128, 2, 2, false, true>, false>(p, a->activation, s);
+  const GemmPlan pl = gemm_plan(a->M, 2 * a->N, a->K, 1);
+  MLA_TRY(gemm_apply(op, p.g, pl, a->workspace, a->workspace_bytes, 2));
+  if (pl.tile == kGemmLarge) gated_launch<GemmCfg<256, 256, 2, 4, false, true>, false>(p, a->activation, s);
+  else if (pl.tile == kGemmHalf) gated_launch<GemmCfg<256, 128, 2, 4, false, true>, false>(p, a->activation, s);
+  else gated_launch<GemmCfg<128, 128, 2, 2, false, true>, false>(p, a->activation, s);
   return launch_status(op);
 }
 
@@ -221,7 +251,7 @@ extern "C" int mla_gated_linear_bwd(const mla_gated_linear_bwd_args* a, void* st
   p.saved = (unsigned char*)const_cast<void*>(a->saved);
   p.os = a->dgu_stride;
   hipStream_t s = (hipStream_t)stream;
-  MLA_TRY(gemm_apply(op, p.g, GemmPlan{0, 1, 0, 0}, nullptr, 0));
-  gated_launch<GemmCfg<128, 2, 2, true, false>, true>(p, a->activation, s);
+  MLA_TRY(gemm_apply(op, p.g, GemmPlan{kGemmSmall, 1, 0, 0}, nullptr, 0));
+  gated_launch<GemmCfg<128, 128, 2, 2, true, false>, true>(p, a->activation, s);
   return launch_status(op);
 }

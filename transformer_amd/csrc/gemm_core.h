@@ -14,6 +14,8 @@
 // groups.  A step's products run under the reads of the next one, the last step's under the next stage's first.
 #pragma once
 
+#include <type_traits>
+
 #include "mla_common.h"
 
 namespace mla {
@@ -21,20 +23,23 @@ namespace mla {
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 
-// T x T outputs of WN x WM waves; KMAJOR: W is [k][n]; PAIR: a tile's W rows come from two weights of N columns each, T / 2
+// TM x TW outputs of WN x WM waves; KMAJOR: W is [k][n]; PAIR: a tile's W rows come from two weights of N columns each, TW / 2
 // of each, a wave's first NB / 2 blocks from w0, the rest from w1 at the same columns
-template <int T_, int WN_, int WM_, bool KMAJOR_, bool PAIR_>
+template <int TM_, int TW_, int WN_, int WM_, bool KMAJOR_, bool PAIR_>
 struct GemmCfg {
-  static constexpr int T = T_, WN = WN_, WM = WM_, BK = 64, HS = BK / 16;
+  static constexpr int TM = TM_, TW = TW_, WN = WN_, WM = WM_, BK = 64, HS = BK / 16;
   static constexpr bool KMAJOR = KMAJOR_, PAIR = PAIR_;
   static constexpr int WAVES = WN * WM, THREADS = 64 * WAVES;
-  static constexpr int NB = T / WN / 32, XJ = T / WM / 32;  // 32 x 32 blocks per wave
-  static constexpr int TN = PAIR ? T / 2 : T;               // columns of the weights that a tile covers
-  static constexpr int SLOT = T * BK * 2;                   // T rows of 64 k, or 64 k rows of T
-  static constexpr int RING = 5;
-  static constexpr int LOADS = SLOT / 1024 / WAVES;         // of a wave per slot
-  static constexpr int LDS = RING * SLOT;
-  static_assert(SLOT % (1024 * WAVES) == 0 && LDS <= 160 * 1024, "the ring fits the LDS");
+  static constexpr int NB = TW / WN / 32, XJ = TM / WM / 32;  // 32 x 32 blocks per wave
+  static constexpr int TN = PAIR ? TW / 2 : TW;               // columns of the weights that a tile covers
+  static constexpr int XSLOT = TM * BK * 2, WSLOT = TW * BK * 2;  // TM, TW rows of 64 k, or 64 k rows of TW
+  static constexpr bool FIVE = TM == TW;                      // one ring of five slots, or rings of three for x and for W
+  static constexpr int RING = FIVE ? 5 : 3;
+  static constexpr int LX = XSLOT / 1024 / WAVES, LW = WSLOT / 1024 / WAVES;  // loads of a wave per slot
+  static constexpr int LDS = FIVE ? RING * XSLOT : RING * (XSLOT + WSLOT);
+  static __device__ __forceinline__ int x_at(int slot) { return slot * XSLOT; }
+  static __device__ __forceinline__ int w_at(int slot) { return FIVE ? slot * XSLOT : RING * XSLOT + slot * WSLOT; }
+  static_assert(XSLOT % (1024 * WAVES) == 0 && WSLOT % (1024 * WAVES) == 0 && LDS <= 160 * 1024, "the ring fits the LDS");
 };
 
 // y (a tile's outputs, as an epilogue defines them) over rows m of x, columns n of W; k runs over `parts` segments of K each:
@@ -117,15 +122,19 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   // ---- loads: a cursor for x and one for W, each (tile, part, stage) with the descriptors of its tile and part, which end at
   // the last valid row; lanes past them load nothing, and the outputs that such rows reach are not stored
   const uint32_t lds0 = lds_addr(lds);
-  uint32_t xoff[C::LOADS], woff[C::LOADS];  // this lane's bytes in each of the wave's loads, at k = 0
-  bool second[C::LOADS];                    // PAIR (wave-uniform): the load is of w1's rows
+  uint32_t xoff[C::LX], woff[C::LW];  // this lane's bytes in each of the wave's loads, at k = 0
+  bool second[C::LW];                    // PAIR (wave-uniform): the load is of w1's rows
 #pragma unroll
-  for (int j = 0; j < C::LOADS; ++j) {
-    const int i = w + C::WAVES * j, row = 8 * i + (lane >> 3);
+  for (int j = 0; j < C::LX; ++j) {
+    const int row = 8 * (w + C::WAVES * j) + (lane >> 3);
     xoff[j] = (uint32_t)(row * p.xs * 2) + (uint32_t)(((lane & 7) ^ gemm_swz(row)) * 16);
+  }
+#pragma unroll
+  for (int j = 0; j < C::LW; ++j) {
+    const int i = w + C::WAVES * j, row = 8 * i + (lane >> 3);
     second[j] = false;
     if (C::KMAJOR) {
-      const int at = i * 1024 + lane * 16, kr = at / (C::T * 2), pos = (at % (C::T * 2)) >> 4;
+      const int at = i * 1024 + lane * 16, kr = at / (C::TW * 2), pos = (at % (C::TW * 2)) >> 4;
       woff[j] = (uint32_t)(kr * p.ws0 * 2) + (uint32_t)((pos ^ (4 * (kr & 3))) * 16);
     } else {
       int src = row;
@@ -161,9 +170,9 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   auto point_x = [&](const Cursor& c) {
     int mt, nt;
     gemm_tile_at(p, gemm_item(p, min(c.item, n_items - 1), n_all).tile, mt, nt);
-    const int m0 = mt * C::T;
+    const int m0 = mt * C::TM;
     rx = gemm_span(p.x + (int64_t)m0 * p.xs + (int64_t)c.part * p.K,
-                   c.item < n_items ? rows_bytes(min(C::T, p.M - m0), p.xs, p.K * 2) : 0u);
+                   c.item < n_items ? rows_bytes(min(C::TM, p.M - m0), p.xs, p.K * 2) : 0u);
   };
   auto point_w = [&](const Cursor& c) {
     int mt, nt;
@@ -184,12 +193,12 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
     if (advance(cx)) point_x(cx);
   };
   auto load_x = [&](const buf_rsrc& r, int slot, int j) {
-    dma16(r, xoff[j] + (uint32_t)(cx.st * C::BK * 2), lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
+    dma16(r, xoff[j] + (uint32_t)(cx.st * C::BK * 2), lds0 + (uint32_t)(C::x_at(slot) + (w + C::WAVES * j) * 1024));
   };
   auto issue_x = [&](int slot) {
     const buf_rsrc r = rx.rsrc();
 #pragma unroll
-    for (int j = 0; j < C::LOADS; ++j) load_x(r, slot, j);
+    for (int j = 0; j < C::LX; ++j) load_x(r, slot, j);
     done_x();
   };
   const uint32_t wstep = C::KMAJOR ? (uint32_t)(C::BK * p.ws0 * 2) : (uint32_t)(C::BK * 2);
@@ -198,12 +207,12 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   };
   auto load_w = [&](const buf_rsrc& r0, const buf_rsrc& r1, int slot, int j) {
     dma16(C::PAIR && second[j] ? r1 : r0, woff[j] + (uint32_t)cw.st * wstep,
-          lds0 + (uint32_t)(slot * C::SLOT + (w + C::WAVES * j) * 1024));
+          lds0 + (uint32_t)(C::w_at(slot) + (w + C::WAVES * j) * 1024));
   };
   auto issue_w = [&](int slot) {
     const buf_rsrc r0 = rw0.rsrc(), r1 = C::PAIR ? rw1.rsrc() : r0;
 #pragma unroll
-    for (int j = 0; j < C::LOADS; ++j) load_w(r0, r1, slot, j);
+    for (int j = 0; j < C::LW; ++j) load_w(r0, r1, slot, j);
     done_w();
   };
 
@@ -216,7 +225,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
 #pragma unroll
     for (int i = 0; i < C::NB; ++i) {
       const int b = wn * C::NB + i;
-      offw[i] = (8 * hk + r2) * (C::T * 2) + 256 * (b >> 2) + 64 * ((b & 3) ^ r2) + 32 * ((lane >> 4) & 1) + 8 * (l16 & 3);
+      offw[i] = (8 * hk + r2) * (C::TW * 2) + 256 * (b >> 2) + 64 * ((b & 3) ^ r2) + 32 * ((lane >> 4) & 1) + 8 * (l16 & 3);
     }
   }
 #pragma unroll
@@ -228,18 +237,18 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   }
   bf16x8 fx[C::HS][C::XJ], fw[2][C::NB];  // x of a stage's four steps, W of this step and the next
   auto read_x = [&](int slot, int h) {
-    const unsigned char* xt = lds + slot * C::SLOT;
+    const unsigned char* xt = lds + C::x_at(slot);
 #pragma unroll
     for (int j = 0; j < C::XJ; ++j) fx[h][j] = as_bf16x8(lds16(xt + offx[h] + j * 32 * 128));
   };
   auto read_w = [&](int slot, int h) {
-    const unsigned char* wt = lds + slot * C::SLOT;
+    const unsigned char* wt = lds + C::w_at(slot);
 #pragma unroll
     for (int i = 0; i < C::NB; ++i) {
       if (C::KMAJOR) {
-        const unsigned char* a = wt + offw[i] + 16 * h * (C::T * 2);
+        const unsigned char* a = wt + offw[i] + 16 * h * (C::TW * 2);
         const s16x4_t lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)a);
-        const s16x4_t hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(a + 4 * (C::T * 2)));
+        const s16x4_t hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(a + 4 * (C::TW * 2)));
         const u32x2 l = __builtin_bit_cast(u32x2, lo4), hh = __builtin_bit_cast(u32x2, hi4);
         fw[h & 1][i] = as_bf16x8(u32x4{l[0], l[1], hh[0], hh[1]});
       } else {
@@ -256,16 +265,16 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   };
   // A step's products with the wave's loads of one slot between them: one behind the other, the loads would wait for each other
   // in the memory pipe, and the wave's next products for them.
-  auto multiply_loading = [&](int h, auto&& load) {
+  auto multiply_loading = [&](int h, auto loads, auto&& load) {
 #pragma unroll
     for (int i = 0; i < C::NB; ++i)
 #pragma unroll
       for (int j = 0; j < C::XJ; ++j) {
-        constexpr int products = C::NB * C::XJ;
+        constexpr int products = C::NB * C::XJ, L = decltype(loads)::value;
         acc.a[i][j] = mfma32(fw[h & 1][i], fx[h][j], acc.a[i][j]);
         const int n = i * C::XJ + j;
 #pragma unroll
-        for (int l = n * C::LOADS / products; l < (n + 1) * C::LOADS / products; ++l) load(l);
+        for (int l = n * L / products; l < (n + 1) * L / products; ++l) load(l);
         __builtin_amdgcn_sched_barrier(0);
       }
   };
@@ -295,23 +304,36 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
   cw = cx;
   point_x(cx);
   point_w(cw);
-  issue_x(0);
-  issue_w(1);
-  issue_x(2);
-  issue_w(3);
-  issue_x(4);
-  gemm_wait_vmem<3 * C::LOADS>();
+  if (C::FIVE) {
+    issue_x(0);
+    issue_w(1);
+    issue_x(2);
+    issue_w(3);
+    issue_x(4);
+    gemm_wait_vmem<2 * C::LX + C::LW>();
+  } else {
+    issue_x(0);
+    issue_w(0);
+    issue_x(1);
+    issue_w(1);
+    gemm_wait_vmem<C::LX + C::LW>();
+  }
   __syncthreads();
-  int sx = 0, sw = 1;  // the slots of the stage being multiplied
+  int sx = 0, sw = C::FIVE ? 1 : 0;  // the slots of the stage being multiplied
   auto next_slots = [&]() {
-    sx = sx >= C::RING - 2 ? sx - (C::RING - 2) : sx + 2;
-    sw = sw >= C::RING - 2 ? sw - (C::RING - 2) : sw + 2;
+    if (C::FIVE) {
+      sx = sx >= C::RING - 2 ? sx - (C::RING - 2) : sx + 2;
+      sw = sw >= C::RING - 2 ? sw - (C::RING - 2) : sw + 2;
+    } else {
+      sx = sw = sx == C::RING - 1 ? 0 : sx + 1;
+    }
   };
   auto read_first = [&]() {  // what a stage's slots give before its first step's products
     read_w(sw, 0);
 #pragma unroll
     for (int h = 0; h + 1 < C::HS; ++h) read_x(sx, h);
   };
+  auto behind = [&](int s) { return s == 0 ? C::RING - 1 : s - 1; };  // rings of three: the slot of the stage after next
   read_first();
   for (int id = blockIdx.x; id < n_items; id += gridDim.x) {
     const GemmItem item = gemm_item(p, id, n_all);
@@ -327,25 +349,42 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
         read_w(sw, 1);
         multiply(0);
         interleave();
-        __syncthreads();  // every wave holds the stage's x in registers
+        if (C::FIVE) __syncthreads();  // every wave holds the stage's x in registers
         read_w(sw, 2);
         __builtin_amdgcn_sched_barrier(0);
         const buf_rsrc r0 = rw0.rsrc(), r1 = C::PAIR ? rw1.rsrc() : r0;
-        multiply_loading(1, [&](int j) { load_w(r0, r1, sx, j); });
+        const int s2 = behind(sx);
+        multiply_loading(1, std::integral_constant<int, C::LW>{}, [&](int j) { load_w(r0, r1, C::FIVE ? sx : s2, j); });
         done_w();
         read_w(sw, 3);
-        multiply(2);
-        interleave();
-        // every wave holds the stage in registers and the next one has landed: all but the one behind it
-        gemm_wait_vmem<2 * C::LOADS>();
-        __syncthreads();
-        const int s1 = sw;
-        next_slots();
-        read_first();
-        __builtin_amdgcn_sched_barrier(0);
-        const buf_rsrc r = rx.rsrc();
-        multiply_loading(3, [&](int j) { load_x(r, s1, j); });
-        done_x();
+        if (C::FIVE) {
+          multiply(2);
+          interleave();
+          // every wave holds the stage in registers and the next one has landed: all but the one behind it
+          gemm_wait_vmem<C::LX + C::LW>();
+          __syncthreads();
+          const int s1 = sw;
+          next_slots();
+          read_first();
+          __builtin_amdgcn_sched_barrier(0);
+          const buf_rsrc r = rx.rsrc();
+          multiply_loading(3, std::integral_constant<int, C::LX>{}, [&](int j) { load_x(r, s1, j); });
+          done_x();
+        } else {
+          __builtin_amdgcn_sched_barrier(0);
+          const buf_rsrc r = rx.rsrc();
+          multiply_loading(2, std::integral_constant<int, C::LX>{}, [&](int j) { load_x(r, s2, j); });
+          done_x();
+          gemm_wait_vmem<C::LX + C::LW>();
+          __syncthreads();
+          next_slots();
+          read_first();
+          multiply(3);
+        }
+      }
+      if (!C::FIVE) {
+        issue_w(behind(sx));
+        issue_x(behind(sx));
       }
       read_x(sx, C::HS - 1);
 #pragma unroll
@@ -355,7 +394,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
         multiply(h);
       }
       cut(C::HS - 1, tail);
-      gemm_wait_vmem<C::LOADS>();
+      gemm_wait_vmem<C::FIVE ? C::LX : C::LX + C::LW>();
       __syncthreads();
       const int s0 = sx, s1 = sw;
       next_slots();
@@ -366,7 +405,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
         if (id >= p.full && p.S > 1) {
           int ln = lane;
           asm volatile("" : "+v"(ln));  // (addresses formed here, not kept through the products)
-          f32x4* const dst = reinterpret_cast<f32x4*>(p.part) + (int64_t)(id - p.full) * (C::T * C::T / 4) +
+          f32x4* const dst = reinterpret_cast<f32x4*>(p.part) + (int64_t)(id - p.full) * (C::TM * C::TW / 4) +
                              w * (C::NB * C::XJ * 256) + ln;
 #pragma unroll
           for (int i = 0; i < C::NB; ++i)
@@ -380,12 +419,14 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
         } else {
           int mt, nt;
           gemm_tile_at(p, item.tile, mt, nt);
-          epi(acc, mt * C::T, nt * C::TN, lds + s0 * C::SLOT, lds + s1 * C::SLOT, 0, C::XJ);
+          epi(acc, mt * C::TM, nt * C::TN, lds + C::x_at(s0), lds + C::w_at(s1), 0, C::XJ);
         }
         gemm_wait_vmem<0>();  // (its stores share the counter that the stages' waits count down)
       }
-      issue_w(s0);
-      issue_x(s1);
+      if (C::FIVE) {
+        issue_w(s0);
+        issue_x(s1);
+      }
       read_first();
     }
   }
@@ -393,13 +434,13 @@ __device__ __forceinline__ void gemm_tiles(const GemmArgs& p, unsigned char* lds
 }
 
 // The tiles that were cut: workgroup (tile, j) adds the pieces' sums of block row j in order and runs the epilogue on it.
-// Bound by reading the pieces, once.  lds: 2 SLOT bytes.
+// Bound by reading the pieces, once.  lds: XSLOT + WSLOT bytes.
 template <class C, class Epi>
 __device__ __forceinline__ void gemm_finish(const GemmArgs& p, unsigned char* lds, Epi&& epi) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rest = p.n_mt * p.n_nt - p.full, t = blockIdx.x / C::XJ, jj = blockIdx.x % C::XJ;
-  const f32x4* src = reinterpret_cast<const f32x4*>(p.part) + (int64_t)t * (C::T * C::T / 4) + w * (C::NB * C::XJ * 256) + lane;
-  const int64_t step = (int64_t)rest * (C::T * C::T / 4);
+  const f32x4* src = reinterpret_cast<const f32x4*>(p.part) + (int64_t)t * (C::TM * C::TW / 4) + w * (C::NB * C::XJ * 256) + lane;
+  const int64_t step = (int64_t)rest * (C::TM * C::TW / 4);
   GemmAcc<C> acc;
 #pragma unroll
   for (int i = 0; i < C::NB; ++i)
@@ -423,7 +464,7 @@ __device__ __forceinline__ void gemm_finish(const GemmArgs& p, unsigned char* ld
     }
   int mt, nt;
   gemm_tile_at(p, p.full + t, mt, nt);
-  epi(acc, mt * C::T, nt * C::TN, lds, lds + C::SLOT, jj, jj + 1);
+  epi(acc, mt * C::TM, nt * C::TN, lds, lds + C::XSLOT, jj, jj + 1);
 }
 
 }  // namespace mla

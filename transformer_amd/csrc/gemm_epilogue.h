@@ -30,7 +30,7 @@ struct WavePos {
 
 template <class C, int COLS>
 struct StagedRows {
-  static constexpr int RB = COLS * 2, CH = COLS / 8, PER = C::SLOT / RB;  // bytes and chunks of a row, rows of a slot
+  static constexpr int RB = COLS * 2, CH = COLS / 8, PER = C::XSLOT / RB;  // bytes and chunks of a row, rows of the first slot
   unsigned char *s0, *s1;
   __device__ __forceinline__ unsigned char* at(int r, int chunk) const {
     unsigned char* row = r < PER ? s0 + r * RB : s1 + (r - PER) * RB;

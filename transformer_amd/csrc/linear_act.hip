@@ -23,9 +23,9 @@ template <class C, int ACT>
 __device__ __forceinline__ void linear_epilogue(const LinearParams& p, GemmAcc<C>& acc, int m0, int n0,
                                                 unsigned char* s0, unsigned char* s1, int j0, int j1) {
   const WavePos<C> at;
-  const StagedRows<C, C::T> st{s0, s1};
-  constexpr int R = 32 * C::WM, CH = C::T / 8;
-  const int mv = min(C::T, p.g.M - m0), nv = min(C::T, p.g.N - n0);
+  const StagedRows<C, C::TW> st{s0, s1};
+  constexpr int R = 32 * C::WM, CH = C::TW / 8;
+  const int mv = min(C::TM, p.g.M - m0), nv = min(C::TW, p.g.N - n0);
   const int sr = 32 * at.wm + at.l32;
 #pragma unroll
   for (int j = 0; j < C::XJ; ++j) {
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void linear_act_kernel(LinearParams 
 
 template <class C, int ACT>
 __global__ __launch_bounds__(C::THREADS, 1) void linear_act_finish_kernel(LinearParams p) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * C::SLOT];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[C::XSLOT + C::WSLOT];
   gemm_finish<C>(p.g, lds, [&](GemmAcc<C>& acc, int m0, int n0, unsigned char* s0, unsigned char* s1, int j0, int j1) {
     linear_epilogue<C, ACT>(p, acc, m0, n0, s0, s1, j0, j1);
   });
@@ -149,10 +149,11 @@ static void linear_act_launch(const LinearParams& p, int act, hipStream_t s) {
 
 template <bool KMAJOR>
 static int linear_tiles(const char* op, LinearParams& p, int act, void* workspace, size_t bytes, hipStream_t s) {
-  const GemmPlan pl = gemm_plan(p.g.M, p.g.N, p.g.K, p.g.parts, true);
+  const GemmPlan pl = gemm_plan(p.g.M, p.g.N, p.g.K, p.g.parts);
   MLA_TRY(gemm_apply(op, p.g, pl, workspace, bytes));
-  if (pl.large) linear_act_launch<GemmCfg<256, 2, 4, KMAJOR, false>>(p, act, s);
-  else linear_act_launch<GemmCfg<128, 2, 2, KMAJOR, false>>(p, act, s);
+  if (pl.tile == kGemmLarge) linear_act_launch<GemmCfg<256, 256, 2, 4, KMAJOR, false>>(p, act, s);
+  else if (pl.tile == kGemmHalf) linear_act_launch<GemmCfg<256, 128, 2, 4, KMAJOR, false>>(p, act, s);
+  else linear_act_launch<GemmCfg<128, 128, 2, 2, KMAJOR, false>>(p, act, s);
   return launch_status(op);
 }
 
@@ -201,7 +202,7 @@ extern "C" size_t mla_linear_saved_size(int64_t M, int64_t N) {
 extern "C" size_t mla_linear_act_workspace_bytes(const mla_linear_act_args* a) {
   // 0 for the sizes mla_linear_act rejects
   if (!a || check_linear_sizes("mla_linear_act", a->M, a->N, a->K) != MLA_OK || a->M <= kRcMaxRows) return 0;
-  return (size_t)gemm_plan(a->M, a->N, a->K, 1, true).part_bytes;
+  return (size_t)gemm_plan(a->M, a->N, a->K, 1).part_bytes;
 }
 
 extern "C" int mla_linear_act(const mla_linear_act_args* a, void* stream) {
@@ -230,7 +231,7 @@ extern "C" int mla_linear_act(const mla_linear_act_args* a, void* stream) {
 extern "C" size_t mla_linear_dx_workspace_bytes(const mla_linear_dx_args* a) {
   // 0 for the sizes mla_linear_dx rejects
   if (!a || check_linear_sizes("mla_linear_dx", a->M, a->N, a->K) != MLA_OK) return 0;
-  return (size_t)gemm_plan(a->M, a->K, a->N, a->w1 ? 2 : 1, true).part_bytes;
+  return (size_t)gemm_plan(a->M, a->K, a->N, a->w1 ? 2 : 1).part_bytes;
 }
 
 extern "C" int mla_linear_dx(const mla_linear_dx_args* a, void* stream) {

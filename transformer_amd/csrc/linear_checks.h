@@ -39,11 +39,11 @@ inline int check_weight_reach(const char* op, const char* name, int64_t rows, in
 // The plan's tiles and pieces; `cols` tile columns of an output column (2 for a pair of weights).  Without a workspace that
 // is large enough a plan that cuts tiles is refused.
 inline int gemm_apply(const char* op, GemmArgs& g, const GemmPlan& pl, void* workspace, size_t bytes, int cols = 1) {
-  const int T = pl.large ? 256 : 128;
-  g.n_mt = (g.M + T - 1) / T;
-  g.n_nt = (int)(((int64_t)g.N * cols + T - 1) / T);
+  const GemmTile t = kGemmTiles[pl.tile];
+  g.n_mt = (int)((g.M + t.m - 1) / t.m);
+  g.n_nt = (int)(((int64_t)g.N * cols + t.n - 1) / t.n);
   g.gm = 8;
-  const int tiles = g.n_mt * g.n_nt, slots = pl.large ? 256 : 512;
+  const int tiles = g.n_mt * g.n_nt, slots = (int)t.slots;
   g.S = pl.S;
   g.per = pl.per;
   g.full = pl.S > 1 ? tiles / slots * slots : tiles;

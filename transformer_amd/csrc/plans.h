@@ -123,39 +123,48 @@ inline WgPlan wg_plan(int64_t M, int64_t N, int64_t K) {
 }
 
 // ---- linear_act.hip's and gated_linear.hip's tiles (gemm_core.h)
+enum { kGemmSmall = 0, kGemmHalf = 1, kGemmLarge = 2 };
+struct GemmTile {
+  int64_t m, n, slots;  // outputs, and how many run at once: one workgroup a CU, or two
+  // us of a stage of 64 k with every slot taken, and of a tile's start and stores; of a stage of a round of r <= 256 workgroups,
+  // one a CU: alone + share r / 256
+  double stage, fixed, alone, share;
+};
+constexpr GemmTile kGemmTiles[3] = {
+    {128, 128, 512, 1.05, 0.0, 0.40, 0.16}, {256, 128, 256, 1.04, 1.2, 0.63, 0.28}, {256, 256, 256, 1.57, 7.0, 0.99, 0.41}};
+
 struct GemmPlan {
-  int large;   // tiles of 256 x 256, one workgroup a CU; else 128 x 128, two
+  int tile;    // of kGemmTiles
   int S, per;  // the tiles of an unfilled last round are cut along k into S pieces of `per` stages (1: not cut)
   int64_t part_bytes;
 };
 
-// The plan of least estimated time (us) for y [M, N] over parts x K, `cut` where tiles may be cut along k.  A round of
-// workgroups takes its stages at a measured time plus what a tile's start and stores take:
-//   large tiles 1.3 us a stage (144 stages of 256 tiles 190 us: the rate that power allows) and 12; small ones, two on a CU, 0.85
-//   (12288 x 9216 over 28 stages: 13.5 rounds in 406 us, the loads' rate) and 6, up to 256 of them, alone on theirs, 0.45 + 0.25
-//   of the CUs in use (2500 x 1000: 160 tiles x 28 stages 19 us; 1999 x 2048: 256 x 72 56 us) and 5.
-// Pieces add the fp32 sums they leave, written and read at 1.5 TB/s together (63 MB took 46 us more), and a
-// second kernel.
-inline GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int64_t parts, bool cut) {
+// The plan of least estimated time (us) for y [M, N] over parts x K: full rounds, the last one, and for pieces their fp32 sums
+// (written and read at 6 TB/s together) and the kernel that adds them.  The constants are fitted to 1000 timings of 100 products
+// (M 65 to 16000; N and K 256 to 5600; every tile, S to 8; inputs of three calls in turn), which they meet within 9 % (rms).  Over
+// the products the rule's choice takes 0.5 % more than the fastest one on average and 12 % at most; without pieces it would take
+// 17 % more, without the tiles of 256 x 128 2 %, without those of 128 x 128 9 %.  Examples (us; 128 x 128, 256 x 128, 256 x 256):
+// 1999 x 2048 over 4608 50, 61, 97; 3001 x 2048 over 5464 101, 85, 114 (95 in two pieces); 12288 x 9216 over 1792 430, 426, 365;
+// 12288 x 1792 over 2 x 4608 430, 403, 413 (348 in three pieces); 159 x 6080 over 5176 47, 62, 98 (31 in four pieces of 128 x 128).
+inline GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int64_t parts) {
   GemmPlan best{};
   double best_t = 1e300;
   const int64_t n = (K + 63) / 64 * parts;
-  for (int large = 1; large >= 0; --large) {
-    const int64_t T = large ? 256 : 128, slots = large ? 256 : 512;
-    const double stage = large ? 1.3 : 0.85, fixed = large ? 12.0 : 6.0;
-    const int64_t tiles = ((M + T - 1) / T) * ((N + T - 1) / T), rest = tiles % slots;
-    for (int64_t S = 1; S <= 16; ++S) {
-      if (S > 1 && (!cut || S * 2 > n || rest == 0 || rest * S > slots)) break;
+  for (int tile = kGemmLarge; tile >= kGemmSmall; --tile) {
+    const GemmTile& T = kGemmTiles[tile];
+    const int64_t tiles = ((M + T.m - 1) / T.m) * ((N + T.n - 1) / T.n), rest = tiles % T.slots;
+    for (int64_t S = 1; S <= 8; ++S) {
+      if (S > 1 && (S * 2 > n || rest == 0 || rest * S > T.slots)) break;
       const int64_t per = (n + S - 1) / S, items = rest * S;
       if ((n + per - 1) / per != S) continue;  // fewer pieces hold the same stages
-      double t = (double)(tiles / slots) * ((double)n * stage + fixed);
-      if (items > 0 && !large && items <= 256) t += (double)per * (0.45 + 0.25 * (double)items / 256) + 5.0;
-      else if (items > 0) t += (double)per * stage + fixed;
-      const int64_t pb = S > 1 ? items * T * T * 4 : 0;
-      if (S > 1) t += 5.0 + (double)pb / 1.5e6;
+      double t = (double)(tiles / T.slots) * ((double)n * T.stage + T.fixed);
+      if (items > 256) t += (double)per * T.stage + T.fixed;
+      else if (items > 0) t += (double)per * (T.alone + T.share * (double)items / 256) + T.fixed;
+      const int64_t pb = S > 1 ? items * T.m * T.n * 4 : 0;
+      if (S > 1) t += 3.0 + 0.6 * (double)S + (double)pb / 6e6;
       if (t < best_t) {
         best_t = t;
-        best = GemmPlan{large, (int)S, (int)per, pb};
+        best = GemmPlan{tile, (int)S, (int)per, pb};
       }
     }
   }

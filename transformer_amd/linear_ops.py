@@ -17,7 +17,7 @@ from ._lib import ACTIVATIONS
 from .kernels import _alloc_workspace, _dt_code, _op, _register_autograd
 
 LINEAR_MAX_STRIDE = 1 << 22
-ROWS_MAX = 64  # rows up to which mla_linear_act needs no workspace
+ROWS_MAX = 64  # rows up to which mla_linear_act and mla_gated_linear need no workspace
 _BF16, _F32 = torch.bfloat16, torch.float32
 _byref, _current_device, _raw_stream = ctypes.byref, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
@@ -340,8 +340,9 @@ def _gated_ffn(x, w_gate, w_up, w_down, residual, activation, save):
     if M:
         wg, wu = _weight_bf16(w_gate), _weight_bf16(w_up)
         args = _lib.GatedLinearArgs(
-            x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), None if saved is None else saved.data_ptr(), M, H, D,
-            _row_stride(x2), _row_stride(wg), _row_stride(wu), H, code)
+            x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), None if saved is None else saved.data_ptr(), None, 0,
+            M, H, D, _row_stride(x2), _row_stride(wg), _row_stride(wu), H, code)
+        ws = _fit_workspace("mla_gated_linear_workspace_bytes", args, h) if M > ROWS_MAX else None  # noqa: F841
         _launch("mla_gated_linear", args, h, op)
         _linear_run(op, h, _weight_bf16(w_down), None, None if residual is None else _matrix(residual, D, True), 0, None, y, M)
     return y, h, saved
