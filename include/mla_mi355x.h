@@ -546,7 +546,8 @@ int mla_linear_dx(const mla_linear_dx_args* a, void* stream);
 
 /* The epilogue's gradient: dz[m][n] = bf16(dy[m][n] act'(z[m][n])) with z as mla_linear_act saved it, and
  * db[n] = sum_m dy act'(z) in fp32, rounded once to db_dtype.  MLA_ACT_NONE: dz = dy is not written and saved not read.
- * db may be NULL, dz too for MLA_ACT_NONE.  dy, dz [M, N] bf16 rows.  The sums run in a fixed order through the workspace.
+ * db may be NULL, dz too for MLA_ACT_NONE.  dy, dz [M, N] bf16 rows.  The sums run in a fixed order, through the workspace where
+ * mla_act_grad_workspace_bytes is not 0 (16-byte aligned).
  *
  * Replaces: autograd of a layer's bias and activation.
  */

@@ -33,7 +33,7 @@ BAD = {
     "mla_linear_dx": (dict(K=0), dict(dy=None), dict(w0=None), dict(w1=8200), dict(dx=8), dict(dy_stride=16),
                       dict(w1_stride=16), dict(w1_stride=32), dict(dx_stride=16), dict(N=1 << 19, dy_stride=1 << 20, w0_stride=1 << 12)),
     "mla_act_grad": (dict(M=0), dict(dy=None), dict(dz=None), dict(saved=None), dict(saved=8), dict(dy_stride=8), dict(dz_stride=8),
-                     dict(db_dtype=3), dict(db=16386), dict(workspace_bytes=0), dict(activation=7)),
+                     dict(db_dtype=3), dict(db=16386), dict(M=200, workspace_bytes=0), dict(activation=7)),
 }
 
 

@@ -3,7 +3,8 @@
 //
 // A wave owns 32 columns and walks 32-row blocks, a lane one row's four quads of a block, as z was kept (act.h).  A lane
 // adds its rows' gradients in fp32; at the end the 32 lanes of a column are added and the segment's sum stored.  A second
-// kernel adds the segments in order: no atomics, results repeat bit for bit.
+// kernel adds the segments in order: no atomics, results repeat bit for bit.  Up to 128 rows are one segment, whose sums are db
+// (four blocks in a row take less than a second launch).  12288 x 4608 with db: 79 us, 5.0 TB/s, and 5 us for the segments.
 #include <algorithm>
 
 #include "act.h"
@@ -15,12 +16,17 @@ struct ActGradParams {
   const bf16* dy;
   const unsigned char* saved;
   bf16* dz;
-  float* part;  // [segments][N], or null
+  float* part;  // [segments][N]; null for one segment
   void* db;
   int M, N, seg;  // 32-row blocks of a segment
   int n_seg, db_f32;
   int64_t dys, dzs;
 };
+
+__device__ __forceinline__ void act_grad_store(const ActGradParams& p, int n, float v) {
+  if (p.db_f32) ((float*)p.db)[n] = v;
+  else ((bf16*)p.db)[n] = (bf16)v;
+}
 
 constexpr int kAgCols = 128;  // columns of a workgroup, 32 a wave
 
@@ -86,7 +92,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p) {
       }
     }
   }
-  if (!p.part || !live) return;
+  if (!p.db || !live) return;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
 #pragma unroll
@@ -96,8 +102,14 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int n = wn + 8 * q + 4 * hk;
-      if (n < p.N) stg16(p.part + (int64_t)blockIdx.y * p.N + n,
-                         __builtin_bit_cast(u32x4, f32x4{sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]}));
+      if (n >= p.N) continue;
+      const f32x4 v{sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]};
+      if (p.part) {
+        stg16(p.part + (int64_t)blockIdx.y * p.N + n, __builtin_bit_cast(u32x4, v));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) act_grad_store(p, n + e, v[e]);
+      }
     }
   }
 }
@@ -113,14 +125,13 @@ __global__ __launch_bounds__(64) void act_grad_sum_kernel(ActGradParams p) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) sum += s0 + e < p.n_seg ? v[e] : 0.f;
   }
-  if (p.db_f32) ((float*)p.db)[n] = sum;
-  else ((bf16*)p.db)[n] = (bf16)sum;
+  act_grad_store(p, n, sum);
 }
 
-// segments of rows so that some 2048 workgroups of four waves share the pass
+// segments of rows so that some 2048 workgroups of four waves share the pass; up to four blocks are one
 static void act_grad_segments(int64_t M, int64_t N, int& seg, int& n_seg) {
   const int64_t blocks = (M + 31) / 32, strips = (N + kAgCols - 1) / kAgCols;
-  const int64_t want = std::min(blocks, std::max<int64_t>(1, 2048 / strips));
+  const int64_t want = blocks <= 4 ? 1 : std::min(blocks, std::max<int64_t>(1, 2048 / strips));
   seg = (int)((blocks + want - 1) / want);
   n_seg = (int)((blocks + seg - 1) / seg);
 }
@@ -133,7 +144,7 @@ extern "C" size_t mla_act_grad_workspace_bytes(const mla_act_grad_args* a) {
   if (!a || a->M <= 0 || a->N <= 0 || a->M >= kLinearMaxM || a->N >= kLinearMaxN || !a->db) return 0;
   int seg, n_seg;
   act_grad_segments(a->M, a->N, seg, n_seg);
-  return (size_t)n_seg * (size_t)a->N * 4;
+  return n_seg == 1 ? 0 : (size_t)n_seg * (size_t)a->N * 4;
 }
 
 extern "C" int mla_act_grad(const mla_act_grad_args* a, void* stream) {
@@ -153,13 +164,14 @@ extern "C" int mla_act_grad(const mla_act_grad_args* a, void* stream) {
     MLA_CHECK(a->db_dtype == MLA_DTYPE_F32 || a->db_dtype == MLA_DTYPE_BF16, MLA_ERR_UNSUPPORTED, "%s: db dtype", op);
     MLA_CHECK(((uintptr_t)a->db & 3) == 0, MLA_ERR_INVALID_ARG, "%s: db must be 4-byte aligned", op);
     const size_t need = mla_act_grad_workspace_bytes(a);
-    MLA_CHECK(a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace & 15) == 0, MLA_ERR_WORKSPACE,
+    MLA_CHECK(need == 0 || (a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace & 15) == 0), MLA_ERR_WORKSPACE,
               "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", op, need, a->workspace_bytes);
   }
   if (!act && !a->db) return MLA_OK;
-  ActGradParams p{(const bf16*)a->dy, (const unsigned char*)a->saved, (bf16*)a->dz, a->db ? (float*)a->workspace : nullptr, a->db,
+  ActGradParams p{(const bf16*)a->dy, (const unsigned char*)a->saved, (bf16*)a->dz, nullptr, a->db,
                   (int)a->M, (int)a->N, 0, 0, a->db_dtype == MLA_DTYPE_F32, a->dy_stride, a->dz_stride};
   act_grad_segments(a->M, a->N, p.seg, p.n_seg);
+  if (a->db && p.n_seg > 1) p.part = (float*)a->workspace;
   const dim3 grid((unsigned)((a->N + kAgCols - 1) / kAgCols), (unsigned)p.n_seg);
   hipStream_t s = (hipStream_t)stream;
   if (a->activation == MLA_ACT_RELU) act_grad_kernel<MLA_ACT_RELU><<<grid, 256, 0, s>>>(p);
@@ -167,7 +179,7 @@ extern "C" int mla_act_grad(const mla_act_grad_args* a, void* stream) {
   else if (a->activation == MLA_ACT_GELU_TANH) act_grad_kernel<MLA_ACT_GELU_TANH><<<grid, 256, 0, s>>>(p);
   else act_grad_kernel<MLA_ACT_NONE><<<grid, 256, 0, s>>>(p);
   MLA_TRY(launch_status(op));
-  if (a->db) {
+  if (p.part) {
     act_grad_sum_kernel<<<dim3((unsigned)((a->N + 63) / 64)), 64, 0, s>>>(p);
     MLA_TRY(launch_status(op));
   }
