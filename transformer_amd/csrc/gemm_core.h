@@ -1,17 +1,29 @@
-// The tile product that the linear layers' kernels share (linear_act.hip): C^T [n][m] = W . x^T over k, bf16 operands, fp32
-// sums, on v_mfma_f32_32x32x16_bf16.  x [M][K] has k contiguous; W either has too (rows of a layer's weight: y = x W^T) or has
-// n contiguous (the same weight read from its other side: dx = dy W), in which case its fragments come by transpose reads.
+// The tile product that the linear layers' kernels share (linear_act.hip, gated_linear.hip): C^T [n][m] = W . x^T over k, bf16
+// operands, fp32 sums, on v_mfma_f32_32x32x16_bf16.  x [M][K] has k contiguous; W either has too (rows of a layer's weight:
+// y = x W^T) or has n contiguous (the same weight read from its other side: dx = dy W), in which case its fragments come by
+// transpose reads.
 //
-// A workgroup of WN x WM waves computes tiles of T x T outputs, one after the other, k in stages of 64.  A stage is two
-// slots of T rows x 64 k, x's and W's, in a ring of five that direct-to-LDS loads fill: when the first step of a stage has
-// read the rest of its x, that slot takes W of the stage after next, and W's, read at the end, x of the one behind it.  The
-// loads run on across the end of a tile, so that the next tile's first stage lands under this tile's last products and its
-// epilogue, which has the two slots last read for its own use.  Loads past the last tile have empty descriptors.
+// A workgroup of WN x WM waves computes tiles of TM x TW outputs, one after the other, k in stages of 64.  A stage is a slot of
+// x's TM rows x 64 k and one of W's TW, filled by direct-to-LDS loads.  Square tiles use one ring of five slots (three stages of
+// 256 x 256 do not fit the LDS): when the first step of a stage has read the rest of its x, that slot takes W of the stage after
+// next, and W's, read at the end, x of the one behind it.  Tiles of 256 x 128 use a ring of three for each, filled two stages
+// ahead with one barrier a stage.  The loads run on across the end of a tile, so that the next tile's first stage lands under
+// this tile's last products and its epilogue, which has the two slots last read for its own use.  Loads past the last tile have
+// empty descriptors.
 //
 // A staged row of 64 k (128 bytes: pieces of 64 bytes reach half the rate, 60 against 95-130 bytes/ns per CU measured) holds
-// its chunk c of 16 bytes at c ^ ((row / 2) mod 8), so that 16 rows x one chunk are free of bank conflicts; a staged k row of T n
-// holds chunk c at c ^ 4 (row mod 4), so that the four rows of a half-wave's transpose read fall on four different 64-byte bank
+// its chunk c of 16 bytes at c ^ ((row / 2) mod 8), so that 16 rows x one chunk are free of bank conflicts; a staged k row of TW
+// n holds chunk c at c ^ 4 (row mod 4), so that the four rows of a half-wave's transpose read fall on four different 64-byte bank
 // groups.  A step's products run under the reads of the next one, the last step's under the next stage's first.
+//
+// What bounds it: a stage of 256 x 256 takes 0.86 us of matrix instructions, 0.96 with its LDS reads, and with random operands on
+// all 256 CUs 1.31 us (1640 TFLOP/s: the clock that power allows), 1.4 to 1.6 us as loads come from beyond the L2.  Smaller
+// tiles read more LDS and load more for their products: 1.05 us a stage for two workgroups of 128 x 128 on a CU, 1.04 for one of
+// 256 x 128 (half the outputs of 1.57); they win where the large ones leave CUs idle (gemm_plan in plans.h).  Operands that lie
+// in HBM and not in the last-level cache add 10 to 40 us where a product has one round of tiles (3001 x 2048 over 5464: 88 and
+// 129 us).  Whole products, 12288 rows, in a training pass: 4608 -> 1792 194 us (1050 TFLOP/s), 2 x 4608 <- 1792 361 us (1120).
+// Measured and not kept: nine slots for a tile of 128 x 128 with eight waves (50 against 56 us at 1999 x 2048 over 4608, slower
+// at larger sizes), waves of their own for loads and for stores (2 %), stores past the caches for y (1 %).
 #pragma once
 
 #include <type_traits>
