@@ -298,3 +298,68 @@ def test_two_captured_graphs_replayed_together():
             for t in out:
                 t.fill_(NAN)
         torch.cuda.synchronize()
+
+
+def test_compiled_with_any_number_of_rows():
+    from transformer_amd import gated_ffn, linear_act
+    g = T.gen("dynamic")
+    w = [T.bf16(g, 136, 72, std=0.1), T.bf16(g, 136, 72, std=0.1), T.bf16(g, 72, 136, std=0.1), T.bf16(g, 72)]
+
+    def f(x, wg, wu, wd, b):
+        return linear_act(gated_ffn(x, wg, wu, wd, x), wd[:, :72], b, None, "gelu_tanh")
+
+    compiled = torch.compile(f, backend="aot_eager", dynamic=True, fullgraph=True)
+    for M in (50, 51, 7, 200):
+        leaves = [t.requires_grad_() for t in (T.bf16(g, M, 72), *(t.clone() for t in w))]
+        dy = T.bf16(g, M, 72)
+        got, want = compiled(*leaves), f(*leaves)
+        assert torch.equal(got, want)
+        assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(got, leaves, dy), torch.autograd.grad(want, leaves, dy)))
+
+
+def test_registered_operators_hold_their_contract():
+    """Schemas, fake kernels and autograd registration; without what the backward keeps, the operator forms it again."""
+    from torch.library import opcheck
+    ops = torch.ops.mla_mi355x
+    g = T.gen("contract")
+    x, wg, wu, wd, r, b = leaves_of(g)
+    dy, dz = T.bf16(g, 40, 136), T.bf16(g, 40, 72)
+    every = ("test_schema", "test_faketensor", "test_autograd_registration")
+    for save in (False, True):
+        opcheck(ops.gated_ffn, (x, wg, wu, wd, r, "silu", save), test_utils=every)
+        opcheck(ops.linear_act, (x, wg, b, None, "silu", save), test_utils=every)
+        opcheck(ops.linear_act, (x, wg, None, None, "none", save), test_utils=every)
+    _, h, saved = ops.gated_ffn(x, wg, wu, wd, None, "silu", True)
+    opcheck(ops.gated_ffn_bwd, (dy, *(t.detach() for t in (x, wg, wu, wd, h)), saved, "silu", True, True, False, True),
+            test_utils=every[:2])
+    saved = ops.linear_act(x, wg, b, None, "silu", True)[1]
+    opcheck(ops.linear_act_bwd, (dz, x.detach(), wg.detach(), saved, "silu", True, True, torch.float32), test_utils=every[:2])
+    for f, of, d in ((lambda save: ops.gated_ffn(x, wg, wu, wd, r, "silu", save)[0], (x, wg, wu, wd, r), dy),
+                     (lambda save: ops.linear_act(x, wg, b, None, "silu", save)[0], (x, wg, b), dz)):
+        kept, formed = (torch.autograd.grad(f(save), of, d) for save in (True, False))
+        assert all(torch.equal(a, c) for a, c in zip(kept, formed))
+
+
+def test_gradients_that_are_views_of_one_buffer_are_used_like_any_other():
+    """The two first weights' gradients share an allocation: accumulated, changed in place, clipped and stepped apart."""
+    from transformer_amd import SwiGLU, clip_grad_norm_
+    torch.manual_seed(5)
+    m = SwiGLU(136, 264).cuda().bfloat16()
+    x = T.bf16(T.gen("views"), 40, 136)
+    m(x, x).float().square().mean().backward()
+    once = [p.grad.clone() for p in m.parameters()]
+    m(x, x).float().square().mean().backward()
+    assert all(torch.equal(p.grad, 2 * q) for p, q in zip(m.parameters(), once))  # (twice a bf16 value is one)
+    m.w1.weight.grad.zero_()
+    assert torch.equal(m.w3.weight.grad, 2 * once[2]) and not m.w1.weight.grad.any()
+    norm = clip_grad_norm_(m.parameters(), 1e-3)
+    left = torch.stack([p.grad.double().square().sum() for p in m.parameters()]).sum().sqrt()
+    assert norm > 1e-3 and abs(float(left) - 1e-3) <= 1e-3 * (T.EPS16 + 1e-5)  # (a rounding to bf16 an element)
+    torch.optim.SGD(m.parameters(), lr=0.1).step()
+
+
+def test_gradients_without_elements():
+    from transformer_amd import clip_grad_norm_, grad_norm
+    p = torch.nn.Parameter(torch.zeros(0, 4, device="cuda"))
+    p.grad = torch.zeros(0, 4, device="cuda")
+    assert float(clip_grad_norm_([p], 1.0)) == 0 and float(grad_norm([p.grad], float("inf"))) == 0

@@ -21,9 +21,12 @@
 // tiles read more LDS and load more for their products: 1.05 us a stage for two workgroups of 128 x 128 on a CU, 1.04 for one of
 // 256 x 128 (half the outputs of 1.57); they win where the large ones leave CUs idle (gemm_plan in plans.h).  Operands that lie
 // in HBM and not in the last-level cache add 10 to 40 us where a product has one round of tiles (3001 x 2048 over 5464: 88 and
-// 129 us).  Whole products, 12288 rows, in a training pass: 4608 -> 1792 194 us (1050 TFLOP/s), 2 x 4608 <- 1792 361 us (1120).
+// 129 us).  Whole products, 12288 rows, in a training pass: 4608 -> 1792 194 us (1050 TFLOP/s), 2 x 4608 <- 1792 361 us (1120);
+// 8192 cubed 840 us (1310; the library 775).
 // Measured and not kept: nine slots for a tile of 128 x 128 with eight waves (50 against 56 us at 1999 x 2048 over 4608, slower
-// at larger sizes), waves of their own for loads and for stores (2 %), stores past the caches for y (1 %).
+// at larger sizes), one such tile a CU with whole stages read ahead into a second set of registers over rings of five stages
+// (53 against 50: its LDS traffic, 64 KiB read and 32 written a stage, bounds it), four waves of 128 x 128 for the large tile (they
+// spill; 907 against 840 at 8192 cubed), waves of their own for loads and for stores (2 %), stores past the caches for y (1 %).
 #pragma once
 
 #include <type_traits>
