@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import math
 from array import array
-from typing import Iterable, List, Union
+from typing import Iterable, List, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -61,26 +61,28 @@ def _refuse(op: str, tensors: List[Tensor]) -> None:
     raise ValueError(f"{op}: gradients on {sorted({str(t.device) for t in tensors})}: one device is needed")
 
 
-def _laid_out(op: str, tensors: List[Tensor]) -> List[Tensor]:
-    """``tensors`` without gaps in memory: those with gaps copied.  (Few look-ups a tensor: they are the host's cost.)"""
+def _laid_out(op: str, tensors: List[Tensor]) -> Tuple[List[Tensor], array]:
+    """``tensors`` without gaps in memory (those with gaps copied) and their types.  (Few look-ups a tensor: they are the host's
+    cost.)"""
     try:
         devices, whole = {t.get_device() for t in tensors}, [t.is_contiguous() for t in tensors]
-    except RuntimeError:  # (sparse)
+        codes = array("i", [_CODES[t.dtype] for t in tensors])
+    except (RuntimeError, KeyError):  # (of a compressed sparse tensor is_contiguous raises)
         _refuse(op, tensors)
-    if len(devices) != 1 or -1 in devices or not _CODES.keys() >= {t.dtype for t in tensors} \
-            or not all(t.layout == torch.strided for t in tensors):
+    if len(devices) != 1 or -1 in devices:
         _refuse(op, tensors)
-    if all(whole):
-        return tensors
-    return [t if w or _dense(t) else t.detach().contiguous() for t, w in zip(tensors, whole)]
+    if not all(whole):
+        if not all(t.layout == torch.strided for t in tensors):
+            _refuse(op, tensors)
+        tensors = [t if w or _dense(t) else t.detach().contiguous() for t, w in zip(tensors, whole)]
+    return tensors, codes
 
 
-def _run(op: str, entry: str, tensors: List[Tensor], is_max: bool, max_norm: float) -> Tensor:
+def _run(op: str, entry: str, tensors: List[Tensor], codes: array, is_max: bool, max_norm: float) -> Tensor:
     n, like = len(tensors), tensors[0]
     norm = torch.empty((), dtype=torch.float32, device=like.device)
     # host tables, read before the entry point returns
     ptrs, numels = array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors])
-    codes = array("i", [_CODES[t.dtype] for t in tensors])
     args = _lib.GradNormArgs(ptrs.buffer_info()[0], numels.buffer_info()[0], codes.buffer_info()[0], n, norm.data_ptr(), None, 0,
                              max_norm, int(is_max))
     ws = _fit_workspace("mla_grad_norm_workspace_bytes", args, like)  # noqa: F841  (kept until the launch)
@@ -95,7 +97,7 @@ def grad_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) 
     is_max = _is_max("grad_norm", norm_type)
     if not tensors:
         return torch.tensor(0.0)
-    return _run("grad_norm", "mla_grad_norm", _laid_out("grad_norm", tensors), is_max, 0.0)
+    return _run("grad_norm", "mla_grad_norm", *_laid_out("grad_norm", tensors), is_max, 0.0)
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -113,17 +115,17 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    flat = _laid_out(op, grads)
+    flat, codes = _laid_out(op, grads)
     if flat is not grads:
         for g in grads:
             if _shares(g):
                 raise ValueError(f"{op}: a gradient with strides {g.stride()} shares memory between its elements")
     if error_if_nonfinite:
-        norm = _run(op, "mla_grad_norm", flat, is_max, 0.0)
+        norm = _run(op, "mla_grad_norm", flat, codes, is_max, 0.0)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it "
                                "cannot be clipped.")
-    norm = _run(op, "mla_grad_clip", flat, is_max, max_norm)
+    norm = _run(op, "mla_grad_clip", flat, codes, is_max, max_norm)
     if flat is not grads:
         with torch.no_grad():
             for g, c in zip(grads, flat):

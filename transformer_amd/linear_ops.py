@@ -46,27 +46,25 @@ def _fit_workspace(entry: str, args, like: Tensor) -> Optional[Tensor]:
     return ws
 
 
-def _matrix(t: Tensor, K: int, one_row: bool = False) -> Tensor:
-    """``t [..., K]`` as rows the linear kernels take: unit inner stride, 16-byte aligned, a row stride that is a multiple of
-    8 and covers a row (``one_row``: or 0, the same row for all); copied where its layout is another."""
+def _rows(t: Tensor, K: int, one_row: bool = False) -> Tuple[Tensor, int]:
+    """``t [..., K]`` as rows the linear kernels take, and their stride: unit inner stride, 16-byte aligned, a row stride that is
+    a multiple of 8 and covers a row (``one_row``: or 0, the same row for all); copied where its layout is another."""
     if t.dim() != 2:
         t = t.reshape(-1, K)
     if t.data_ptr() % 16 == 0:
         if t.is_contiguous():
-            return t
-        if t.stride(1) == 1:
-            s = t.stride(0)
-            if t.size(0) <= 1 or (s % 8 == 0 and s < LINEAR_MAX_STRIDE and (s >= K or (one_row and s == 0))):
-                return t
-    return t.clone(memory_format=torch.contiguous_format)
+            return t, K
+        s, inner = t.stride()
+        if inner == 1:
+            if t.size(0) <= 1:
+                return t, K
+            if s % 8 == 0 and s < LINEAR_MAX_STRIDE and (s >= K or (one_row and s == 0)):
+                return t, s
+    return t.clone(memory_format=torch.contiguous_format), K
 
 
-def _row_stride(t: Tensor) -> int:
-    return t.stride(0) if t.size(0) > 1 else t.size(1)
-
-
-def _weight_bf16(w: Tensor) -> Tensor:
-    return _matrix(w if w.dtype == _BF16 else w.to(_BF16), w.size(1))
+def _weight_rows(w: Tensor, K: int) -> Tuple[Tensor, int]:  # (and a gradient's)
+    return _rows(w if w.dtype == _BF16 else w.to(_BF16), K)
 
 
 def _activation(op: str, name: str, gate: bool = False) -> int:
@@ -116,13 +114,13 @@ def _saved_size(M: int, N: int) -> int:
     return 3072 * ((M + 31) // 32) * ((N + 31) // 32)  # mla_linear_saved_size
 
 
-def _linear_run(op, x2, w, bias, res2, code, saved, y, M):
-    """``y = act(x2 w^T + bias) + res2`` on bf16 matrices as :func:`_matrix` leaves them."""
-    N, K = w.shape
+def _linear_run(op, x2, x_stride, weight, bias, residual, code, saved, y, M, N, K):
+    """``y = act(x2 weight^T + bias) + residual`` on bf16 rows as :func:`_rows` leaves them."""
+    w, w_stride = _weight_rows(weight, K)
+    res2, r_stride = (None, 0) if residual is None else _rows(residual, N, True)
     args = _lib.LinearActArgs(
         x2.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(), None if res2 is None else res2.data_ptr(),
-        y.data_ptr(), None if saved is None else saved.data_ptr(), None, 0, M, N, K, _row_stride(x2), _row_stride(w),
-        0 if res2 is None else _row_stride(res2), N, code)
+        y.data_ptr(), None if saved is None else saved.data_ptr(), None, 0, M, N, K, x_stride, w_stride, r_stride, N, code)
     ws = _fit_workspace("mla_linear_act_workspace_bytes", args, y) if M > ROWS_MAX else None  # noqa: F841  (kept until the launch)
     _launch("mla_linear_act", args, y, op)
 
@@ -139,17 +137,17 @@ def _linear_act(x, weight, bias, residual, activation, save):
                          f"{None if bias is None else tuple(bias.shape)}")
     N, K = weight.shape
     _check(op, x, (weight, bias), ("weight", "bias"), residual, N)
-    x2 = _matrix(x, K)
+    x2, x_stride = _rows(x, K)
     M = x2.size(0)
-    y = torch.empty((*x.shape[:-1], N), dtype=_BF16, device=x.device)
-    saved = torch.empty(_saved_size(M, N), dtype=torch.uint8, device=x.device) if save and code else None
+    y = x.new_empty((*x.shape[:-1], N))
+    saved = x.new_empty(_saved_size(M, N), dtype=torch.uint8) if save and code else None
     if M:
         b = bias
         if b is not None:
             b = b.to(_BF16).contiguous()
             if b.data_ptr() % 8:
                 b = b.clone()
-        _linear_run(op, x2, _weight_bf16(weight), b, None if residual is None else _matrix(residual, N, True), code, saved, y, M)
+        _linear_run(op, x2, x_stride, weight, b, residual, code, saved, y, M, N, K)
     return y, saved
 
 
@@ -174,13 +172,12 @@ def _(x, weight, bias, residual, activation, save):
     return x.new_empty(*x.shape[:-1], N), _saved_fake(x, K, N, 1, save and activation != "none")
 
 
-def _weight_grad(dy: Tensor, x: Tensor, dtype: torch.dtype) -> Tensor:
-    """``dy^T x`` in ``dtype`` for rows as :func:`_matrix` leaves them, any number of them: those beyond the kernel's 32-bit reach
-    in several parts, added in fp32."""
+def _weight_grad(dy: Tensor, sy: int, x: Tensor, sx: int, dtype: torch.dtype) -> Tensor:
+    """``dy^T x`` in ``dtype`` for rows of strides ``sy`` and ``sx`` as :func:`_rows` leaves them, any number of them: those beyond
+    the kernel's 32-bit reach in several parts, added in fp32."""
     (M, N), K = dy.shape, x.size(1)
     if M == 0:
         return torch.zeros(N, K, dtype=dtype, device=dy.device)
-    sy, sx = _row_stride(dy), _row_stride(x)
     if kernels.weight_grad_fits(M, N, K, sy, sx):
         dw = torch.empty((N, K), dtype=dtype, device=dy.device)
         args = _lib.WeightGradArgs(dy.data_ptr(), x.data_ptr(), dw.data_ptr(), None, 0, M, N, K, sy, sx, K, _dt_code(dw))
@@ -197,16 +194,17 @@ def _weight_grad(dy: Tensor, x: Tensor, dtype: torch.dtype) -> Tensor:
     return dw.to(dtype)
 
 
-def _linear_dx(op: str, dy: Tensor, weights, shape) -> Tensor:
-    """``sum_p dy_p W_p`` for bf16 rows ``dy [M, P N]`` and P = 1 or 2 weights ``[N, K]``, as ``shape``."""
-    w0, w1 = _weight_bf16(weights[0]), _weight_bf16(weights[1]) if len(weights) > 1 else None
-    if w1 is not None and _row_stride(w1) != _row_stride(w0):
-        w0, w1 = w0.contiguous(), w1.contiguous()
-    (N, K), M = w0.shape, dy.size(0)
-    dx = torch.empty(shape, dtype=_BF16, device=dy.device)
+def _linear_dx(op: str, dy: Tensor, sy: int, weights, shape) -> Tensor:
+    """``sum_p dy_p W_p`` for bf16 rows ``dy [M, P N]`` of stride ``sy`` and P = 1 or 2 weights ``[N, K]``, as ``shape``."""
+    (N, K), M = weights[0].shape, dy.size(0)
+    w0, s0 = _weight_rows(weights[0], K)
+    w1, s1 = _weight_rows(weights[1], K) if len(weights) > 1 else (None, 0)
+    if w1 is not None and s1 != s0:  # (one stride for both)
+        w0, w1, s0, s1 = w0.contiguous(), w1.contiguous(), K, K
+    dx = dy.new_empty(shape)
     if M:
         args = _lib.LinearDxArgs(dy.data_ptr(), w0.data_ptr(), None if w1 is None else w1.data_ptr(), dx.data_ptr(), None, 0,
-                                 M, N, K, _row_stride(dy), _row_stride(w0), 0 if w1 is None else _row_stride(w1), K)
+                                 M, N, K, sy, s0, s1, K)
         ws = _fit_workspace("mla_linear_dx_workspace_bytes", args, dx)  # noqa: F841  (kept until the launch)
         _launch("mla_linear_dx", args, dx, op)
     return dx
@@ -217,7 +215,7 @@ def _linear_act_bwd(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype
     op = "mla_mi355x::linear_act_bwd"
     code = _activation(op, activation)
     N, K = weight.shape
-    dy2, x2 = _matrix(dy if dy.dtype == _BF16 else dy.to(_BF16), N), _matrix(x, K)
+    (dy2, sy), (x2, sx) = _weight_rows(dy, N), _rows(x, K)
     M = x2.size(0)
     if dy2.size(0) != M or (code and saved.numel() != _saved_size(M, N)):
         raise ValueError(f"{op}: dy {tuple(dy.shape)} and saved do not belong to x {tuple(x.shape)} and weight "
@@ -227,14 +225,15 @@ def _linear_act_bwd(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype
         db = (torch.empty if M else torch.zeros)(N, dtype=db_dtype, device=x.device)
     if M and (code or db is not None):
         if code:
-            dz = torch.empty(M, N, dtype=_BF16, device=x.device)
+            dz = x.new_empty((M, N))
         args = _lib.ActGradArgs(dy2.data_ptr(), saved.data_ptr() if code else None, dz.data_ptr() if code else None,
-                                None if db is None else db.data_ptr(), None, 0, M, N, _row_stride(dy2), N, code,
+                                None if db is None else db.data_ptr(), None, 0, M, N, sy, N, code,
                                 0 if db is None else _dt_code(db))
         ws = None if db is None else _fit_workspace("mla_act_grad_workspace_bytes", args, dy2)  # noqa: F841
         _launch("mla_act_grad", args, dy2, op)
-    return (_linear_dx(op, dz, (weight,), x.shape) if need_dx else None,
-            _weight_grad(dz, x2, weight.dtype) if need_dw else None, db)
+    sz = N if code else sy
+    return (_linear_dx(op, dz, sz, (weight,), x.shape) if need_dx else None,
+            _weight_grad(dz, sz, x2, sx, weight.dtype) if need_dw else None, db)
 
 
 @_op("linear_act_bwd", mutates_args=())
@@ -332,19 +331,19 @@ def _gated_ffn(x, w_gate, w_up, w_down, residual, activation, save):
                          f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
     H, D = w_gate.shape
     _check(op, x, (w_gate, w_up, w_down), ("w_gate", "w_up", "w_down"), residual, D)
-    x2 = _matrix(x, D)
+    x2, x_stride = _rows(x, D)
     M = x2.size(0)
-    y = torch.empty(x.shape, dtype=_BF16, device=x.device)
-    h = torch.empty((M, H), dtype=_BF16, device=x.device)
-    saved = torch.empty(2 * _saved_size(M, H), dtype=torch.uint8, device=x.device) if save else None
+    y = x.new_empty(x.shape)
+    h = x.new_empty((M, H))
+    saved = x.new_empty(2 * _saved_size(M, H), dtype=torch.uint8) if save else None
     if M:
-        wg, wu = _weight_bf16(w_gate), _weight_bf16(w_up)
+        (wg, sg), (wu, su) = _weight_rows(w_gate, D), _weight_rows(w_up, D)
         args = _lib.GatedLinearArgs(
             x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), None if saved is None else saved.data_ptr(), None, 0,
-            M, H, D, _row_stride(x2), _row_stride(wg), _row_stride(wu), H, code)
+            M, H, D, x_stride, sg, su, H, code)
         ws = _fit_workspace("mla_gated_linear_workspace_bytes", args, h) if M > ROWS_MAX else None  # noqa: F841
         _launch("mla_gated_linear", args, h, op)
-        _linear_run(op, h, _weight_bf16(w_down), None, None if residual is None else _matrix(residual, D, True), 0, None, y, M)
+        _linear_run(op, h, H, w_down, None, residual, 0, None, y, M, D, H)
     return y, h, saved
 
 
@@ -370,26 +369,26 @@ def _gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, n
     op = "mla_mi355x::gated_ffn_bwd"
     code = _activation(op, activation, gate=True)
     H, D = w_gate.shape
-    dy2, x2 = _matrix(dy if dy.dtype == _BF16 else dy.to(_BF16), D), _matrix(x, D)
+    (dy2, sy), (x2, sx) = _weight_rows(dy, D), _rows(x, D)
     M = x2.size(0)
     if dy2.size(0) != M or tuple(h.shape) != (M, H) or not h.is_contiguous() or saved.numel() != 2 * _saved_size(M, H):
         raise ValueError(f"{op}: dy {tuple(dy.shape)}, h {tuple(h.shape)} and saved do not belong to x {tuple(x.shape)}")
     dx = dwg = dwu = None
-    dwd = _weight_grad(dy2, h, w_down.dtype) if need_down else None
+    dwd = _weight_grad(dy2, sy, h, H, w_down.dtype) if need_down else None
     if need_dx or need_gate or need_up:
-        dgu = torch.empty((M, 2 * H), dtype=_BF16, device=x.device)
+        dgu = x.new_empty((M, 2 * H))
         if M:
-            wd = _weight_bf16(w_down)
+            wd, sd = _weight_rows(w_down, H)
             args = _lib.GatedLinearBwdArgs(dy2.data_ptr(), wd.data_ptr(), saved.data_ptr(), dgu.data_ptr(), M, H, D,
-                                           _row_stride(dy2), _row_stride(wd), 2 * H, code)
+                                           sy, sd, 2 * H, code)
             _launch("mla_gated_linear_bwd", args, dgu, op)
         if need_dx:
-            dx = _linear_dx(op, dgu, (w_gate, w_up), x.shape)
+            dx = _linear_dx(op, dgu, 2 * H, (w_gate, w_up), x.shape)
         if need_gate and need_up and w_gate.dtype == w_up.dtype:  # one product, its rows the two gradients
-            dwg, dwu = _weight_grad(dgu, x2, w_gate.dtype).split(H)
+            dwg, dwu = _weight_grad(dgu, 2 * H, x2, sx, w_gate.dtype).split(H)
         else:
-            dwg = _weight_grad(dgu[:, :H], x2, w_gate.dtype) if need_gate else None
-            dwu = _weight_grad(dgu[:, H:], x2, w_up.dtype) if need_up else None
+            dwg = _weight_grad(dgu[:, :H], 2 * H, x2, sx, w_gate.dtype) if need_gate else None
+            dwu = _weight_grad(dgu[:, H:], 2 * H, x2, sx, w_up.dtype) if need_up else None
     return dx, dwg, dwu, dwd
 
 
