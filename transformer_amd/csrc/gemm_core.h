@@ -23,10 +23,12 @@
 // in HBM and not in the last-level cache add 10 to 40 us where a product has one round of tiles (3001 x 2048 over 5464: 88 and
 // 129 us).  Whole products, 12288 rows, in a training pass: 4608 -> 1792 194 us (1050 TFLOP/s), 2 x 4608 <- 1792 361 us (1120);
 // 8192 cubed 840 us (1310; the library 775).
-// Measured and not kept: nine slots for a tile of 128 x 128 with eight waves (50 against 56 us at 1999 x 2048 over 4608, slower
-// at larger sizes), one such tile a CU with whole stages read ahead into a second set of registers over rings of five stages
-// (53 against 50: its LDS traffic, 64 KiB read and 32 written a stage, bounds it), four waves of 128 x 128 for the large tile (they
-// spill; 907 against 840 at 8192 cubed), waves of their own for loads and for stores (2 %), stores past the caches for y (1 %).
+// Measured and not kept, for a tile of 128 x 128 alone on its CU (50 us at 1999 x 2048 over 4608; its LDS traffic, 64 KiB read and
+// 32 written a stage, is 0.42 us of the 0.55 a stage takes): nine slots and eight waves (the same there, slower at larger sizes),
+// whole stages read ahead into a second set of registers over rings of five (53), two groups of waves that share its k (51; 5 us
+// less with the operands in HBM, 1 to 2 more at short k).  For 256 x 128, four waves of 128 x 64 (3 to 10 % slower).  For 256 x
+// 256, four waves of 128 x 128 (they spill; 907 against 840 at 8192 cubed).  Waves of their own for loads and for stores (2 %),
+// stores past the caches for y (1 %).
 #pragma once
 
 #include <type_traits>
