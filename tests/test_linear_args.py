@@ -84,5 +84,5 @@ def test_workspaces_and_saved_sizes():
     lib = _lib.load()
     a, _ = _norm_args([65536] * 3, [1] * 3, [1] * 3)
     assert 0 < lib.mla_grad_norm_workspace_bytes(ctypes.byref(a)) <= 1 << 14
-    assert lib.mla_linear_saved_size(1, 8) == 3072 and lib.mla_linear_saved_size(33, 40) == 4 * 3072
+    assert lib.mla_linear_saved_size(1, 8) == 3 << 10 and lib.mla_linear_saved_size(33, 40) == 12 << 10
     assert lib.mla_linear_saved_size(0, 8) == lib.mla_linear_saved_size(-5, 8) == lib.mla_linear_saved_size(1 << 62, 8) == 0

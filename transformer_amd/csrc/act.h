@@ -44,7 +44,7 @@ __device__ __forceinline__ void act_both(float z, float& value, float& slope) {
 // lanes (32 m x 32 n, see gemm_core.h): 2 x 16 bytes of upper halves and 16 bytes of the next 8 bits per lane, 3 KiB a block.
 // Written and read by whole 1 KiB runs straight from registers.  In bf16 they would cost 2 KiB and their rounding would add
 // to that of the gradients computed from them: an rms error of 1.7 to 2 times a single rounding's instead of 1.4.
-constexpr int kSavedBlock = 3072;
+constexpr int kSavedBlock = 3 << 10;
 
 __device__ __forceinline__ void saved_store(unsigned char* block, int lane, const f32x16& v) {
   u32x4 hi[2], lo;

@@ -111,7 +111,7 @@ def _refuse(op: str, x: Tensor, weights, names, residual: Optional[Tensor], n_ou
 
 
 def _saved_size(M: int, N: int) -> int:
-    return 3072 * ((M + 31) // 32) * ((N + 31) // 32)  # mla_linear_saved_size
+    return (3 << 10) * ((M + 31) // 32) * ((N + 31) // 32)  # mla_linear_saved_size
 
 
 def _linear_run(op, x2, x_stride, weight, bias, residual, code, saved, y, M, N, K):
