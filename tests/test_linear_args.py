@@ -86,3 +86,25 @@ def test_workspaces_and_saved_sizes():
     assert 0 < lib.mla_grad_norm_workspace_bytes(ctypes.byref(a)) <= 1 << 14
     assert lib.mla_linear_saved_size(1, 8) == 3 << 10 and lib.mla_linear_saved_size(33, 40) == 12 << 10
     assert lib.mla_linear_saved_size(0, 8) == lib.mla_linear_saved_size(-5, 8) == lib.mla_linear_saved_size(1 << 62, 8) == 0
+
+
+NEED = {  # sizes whose products are cut along k, or whose column sums come in several segments
+    "mla_linear_act": dict(M=4090, N=328, K=4072, x_stride=4072, w_stride=4072, y_stride=328),
+    "mla_gated_linear": dict(M=1000, N=264, K=1800, x_stride=1800, w_gate_stride=1800, w_up_stride=1800, h_stride=264),
+    "mla_linear_dx": dict(M=300, N=1000, K=64, dy_stride=2000, w0_stride=64, w1_stride=64, dx_stride=64),
+    "mla_act_grad": dict(M=200),
+}
+
+
+@pytest.mark.parametrize("entry", sorted(NEED))
+def test_missing_short_and_unaligned_workspaces_are_refused(entry):
+    lib = _lib.load()
+    struct, good = BASE[entry]
+    a = struct(**{**good, **NEED[entry]})
+    need = getattr(lib, entry + "_workspace_bytes")(ctypes.byref(a))
+    assert 0 < need <= 64 << 20
+    for at, size in ((None, need), (1 << 20, need - 1), (1 << 20, 0), ((1 << 20) + 8, need)):
+        a.workspace, a.workspace_bytes = at, size
+        assert getattr(lib, entry)(ctypes.byref(a), None) == _lib.MLA_ERR_WORKSPACE, (at, size)
+    small = struct(**{**good, "M": 64})
+    assert getattr(lib, entry + "_workspace_bytes")(ctypes.byref(small)) == 0 or entry == "mla_linear_dx"

@@ -75,6 +75,5 @@ __device__ __forceinline__ float saved_value(const SavedRegs& r, int e) {
   const uint32_t top = (e & 1) ? (h & 0xffff0000u) : (h << 16);
   return __uint_as_float(top | (((l >> (8 * (e & 3))) & 255u) << 8));
 }
-__device__ __forceinline__ int64_t saved_blocks(int64_t n) { return (n + 31) / 32; }
 
 }  // namespace mla

@@ -6,7 +6,6 @@
 // gelu and the kept pre-activations (302 MB out) 224 + 20 for the tiles cut along k (830 TFLOP/s; the epilogue's arithmetic and
 // stores run with the matrix units idle), 4608 -> 1792 178 + 16, dx of the former 187 + 14, of two layers 1792 -> 4608 together
 // 346 + 15 (1120 TFLOP/s).
-#include <algorithm>
 
 #include "gemm_epilogue.h"
 #include "linear_checks.h"

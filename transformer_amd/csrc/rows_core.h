@@ -11,8 +11,6 @@
 // A staged row's chunk c of 16 bytes lies at c ^ (row mod 16): the 16 rows of a fragment fall on different banks.
 #pragma once
 
-#include <algorithm>
-
 #include "act.h"
 #include "gemm_core.h"
 
