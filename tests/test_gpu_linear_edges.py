@@ -151,6 +151,44 @@ def test_outputs_past_two_to_the_31_elements():
         T.near(db, sums, "db")
 
 
+def test_more_rows_than_a_weight_gradient_takes_at_once():
+    from transformer_amd import gated_ffn, linear_act
+    M = (1 << 24) + 1000
+    g = T.gen("many rows")
+    x, w, b, dy = T.bf16(g, M, 8), T.bf16(g, 16, 8, std=0.3), T.bf16(g, 16), T.bf16(g, M, 16)
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = linear_act(x, w, b, None, "relu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    with torch.no_grad():
+        z = x.double() @ w.double().t() + b.double()
+        dz = dy.double() * (z > 0)
+        T.near(dx, dz @ w.double(), "dx")
+        T.near(dw, dz.t() @ x.double(), "dw")
+        T.near(db, dz.sum(0), "db")
+        T.near(y, torch.relu(z), "y")
+    wd = T.bf16(g, 8, 16, std=0.3).requires_grad_()
+    y = gated_ffn(x, w, w, wd, None, "relu")
+    got = torch.autograd.grad(y, (w, wd), x.detach())
+    with torch.no_grad():
+        z, d = x.double() @ w.double().t(), x.double()
+        dh = d @ wd.double()
+        T.near(got[0], (dh * 2 * torch.relu(z)).t() @ d, "dw of both")
+        T.near(got[1], d.t() @ torch.relu(z).square(), "dwd")
+
+
+def test_rows_that_lie_far_apart():
+    from transformer_amd import linear_act
+    g = T.gen("far apart")
+    buf = torch.zeros(300, (1 << 22) - 8, dtype=torch.bfloat16, device="cuda")  # 2.5 GB
+    x, w, dy = buf[:, 16:152], T.bf16(g, 72, 136, std=0.1).requires_grad_(), T.bf16(g, 300, 72)
+    x.copy_(T.bf16(g, 300, 136))
+    near, far = (linear_act(t, w, None, None, "silu") for t in (x.contiguous(), x))
+    assert torch.equal(near, far)
+    (a,), (c,) = (torch.autograd.grad(t, w, dy) for t in (near, far))
+    T.near(c, a.double(), "dw")
+
+
 def test_slopes_of_huge_pre_activations():
     """z up to 3e38: the slope is 0 or 1 there, and 0 times a square past the range is not formed."""
     from transformer_amd import gated_ffn, linear_act

@@ -174,7 +174,7 @@ def _(x, weight, bias, residual, activation, save):
 
 def _weight_grad(dy: Tensor, sy: int, x: Tensor, sx: int, dtype: torch.dtype) -> Tensor:
     """``dy^T x`` in ``dtype`` for rows of strides ``sy`` and ``sx`` as :func:`_rows` leaves them, any number of them: those beyond
-    the kernel's 32-bit reach in several parts, added in fp32."""
+    the kernel's reach in several parts, added in fp32."""
     (M, N), K = dy.shape, x.size(1)
     if M == 0:
         return torch.zeros(N, K, dtype=dtype, device=dy.device)
@@ -184,9 +184,9 @@ def _weight_grad(dy: Tensor, sy: int, x: Tensor, sx: int, dtype: torch.dtype) ->
         ws = _fit_workspace("mla_weight_grad_workspace_bytes", args, dw)  # noqa: F841  (kept until the launch)
         _launch("mla_weight_grad", args, dw, "mla_mi355x::weight_grad")
         return dw
-    rows = (1 << 30) // max(sy, sx) - 257
-    if rows < 32:
-        raise ValueError(f"mla_mi355x::weight_grad: rows of {N} and {K} are too wide")
+    if max(sy, sx) > 1 << 20:  # (few rows would be within reach: closer together)
+        dy, x, sy, sx = dy.contiguous(), x.contiguous(), N, K
+    rows = min((1 << 30) // max(sy, sx) - 257, (1 << 24) - 1)
     dw = None
     for r in range(0, M, rows):
         part = kernels.weight_grad(dy[r:r + rows], x[r:r + rows], True)
