@@ -8,7 +8,7 @@
 // The second pass walks the chunks backwards: what the first one read last is still in the last-level cache.
 // 1228 million fp32 gradients in 338 tensors (4.9 GB, three launches a pass): norm 876 us, 5.6 TB/s, factor 1912 us, 5.1 TB/s, what
 // a large copy reaches; twice the grid, eight loads in flight and stores past the caches changed nothing.  50 tensors of 4
-// million: 7 and 12 us.
+// million: 7 and 12 us (chunks of 16 KiB: 2 us less at 1 million elements, 3 more at 8).
 #include <algorithm>
 #include <cmath>
 #include <vector>
