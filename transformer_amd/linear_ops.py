@@ -110,6 +110,23 @@ def _refuse(op: str, x: Tensor, weights, names, residual: Optional[Tensor], n_ou
                      f"{residual.device}")
 
 
+def _check_bwd(op: str, fits: bool, x: Tensor, dy: Tensor, weights, saved: Optional[Tensor], h: Optional[Tensor] = None) -> None:
+    """What a backward's launches take for granted, before the first of them; ``fits``: whether the shapes belong together."""
+    if not fits:
+        raise ValueError(f"{op}: dy {tuple(dy.shape)}, x {tuple(x.shape)}, weights {[tuple(w.shape) for w in weights]}"
+                         f"{'' if h is None else f', h {tuple(h.shape)}'} and saved "
+                         f"{'(none)' if saved is None else tuple(saved.shape)} do not belong together")
+    if x.dtype != _BF16 or (h is not None and h.dtype != _BF16) or (saved is not None and saved.dtype != torch.uint8) \
+            or any(w.dtype != _BF16 and w.dtype != _F32 for w in weights):
+        raise TypeError(f"{op}: x and h must be bfloat16, weights bfloat16 or float32 and saved uint8")
+    if any(t is not None and not t.is_contiguous() for t in (h, saved)):
+        raise ValueError(f"{op}: h and saved must be contiguous")
+    dev = x.get_device()
+    if dev < 0 or any(t is not None and t.get_device() != dev for t in (dy, *weights, h, saved)):
+        kernels._require_gpu(op, x, dy, *weights, h, saved)
+        raise ValueError(f"{op}: all tensors must be on one device")
+
+
 def _saved_size(M: int, N: int) -> int:
     return (3 << 10) * ((M + 31) // 32) * ((N + 31) // 32)  # mla_linear_saved_size
 
@@ -214,12 +231,13 @@ def _linear_act_bwd(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype
     """``(dx, dw, db)``, None where not needed; see :func:`linear_act_bwd`."""
     op = "mla_mi355x::linear_act_bwd"
     code = _activation(op, activation)
-    N, K = weight.shape
+    if db_dtype is not None and db_dtype != _BF16 and db_dtype != _F32:
+        raise TypeError(f"{op}: db_dtype must be bfloat16 or float32, got {db_dtype}")
+    N, K = weight.shape if weight.dim() == 2 else (0, 0)
+    M = x.numel() // K if K else 0
+    _check_bwd(op, N > 0 and x.dim() > 0 and x.size(-1) == K and dy.shape == (*x.shape[:-1], N)
+               and (not code or saved.numel() == _saved_size(M, N)), x, dy, (weight,), saved if code else None)
     (dy2, sy), (x2, sx) = _weight_rows(dy, N), _rows(x, K)
-    M = x2.size(0)
-    if dy2.size(0) != M or (code and saved.numel() != _saved_size(M, N)):
-        raise ValueError(f"{op}: dy {tuple(dy.shape)} and saved do not belong to x {tuple(x.shape)} and weight "
-                         f"{tuple(weight.shape)}")
     dz, db = dy2, None
     if db_dtype is not None:
         db = (torch.empty if M else torch.zeros)(N, dtype=db_dtype, device=x.device)
@@ -241,8 +259,6 @@ def linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, saved: Tensor, activat
                    db_dtype: Optional[torch.dtype]) -> Tuple[Tensor, Tensor, Tensor]:
     """Gradients ``(dx, dw, db)`` of :func:`linear_act` from ``dy`` and what it saved; ``dw`` in the weight's dtype, ``db`` in
     ``db_dtype`` (None: no bias).  Empty tensors where a gradient is not needed."""
-    kernels._require_gpu("mla_mi355x::linear_act_bwd", dy, x, weight, saved)
-    kernels._bf16("mla_mi355x::linear_act_bwd", x=x)
     got = _linear_act_bwd(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype)
     return tuple(x.new_empty(0) if t is None else t for t in got)
 
@@ -368,11 +384,12 @@ def _gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, n
     """``(dx, dw_gate, dw_up, dw_down)``, None where not needed; see :func:`gated_ffn_bwd`."""
     op = "mla_mi355x::gated_ffn_bwd"
     code = _activation(op, activation, gate=True)
-    H, D = w_gate.shape
+    H, D = w_gate.shape if w_gate.dim() == 2 else (0, 0)
+    M = x.numel() // D if D else 0
+    _check_bwd(op, H > 0 and x.dim() > 0 and x.size(-1) == D and dy.shape == x.shape and w_up.shape == w_gate.shape
+               and w_down.shape == (D, H) and h.shape == (M, H) and saved.numel() == 2 * _saved_size(M, H),
+               x, dy, (w_gate, w_up, w_down), saved, h)
     (dy2, sy), (x2, sx) = _weight_rows(dy, D), _rows(x, D)
-    M = x2.size(0)
-    if dy2.size(0) != M or tuple(h.shape) != (M, H) or not h.is_contiguous() or saved.numel() != 2 * _saved_size(M, H):
-        raise ValueError(f"{op}: dy {tuple(dy.shape)}, h {tuple(h.shape)} and saved do not belong to x {tuple(x.shape)}")
     dx = dwg = dwu = None
     dwd = _weight_grad(dy2, sy, h, H, w_down.dtype) if need_down else None
     if need_dx or need_gate or need_up:
@@ -398,8 +415,6 @@ def gated_ffn_bwd(dy: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: T
                   need_down: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
     """Gradients ``(dx, dw_gate, dw_up, dw_down)`` of :func:`gated_ffn` from ``dy`` and what it saved, the weights' in their
     dtypes.  Empty tensors where a gradient is not needed."""
-    kernels._require_gpu("mla_mi355x::gated_ffn_bwd", dy, x, w_gate, w_up, w_down, h, saved)
-    kernels._bf16("mla_mi355x::gated_ffn_bwd", x=x, h=h)
     dx, dwg, dwu, dwd = _gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, need_gate, need_up, need_down)
     if dwg is not None and dwu is not None and dwu.untyped_storage().data_ptr() == dwg.untyped_storage().data_ptr():
         dwu = dwu.clone()  # (an operator's outputs share no memory)
