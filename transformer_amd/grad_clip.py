@@ -51,6 +51,8 @@ def _is_max(op: str, norm_type: float) -> bool:
 
 def _refuse(op: str, tensors: List[Tensor]) -> None:
     """The error of a list that the kernels do not take."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"transformer_amd.{op} is no registered operator: torch.jit.trace would not record its launches")
     for t in tensors:
         if t.layout != torch.strided:
             raise ValueError(f"{op}: sparse gradients are not built")
@@ -69,7 +71,7 @@ def _laid_out(op: str, tensors: List[Tensor]) -> Tuple[List[Tensor], array]:
         codes = array("i", [_CODES[t.dtype] for t in tensors])
     except (RuntimeError, KeyError):  # (of a compressed sparse tensor is_contiguous raises)
         _refuse(op, tensors)
-    if len(devices) != 1 or -1 in devices:
+    if len(devices) != 1 or -1 in devices or torch._C._get_tracing_state() is not None:
         _refuse(op, tensors)
     if not all(whole):
         if not all(t.layout == torch.strided for t in tensors):

@@ -1043,9 +1043,10 @@ def _(logits, targets, lse, g_vec, g_scale, v0):
 # ----------------------------------------------------------------- eager calls
 
 def _not_plain(args) -> bool:
-    """Tracing (torch.compile), a dispatch mode, a functorch transform, tensor subclasses, or tensors off the GPU."""
+    """Tracing (torch.compile, torch.jit.trace), a dispatch mode, a functorch transform, tensor subclasses, or tensors off
+    the GPU."""
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 \
-            or torch._C._functorch.peek_interpreter_stack() is not None:
+            or torch._C._get_tracing_state() is not None or torch._C._functorch.peek_interpreter_stack() is not None:
         return True
     for a in args:
         if isinstance(a, Tensor) and ((type(a) is not Tensor and type(a) is not torch.nn.Parameter) or not a.is_cuda):
@@ -1069,7 +1070,7 @@ def _needs_grad(args) -> bool:
 
 def dispatcher_needed(args) -> bool:
     """Whether a call with ``args`` must go through the registered operator: under tracing
-    (torch.compile), a dispatch mode (fake tensors, functionalization), a functorch transform,
+    (torch.compile, torch.jit.trace), a dispatch mode (fake tensors, functionalization), a functorch transform,
     tensor subclasses, tensors off the GPU (meta tensors take the fake kernels), or an input
     that needs a gradient while grad mode is on (the autograd formulas live on the
     operators).  Otherwise the operator adds only dispatch time (about 15 us of Python per
@@ -1079,9 +1080,9 @@ def dispatcher_needed(args) -> bool:
 
 def function_fits(args) -> bool:
     """Whether an autograd.Function may stand in for a registered operator whose gradient is needed: nothing else in
-    :func:`dispatcher_needed` holds, and no forward-mode level, jit trace or torch-function mode would see less."""
+    :func:`dispatcher_needed` holds, and no forward-mode level or torch-function mode would see less."""
     return torch.autograd.forward_ad._current_level < 0 and torch._C._len_torch_function_stack() == 0 \
-        and torch._C._get_tracing_state() is None and not _not_plain(args)
+        and not _not_plain(args)
 
 
 def below_autograd():

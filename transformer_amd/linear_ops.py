@@ -270,9 +270,8 @@ def _(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype):
 
 
 def _plain_backward(dy: Tensor) -> bool:
-    """Whether a backward may run the bodies: it is not itself differentiated, batched or under a dispatch mode."""
-    return not (torch.is_grad_enabled() or type(dy) is not Tensor or kernels.batched_grad(dy)
-                or torch._C._len_torch_dispatch_stack() > 0 or torch._C._functorch.peek_interpreter_stack() is not None)
+    """Whether a backward may run the bodies: it is not itself differentiated, batched, traced or under a dispatch mode."""
+    return not (torch.is_grad_enabled() or type(dy) is not Tensor or kernels.batched_grad(dy) or kernels._not_plain((dy,)))
 
 
 def _linear_act_grads(ctx, dy, need):

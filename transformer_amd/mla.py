@@ -216,7 +216,7 @@ class MLA(nn.Module):
         bf16 weights and a bf16 input; under bf16 autocast, bf16 or fp32 weights and a bf16 or fp32
         input (fp32 weights under bf16 autocast is how the reference's generation loop runs,
         CLI.py:294); q_up and o_proj plain layers (the recording reads their weights: a hooked, wrapped or
-        parametrized one is called eagerly); not inside a graph capture or torch.compile, and the module has
+        parametrized one is called eagerly); not inside a graph capture, torch.compile or torch.jit.trace, and the module has
         not given up recording.  The recording keeps its cache in bf16, which is the reference's cache dtype in
         those cases; an fp32 module outside autocast takes the eager kernels, whose cache stays
         fp32 as the reference's does (transformer.py:215-218, :241-244)."""
@@ -232,7 +232,7 @@ class MLA(nn.Module):
         else:
             ok = wdt == torch.bfloat16 and x.dtype == wdt
         return (ok and not self.__dict__.get("_graph_off", False) and not torch.compiler.is_compiling()
-                and not torch.cuda.is_current_stream_capturing())
+                and torch._C._get_tracing_state() is None and not torch.cuda.is_current_stream_capturing())
 
     def _step_graph(self, store, L0, B):
         """The recorded step bound to ``store``'s buffers, recorded again when the buffers
