@@ -41,6 +41,53 @@ def _shares(t: Tensor) -> bool:
     return False
 
 
+def _layout(t: Tensor) -> Tuple[int, tuple]:
+    """Where ``t``'s bytes lie: their first address, and (stride, count) of each dimension in bytes, the longest first and
+    the last one a run."""
+    dims = [(1, t.element_size())]
+    for stride, size in sorted((s * t.element_size(), n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        below, count = dims[-1]
+        if stride == below * count:
+            dims[-1] = below, count * size
+        else:
+            dims.append((stride, size))
+    return t.data_ptr(), tuple(reversed(dims))
+
+
+def _reach(dims: tuple) -> int:
+    return 1 + sum(s * (n - 1) for s, n in dims)
+
+
+def _meet(a: int, da: tuple, b: int, db: tuple) -> bool:
+    """Whether two layouts of :func:`_layout` share a byte."""
+    if a + _reach(da) <= b or b + _reach(db) <= a:
+        return False
+    if len(da) == len(db) == 1:
+        return True
+    if da[0][0] < db[0][0]:
+        a, da, b, db = b, db, a, da
+    (s, n), inner = da[0], da[1:]
+    if s == db[0][0]:  # rows of one stride: which of them meet goes by their distance alone
+        first, other, within = 1 - db[0][1], db[1:], _reach(db[1:])
+    else:              # the rows of the one with the longer stride, against all of the other
+        first, other, within = 0, db, _reach(db)
+    lo, hi = max(first, (b - a - _reach(inner)) // s + 1), min(n - 1, (b - a + within - 1) // s)
+    return any(_meet(a + i * s, inner, b, other) for i in range(lo, hi + 1))
+
+
+def _refuse_shared(op: str, grads: List[Tensor]) -> None:
+    """An error where an element of ``grads`` lies in the memory of another one."""
+    for g in grads:
+        if _shares(g):
+            raise ValueError(f"{op}: a gradient with strides {g.stride()} shares memory between its elements")
+    near: List[Tuple[int, tuple]] = []  # those that reach past the start of the next one
+    for at, dims in sorted(_layout(g) for g in grads if g.numel()):
+        near = [o for o in near if o[0] + _reach(o[1]) > at]
+        if any(_meet(*o, at, dims) for o in near):
+            raise ValueError(f"{op}: two gradients share memory")
+        near.append((at, dims))
+
+
 def _is_max(op: str, norm_type: float) -> bool:
     """Whether the norm is the largest magnitude (else the 2-norm)."""
     norm_type = float(norm_type)
@@ -118,10 +165,8 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     if not grads:
         return torch.tensor(0.0)
     flat, codes = _laid_out(op, grads)
-    if flat is not grads:
-        for g in grads:
-            if _shares(g):
-                raise ValueError(f"{op}: a gradient with strides {g.stride()} shares memory between its elements")
+    if any(g is not c for g, c in zip(grads, flat)):  # (the entry point would compare the copies)
+        _refuse_shared(op, grads)
     if error_if_nonfinite:
         norm = _run(op, "mla_grad_norm", flat, codes, is_max, 0.0)
         if not bool(torch.isfinite(norm)):
