@@ -74,3 +74,21 @@ def test_a_jit_trace_records_the_operators():
     dy = T.bf16(g, 40, 72)
     want = torch.autograd.grad(gated_ffn(linear_act(y, wd @ w, None, y, "silu"), w, w, wd), y, dy)[0]
     assert torch.equal(torch.autograd.grad(traced(y), y, dy)[0], want)
+
+
+@pytest.mark.parametrize("H", [(1 << 19) - 8, 1 << 19, (1 << 20) - 8])
+def test_gradients_of_the_widest_hidden_layers(H):
+    """From 2^19 on, both first weights' gradients are more rows than one weight gradient takes."""
+    from transformer_amd import gated_ffn
+    g = T.gen("wide", H)
+    M, D = 5, 16
+    t = [T.bf16(g, M, D), T.bf16(g, H, D, std=0.2), T.bf16(g, H, D, std=0.2), T.bf16(g, D, H, std=1e-3)]
+    dy = T.bf16(g, M, D)
+    leaves = [v.clone().requires_grad_() for v in t]
+    got = torch.autograd.grad(gated_ffn(*leaves), leaves, dy)
+    x, wg, wu, wd = (v.double() for v in t)
+    a, u, dh = T.act64(x @ wg.t(), "silu"), x @ wu.t(), dy.double() @ wd
+    dg, du = dh * u * T.slope64(x @ wg.t(), "silu"), dh * a
+    for name, v, ref in zip(("dx", "dw_gate", "dw_up", "dw_down"), got,
+                            (dg @ wg + du @ wu, dg.t() @ x, du.t() @ x, dy.double().t() @ (a * u))):
+        T.near(v, ref, name)

@@ -400,7 +400,8 @@ def _gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, n
             _launch("mla_gated_linear_bwd", args, dgu, op)
         if need_dx:
             dx = _linear_dx(op, dgu, 2 * H, (w_gate, w_up), x.shape)
-        if need_gate and need_up and w_gate.dtype == w_up.dtype:  # one product, its rows the two gradients
+        # one product, its rows the two gradients (which a weight gradient takes below 2^20 of)
+        if need_gate and need_up and w_gate.dtype == w_up.dtype and 2 * H < 1 << 20:
             dwg, dwu = _weight_grad(dgu, 2 * H, x2, sx, w_gate.dtype).split(H)
         else:
             dwg = _weight_grad(dgu[:, :H], 2 * H, x2, sx, w_gate.dtype) if need_gate else None
