@@ -92,3 +92,62 @@ def test_gradients_of_the_widest_hidden_layers(H):
     for name, v, ref in zip(("dx", "dw_gate", "dw_up", "dw_down"), got,
                             (dg @ wg + du @ wu, dg.t() @ x, du.t() @ x, dy.double().t() @ (a * u))):
         T.near(v, ref, name)
+
+
+def _gradients_of_few_rows(g, x, w, wg, wu, wd):
+    """dx of both operators, and the gated block's first weight gradients, against 64 bits (in parts of the wide sizes)."""
+    from transformer_amd import gated_ffn, linear_act
+    x = x.detach().requires_grad_()
+    y = linear_act(x, w, None, None, "relu")
+    dy = T.bf16(g, *y.shape)
+    dx, = torch.autograd.grad(y, x, dy)
+    x6, ref = x.detach().double(), torch.zeros(x.shape, dtype=torch.float64, device="cuda")
+    for part, d in zip(w.split(4096), dy.split(4096, 1)):
+        ref += (d.double() * (x6 @ part.double().t() > 0)) @ part.double()
+    T.near(dx, ref, "dx")
+    leaves = [x, wg.detach().requires_grad_()]
+    y = gated_ffn(x, leaves[1], wu, wd, x)
+    dy = T.bf16(g, *y.shape)
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    ref = dy.double()
+    for s in range(0, wg.size(0), 4096):
+        a, b, c = wg[s:s + 4096].double(), wu[s:s + 4096].double(), wd[:, s:s + 4096].double()
+        p, u, dh = x6 @ a.t(), x6 @ b.t(), dy.double() @ c
+        dg = dh * u * T.slope64(p, "silu")
+        ref = ref + dg @ a + (dh * T.act64(p, "silu")) @ b
+        T.near(dw[s:s + 4096], dg.t() @ x6, "dw_gate")
+    T.near(dx, ref, "gated dx")
+
+
+@pytest.mark.parametrize("M,H,D", [(5, 520, 808), (200, 1032, 264), (300, 264, 1032)])
+def test_gradients_through_weights_in_parts(M, H, D, monkeypatch):
+    from transformer_amd import linear_ops
+    g = T.gen("parts", M, H, D)
+    t = [T.bf16(g, M, D), *(T.bf16(g, H, D, std=D ** -0.5) for _ in range(3)), T.bf16(g, D, H, std=H ** -0.5)]
+    monkeypatch.setattr(linear_ops, "REACH", 257 * (max(H, D) + 64))
+    launches = []
+    launch = linear_ops._launch
+    monkeypatch.setattr(linear_ops, "_launch", lambda entry, *a: launches.append(entry) or launch(entry, *a))
+    _gradients_of_few_rows(g, *t)
+    parts = {"mla_linear_dx": -(-D // linear_ops._columns(H, D, D)), "mla_gated_linear_bwd": -(-H // linear_ops._columns(D, H, H))}
+    assert min(parts.values()) > 1
+    assert launches.count("mla_linear_dx") == 2 * parts["mla_linear_dx"]  # (linear_act's and the gated block's)
+    assert launches.count("mla_gated_linear_bwd") == parts["mla_gated_linear_bwd"]
+
+
+def test_gradients_through_weights_whose_rows_lie_far_apart():
+    g = T.gen("far weights")
+    M, H, D = 40, 304, 264
+    buf = torch.zeros(304, (1 << 22) - 8, dtype=torch.bfloat16, device="cuda")  # 2.6 GB
+    w, wg, wd = buf[:, 64:64 + D], buf[:, 1024:1024 + D], buf[:D, 4096:4096 + H]
+    for t in (w, wg, wd):
+        t.copy_(T.bf16(g, *t.shape, std=0.06))
+    _gradients_of_few_rows(g, T.bf16(g, M, D), w, wg, T.bf16(g, H, D, std=0.06), wd)
+
+
+def test_gradients_through_weights_of_two_gib():
+    g = T.gen("large weights")
+    H, D = (1 << 15) + 8, 1 << 15
+    make = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device="cuda").normal_(0, 2.0 ** -7, generator=g)
+    wg = make(H, D)
+    _gradients_of_few_rows(g, T.bf16(g, 3, D), wg, wg, make(H, D), make(D, H))

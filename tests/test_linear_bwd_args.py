@@ -65,3 +65,14 @@ def test_what_belongs_together_is_refused_for_its_device_alone():
     for change in ({}, dict(dy=z(5, 8, K), x=z(5, 8, K)), dict(w_down=z(K, N, dt=torch.float32))):
         with pytest.raises(RuntimeError, match="GPU"):
             ops.gated_ffn_bwd(*{**GATED, **change}.values())
+
+
+def test_parts_of_a_weight_lie_within_the_kernels_reach():
+    for rows in (8, 264, 1 << 14, 1 << 15, (1 << 20) - 8):
+        for cols in (8, 264, 1 << 15, (1 << 20) - 8):
+            for stride in (cols, 1 << 21, (1 << 22) - 8):
+                if stride < cols:
+                    continue
+                n = linear_ops._columns(rows, cols, stride)
+                assert (rows + 64) * n < linear_ops.REACH  # (as mla_linear_dx and mla_gated_linear_bwd ask of a contiguous one)
+                assert n == cols or (n >= 256 and n % 256 == 0 and (rows + 64) * cols >= linear_ops.REACH)

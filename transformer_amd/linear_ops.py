@@ -17,6 +17,7 @@ from ._lib import ACTIVATIONS
 from .kernels import _alloc_workspace, _dt_code, _op, _register_autograd
 
 LINEAR_MAX_STRIDE = 1 << 22
+REACH = 1 << 30  # elements that a weight read across its rows, and 64 rows more, lie within (mla_linear_dx, mla_gated_linear_bwd)
 ROWS_MAX = 64  # rows up to which mla_linear_act and mla_gated_linear need no workspace
 _BF16, _F32 = torch.bfloat16, torch.float32
 _byref, _current_device, _raw_stream = ctypes.byref, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
@@ -211,17 +212,31 @@ def _weight_grad(dy: Tensor, sy: int, x: Tensor, sx: int, dtype: torch.dtype) ->
     return dw.to(dtype)
 
 
+def _columns(rows: int, cols: int, stride: int) -> int:
+    """How many of the columns of a weight that is read across its rows one call takes: all of them, as they lie or closer
+    together, or else whole blocks of 256 within its reach, copied."""
+    if (rows + 64) * min(stride, cols) < REACH:
+        return cols
+    return (REACH - 1) // (rows + 64) // 256 * 256
+
+
 def _linear_dx(op: str, dy: Tensor, sy: int, weights, shape) -> Tensor:
     """``sum_p dy_p W_p`` for bf16 rows ``dy [M, P N]`` of stride ``sy`` and P = 1 or 2 weights ``[N, K]``, as ``shape``."""
     (N, K), M = weights[0].shape, dy.size(0)
-    w0, s0 = _weight_rows(weights[0], K)
-    w1, s1 = _weight_rows(weights[1], K) if len(weights) > 1 else (None, 0)
-    if w1 is not None and s1 != s0:  # (one stride for both)
-        w0, w1, s0, s1 = w0.contiguous(), w1.contiguous(), K, K
     dx = dy.new_empty(shape)
-    if M:
-        args = _lib.LinearDxArgs(dy.data_ptr(), w0.data_ptr(), None if w1 is None else w1.data_ptr(), dx.data_ptr(), None, 0,
-                                 M, N, K, sy, s0, s1, K)
+    if not M:
+        return dx
+    given = [_weight_rows(w, K) for w in weights]
+    cols = _columns(N, K, max(s for _, s in given))
+    for c in range(0, K, cols):
+        n = min(cols, K - c)
+        if n < K or len({s for _, s in given}) > 1 or (N + 64) * given[0][1] >= REACH:  # (one stride for both)
+            part = [(w[:, c:c + n].contiguous(), n) for w, _ in given]
+        else:
+            part = given
+        (w0, s), w1 = part[0], part[1][0] if len(part) > 1 else None
+        args = _lib.LinearDxArgs(dy.data_ptr(), w0.data_ptr(), None if w1 is None else w1.data_ptr(), dx.data_ptr() + 2 * c, None, 0,
+                                 M, N, n, sy, s, 0 if w1 is None else s, K)
         ws = _fit_workspace("mla_linear_dx_workspace_bytes", args, dx)  # noqa: F841  (kept until the launch)
         _launch("mla_linear_dx", args, dx, op)
     return dx
@@ -379,6 +394,24 @@ def _(x, w_gate, w_up, w_down, residual, activation, save):
     return (x.new_empty(x.shape), x.new_empty((x.numel() // D, H) if save else 0), _saved_fake(x, D, H, 2, save))
 
 
+def _gated_grads(op, dy, sy, w_down, saved, dgu, code):
+    """The gradients ``dgu [M, 2 H]`` of both first products from bf16 rows ``dy [M, D]`` of stride ``sy`` and what they saved."""
+    (D, H), M = w_down.shape, dy.size(0)
+    wd, sd = _weight_rows(w_down, H)
+    cols = _columns(D, H, sd)
+    if (D + 64) * sd >= REACH and cols == H:
+        wd, sd = wd.contiguous(), H
+    for c in range(0, H, cols):
+        n, w, s, kept, out = min(cols, H - c), wd, sd, saved, dgu
+        if n < H:  # (the blocks of the kept values that lie in these columns)
+            w, s, out = wd[:, c:c + n].contiguous(), n, dgu.new_empty((M, 2 * n))
+            kept = saved.view((M + 31) // 32, (H + 31) // 32, -1)[:, c // 32:(c + n + 31) // 32].contiguous()
+        args = _lib.GatedLinearBwdArgs(dy.data_ptr(), w.data_ptr(), kept.data_ptr(), out.data_ptr(), M, n, D, sy, s, 2 * n, code)
+        _launch("mla_gated_linear_bwd", args, out, op)
+        if n < H:
+            dgu[:, c:c + n], dgu[:, H + c:H + c + n] = out[:, :n], out[:, n:]
+
+
 def _gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, need_gate, need_up, need_down):
     """``(dx, dw_gate, dw_up, dw_down)``, None where not needed; see :func:`gated_ffn_bwd`."""
     op = "mla_mi355x::gated_ffn_bwd"
@@ -394,10 +427,7 @@ def _gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, n
     if need_dx or need_gate or need_up:
         dgu = x.new_empty((M, 2 * H))
         if M:
-            wd, sd = _weight_rows(w_down, H)
-            args = _lib.GatedLinearBwdArgs(dy2.data_ptr(), wd.data_ptr(), saved.data_ptr(), dgu.data_ptr(), M, H, D,
-                                           sy, sd, 2 * H, code)
-            _launch("mla_gated_linear_bwd", args, dgu, op)
+            _gated_grads(op, dy2, sy, w_down, saved, dgu, code)
         if need_dx:
             dx = _linear_dx(op, dgu, 2 * H, (w_gate, w_up), x.shape)
         # one product, its rows the two gradients (which a weight gradient takes below 2^20 of)
