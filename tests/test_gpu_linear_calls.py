@@ -151,3 +151,21 @@ def test_gradients_through_weights_of_two_gib():
     make = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device="cuda").normal_(0, 2.0 ** -7, generator=g)
     wg = make(H, D)
     _gradients_of_few_rows(g, T.bf16(g, 3, D), wg, wg, make(H, D), make(D, H))
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 72), (72,), (3, 40, 1), (2, 3, 40, 72), (1, 40, 72), ()])
+def test_residuals_of_another_shape_are_refused_in_every_type(shape):
+    from transformer_amd import SwiGLU, gated_ffn, linear_act
+    g = T.gen("residual")
+    x, w, wd = T.bf16(g, 3, 40, 72), T.bf16(g, 72, 72, std=0.1), T.bf16(g, 72, 72, std=0.1)
+    with torch.device("cuda"):
+        ffn, hooked = SwiGLU(72, 72), SwiGLU(72, 72)
+    hooked.w1.register_forward_hook(lambda *a: None)
+    for dt in (torch.bfloat16, torch.float32):
+        bad, good = torch.zeros(shape, dtype=dt, device="cuda"), torch.ones(3, 40, 72, dtype=dt, device="cuda")
+        for call in (lambda r: linear_act(x, w, None, r, "silu"), lambda r: gated_ffn(x, w, w, wd, r), lambda r: ffn(x, r),
+                     lambda r: hooked(x, r)):
+            with torch.autocast("cuda", dtype=torch.bfloat16):
+                with pytest.raises(ValueError, match="residual"):
+                    call(bad)
+                assert call(good).shape == x.shape and call(good).dtype == dt

@@ -33,12 +33,20 @@ def _inputs(op: str, x: Tensor, residual):
     return x, residual, None
 
 
+def _add(op: str, residual, y: Tensor) -> Tensor:
+    """``residual + y`` by torch, for residuals that the kernels take: of the result's shape."""
+    if residual is None:
+        return y
+    if residual.shape != y.shape:
+        raise ValueError(f"{op}: residual must be {tuple(y.shape)}, got {tuple(residual.shape)}")
+    return residual + y
+
+
 def linear_act(x: Tensor, weight: Tensor, bias: Tensor = None, residual: Tensor = None, activation: str = "none") -> Tensor:
     """``act(x W^T + bias) + residual`` for ``x [..., K]``, ``weight [N, K]``, ``bias [N]`` and ``residual [..., N]``, K and N
     multiples of 8; ``activation``: "none", "relu", "silu" or "gelu_tanh".  fp32 sums and epilogue, one rounding to bf16."""
     x, res, after = _inputs("linear_act", x, residual)
-    y = linear_ops.linear(x, weight, bias, res, activation)
-    return y if after is None else after + y
+    return _add("linear_act", after, linear_ops.linear(x, weight, bias, res, activation))
 
 
 def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, residual: Tensor = None,
@@ -48,8 +56,7 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, residual:
     and the result are rounded to bf16 once each.  With gradients the block keeps the hidden layer (bf16) and both first
     products (24 bits each): 8 bytes per hidden value."""
     x, res, after = _inputs("gated_ffn", x, residual)
-    y = linear_ops.gated(x, w_gate, w_up, w_down, res, activation)
-    return y if after is None else after + y
+    return _add("gated_ffn", after, linear_ops.gated(x, w_gate, w_up, w_down, res, activation))
 
 
 class SwiGLU(nn.Module):
@@ -67,5 +74,4 @@ class SwiGLU(nn.Module):
             raise RuntimeError("transformer_amd.SwiGLU runs on a ROCm GPU only (no CPU path)")
         if all(training.plain_linear(m) for m in (self.w1, self.w2, self.w3)):
             return gated_ffn(x, self.w1.weight, self.w3.weight, self.w2.weight, residual)
-        y = self.w2(F.silu(self.w1(x)) * self.w3(x))
-        return y if residual is None else residual + y
+        return _add("SwiGLU", residual, self.w2(F.silu(self.w1(x)) * self.w3(x)))
