@@ -169,3 +169,29 @@ def test_residuals_of_another_shape_are_refused_in_every_type(shape):
                 with pytest.raises(ValueError, match="residual"):
                     call(bad)
                 assert call(good).shape == x.shape and call(good).dtype == dt
+
+
+@pytest.mark.parametrize("dims,weights,rows,amp", [
+    ((72, 136), torch.float32, torch.float32, None), ((72, 136), torch.float16, torch.float16, None),
+    ((20, 36), torch.bfloat16, torch.bfloat16, None), ((72, 140), torch.bfloat16, torch.bfloat16, None),
+    ((72, 136), torch.float64, torch.float64, None), ((72, 136), torch.float32, torch.bfloat16, torch.float16),
+    ((72, 136), torch.float32, torch.float32, torch.float16), ((20, 136), torch.float32, torch.float32, torch.bfloat16),
+    ((72, 136), torch.float16, torch.float32, torch.bfloat16)])
+def test_blocks_that_the_kernels_do_not_take_run_in_torch(dims, weights, rows, amp):
+    import torch.nn.functional as F
+    from transformer_amd import SwiGLU
+    torch.manual_seed(6)
+    with torch.device("cuda"):
+        m = SwiGLU(*dims).to(weights)
+    g = T.gen("torch", dims)
+    x, r, dy = (torch.randn(2, 30, dims[0], generator=g, device="cuda").to(rows) for _ in range(3))
+
+    def run(f):
+        leaf = x.clone().requires_grad_()
+        with torch.autocast("cuda", dtype=amp or torch.bfloat16, enabled=amp is not None):
+            y = f(leaf)
+        return [y, *torch.autograd.grad(y, (leaf, *m.parameters()), dy.to(y.dtype))]
+
+    for got, want in ((run(m), run(lambda t: m.w2(F.silu(m.w1(t)) * m.w3(t)))),
+                      (run(lambda t: m(t, r)), run(lambda t: r + m.w2(F.silu(m.w1(t)) * m.w3(t))))):
+        assert all(a.dtype == c.dtype and torch.equal(a, c) for a, c in zip(got, want))

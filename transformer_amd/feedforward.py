@@ -24,7 +24,7 @@ def _inputs(op: str, x: Tensor, residual):
     if not x.is_cuda:
         raise RuntimeError(f"transformer_amd.{op} runs on a ROCm GPU only (no CPU path)")
     if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16 \
-            and x.dtype in (torch.bfloat16, torch.float16, torch.float32):
+            and x.dtype in training._AUTOCAST_INPUTS:
         x = x.to(torch.bfloat16)
         if residual is not None and residual.dtype != torch.bfloat16:
             return x, None, residual
@@ -61,7 +61,9 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, residual:
 
 class SwiGLU(nn.Module):
     """``w2(silu(w1 x) * w3 x)`` (transformer.py:117-125); ``forward(x, residual)`` adds the block's residual stream in the
-    second product's epilogue.  Layers that are not plain ``nn.Linear`` (hooks, adapters, a parametrization) run as they are."""
+    second product's epilogue.  What the kernels do not take runs through the layers as they are, in torch: layers that are not
+    plain ``nn.Linear`` (hooks, adapters, a parametrization), other arithmetic than bf16 (fp32 or fp16 without bf16 autocast,
+    fp16 autocast), sizes that are not multiples of 8."""
 
     def __init__(self, dim: int, hidden: int):
         super().__init__()
@@ -69,9 +71,21 @@ class SwiGLU(nn.Module):
         self.w2 = nn.Linear(hidden, dim, bias=False)
         self.w3 = nn.Linear(dim, hidden, bias=False)
 
+    def _fits(self, x: Tensor) -> bool:
+        """Whether the kernels take the layers and ``x``."""
+        if not all(training.plain_linear(m) for m in (self.w1, self.w2, self.w3)):
+            return False
+        if torch.is_autocast_enabled("cuda"):
+            ok = torch.get_autocast_dtype("cuda") == torch.bfloat16 and x.dtype in training._AUTOCAST_INPUTS
+        else:
+            ok = x.dtype == torch.bfloat16
+        w = self.w1.weight
+        return ok and w.size(0) % 8 == 0 and w.size(1) % 8 == 0 \
+            and all(m.weight.dtype in (torch.bfloat16, torch.float32) for m in (self.w1, self.w2, self.w3))
+
     def forward(self, x: Tensor, residual: Tensor = None) -> Tensor:
         if not x.is_cuda:
             raise RuntimeError("transformer_amd.SwiGLU runs on a ROCm GPU only (no CPU path)")
-        if all(training.plain_linear(m) for m in (self.w1, self.w2, self.w3)):
+        if self._fits(x):
             return gated_ffn(x, self.w1.weight, self.w3.weight, self.w2.weight, residual)
         return _add("SwiGLU", residual, self.w2(F.silu(self.w1(x)) * self.w3(x)))
