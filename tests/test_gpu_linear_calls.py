@@ -195,3 +195,40 @@ def test_blocks_that_the_kernels_do_not_take_run_in_torch(dims, weights, rows, a
     for got, want in ((run(m), run(lambda t: m.w2(F.silu(m.w1(t)) * m.w3(t)))),
                       (run(lambda t: m(t, r)), run(lambda t: r + m.w2(F.silu(m.w1(t)) * m.w3(t))))):
         assert all(a.dtype == c.dtype and torch.equal(a, c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 24, 40), (20, 264, 72), (64, 4104, 40), (65, 264, 128), (300, 1000, 64), (4090, 328, 4072),
+                                   (4750, 3496, 3144)])
+def test_an_fp32_bias_is_added_as_it_is(M, N, K):
+    from transformer_amd import linear_act
+    g = T.gen("fp32 bias", M, N, K)
+    x, w, dy = T.bf16(g, M, K), T.bf16(g, N, K, std=K ** -0.5), T.bf16(g, M, N)
+    b = torch.randn(N + 1, generator=g, device="cuda")[1:]  # (off 16 bytes)
+    r = (-b).bfloat16().expand(M, N)
+    # without a product: what is left of the bias once its own bf16 value is taken away, rounded once
+    assert torch.equal(linear_act(torch.zeros_like(x), w, b, r), (b + r.float()).bfloat16())
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = linear_act(*leaves, r, "silu")
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    z = x.double() @ w.double().t() + b.double()
+    mag = x.double().abs() @ w.double().abs().t() + b.double().abs()
+    ref = T.act64(z, "silu") + r.double()
+    T.within(y.detach(), ref, 1.13 * mag * (K + 8) * T.EPS32 + T.act_error(z) + ref.abs() * T.EPS32, "y")
+    dz = dy.double() * T.slope64(z, "silu")
+    assert db.dtype == torch.float32 and y.dtype == torch.bfloat16
+    # (z kept to 24 bits, a slope's derivative below 1 / 2, fp32 sums)
+    T.within(db, dz.sum(0), (dy.double().abs() * (z.abs() * 2.0 ** -16 + mag * (K + 8) * T.EPS32 + 16 * T.EPS32 * (1 + z.abs()) ** 2)
+                             + dz.abs() * (M + 8) * T.EPS32).sum(0), "db")
+    if min(M, N, K) >= 20:
+        T.near(dx, dz @ w.double(), "dx")
+        T.near(dw, dz.t() @ x.double(), "dw")
+
+
+def test_a_compiled_block():
+    from transformer_amd import SwiGLU
+    torch.manual_seed(8)
+    m = SwiGLU(72, 136).cuda().bfloat16()
+    x, dy = T.bf16(T.gen("block"), 50, 72), T.bf16(T.gen("block dy"), 50, 72)
+    compiled = torch.compile(m, backend="aot_eager", fullgraph=True)
+    want, got = (torch.autograd.grad(f(x, x), tuple(m.parameters()), dy) for f in (m, compiled))
+    assert all(torch.equal(a, c) for a, c in zip(got, want))

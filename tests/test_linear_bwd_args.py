@@ -76,3 +76,14 @@ def test_parts_of_a_weight_lie_within_the_kernels_reach():
                 n = linear_ops._columns(rows, cols, stride)
                 assert (rows + 64) * n < linear_ops.REACH  # (as mla_linear_dx and mla_gated_linear_bwd ask of a contiguous one)
                 assert n == cols or (n >= 256 and n % 256 == 0 and (rows + 64) * cols >= linear_ops.REACH)
+
+
+def test_a_bias_is_refused_off_its_alignment_or_in_another_type():
+    import ctypes
+    from tests.test_linear_args import BASE
+    from transformer_amd import _lib
+    lib, (struct, good) = _lib.load(), BASE["mla_linear_act"]
+    for change in (dict(bias=4096, bias_dtype=2), dict(bias=4096, bias_dtype=-1), dict(bias=4104, bias_dtype=1),
+                   dict(bias=4100, bias_dtype=0), dict(bias=4100, bias_dtype=1)):
+        assert lib.mla_linear_act(ctypes.byref(struct(**{**good, **change})), None) < 0, change
+        assert b"bias" in lib.mla_last_error()

@@ -180,7 +180,7 @@ class LinearActArgs(ctypes.Structure):
         ("x", c_void_p), ("w", c_void_p), ("bias", c_void_p), ("residual", c_void_p), ("y", c_void_p), ("saved", c_void_p),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t),
         ("M", c_int64), ("N", c_int64), ("K", c_int64), ("x_stride", c_int64), ("w_stride", c_int64),
-        ("residual_stride", c_int64), ("y_stride", c_int64), ("activation", c_int32),
+        ("residual_stride", c_int64), ("y_stride", c_int64), ("activation", c_int32), ("bias_dtype", c_int32),
     ]
 
 

@@ -15,12 +15,20 @@ namespace mla {
 
 struct LinearParams {
   GemmArgs g;
-  const bf16* bias;
+  const void* bias;
   const bf16* residual;
   bf16* y;
   unsigned char* saved;
   int64_t rs, ys;
+  bool bias_f32;
 };
+
+// bias[n .. n + 3], n a multiple of 4
+__device__ __forceinline__ f32x4 linear_bias(const LinearParams& p, int n) {
+  if (p.bias_f32) return __builtin_bit_cast(f32x4, ldg16((const float*)p.bias + n));
+  const u32x2 b = ldg8((const bf16*)p.bias + n);
+  return f32x4{lo_bf16(b[0]), hi_bf16(b[0]), lo_bf16(b[1]), hi_bf16(b[1])};
+}
 
 // The epilogue of the blocks [j0, j1) of each wave
 template <class C, int ACT>
@@ -50,11 +58,9 @@ __device__ __forceinline__ void linear_epilogue(const LinearParams& p, GemmAcc<C
       if (p.bias) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const u32x2 b = ldg8(p.bias + n0 + min(nb + 8 * q + 4 * at.hk, nv - 4));  // (columns past the last are not stored)
-          a[4 * q] += lo_bf16(b[0]);
-          a[4 * q + 1] += hi_bf16(b[0]);
-          a[4 * q + 2] += lo_bf16(b[1]);
-          a[4 * q + 3] += hi_bf16(b[1]);
+          const f32x4 b = linear_bias(p, n0 + min(nb + 8 * q + 4 * at.hk, nv - 4));  // (columns past the last are not stored)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[4 * q + e] += b[e];
         }
       }
       const int mb = 32 * (C::XJ * at.wm + j);
@@ -106,10 +112,7 @@ __global__ __launch_bounds__(64 * kRcWaves) void linear_act_rows_kernel(LinearPa
   t.run(r, lds);
   if (!t.mine) return;
   f32x4 v = t.sum[0];
-  if (p.bias) {
-    const u32x2 b = ldg8(p.bias + t.n);
-    v += f32x4{lo_bf16(b[0]), hi_bf16(b[0]), lo_bf16(b[1]), hi_bf16(b[1])};
-  }
+  if (p.bias) v += linear_bias(p, t.n);
   if (p.saved) saved_store4(p.saved + ((int64_t)(t.m >> 5) * ((r.N + 31) >> 5) + (t.n >> 5)) * kSavedBlock, t.m, t.n, v);
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(v[e]);
@@ -171,7 +174,11 @@ static int linear_act_check(const mla_linear_act_args* a) {
   MLA_TRY(check_rows(op, "x", a->x, a->K, a->x_stride));
   MLA_TRY(check_rows(op, "w", a->w, a->K, a->w_stride));
   MLA_TRY(check_rows(op, "y", a->y, a->N, a->y_stride));
-  MLA_CHECK(((uintptr_t)a->bias & 7) == 0, MLA_ERR_INVALID_ARG, "%s: bias must be 8-byte aligned", op);
+  if (a->bias) {
+    MLA_CHECK(a->bias_dtype == MLA_DTYPE_BF16 || a->bias_dtype == MLA_DTYPE_F32, MLA_ERR_UNSUPPORTED, "%s: bias dtype", op);
+    const uintptr_t at = a->bias_dtype == MLA_DTYPE_F32 ? 16 : 8;
+    MLA_CHECK((uintptr_t)a->bias % at == 0, MLA_ERR_INVALID_ARG, "%s: bias must be %d-byte aligned", op, (int)at);
+  }
   if (a->residual) MLA_TRY(check_rows(op, "residual", a->residual, a->residual_stride ? a->N : 0, a->residual_stride));
   MLA_CHECK(((uintptr_t)a->saved & 15) == 0, MLA_ERR_INVALID_ARG, "%s: saved must be 16-byte aligned", op);
   return MLA_OK;
@@ -217,7 +224,8 @@ extern "C" int mla_linear_act(const mla_linear_act_args* a, void* stream) {
   p.g.x = (const bf16*)a->x, p.g.w0 = (const bf16*)a->w;
   p.g.xs = a->x_stride, p.g.ws0 = a->w_stride;
   p.g.M = (int)a->M, p.g.N = (int)a->N, p.g.K = (int)a->K, p.g.parts = 1;
-  p.bias = (const bf16*)a->bias;
+  p.bias = a->bias;
+  p.bias_f32 = a->bias_dtype == MLA_DTYPE_F32;
   p.residual = (const bf16*)a->residual;
   p.y = (bf16*)a->y;
   p.saved = (unsigned char*)a->saved;

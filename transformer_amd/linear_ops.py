@@ -133,12 +133,14 @@ def _saved_size(M: int, N: int) -> int:
 
 
 def _linear_run(op, x2, x_stride, weight, bias, residual, code, saved, y, M, N, K):
-    """``y = act(x2 weight^T + bias) + residual`` on bf16 rows as :func:`_rows` leaves them."""
+    """``y = act(x2 weight^T + bias) + residual`` on bf16 rows as :func:`_rows` leaves them; bias contiguous, aligned to four of
+    its elements."""
     w, w_stride = _weight_rows(weight, K)
     res2, r_stride = (None, 0) if residual is None else _rows(residual, N, True)
     args = _lib.LinearActArgs(
         x2.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(), None if res2 is None else res2.data_ptr(),
-        y.data_ptr(), None if saved is None else saved.data_ptr(), None, 0, M, N, K, x_stride, w_stride, r_stride, N, code)
+        y.data_ptr(), None if saved is None else saved.data_ptr(), None, 0, M, N, K, x_stride, w_stride, r_stride, N, code,
+        0 if bias is None else _dt_code(bias))
     ws = _fit_workspace("mla_linear_act_workspace_bytes", args, y) if M > ROWS_MAX else None  # noqa: F841  (kept until the launch)
     _launch("mla_linear_act", args, y, op)
 
@@ -162,8 +164,8 @@ def _linear_act(x, weight, bias, residual, activation, save):
     if M:
         b = bias
         if b is not None:
-            b = b.to(_BF16).contiguous()
-            if b.data_ptr() % 8:
+            b = b.contiguous()
+            if b.data_ptr() % (4 * b.element_size()):
                 b = b.clone()
         _linear_run(op, x2, x_stride, weight, b, residual, code, saved, y, M, N, K)
     return y, saved
@@ -173,7 +175,7 @@ def _linear_act(x, weight, bias, residual, activation, save):
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], activation: str,
                save: bool) -> Tuple[Tensor, Tensor]:
     """``y = act(x W^T + bias) + residual`` for bf16 ``x [..., K]``, ``weight [N, K]`` (bf16, or fp32 read as bf16), ``bias
-    [N]``, ``residual [..., N]`` bf16: fp32 sums and epilogue, one rounding.  ``activation``: none, relu, silu, gelu_tanh.
+    [N]`` (bf16 or fp32), ``residual [..., N]`` bf16: fp32 sums and epilogue, one rounding.  ``activation``: none, relu, silu, gelu_tanh.
     Returns ``y`` and, with ``save`` and an activation, what the backward keeps of the pre-activation (else an empty
     tensor).  K and N multiples of 8."""
     y, saved = _linear_act(x, weight, bias, residual, activation, save)
