@@ -23,11 +23,19 @@ struct LinearParams {
   bool bias_f32;
 };
 
-// bias[n .. n + 3], n a multiple of 4
-__device__ __forceinline__ f32x4 linear_bias(const LinearParams& p, int n) {
-  if (p.bias_f32) return __builtin_bit_cast(f32x4, ldg16((const float*)p.bias + n));
-  const u32x2 b = ldg8((const bf16*)p.bias + n);
-  return f32x4{lo_bf16(b[0]), hi_bf16(b[0]), lo_bf16(b[1]), hi_bf16(b[1])};
+// b[q] = bias[n .. n + 3] for n = at(q), a multiple of 4
+template <int Q, class At>
+__device__ __forceinline__ void linear_bias(const LinearParams& p, f32x4 (&b)[Q], At&& at) {
+  if (p.bias_f32) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) b[q] = __builtin_bit_cast(f32x4, ldg16((const float*)p.bias + at(q)));
+  } else {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const u32x2 v = ldg8((const bf16*)p.bias + at(q));
+      b[q] = f32x4{lo_bf16(v[0]), hi_bf16(v[0]), lo_bf16(v[1]), hi_bf16(v[1])};
+    }
+  }
 }
 
 // The epilogue of the blocks [j0, j1) of each wave
@@ -55,13 +63,11 @@ __device__ __forceinline__ void linear_epilogue(const LinearParams& p, GemmAcc<C
     for (int i = 0; i < C::NB; ++i) {
       f32x16 a = acc.a[i][j];
       const int nb = (at.wn * C::NB + i) * 32;  // the block's first column within the tile
-      if (p.bias) {
+      if (p.bias) {  // (columns past the last are not stored; one branch on the type a block, whose loads go out together)
+        f32x4 b[4];
+        linear_bias(p, b, [&](int q) { return n0 + min(nb + 8 * q + 4 * at.hk, nv - 4); });
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 b = linear_bias(p, n0 + min(nb + 8 * q + 4 * at.hk, nv - 4));  // (columns past the last are not stored)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) a[4 * q + e] += b[e];
-        }
+        for (int e = 0; e < 16; ++e) a[e] += b[e >> 2][e & 3];
       }
       const int mb = 32 * (C::XJ * at.wm + j);
       if (p.saved && mb < mv && nb < nv)
@@ -112,7 +118,11 @@ __global__ __launch_bounds__(64 * kRcWaves) void linear_act_rows_kernel(LinearPa
   t.run(r, lds);
   if (!t.mine) return;
   f32x4 v = t.sum[0];
-  if (p.bias) v += linear_bias(p, t.n);
+  if (p.bias) {
+    f32x4 b[1];
+    linear_bias(p, b, [&](int) { return t.n; });
+    v += b[0];
+  }
   if (p.saved) saved_store4(p.saved + ((int64_t)(t.m >> 5) * ((r.N + 31) >> 5) + (t.n >> 5)) * kSavedBlock, t.m, t.n, v);
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(v[e]);

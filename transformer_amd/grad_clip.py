@@ -165,7 +165,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     if not grads:
         return torch.tensor(0.0)
     flat, codes = _laid_out(op, grads)
-    if any(g is not c for g, c in zip(grads, flat)):  # (the entry point would compare the copies)
+    if flat is not grads and any(g is not c for g, c in zip(grads, flat)):  # (the entry point would compare the copies)
         _refuse_shared(op, grads)
     if error_if_nonfinite:
         norm = _run(op, "mla_grad_norm", flat, codes, is_max, 0.0)
