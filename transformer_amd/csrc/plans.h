@@ -171,4 +171,8 @@ inline GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int64_t parts) {
   return best;
 }
 
+// ---- rows_core.h's columns of a workgroup: 16, or 32 where 16 would make a second round (a CU alone moves several times its
+// share of the memory's rate, and the wider workgroup reads x half as often).
+inline int rows_columns(int64_t N) { return N <= 16 * 256 ? 16 : 32; }
+
 }  // namespace mla

@@ -133,10 +133,6 @@ struct RowsProduct {
   }
 };
 
-// Columns of a workgroup: 16, or 32 where 16 would make a second round (a CU alone moves several times its share of the
-// memory's rate, and the wider workgroup reads x half as often).
-inline int rows_columns(int64_t N) { return N <= 16 * 256 ? 16 : 32; }
-
 // the 4 consecutive n that a lane holds, in the layout of act.h's blocks
 __device__ __forceinline__ void saved_store4(unsigned char* block, int m, int n, const f32x4& v) {
   const int lane = 32 * ((n >> 2) & 1) + (m & 31), e = 4 * ((n & 31) >> 3);
