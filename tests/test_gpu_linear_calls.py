@@ -232,3 +232,27 @@ def test_a_compiled_block():
     compiled = torch.compile(m, backend="aot_eager", fullgraph=True)
     want, got = (torch.autograd.grad(f(x, x), tuple(m.parameters()), dy) for f in (m, compiled))
     assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_the_operators_without_rows_and_without_what_they_keep():
+    ops = torch.ops.mla_mi355x
+    z = lambda *s: torch.zeros(*s, device="cuda").bfloat16().requires_grad_()
+    for shape in ((0, 16), (2, 0, 16)):
+        x, w, wd, b = z(*shape), z(24, 16), z(16, 24), z(24)
+        for save in (False, True):
+            for y, of in ((ops.gated_ffn(x, w, w, wd, None, "silu", save)[0], (x, w, wd)),
+                          (ops.linear_act(x, w, b, None, "silu", save)[0], (x, w, b))):
+                got = torch.autograd.grad(y, of, torch.zeros_like(y))
+                assert all(t.shape == o.shape and not t.any() for t, o in zip(got, of))
+
+
+def test_one_row_of_one_dimension():
+    from transformer_amd import gated_ffn, linear_act
+    g = T.gen("one row")
+    x, w, wd, b, r = T.bf16(g, 72), T.bf16(g, 136, 72, std=0.1), T.bf16(g, 72, 136, std=0.1), T.bf16(g, 136), T.bf16(g, 136)
+    for f, dy in ((lambda t: linear_act(t, w, b, r.view(*t.shape[:-1], 136), "silu"), T.bf16(g, 136)),
+                  (lambda t: gated_ffn(t, w, w, wd, t), T.bf16(g, 72))):
+        one, row = x.clone().requires_grad_(), x.view(1, 72).clone().requires_grad_()
+        y, want = f(one), f(row)
+        assert y.dim() == 1 and torch.equal(y, want[0])
+        assert torch.equal(torch.autograd.grad(y, one, dy)[0], torch.autograd.grad(want, row, dy.view(1, -1))[0][0])

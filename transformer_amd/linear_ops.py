@@ -463,7 +463,7 @@ def _gated_ffn_grads(ctx, dy, need):
     """The gradients for (x, w_gate, w_up, w_down) from the saved tensors of either autograd path."""
     x, w_gate, w_up, w_down, h, saved = ctx.saved_tensors
     plain = _plain_backward(dy)
-    if not saved.numel() and x.numel():  # not kept: the first half again
+    if not saved.numel():  # not kept: the first half again (without rows: h's shape)
         _, h, saved = torch.ops.mla_mi355x.gated_ffn(x.detach(), w_gate.detach(), w_up.detach(), w_down.detach(), None,
                                                      ctx.activation, True)
     run = _gated_ffn_bwd if plain else torch.ops.mla_mi355x.gated_ffn_bwd
