@@ -234,6 +234,18 @@ def test_a_compiled_block():
     assert all(torch.equal(a, c) for a, c in zip(got, want))
 
 
+def test_a_block_whose_last_layer_has_another_width_runs_in_torch():
+    import torch.nn.functional as F
+    from transformer_amd import SwiGLU
+    torch.manual_seed(9)
+    with torch.device("cuda"):
+        m = SwiGLU(72, 136)
+        m.w2 = torch.nn.Linear(136, 40, bias=False)
+        m.bfloat16()
+        x = torch.randn(30, 72).bfloat16()
+    assert torch.equal(m(x), m.w2(F.silu(m.w1(x)) * m.w3(x)))
+
+
 def test_the_operators_without_rows_and_without_what_they_keep():
     ops = torch.ops.mla_mi355x
     z = lambda *s: torch.zeros(*s, device="cuda").bfloat16().requires_grad_()

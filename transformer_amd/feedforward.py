@@ -63,7 +63,7 @@ class SwiGLU(nn.Module):
     """``w2(silu(w1 x) * w3 x)`` (transformer.py:117-125); ``forward(x, residual)`` adds the block's residual stream in the
     second product's epilogue.  What the kernels do not take runs through the layers as they are, in torch: layers that are not
     plain ``nn.Linear`` (hooks, adapters, a parametrization), other arithmetic than bf16 (fp32 or fp16 without bf16 autocast,
-    fp16 autocast), sizes that are not multiples of 8."""
+    fp16 autocast), sizes that are not multiples of 8, a layer replaced by one of another shape."""
 
     def __init__(self, dim: int, hidden: int):
         super().__init__()
@@ -79,9 +79,9 @@ class SwiGLU(nn.Module):
             ok = torch.get_autocast_dtype("cuda") == torch.bfloat16 and x.dtype in training._AUTOCAST_INPUTS
         else:
             ok = x.dtype == torch.bfloat16
-        w = self.w1.weight
-        return ok and w.size(0) % 8 == 0 and w.size(1) % 8 == 0 \
-            and all(m.weight.dtype in (torch.bfloat16, torch.float32) for m in (self.w1, self.w2, self.w3))
+        w1, w2, w3 = self.w1.weight, self.w2.weight, self.w3.weight
+        return ok and w1.shape == w3.shape == w2.shape[::-1] and w1.size(0) % 8 == 0 and w1.size(1) % 8 == 0 and w1.numel() > 0 \
+            and all(w.dtype in (torch.bfloat16, torch.float32) for w in (w1, w2, w3))
 
     def forward(self, x: Tensor, residual: Tensor = None) -> Tensor:
         if not x.is_cuda:
