@@ -129,7 +129,7 @@ def test_gradients_through_weights_in_parts(M, H, D, monkeypatch):
     launch = linear_ops._launch
     monkeypatch.setattr(linear_ops, "_launch", lambda entry, *a: launches.append(entry) or launch(entry, *a))
     _gradients_of_few_rows(g, *t)
-    parts = {"mla_linear_dx": -(-D // linear_ops._columns(H, D, D)), "mla_gated_linear_bwd": -(-H // linear_ops._columns(D, H, H))}
+    parts = {"mla_linear_dx": -(-D // linear_ops._columns(H, D)), "mla_gated_linear_bwd": -(-H // linear_ops._columns(D, H))}
     assert min(parts.values()) > 1
     assert launches.count("mla_linear_dx") == 2 * parts["mla_linear_dx"]  # (linear_act's and the gated block's)
     assert launches.count("mla_gated_linear_bwd") == parts["mla_gated_linear_bwd"]

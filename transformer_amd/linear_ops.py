@@ -111,8 +111,8 @@ def _refuse(op: str, x: Tensor, weights, names, residual: Optional[Tensor], n_ou
                      f"{residual.device}")
 
 
-def _check_bwd(op: str, fits: bool, x: Tensor, dy: Tensor, weights, saved: Optional[Tensor], h: Optional[Tensor] = None) -> None:
-    """What a backward's launches take for granted, before the first of them; ``fits``: whether the shapes belong together."""
+def _refuse_bwd(op: str, fits: bool, x: Tensor, dy: Tensor, weights, saved: Optional[Tensor], h: Optional[Tensor] = None) -> None:
+    """The error of a backward's operands that its launches must not see; ``fits``: whether the shapes belong together."""
     if not fits:
         raise ValueError(f"{op}: dy {tuple(dy.shape)}, x {tuple(x.shape)}, weights {[tuple(w.shape) for w in weights]}"
                          f"{'' if h is None else f', h {tuple(h.shape)}'} and saved "
@@ -122,10 +122,8 @@ def _check_bwd(op: str, fits: bool, x: Tensor, dy: Tensor, weights, saved: Optio
         raise TypeError(f"{op}: x and h must be bfloat16, weights bfloat16 or float32 and saved uint8")
     if any(t is not None and not t.is_contiguous() for t in (h, saved)):
         raise ValueError(f"{op}: h and saved must be contiguous")
-    dev = x.get_device()
-    if dev < 0 or any(t is not None and t.get_device() != dev for t in (dy, *weights, h, saved)):
-        kernels._require_gpu(op, x, dy, *weights, h, saved)
-        raise ValueError(f"{op}: all tensors must be on one device")
+    kernels._require_gpu(op, x, dy, *weights, h, saved)
+    raise ValueError(f"{op}: all tensors must be on one device")
 
 
 def _saved_size(M: int, N: int) -> int:
@@ -214,12 +212,10 @@ def _weight_grad(dy: Tensor, sy: int, x: Tensor, sx: int, dtype: torch.dtype) ->
     return dw.to(dtype)
 
 
-def _columns(rows: int, cols: int, stride: int) -> int:
-    """How many of the columns of a weight that is read across its rows one call takes: all of them, as they lie or closer
-    together, or else whole blocks of 256 within its reach, copied."""
-    if (rows + 64) * min(stride, cols) < REACH:
-        return cols
-    return (REACH - 1) // (rows + 64) // 256 * 256
+def _columns(rows: int, cols: int) -> int:
+    """How many of the columns of a weight that is read across its rows one call takes from a copy: all of them, or whole
+    blocks of 256 within its reach."""
+    return cols if (rows + 64) * cols < REACH else (REACH - 1) // (rows + 64) // 256 * 256
 
 
 def _linear_dx(op: str, dy: Tensor, sy: int, weights, shape) -> Tensor:
@@ -228,17 +224,16 @@ def _linear_dx(op: str, dy: Tensor, sy: int, weights, shape) -> Tensor:
     dx = dy.new_empty(shape)
     if not M:
         return dx
-    given = [_weight_rows(w, K) for w in weights]
-    cols = _columns(N, K, max(s for _, s in given))
+    w0, s0 = _weight_rows(weights[0], K)
+    w1, s1 = _weight_rows(weights[1], K) if len(weights) > 1 else (None, s0)
+    as_they_lie = s1 == s0 and (N + 64) * s0 < REACH  # (one stride for both)
+    cols = K if as_they_lie else _columns(N, K)
     for c in range(0, K, cols):
-        n = min(cols, K - c)
-        if n < K or len({s for _, s in given}) > 1 or (N + 64) * given[0][1] >= REACH:  # (one stride for both)
-            part = [(w[:, c:c + n].contiguous(), n) for w, _ in given]
-        else:
-            part = given
-        (w0, s), w1 = part[0], part[1][0] if len(part) > 1 else None
-        args = _lib.LinearDxArgs(dy.data_ptr(), w0.data_ptr(), None if w1 is None else w1.data_ptr(), dx.data_ptr() + 2 * c, None, 0,
-                                 M, N, n, sy, s, 0 if w1 is None else s, K)
+        n, s, p0, p1 = min(cols, K - c), s0, w0, w1
+        if not as_they_lie:
+            s, p0, p1 = n, w0[:, c:c + n].contiguous(), None if w1 is None else w1[:, c:c + n].contiguous()
+        args = _lib.LinearDxArgs(dy.data_ptr(), p0.data_ptr(), None if p1 is None else p1.data_ptr(), dx.data_ptr() + 2 * c, None, 0,
+                                 M, N, n, sy, s, 0 if p1 is None else s, K)
         ws = _fit_workspace("mla_linear_dx_workspace_bytes", args, dx)  # noqa: F841  (kept until the launch)
         _launch("mla_linear_dx", args, dx, op)
     return dx
@@ -251,9 +246,14 @@ def _linear_act_bwd(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype
     if db_dtype is not None and db_dtype != _BF16 and db_dtype != _F32:
         raise TypeError(f"{op}: db_dtype must be bfloat16 or float32, got {db_dtype}")
     N, K = weight.shape if weight.dim() == 2 else (0, 0)
-    M = x.numel() // K if K else 0
-    _check_bwd(op, N > 0 and x.dim() > 0 and x.size(-1) == K and dy.shape == (*x.shape[:-1], N)
-               and (not code or saved.numel() == _saved_size(M, N)), x, dy, (weight,), saved if code else None)
+    M, dev = x.numel() // K if K else 0, x.get_device()
+    # (without generators: a training pass of few rows is bound by the host)
+    fits = N > 0 and x.dim() > 0 and x.size(-1) == K and dy.shape == (*x.shape[:-1], N) \
+        and (not code or saved.numel() == _saved_size(M, N))
+    if not (fits and x.dtype == _BF16 and (weight.dtype == _BF16 or weight.dtype == _F32)
+            and 0 <= dev == dy.get_device() == weight.get_device()
+            and (not code or (saved.dtype == torch.uint8 and saved.is_contiguous() and saved.get_device() == dev))):
+        _refuse_bwd(op, fits, x, dy, (weight,), saved if code else None)
     (dy2, sy), (x2, sx) = _weight_rows(dy, N), _rows(x, K)
     dz, db = dy2, None
     if db_dtype is not None:
@@ -288,7 +288,9 @@ def _(dy, x, weight, saved, activation, need_dx, need_dw, db_dtype):
 
 def _plain_backward(dy: Tensor) -> bool:
     """Whether a backward may run the bodies: it is not itself differentiated, batched, traced or under a dispatch mode."""
-    return not (torch.is_grad_enabled() or type(dy) is not Tensor or kernels.batched_grad(dy) or kernels._not_plain((dy,)))
+    return not (torch.is_grad_enabled() or type(dy) is not Tensor or kernels.batched_grad(dy)
+                or torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() > 0
+                or torch._C._functorch.peek_interpreter_stack() is not None)
 
 
 def _linear_act_grads(ctx, dy, need):
@@ -400,13 +402,14 @@ def _gated_grads(op, dy, sy, w_down, saved, dgu, code):
     """The gradients ``dgu [M, 2 H]`` of both first products from bf16 rows ``dy [M, D]`` of stride ``sy`` and what they saved."""
     (D, H), M = w_down.shape, dy.size(0)
     wd, sd = _weight_rows(w_down, H)
-    cols = _columns(D, H, sd)
-    if (D + 64) * sd >= REACH and cols == H:
-        wd, sd = wd.contiguous(), H
+    as_it_lies = (D + 64) * sd < REACH
+    cols = H if as_it_lies else _columns(D, H)
     for c in range(0, H, cols):
         n, w, s, kept, out = min(cols, H - c), wd, sd, saved, dgu
+        if not as_it_lies:
+            w, s = wd[:, c:c + n].contiguous(), n
         if n < H:  # (the blocks of the kept values that lie in these columns)
-            w, s, out = wd[:, c:c + n].contiguous(), n, dgu.new_empty((M, 2 * n))
+            out = dgu.new_empty((M, 2 * n))
             kept = saved.view((M + 31) // 32, (H + 31) // 32, -1)[:, c // 32:(c + n + 31) // 32].contiguous()
         args = _lib.GatedLinearBwdArgs(dy.data_ptr(), w.data_ptr(), kept.data_ptr(), out.data_ptr(), M, n, D, sy, s, 2 * n, code)
         _launch("mla_gated_linear_bwd", args, out, op)
@@ -419,10 +422,15 @@ def _gated_ffn_bwd(dy, x, w_gate, w_up, w_down, h, saved, activation, need_dx, n
     op = "mla_mi355x::gated_ffn_bwd"
     code = _activation(op, activation, gate=True)
     H, D = w_gate.shape if w_gate.dim() == 2 else (0, 0)
-    M = x.numel() // D if D else 0
-    _check_bwd(op, H > 0 and x.dim() > 0 and x.size(-1) == D and dy.shape == x.shape and w_up.shape == w_gate.shape
-               and w_down.shape == (D, H) and h.shape == (M, H) and saved.numel() == 2 * _saved_size(M, H),
-               x, dy, (w_gate, w_up, w_down), saved, h)
+    M, dev = x.numel() // D if D else 0, x.get_device()
+    fits = H > 0 and x.dim() > 0 and x.size(-1) == D and dy.shape == x.shape and w_up.shape == w_gate.shape \
+        and w_down.shape == (D, H) and h.shape == (M, H) and saved.numel() == 2 * _saved_size(M, H)
+    if not (fits and x.dtype == _BF16 and h.dtype == _BF16 and saved.dtype == torch.uint8 and h.is_contiguous()
+            and saved.is_contiguous() and (w_gate.dtype == _BF16 or w_gate.dtype == _F32)
+            and (w_up.dtype == _BF16 or w_up.dtype == _F32) and (w_down.dtype == _BF16 or w_down.dtype == _F32)
+            and 0 <= dev == dy.get_device() == w_gate.get_device() == w_up.get_device() == w_down.get_device()
+            == h.get_device() == saved.get_device()):
+        _refuse_bwd(op, fits, x, dy, (w_gate, w_up, w_down), saved, h)
     (dy2, sy), (x2, sx) = _weight_rows(dy, D), _rows(x, D)
     dx = dwg = dwu = None
     dwd = _weight_grad(dy2, sy, h, H, w_down.dtype) if need_down else None
