@@ -40,7 +40,8 @@ __device__ __forceinline__ void act_both(float z, float& value, float& slope) {
   }
 }
 
-// Pre-activations kept for a backward: the upper 24 bits of the fp32 value, as a 32 x 32 block's accumulators lie in the
+// Pre-activations kept for a backward: the upper 24 bits of the fp32 value (cut, not rounded: off by less than 2^-15 of it, a
+// hundredth of the bf16 rounding of what is computed from it, for no instruction), as a 32 x 32 block's accumulators lie in the
 // lanes (32 m x 32 n, see gemm_core.h): 2 x 16 bytes of upper halves and 16 bytes of the next 8 bits per lane, 3 KiB a block.
 // Written and read by whole 1 KiB runs straight from registers.  In bf16 they would cost 2 KiB and their rounding would add
 // to that of the gradients computed from them: an rms error of 1.7 to 2 times a single rounding's instead of 1.4.

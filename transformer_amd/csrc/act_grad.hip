@@ -1,4 +1,5 @@
-// The gradient of a linear layer's epilogue (gfx950): dz = bf16(dy act'(z)) from the z that the forward kept, and the bias
+// The gradient of a linear layer's epilogue (gfx950): dz = bf16(dy act'(z)) from the z that the forward kept (rounded because the
+// products that follow take bf16 operands; the bias gradient is summed from the fp32 values), and the bias
 // gradient db = sum over rows of dy act'(z), in one pass over dy.  HBM bound: 2 + 3 bytes read and 2 written per element.
 //
 // A wave owns 32 columns and walks 32-row blocks, a lane one row's four quads of a block, as z was kept (act.h).  A lane

@@ -5,6 +5,10 @@
 // One kernel for both products reads x once and leaves h alone: apart, g and u would be written and read again (12288 x 4608:
 // 453 MB of traffic more).  12288 rows, 1792 -> 2 x 4608, us: 331 without and 378 with the kept g and u (340 MB; 1070 TFLOP/s),
 // backward 279 (730 TFLOP/s beside 340 MB of kept values read and 226 MB stored).
+//
+// Rounded to bf16 once each: h, dg and du, because the next products' matrix instructions take bf16 operands (fp32 ones would
+// run at a sixteenth of the rate and move twice the bytes).  Relative rms of y against 64 bits 0.0018 to 0.0019 (a lone rounding of
+// y 0.0017), of the gradients 0.0023 to 0.0024 (0.0017).
 #include "gemm_epilogue.h"
 #include "linear_checks.h"
 #include "rows_core.h"

@@ -146,6 +146,11 @@ struct GemmPlan {
 // 17 % more, without the tiles of 256 x 128 2 %, without those of 128 x 128 9 %.  Examples (us; 128 x 128, 256 x 128, 256 x 256):
 // 1999 x 2048 over 4608 50, 61, 97; 3001 x 2048 over 5464 101, 85, 114 (95 in two pieces); 12288 x 9216 over 1792 430, 426, 365;
 // 12288 x 1792 over 2 x 4608 430, 403, 413 (348 in three pieces); 159 x 6080 over 5176 47, 62, 98 (31 in four pieces of 128 x 128).
+// The timings are of products with a plain store, K a multiple of 64, operands near the caches.  Elsewhere calls take longer than
+// estimated (estimate, call): 2500 x 1000 over 1800 with bias and silu 15, 25 (over 1792 14, 21: rows that no 128 bytes divide);
+// 1999 x 2048 over 4608 40, 48; 12288 x 4608 over 1792 with kept values 191, 225; 12288 x 1792 over 2 x 4608 321, 359.  The choice
+// holds there too: in twelve such calls, kept values, activations and both directions among them, it was within 2 % of the fastest
+// tile (12288 x 4608 over 1792, gelu, kept: 240, 238, 224; profiles/linear_sizes.txt).
 inline GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int64_t parts) {
   GemmPlan best{};
   double best_t = 1e300;

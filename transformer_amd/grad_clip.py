@@ -153,8 +153,9 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
                     error_if_nonfinite: bool = False, foreach: bool = None) -> Tensor:
     """Scales the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))`` and returns their norm before
     that, as ``torch.nn.utils.clip_grad_norm_`` does; parameters without a gradient are passed over.  ``norm_type``: 2 or inf.
-    ``error_if_nonfinite`` waits for the norm and raises before anything is scaled.  ``foreach`` is accepted and ignored.
-    Gradients are fp32 or bf16 on one device; two that share memory are refused."""
+    ``error_if_nonfinite`` waits for the norm (one more pass over the gradients) and raises before anything is scaled.
+    ``foreach`` is accepted and ignored.  Gradients are fp32 or bf16 on one device, of any layout; two that share memory are
+    refused, and so is torch.jit.trace, which would not record the launches."""
     op = "clip_grad_norm_"
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
