@@ -474,10 +474,10 @@ size_t mla_linear_saved_size(int64_t M, int64_t N);
 /* A linear layer with its epilogue:
  *   z[m][n] = sum_k x[m][k] W[n][k] + bias[n],   y[m][n] = bf16(act(z[m][n]) + residual[m][n])
  * fp32 sums and epilogue, one rounding.  x [M, K], W [N, K] (an nn.Linear weight), residual and y [M, N]: bf16 rows with row
- * strides; bias [N] in bias_dtype (bf16 or fp32, added as it is) or NULL, residual or NULL (it may be y itself).  saved: NULL, or mla_linear_saved_size(M, N) bytes
- * that receive z for mla_act_grad.  N and K multiples of 8; all pointers 16-byte aligned (a bf16 bias 8), strides multiples of 8
- * that cover a row (residual's may also be 0: one row for all).  The workspace (mla_linear_act_workspace_bytes, 256-byte
- * aligned) holds fp32 partials where a product is cut along k.  Deterministic.
+ * strides; bias [N] in bias_dtype (bf16 or fp32, added as it is) or NULL, residual or NULL (it may be y itself).  saved: NULL,
+ * or mla_linear_saved_size(M, N) bytes that receive z for mla_act_grad.  N and K multiples of 8; all pointers 16-byte aligned
+ * (a bf16 bias 8), strides multiples of 8 that cover a row (residual's may also be 0: one row for all).  The workspace
+ * (mla_linear_act_workspace_bytes, 256-byte aligned) holds fp32 partials where a product is cut along k.  Deterministic.
  *
  * Replaces: o_proj with the block's residual sum (transformer.py:300, :348) and the feed-forward's second product with
  *           its own (:125, :351).

@@ -1,6 +1,6 @@
 // The gradient of a linear layer's epilogue (gfx950): dz = bf16(dy act'(z)) from the z that the forward kept (rounded because the
-// products that follow take bf16 operands; the bias gradient is summed from the fp32 values), and the bias
-// gradient db = sum over rows of dy act'(z), in one pass over dy.  HBM bound: 2 + 3 bytes read and 2 written per element.
+// products that follow take bf16 operands), and the bias gradient db = sum over rows of dy act'(z), of the fp32 values, in one
+// pass over dy.  HBM bound: 2 + 3 bytes read and 2 written per element.
 //
 // A wave owns 32 columns and walks 32-row blocks, a lane one row's four quads of a block, as z was kept (act.h).  A lane
 // adds its rows' gradients in fp32; at the end the 32 lanes of a column are added and the segment's sum stored.  A second

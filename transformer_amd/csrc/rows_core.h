@@ -7,10 +7,10 @@
 // instruction, in brackets): one row against 2 x 4608 x 1792 7.6 (10.3), 4.4 TB/s; 32 against 2 x 4608 x 2048 9.4 (18.0), 4.0
 // TB/s; 64 against 2 x 4608 x 1792 10.7 (22); one against 1792 x 4608 7.0 (7.3), 32 against 2048 x 4608 9.2 (14.3): 112 and 128
 // workgroups, whose chunks follow each other at the latency of the ring.
-// mla_linear_rows is the framework's other product of few rows: over groups, K a multiple of 128 up to 4096, no epilogue.  Against it
-// (replayed graphs, us, linear_rows in brackets) 1 row of 4608 x 1792 6.3 (6.1), 16 rows 6.4 (8.3), 64 rows 8.3 (22); 1 row of 9216
-// x 2048 14.2 (11.1), 32 rows 16.2 (20.6); 2048 x 2048 5.3 (4.7), 5.5 (6.1), 7.5 (8.8).  Neither calls the other: the decode step's
-// projections, which read the cache's rows beside them, keep linear_rows, and what has an epilogue or another K runs here.
+// mla_linear_rows is the framework's other product of few rows: over groups, K a multiple of 128 up to 4096, no epilogue.  Against
+// it (replayed graphs, us, linear_rows in brackets) 1 row of 4608 x 1792 6.3 (6.1), 16 rows 6.4 (8.3), 64 rows 8.3 (22); 1 row of 9216
+// x 2048 14.2 (11.1), 32 rows 16.2 (20.6); 2048 x 2048 5.3 (4.7), 5.5 (6.1), 7.5 (8.8).  The decode step keeps linear_rows (one of
+// its launches holds the RoPE append too); what has an epilogue or another K runs here.
 //
 // A staged row's chunk c of 16 bytes lies at c ^ (row mod 16): the 16 rows of a fragment fall on different banks.
 #pragma once

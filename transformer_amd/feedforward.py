@@ -7,7 +7,8 @@ in two: both first products with the activation and the product of the two, then
 reference's state-dict keys ``w1.weight``, ``w2.weight``, ``w3.weight``.
 
 Arithmetic is bf16 with fp32 sums: inputs are bf16, or anything that bf16 autocast casts; weights may be fp32 (read as bf16,
-their gradients fp32).  The gradients of ``w_gate`` and ``w_up`` are the halves of one allocation.  Under autocast a residual stream in fp32 stays fp32: the sum with it is then torch's.
+their gradients fp32).  The gradients of ``w_gate`` and ``w_up`` are the halves of one allocation.  Under autocast a residual
+stream in fp32 stays fp32: the sum with it is then torch's.
 """
 from __future__ import annotations
 
@@ -44,7 +45,8 @@ def _add(op: str, residual, y: Tensor) -> Tensor:
 
 def linear_act(x: Tensor, weight: Tensor, bias: Tensor = None, residual: Tensor = None, activation: str = "none") -> Tensor:
     """``act(x W^T + bias) + residual`` for ``x [..., K]``, ``weight [N, K]``, ``bias [N]`` (bf16 or fp32, added as it is) and
-    ``residual [..., N]``, K and N multiples of 8; ``activation``: "none", "relu", "silu" or "gelu_tanh".  fp32 sums and epilogue, one rounding to bf16."""
+    ``residual [..., N]``, K and N multiples of 8; ``activation``: "none", "relu", "silu" or "gelu_tanh".  fp32 sums and
+    epilogue, one rounding to bf16."""
     x, res, after = _inputs("linear_act", x, residual)
     return _add("linear_act", after, linear_ops.linear(x, weight, bias, res, activation))
 

@@ -173,8 +173,8 @@ def _linear_act(x, weight, bias, residual, activation, save):
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], activation: str,
                save: bool) -> Tuple[Tensor, Tensor]:
     """``y = act(x W^T + bias) + residual`` for bf16 ``x [..., K]``, ``weight [N, K]`` (bf16, or fp32 read as bf16), ``bias
-    [N]`` (bf16 or fp32), ``residual [..., N]`` bf16: fp32 sums and epilogue, one rounding.  ``activation``: none, relu, silu, gelu_tanh.
-    Returns ``y`` and, with ``save`` and an activation, what the backward keeps of the pre-activation (else an empty
+    [N]`` (bf16 or fp32), ``residual [..., N]`` bf16: fp32 sums and epilogue, one rounding.  ``activation``: none, relu, silu,
+    gelu_tanh.  Returns ``y`` and, with ``save`` and an activation, what the backward keeps of the pre-activation (else an empty
     tensor).  K and N multiples of 8."""
     y, saved = _linear_act(x, weight, bias, residual, activation, save)
     return y, x.new_empty(0, dtype=torch.uint8) if saved is None else saved
