@@ -620,13 +620,127 @@ typedef struct {
 } mla_ce_chunk_args;
 int mla_ce_chunk(const mla_ce_chunk_args* a, void* stream);
 
+/* -------------------------------------------------------- paged cache --
+ * A latent cache in pages of `page_size` tokens (a multiple of 16, up to 4096), shared by many sequences.  A token's row is
+ * [latent | rotated keys], W = d_latent + 64 n_k_rope_heads values (head hr's key at d_latent + 64 hr), and position p of
+ * sequence b is row p % page_size of page block_table[b][p / page_size].
+ *   16 bits (scales NULL): pages is bf16 [n_pages][page_size][W].
+ *   4 bits:  pages is uint8 [n_pages][page_size][W / 2], value 2 i of a row in the low half of byte i, and scales bf16
+ *            [n_pages][W / 64][page_size]: run g of 64 values of a row (a rotated key is one run) stands for (code - 8) scale with
+ *            scale = bf16(max |x| / 7) and code = 8 + rint(x / scale) within 1 .. 15 (8 where the scale is 0).  A run with an
+ *            infinity or a NaN in it reads back as NaN.
+ * page_stride: bytes between pages; scale_stride: elements between their scales; rows of a page lie close together.
+ * block_table: int32 [B][table_pages], rows table_stride apart.  An entry outside [0, n_pages) is no page: nothing is written there,
+ * its tokens read as zeros and take no part in an attention.  Positions past table_pages * page_size do not exist.
+ * pages, scales: 16-byte aligned, page_stride a multiple of 16, scale_stride of 8.  d_latent in {64, 128, 256, 384, 512}.
+ * No two tokens of a call may be appended to one place of a page: which of them it then holds, or a mix, is not defined.
+ * No counterpart in the reference, whose cache is one tensor a batch of equally long sequences (transformer.py:215-218, :241-244).
+ */
+typedef struct {
+  void* pages;
+  void* scales;
+  const int32_t* block_table;
+  int64_t n_pages, page_size, page_stride, scale_stride, table_pages, table_stride, d_latent, n_k_rope_heads;
+} mla_paged_cache;
+
+/* RoPE of up to T new tokens a sequence with their append: for t < counts[b] (counts NULL: T) and p = starts[b] + t,
+ *   q heads 0 .. H-1 of qk    -> q_out[b][t][h]     (rotated at p; zeros for the other t)
+ *   k heads H .. H+Hr-1       -> the row of p       (rotated, rounded to bf16, then to 4 bits in a 4-bit cache)
+ *   c_new[b][t]               -> the row of p
+ * A token with p < 0, p >= table_rows or p >= table_pages * page_size is skipped, its q_out zero.  qk bf16 [B, T, H + Hr, 64]
+ * (qk_stride), c_new bf16 [B, T, d_latent] (c_new_sb, c_new_st), q_out bf16 [B, T, H, 64] contiguous; cos, sin bf16
+ * [table_rows, 32]; pointers 16-byte aligned, strides multiples of 8.
+ */
+typedef struct {
+  mla_paged_cache cache;
+  const void* qk;
+  const void* c_new;
+  void* q_out;
+  const void* cos;
+  const void* sin;
+  const int32_t* starts;
+  const int32_t* counts;
+  int64_t B, T, H, table_rows;
+  mla_strides qk_stride;
+  int64_t c_new_sb, c_new_st;
+} mla_paged_append_args;
+int mla_paged_append(const mla_paged_append_args* a, void* stream);
+
+/* The rows of positions starts[b] + t, t < counts[b] (starts NULL: 0; counts NULL: T), out of their pages:
+ *   latent bf16 [B, T, d_latent], k_rope bf16 [B, Hr, T, 64], contiguous, 16-byte aligned; zeros for the other t, for positions
+ *   that do not exist and where there is no page.  4-bit values are rounded to bf16 once.
+ */
+typedef struct {
+  mla_paged_cache cache;
+  void* latent;
+  void* k_rope;
+  const int32_t* starts;
+  const int32_t* counts;
+  int64_t B, T;
+} mla_paged_read_args;
+int mla_paged_read(const mla_paged_read_args* a, void* stream);
+
+/* mla_decode over a paged cache: sequence b attends to its first seq_lens[b] positions (int32 [B], read on the device, so a
+ * recorded call follows the lengths).  A sequence with none gets ctx = 0, lse = -inf.
+ *   q_lat bf16 [B, H, d_latent] (q_lat_sb, q_lat_sh), q_rope bf16 [B, H, 64] (q_rope_sb, q_rope_sh), n_k_rope_heads 1 or H
+ *   ctx bf16 [B, H, d_latent] contiguous, lse fp32 [B, H] contiguous, natural log
+ * The sequences' tiles are divided evenly over the workgroups whatever their lengths; a sequence that spans several leaves fp32
+ * partials in the workspace, which a second kernel on the same stream adds in order: results repeat bit for bit.  Needs
+ * mla_paged_decode_workspace_bytes() bytes of 256-byte aligned device memory of this call's own; what they hold does not matter.
+ */
+typedef struct {
+  mla_paged_cache cache;
+  const void* q_lat;
+  const void* q_rope;
+  const int32_t* seq_lens;
+  void* ctx;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t B, H;
+  int64_t q_lat_sb, q_lat_sh, q_rope_sb, q_rope_sh;
+  float scale;
+} mla_paged_decode_args;
+size_t mla_paged_decode_workspace_bytes(const mla_paged_decode_args* a);
+int mla_paged_decode(const mla_paged_decode_args* a, void* stream);
+
+/* ------------------------------------------------------------ sampling --
+ * One token for each row of logits [B, V] (bf16 or fp32, row stride `stride`, V up to 2^19) from the given u[b] in [0, 1):
+ *   w_i = exp((x_i - max x) / temperature)     (a NaN counts as -inf; infinities share all the weight)
+ *   K1 = the top_k largest x                   (top_k <= 0: all)
+ *   K2 = the shortest run of K1, largest first, that holds top_p of its weight, one token at least  (top_p >= 1: all)
+ *   K3 = what of K2 has w_i >= min(min_p, 1)
+ *   tokens[b] = the first i, in the order of the vocabulary, with sum_{j <= i in K3} w_j > u[b] sum_{K3} w
+ *   logprobs[b] = log(w_token / sum_{K3} w)
+ * Of equal logits the lower index counts as the larger.  temperature <= 0: the largest (logprob 0).  A row without a logit above
+ * -inf: token -1, logprob -inf.  The settings are one number for all rows or, where the *_rows pointer is set, fp32 (top_k: int32)
+ * [B].  Weights are fixed-point numbers of 2^-44 of the largest, from fp64 exponentials: sums do not depend on their order.
+ *
+ * Replaces: the sampling of the generation loop (CLI.py:139-187), without its host synchronisation.
+ */
+typedef struct {
+  const void* logits;
+  const float* u;
+  const float* temperature_rows;
+  const int32_t* top_k_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+  int64_t* tokens;
+  float* logprobs;
+  int64_t B, V, stride;
+  float temperature, top_p, min_p;
+  int32_t top_k, dtype;
+} mla_sample_args;
+int mla_sample(const mla_sample_args* a, void* stream);
+
 /* --------------------------------------------------------------- misc --
  * mla_last_error: description of the last non-zero return on this thread.
  * mla_abi_version: MLA_ABI_VERSION of the built library.
  * mla_args_size: sizeof() of the argument structs, for binding checks
  *   (0 rope, 1 prefill_fwd, 2 prefill_bwd, 3 decode, 4 rmsnorm, 5 rmsnorm_bwd, 6 decode_out,
  *    7 rope_append, 8 absorb_q, 9 ce_chunk, 10 linear_rows, 11 prefill_cached, 12 norm_linear,
- *    13 weight_grad, 14 linear_act, 15 gated_linear, 16 gated_linear_bwd, 17 linear_dx, 18 act_grad, 19 grad_norm).
+ *    13 weight_grad, 14 linear_act, 15 gated_linear, 16 gated_linear_bwd, 17 linear_dx, 18 act_grad, 19 grad_norm,
+ *    20 paged_append, 21 paged_read, 22 paged_decode, 23 sample).
  */
 const char* mla_last_error(void);
 int mla_abi_version(void);

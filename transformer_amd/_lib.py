@@ -228,10 +228,54 @@ class GradNormArgs(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    _fields_ = [
+        ("pages", c_void_p), ("scales", c_void_p), ("block_table", c_void_p),
+        ("n_pages", c_int64), ("page_size", c_int64), ("page_stride", c_int64), ("scale_stride", c_int64),
+        ("table_pages", c_int64), ("table_stride", c_int64), ("d_latent", c_int64), ("n_k_rope_heads", c_int64),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("qk", c_void_p), ("c_new", c_void_p), ("q_out", c_void_p), ("cos", c_void_p), ("sin", c_void_p),
+        ("starts", c_void_p), ("counts", c_void_p),
+        ("B", c_int64), ("T", c_int64), ("H", c_int64), ("table_rows", c_int64),
+        ("qk_stride", Strides), ("c_new_sb", c_int64), ("c_new_st", c_int64),
+    ]
+
+
+class PagedReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("latent", c_void_p), ("k_rope", c_void_p), ("starts", c_void_p), ("counts", c_void_p),
+        ("B", c_int64), ("T", c_int64),
+    ]
+
+
+class PagedDecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("q_lat", c_void_p), ("q_rope", c_void_p), ("seq_lens", c_void_p), ("ctx", c_void_p),
+        ("lse", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("B", c_int64), ("H", c_int64),
+        ("q_lat_sb", c_int64), ("q_lat_sh", c_int64), ("q_rope_sb", c_int64), ("q_rope_sh", c_int64),
+        ("scale", c_float),
+    ]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p), ("u", c_void_p), ("temperature_rows", c_void_p), ("top_k_rows", c_void_p),
+        ("top_p_rows", c_void_p), ("min_p_rows", c_void_p), ("tokens", c_void_p), ("logprobs", c_void_p),
+        ("B", c_int64), ("V", c_int64), ("stride", c_int64),
+        ("temperature", c_float), ("top_p", c_float), ("min_p", c_float), ("top_k", c_int32), ("dtype", c_int32),
+    ]
+
+
 ARGS_STRUCTS = {0: RopeArgs, 1: PrefillFwdArgs, 2: PrefillBwdArgs, 3: DecodeArgs, 4: RmsNormArgs,
                 5: RmsNormBwdArgs, 6: DecodeOutArgs, 7: RopeAppendArgs, 8: AbsorbQArgs, 9: CeChunkArgs,
                 10: LinearRowsArgs, 11: PrefillCachedArgs, 12: NormLinearArgs, 13: WeightGradArgs, 14: LinearActArgs,
-                15: GatedLinearArgs, 16: GatedLinearBwdArgs, 17: LinearDxArgs, 18: ActGradArgs, 19: GradNormArgs}
+                15: GatedLinearArgs, 16: GatedLinearBwdArgs, 17: LinearDxArgs, 18: ActGradArgs, 19: GradNormArgs,
+                20: PagedAppendArgs, 21: PagedReadArgs, 22: PagedDecodeArgs, 23: SampleArgs}
 
 # exported symbol -> (restype, argtypes)
 SIGNATURES = {
@@ -272,6 +316,11 @@ SIGNATURES = {
     "mla_grad_norm_workspace_bytes": (c_size_t, [POINTER(GradNormArgs)]),
     "mla_grad_norm": (c_int, [POINTER(GradNormArgs), c_void_p]),
     "mla_grad_clip": (c_int, [POINTER(GradNormArgs), c_void_p]),
+    "mla_paged_append": (c_int, [POINTER(PagedAppendArgs), c_void_p]),
+    "mla_paged_read": (c_int, [POINTER(PagedReadArgs), c_void_p]),
+    "mla_paged_decode_workspace_bytes": (c_size_t, [POINTER(PagedDecodeArgs)]),
+    "mla_paged_decode": (c_int, [POINTER(PagedDecodeArgs), c_void_p]),
+    "mla_sample": (c_int, [POINTER(SampleArgs), c_void_p]),
     "mla_last_error": (ctypes.c_char_p, []),
     "mla_abi_version": (c_int, []),
     "mla_args_size": (c_size_t, [c_int]),

@@ -72,6 +72,10 @@ extern "C" size_t mla_args_size(int which) {
     case 17: return sizeof(mla_linear_dx_args);
     case 18: return sizeof(mla_act_grad_args);
     case 19: return sizeof(mla_grad_norm_args);
+    case 20: return sizeof(mla_paged_append_args);
+    case 21: return sizeof(mla_paged_read_args);
+    case 22: return sizeof(mla_paged_decode_args);
+    case 23: return sizeof(mla_sample_args);
     default: return 0;
   }
 }
