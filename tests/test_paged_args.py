@@ -16,8 +16,8 @@ BASE = {
     "mla_paged_append": (_lib.PagedAppendArgs, dict(qk=4096, c_new=4096, q_out=4096, cos=4096, sin=4096, starts=4096, counts=None, B=2,
                                                     T=1, H=16, table_rows=100, qk_stride=ST, c_new_sb=512, c_new_st=512)),
     "mla_paged_read": (_lib.PagedReadArgs, dict(latent=4096, k_rope=4096, starts=None, counts=None, B=2, T=5)),
-    "mla_paged_decode": (_lib.PagedDecodeArgs, dict(q_lat=4096, q_rope=4096, seq_lens=4096, ctx=4096, lse=4096, workspace=None,
-                                                    workspace_bytes=0, B=2, H=16, q_lat_sb=8192, q_lat_sh=512, q_rope_sb=1024,
+    "mla_paged_decode": (_lib.PagedDecodeArgs, dict(q_lat=4096, q_rope=4096, seq_lens=4096, ctx=4096, lse=4096, workspace=4096,
+                                                    workspace_bytes=1 << 30, B=2, H=16, q_lat_sb=8192, q_lat_sh=512, q_rope_sb=1024,
                                                     q_rope_sh=64, scale=0.1)),
 }
 BAD_CACHE = (dict(pages=None), dict(pages=4104), dict(scales=8196), dict(block_table=None), dict(block_table=2), dict(n_pages=-1),
@@ -32,7 +32,7 @@ BAD = {
                          dict(B=(1 << 24) - 1, T=(1 << 24) - 1)),
     "mla_paged_read": (dict(B=-1), dict(T=-2), dict(latent=None), dict(k_rope=None), dict(latent=4104), dict(starts=3), dict(counts=2),
                        dict(B=(1 << 24) - 1, T=(1 << 24) - 1)),
-    "mla_paged_decode": (dict(B=-1), dict(H=0), dict(H=2000), dict(B=1 << 20), dict(q_lat=None), dict(q_rope=4100), dict(ctx=None), dict(ctx=4104),
+    "mla_paged_decode": (dict(workspace_bytes=1000), dict(workspace=4100), dict(B=-1), dict(H=0), dict(H=2000), dict(B=1 << 20), dict(q_lat=None), dict(q_rope=4100), dict(ctx=None), dict(ctx=4104),
                          dict(lse=None), dict(lse=4098), dict(seq_lens=None), dict(seq_lens=4099), dict(q_lat_sb=-8), dict(q_rope_sh=12),
                          dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf)),
 }

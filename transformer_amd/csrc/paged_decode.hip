@@ -1,7 +1,30 @@
 // Absorbed latent decode over a paged cache in 16 or 4 bits (gfx950): one query token a sequence.
+//
+//   s_j = (q_lat . c_j + q_rope . k_j) scale,   ctx = softmax(s) c,   lse = logsumexp(s)
+//
+// over the rows [c | k] of a sequence's pages, each read once for the 16 heads of a head group.  HBM bound: 1152 bytes a token in 16
+// bits (d_latent 512, one rotated key), 306 in 4.
+//
+// Work.  A unit is a sequence and head group, a tile 16 tokens of it (16 bits) or 64 (4 bits).  The tiles of all units in a row are
+// cut into equal runs, one a workgroup, whatever the sequences' lengths: every workgroup adds the lengths up and finds its place
+// itself, so nothing is planned on the host and a recorded call follows the lengths.  A unit that lies in one run is finished there;
+// one that spans several leaves (m, l, O) of each in fp32, which the merge kernel adds in the runs' order (no atomics: results
+// repeat bit for bit).
+//
+// A workgroup's tiles come through a ring of LDS slots by direct-to-LDS loads, which run on across its units.  16 tokens never
+// straddle a page, so a buffer descriptor of the tokens that exist (none, where the entry is no page) bounds each load: what lies
+// behind a sequence's end reads as zero and never reaches a product.  The four waves share the scores through LDS and then own a
+// quarter of the latent's columns each, so no wave's O has to be merged with another's.  One barrier a tile.
+#include <algorithm>
+
 #include "paged.h"
 
 namespace mla {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
 struct PagedDecodeParams {
   PagedParams c;
@@ -9,85 +32,776 @@ struct PagedDecodeParams {
   const int32_t* seq_lens;
   bf16* ctx;
   float* lse;
-  int H, Hr, DL;
+  float* part_o;   // [2 runs][16][DL]: slot 2 run for a unit that begins before the run, 2 run + 1 for one that ends after it
+  float* part_ml;  // [2 runs][16][2]: m (log2) and l
+  int B, H, n_hg, runs;
+  int pieces;          // 16-token pieces of a page
+  uint32_t piece_magic;  // ceil(2^32 / pieces): the page of piece s < 2^24 is the high half of s times this (pieces > 1)
   int64_t q_lat_sb, q_lat_sh, q_rope_sb, q_rope_sh;
   float scale_log2;
 };
 
-// One workgroup a head of a sequence; its waves take the tokens in turn, a lane DL / 64 of the latent's values and one of the key's.
-template <bool FOUR>
-__global__ __launch_bounds__(256) void paged_decode_kernel(PagedDecodeParams a) {
-  __shared__ float m_s[4], l_s[4], o_s[4][512];
-  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int n = a.DL / 64;
-  float q[8], o[8], v[8];
-  for (int i = 0; i < n; ++i) {
-    q[i] = (float)a.q_lat[b * a.q_lat_sb + h * a.q_lat_sh + 64 * i + lane];
-    o[i] = 0.f;
-  }
-  const float qr = (float)a.q_rope[b * a.q_rope_sb + h * a.q_rope_sh + lane];
-  const int64_t len = min((int64_t)max(a.seq_lens[b], 0), (int64_t)a.c.table_pages * a.c.size);
-  float m = -INFINITY, l = 0.f;
-  const int kr = a.DL + (a.Hr > 1 ? 64 * h : 0);
-  for (int64_t t = w; t < len; t += 4) {
-    const int id = page_of(a.c, b, t / a.c.size);
-    if (id < 0) continue;
-    const int slot = (int)(t % a.c.size);
-    const unsigned char* row = a.c.pages + id * a.c.page_stride + (int64_t)slot * a.c.row_bytes;
-    auto value = [&](int col) {
-      if (!FOUR) return (float)reinterpret_cast<const bf16*>(row)[col];
-      const int byte = row[col >> 1];
-      return (float)((col & 1 ? byte >> 4 : byte & 15) - 8) *
-             (float)a.c.scales[id * a.c.scale_stride + (col >> 6) * a.c.size + slot];
-    };
-    float s = qr * value(kr + lane);
-    for (int i = 0; i < n; ++i) {
-      v[i] = value(64 * i + lane);
-      s += q[i] * v[i];
-    }
-    for (int x = 32; x; x >>= 1) s += wave_shfl_xor(s, x);
-    s *= a.scale_log2;
-    const float m_new = fmaxf(m, s), r = m == -INFINITY ? 0.f : fast_exp2(m - m_new), p = fast_exp2(s - m_new);
-    m = m_new;
-    l = l * r + p;
-    for (int i = 0; i < n; ++i) o[i] = o[i] * r + p * v[i];
-  }
-  if (lane == 0) {
-    m_s[w] = m;
-    l_s[w] = l;
-  }
-  for (int i = 0; i < n; ++i) o_s[w][64 * i + lane] = o[i];
-  __syncthreads();
-  const float M = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
-  float L = 0.f, f[4];
-  for (int i = 0; i < 4; ++i) {
-    f[i] = M == -INFINITY ? 0.f : fast_exp2(m_s[i] - M);
-    L += f[i] * l_s[i];
-  }
-  for (int c = threadIdx.x; c < a.DL; c += 256) {
-    const float s = f[0] * o_s[0][c] + f[1] * o_s[1][c] + f[2] * o_s[2][c] + f[3] * o_s[3][c];
-    a.ctx[(int64_t)blockIdx.x * a.DL + c] = (bf16)(L > 0.f ? s / L : 0.f);
-  }
-  if (threadIdx.x == 0) a.lse[blockIdx.x] = L > 0.f ? (M + fast_log2(L)) * kLn2 : -INFINITY;
+constexpr uint32_t kPdNothing = 0x40000000u;  // an offset past every descriptor: reads as zero
+constexpr float kPdRescale = 8.0f;  // growth of a head's running max (log2) that makes O be scaled again
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
 }
+// a barrier that leaves the loads in flight alone
+__device__ __forceinline__ void pd_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ int pd_len(const PagedDecodeParams& p, int b) {
+  return min(max(p.seq_lens[b], 0), p.c.table_pages * p.c.size);
+}
+__device__ __forceinline__ int pd_page(const PagedDecodeParams& p, int piece) {
+  return p.pieces == 1 ? piece : (int)__umulhi((uint32_t)piece, p.piece_magic);
+}
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// A place in the units' tiles: tile `tile` of the `n` of (b, hg), `left` tiles to go from here.
+template <int TT>
+struct PdCursor {
+  int b, hg, tile, n, len;
+  int64_t left;
+
+  __device__ __forceinline__ void next(const PagedDecodeParams& p) {
+    --left;
+    if (++tile < n) return;
+    tile = 0;
+    if (++hg < p.n_hg || left <= 0) return;
+    hg = 0;
+    do {
+      len = pd_len(p, ++b);
+      n = (len + TT - 1) / TT;
+    } while (n == 0 && b + 1 < p.B);
+  }
+};
+
+// The tiles of sequences up to and with lane's (64 b0 + lane); 64-bit sums, as every lane's n is below 2^28.
+template <int TT>
+__device__ __forceinline__ int64_t pd_scan(const PagedDecodeParams& p, int b0, int lane, int& n) {
+  const int b = b0 + lane;
+  n = b < p.B ? (pd_len(p, b) + TT - 1) / TT : 0;
+  int64_t s = n;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int64_t o = __shfl_up(s, m, 64);
+    s += lane >= m ? o : 0;
+  }
+  return s;
+}
+// All units' tiles, as tiles a run: runs are of ceil(total / runs).
+template <int TT>
+__device__ __forceinline__ int64_t pd_run(const PagedDecodeParams& p, int lane) {
+  int64_t total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    int n;
+    total += lane_value(pd_scan<TT>(p, b0, lane, n), 63);
+  }
+  total *= p.n_hg;
+  return (total + p.runs - 1) / p.runs;
+}
+// The cursor of this workgroup's run; left = 0 where there is none.
+template <int TT>
+__device__ __forceinline__ PdCursor<TT> pd_begin(const PagedDecodeParams& p, int run, int lane) {
+  PdCursor<TT> c = {0, 0, 0, 0, 0, 0};
+  int n = 0;
+  int64_t upto = 0, before = 0, total = 0;
+  if (p.B <= 64) {
+    upto = pd_scan<TT>(p, 0, lane, n);
+    total = lane_value(upto, 63);
+  } else {
+    for (int b0 = 0; b0 < p.B; b0 += 64) total += lane_value(pd_scan<TT>(p, b0, lane, n), 63);
+  }
+  total *= p.n_hg;
+  const int64_t each = (total + p.runs - 1) / p.runs, from = run * each;
+  if (from >= total) return c;
+  for (int b0 = 0;; b0 += 64) {
+    if (p.B > 64) upto = pd_scan<TT>(p, b0, lane, n);
+    const uint64_t past = __ballot((before + upto) * p.n_hg > from);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      c.b = b0 + at;
+      c.n = __builtin_amdgcn_readlane(n, at);
+      const int64_t in = from - (before + lane_value(upto, at) - c.n) * p.n_hg;
+      c.hg = (int)(in / c.n);
+      c.tile = (int)(in - (int64_t)c.hg * c.n);
+      break;
+    }
+    before += lane_value(upto, 63);
+  }
+  c.len = pd_len(p, c.b);
+  c.left = min(each, total - from);
+  return c;
+}
+
+// The pages of a wave's next 64 tiles, one a lane: 16-token piece tile * PIECES + piece of each.
+template <int TT>
+struct PdPages {
+  static constexpr int PIECES = TT / 16;
+  int ids, first, b;
+
+  __device__ __forceinline__ int at(const PagedDecodeParams& p, const PdCursor<TT>& c, int piece, int lane) {
+    if (c.b != b || c.tile - first >= 64 || c.tile < first) {
+      b = c.b;
+      first = c.tile;
+      const int sub = (first + lane) * PIECES + piece;
+      ids = sub * 16 < c.len ? page_of(p.c, b, pd_page(p, sub)) : -1;
+    }
+    return __builtin_amdgcn_readlane(ids, c.tile - first);
+  }
+};
+
+// Stores of a unit's 16 heads x 4 columns a lane: the result, or the run's part.
+template <int DL, int TT>
+struct PdOut {
+  bool whole;
+  int slot;
+  __device__ __forceinline__ void columns(const PagedDecodeParams& p, int b, int h, int l16, int col, f32x4 o, float inv) const {
+    if (!whole) {
+      *reinterpret_cast<f32x4*>(p.part_o + ((int64_t)slot * 16 + l16) * DL + col) = o;
+    } else if (h < p.H) {
+      o *= inv;
+      stg8(p.ctx + ((int64_t)b * p.H + h) * DL + col, u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])});
+    }
+  }
+  __device__ __forceinline__ void sums(const PagedDecodeParams& p, int b, int h, int l16, float m, float l) const {
+    if (!whole) {
+      p.part_ml[(slot * 16 + l16) * 2] = m;
+      p.part_ml[(slot * 16 + l16) * 2 + 1] = l;
+    } else if (h < p.H) {
+      p.lse[(int64_t)b * p.H + h] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ 16 bits
+
+// Rows [latent | shared key] (or the latent alone) lie in a slot as 16-byte chunks, chunk c of token t at c ^ tok_swz(t), RS chunks a
+// row (RS = 8 mod 16): the QK reads (16 tokens x one chunk) and the transpose reads (4 tokens x 2 chunks a 16 lanes) are free of bank
+// conflicts.  Keys of their own lie head by head, 16 tokens x 8 chunks, chunk c at c ^ (t / 2): in a ring one slot shorter, since only
+// the scores read them.
+template <int DL, bool SHARED>
+struct Pd16 {
+  static constexpr int TT = 16;
+  static constexpr int NCH = DL / 8 + (SHARED ? 8 : 0), RS = NCH % 16 == 8 ? NCH : NCH + 8;
+  static constexpr int NKS = NCH / 4, NKW = (NKS + 3) / 4;  // k-steps of the scores; of a wave
+  static constexpr int NB = DL / 64;                        // column blocks of 16 a wave
+  static constexpr int SLOT = 16 * RS * 16, ROPE = SHARED ? 0 : 16 * 2048, SX = 2 * 4096;
+  static constexpr int LIMIT = 160 * 1024;
+  static constexpr int NS = SHARED ? std::min(8, (LIMIT - SX) / SLOT) : 4 * SLOT + 3 * ROPE + SX <= LIMIT ? 4 : 3;
+  static constexpr int LDS = NS * SLOT + (NS - 1) * ROPE + SX;
+  static constexpr int NI = RS / 4 + (SHARED ? 0 : 32);  // loads of 1 KiB a tile
+  static constexpr int ND = (NI + 3) / 4;                // of waves 0 .. (NI - 1) % 4; one less of the others
+  static_assert((NS - 2) * ND < 63, "vmcnt");
+};
+
+__device__ __forceinline__ int tok_swz16(int t) { return ((t >> 2) & 1) | (((t >> 3) & 1) << 1) | (((t >> 1) & 1) << 2); }
+
+template <int DL, bool SHARED>
+__global__ __launch_bounds__(256, 1) void paged_decode16_kernel(PagedDecodeParams p) {
+  using C = Pd16<DL, SHARED>;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
+  unsigned char* ropes = lds + C::NS * C::SLOT;
+  f32x4* sx = reinterpret_cast<f32x4*>(ropes + (C::NS - 1) * C::ROPE);  // [2][4 waves][64]
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, G = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  PdCursor<16> use = pd_begin<16>(p, blockIdx.x, lane), load = use;
+  if (use.left == 0) return;
+  PdPages<16> pages = {0, 0, -1};
+
+  // what a lane loads of a tile's row chunks: instruction i of the wave is piece w + 4 i of the slot
+  constexpr int NR = C::RS / 4;  // row pieces; then 32 key pieces (head j / 2, tokens 8 (j % 2) ..)
+  uint32_t off[(NR + 3) / 4], roff[2];
+#pragma unroll
+  for (int i = 0; i < (NR + 3) / 4; ++i) {
+    const int q = 64 * (w + 4 * i) + lane, row = q / C::RS, c = (q - row * C::RS) ^ tok_swz16(row);
+    off[i] = c < C::NCH ? (uint32_t)(row * p.c.row_bytes + 16 * c) : kPdNothing;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = 8 * i + (lane >> 3);
+    roff[i] = (uint32_t)(t * p.c.row_bytes + 2 * DL + 16 * ((lane & 7) ^ (t >> 1)));
+  }
+  uint64_t tokens = 0;  // of the tiles in the ring, a byte each, the oldest lowest
+  int slot_in = 0, rope_in = 0;
+  auto issue = [&]() {
+    int nv = 0;
+    const unsigned char* base = p.c.pages;
+    int hg = 0;
+    if (load.left > 0) {
+      const int id = pages.at(p, load, 0, lane);
+      if (id >= 0) {
+        const int piece = load.tile - pd_page(p, load.tile) * p.pieces;
+        base += id * p.c.page_stride + (int64_t)piece * 16 * p.c.row_bytes;
+        nv = min(16, load.len - load.tile * 16);
+      }
+      hg = load.hg;
+      load.next(p);
+    }
+    const buf_rsrc r = make_rsrc(base, (uint32_t)(nv * p.c.row_bytes));
+    const uint32_t to = lds_addr(lds) + slot_in * C::SLOT;
+#pragma unroll
+    for (int i = 0; i < (NR + 3) / 4; ++i)
+      if (w + 4 * i < NR) dma16(r, off[i], to + (w + 4 * i) * 1024);
+    if constexpr (!SHARED) {
+      const uint32_t rto = lds_addr(ropes) + rope_in * C::ROPE;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = ((w - NR) & 3) + 4 * i;  // so that the wave's pieces go on where its row pieces ended
+        const int h = hg * 16 + (j >> 1);
+        dma16(r, h < p.H ? (j & 1 ? roff[1] : roff[0]) + (uint32_t)h * 128 : kPdNothing, rto + j * 1024);
+      }
+      rope_in = rope_in + 1 == C::NS - 1 ? 0 : rope_in + 1;
+    }
+    slot_in = slot_in + 1 == C::NS ? 0 : slot_in + 1;
+    tokens |= (uint64_t)nv << (8 * (C::NS - 2));
+  };
+  const bool more_loads = w <= (C::NI - 1) % 4;  // ND loads a tile, or one less
+#pragma unroll
+  for (int i = 0; i < C::NS - 1; ++i) {
+    tokens >>= 8;
+    issue();
+  }
+
+  const int swA = tok_swz16(l16);
+  const int offA = l16 * C::RS * 16 + ((4 * (w & 1) + G) ^ swA) * 16 + (w >> 1) * 128;  // k-step w; w + 4 i: + 256 i
+  const int rowB = 4 * G + (l16 >> 2), swB = tok_swz16(rowB);
+  const int offB = rowB * C::RS * 16 + (((2 * w) ^ (swB & 6)) + ((((l16 & 3) >> 1) ^ swB) & 1)) * 16 + (l16 & 1) * 8;  // block w + 4 i: + 128 i
+  const int offR = l16 * 128 + ((G ^ (l16 >> 1)) * 16);  // k-step 1: chunk 4 further, ^ 64
+
+  u32x4 q[C::NKW], qr[SHARED ? 1 : 8];
+  f32x4 o[C::NB];
+  float m_run = 0.f, l_part = 0.f;
+  int slot = 0, rope = 0, par = 0;
+  bool first = true;
+  int from = 0;
+
+  if (more_loads)
+    wait_loads<(C::NS - 2) * C::ND>();
+  else
+    wait_loads<(C::NS - 2) * (C::ND - 1)>();
+  pd_barrier();
+  while (true) {
+    if (first) {  // a unit begins
+      const int h = use.hg * 16 + l16;
+      const bf16* ql = p.q_lat + use.b * p.q_lat_sb + (int64_t)h * p.q_lat_sh;
+      const bf16* qp = p.q_rope + use.b * p.q_rope_sb + (int64_t)h * p.q_rope_sh;
+#pragma unroll
+      for (int i = 0; i < C::NKW; ++i) {
+        const int c = 4 * (w + 4 * i) + G;
+        q[i] = u32x4{0u, 0u, 0u, 0u};
+        if (w + 4 * i < C::NKS && h < p.H) q[i] = c < DL / 8 ? ldg16(ql + 8 * c) : ldg16(qp + 8 * (c - DL / 8));
+      }
+      if constexpr (!SHARED) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // heads 4 w + j / 2, the same in every column
+          const int hj = min(use.hg * 16 + 4 * w + (j >> 1), p.H - 1);
+          qr[j] = ldg16(p.q_rope + use.b * p.q_rope_sb + (int64_t)hj * p.q_rope_sh + 32 * (j & 1) + 8 * G);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run = -INFINITY;
+      l_part = 0.f;
+      from = use.tile;
+      first = false;
+    }
+    const unsigned char* buf = lds + slot * C::SLOT;
+    // the wave's part of S^T: S[token 4 G + r][head l16]
+    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < C::NKW; ++i)
+      if (w + 4 * i < C::NKS) s = mfma16(as_bf16x8(lds16(buf + offA + 256 * i)), as_bf16x8(q[i]), s);
+    if constexpr (!SHARED) {
+      const unsigned char* rb = ropes + rope * C::ROPE + 4 * w * 2048 + offR;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 d = mfma16(as_bf16x8(lds16(rb + j * 2048)), as_bf16x8(qr[2 * j]), f32x4{0.f, 0.f, 0.f, 0.f});
+        d = mfma16(as_bf16x8(lds16(ropes + rope * C::ROPE + (4 * w + j) * 2048 + (offR ^ 64))), as_bf16x8(qr[2 * j + 1]), d);
+        // (each head's own product: one chain over the heads would carry a head's infinities into the others)
+        const bool mine = l16 == 4 * w + j;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] += mine ? d[r] : 0.f;
+      }
+      rope = rope + 1 == C::NS - 1 ? 0 : rope + 1;
+    }
+    sx[(par * 4 + w) * 64 + lane] = s;
+    if (more_loads)
+      wait_loads<(C::NS - 3) * C::ND>();
+    else
+      wait_loads<(C::NS - 3) * (C::ND - 1)>();
+    pd_barrier();  // every part of S, the next tile, and every wave done with the last one's slot
+    const int nv = (int)(tokens & 255);
+    tokens >>= 8;
+    issue();
+
+    f32x4 x = sx[(par * 4) * 64 + lane];
+    x += sx[(par * 4 + 1) * 64 + lane];
+    x += sx[(par * 4 + 2) * 64 + lane];
+    x += sx[(par * 4 + 3) * 64 + lane];
+    par ^= 1;
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[r] = 4 * G + r < nv ? x[r] * p.scale_log2 : -INFINITY;
+      top = fmaxf(top, x[r]);
+    }
+    top = xor32_max(xor16_max(top));
+    if (__any(top > m_run + kPdRescale)) {
+      const float m_new = fmaxf(m_run, top), alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_part *= alpha;
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) o[i] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[r] = fast_exp2(x[r] - m_use);
+      l_part += x[r];
+    }
+    const s16x4 pa = __builtin_bit_cast(s16x4, u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])});
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i) {
+      const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(buf + offB + 128 * i));
+      o[i] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v, pa, o[i], 0, 0, 0);
+    }
+    slot = slot + 1 == C::NS ? 0 : slot + 1;
+
+    const int b = use.b, hg = use.hg, n = use.n, tile = use.tile;
+    use.next(p);
+    if (tile + 1 == n || use.left == 0) {
+      const PdOut<DL, 16> out = {from == 0 && tile + 1 == n, 2 * (int)blockIdx.x + (from == 0 ? 1 : 0)};
+      const float l = xor32_sum(xor16_sum(l_part)), inv = l == 0.f ? 0.f : 1.f / l;
+      const int h = hg * 16 + l16;
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) out.columns(p, b, h, l16, 16 * (w + 4 * i) + 4 * G, o[i], inv);
+      if (w == 0 && G == 0) out.sums(p, b, h, l16, m_run, l);
+      first = true;
+      if (use.left == 0) break;
+    }
+  }
+  wait_loads<0>();  // (loads of nothing into the ring)
+}
+
+// ------------------------------------------------------------------------------------------------ 4 bits
+
+// Codes are never turned into their values: (w >> s) & 0x00780078 | 0x41804180 makes two of a word's eight codes the bf16 numbers 16 +
+// code, which the matrix instructions take as they are.  With u = 16 + code a run of 64 adds scale (sum u q - 24 sum q) to a score:
+// -24 sum q is the accumulator's start, the scale a factor on the result, one a run and token.  For O the scale goes into p
+// before it is rounded to bf16, and -24 sum p' is an accumulator of its own, added at the end.  A code costs one VALU operation each
+// time, twice a token (scores, O).
+//
+// A wave scores its own 16 of the tile's 64 tokens, whose rows it loaded itself.  p goes through LDS in fp32; ds_read_b64_tr_b4 then
+// gives each lane one column's 16 tokens, those whose p the same lane's accumulator layout holds: token 16 t + 4 G + r for t, r < 4.
+// Rows of RS chunks, RS odd, and every second 16 rows 128 bytes further: 2-way bank conflicts in the transpose reads, none in the
+// scores' reads.
+template <int DL, bool SHARED>
+struct Pd4 {
+  static constexpr int TT = 64;
+  static constexpr int NCH = DL / 32 + (SHARED ? 2 : 32), RS = NCH + 1;
+  static constexpr int NL = DL / 64, NG = NL + (SHARED ? 1 : 16);  // runs of a row: the latent's; with the keys
+  static constexpr int NB = DL / 64;                               // column blocks of 16 a wave
+  static constexpr int SUB = 16 * RS * 16, ROWS = 4 * SUB + 256;
+  static constexpr int SC = NG * 32;  // bytes of 16 tokens' scales
+  static constexpr int SLOT = ROWS + 4 * SC, SX = 2 * 4096 + 512 + 256 + (SHARED ? 0 : 16 * 128 + 64);
+  static constexpr int NS = 3 * SLOT + SX <= 160 * 1024 ? 3 : 2;
+  static constexpr int LDS = NS * SLOT + SX;
+  static constexpr int NR = (16 * RS + 63) / 64, ND = NR + 1;  // loads of a wave a tile
+  static_assert(LDS <= 160 * 1024 && ND < 63 && 2 * NG <= 64, "");
+};
+// where 16-token piece t of a slot begins: pieces 1 and 3 lie 128 bytes off the others
+template <int SUB>
+__device__ __forceinline__ int piece_at(int t) { return t * SUB + (((t + 1) >> 1) << 7); }
+
+__device__ __forceinline__ bf16x8 codes8(uint32_t w) {
+  const uint32_t m = 0x00780078u, k = 0x41804180u;
+  return as_bf16x8(u32x4{((w << 3) & m) | k, ((w >> 1) & m) | k, ((w >> 5) & m) | k, ((w >> 9) & m) | k});
+}
+// 8 values in the order in which codes8 leaves the codes: 0 4 1 5 2 6 3 7
+__device__ __forceinline__ u32x4 order8(u32x4 v) {
+  return u32x4{pack_lo16(v[0], v[2]), pack_hi16(v[0], v[2]), pack_lo16(v[1], v[3]), pack_hi16(v[1], v[3])};
+}
+__device__ __forceinline__ f32x4 floats4(u32x2 v) { return f32x4{lo_bf16(v[0]), hi_bf16(v[0]), lo_bf16(v[1]), hi_bf16(v[1])}; }
+
+template <int DL, bool SHARED>
+__global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(PagedDecodeParams p) {
+  using C = Pd4<DL, SHARED>;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
+  f32x4* px = reinterpret_cast<f32x4*>(lds + C::NS * C::SLOT);         // [2][4 waves][64]
+  float* mx = reinterpret_cast<float*>(lds + C::NS * C::SLOT + 8192);  // [2][4][16]
+  float* lx = mx + 128;                                                // [4][16]
+  float* qstart = lx + 64;                                             // [16], keys of their own: -24 sum q of each head
+  unsigned char* qs = reinterpret_cast<unsigned char*>(qstart + 16);   // [16][128], their queries in codes8's order
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, G = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  PdCursor<64> use = pd_begin<64>(p, blockIdx.x, lane), load = use;
+  if (use.left == 0) return;
+  PdPages<64> pages = {0, 0, -1};
+
+  uint32_t off[C::NR];
+#pragma unroll
+  for (int i = 0; i < C::NR; ++i) {
+    const int q = 64 * i + lane, row = q / C::RS, c = q - row * C::RS;
+    off[i] = c < C::NCH ? (uint32_t)(row * p.c.row_bytes + 16 * c) : kPdNothing;
+  }
+  const int key_chunk = DL / 32;  // keys of their own: chunks and runs of head group hg
+  uint64_t tokens = 0;            // of the wave's piece of the tiles in the ring
+  int slot_in = 0;
+  auto issue = [&]() {
+    int nv = 0, hg = 0;
+    const unsigned char* base = p.c.pages;
+    const bf16* sc = p.c.scales;
+    if (load.left > 0) {
+      const int id = pages.at(p, load, w, lane);
+      const int sub = load.tile * 4 + w;
+      if (id >= 0) {
+        const int piece = sub - pd_page(p, sub) * p.pieces;
+        base += id * p.c.page_stride + (int64_t)piece * 16 * p.c.row_bytes;
+        sc += id * p.c.scale_stride + piece * 16;
+        nv = max(0, min(16, load.len - sub * 16));
+      }
+      hg = load.hg;
+      load.next(p);
+    }
+    const buf_rsrc r = make_rsrc(base, (uint32_t)(nv * p.c.row_bytes));
+    const uint32_t to = lds_addr(lds) + slot_in * C::SLOT;
+    const uint32_t rows_to = to + piece_at<C::SUB>(w);
+#pragma unroll
+    for (int i = 0; i < C::NR; ++i) {
+      uint32_t v = off[i];
+      if constexpr (!SHARED) {
+        const int q = 64 * i + lane, c = q - q / C::RS * C::RS;
+        const bool key = c >= key_chunk && c < C::NCH;
+        v = key && c - key_chunk + 32 * hg >= 2 * p.H ? kPdNothing : key ? v + 512 * hg : v;
+      }
+      if (64 * i + lane < 16 * C::RS) dma16(r, v, rows_to + i * 1024);
+    }
+    const buf_rsrc rs = make_rsrc(sc, nv ? (uint32_t)((p.c.groups - 1) * p.c.size + 16) * 2 : 0u);
+    int g = lane >> 1;
+    if (!SHARED && g >= C::NL) g += 16 * hg;
+    const uint32_t sv = g < p.c.groups ? (uint32_t)(g * p.c.size * 2 + 16 * (lane & 1)) : kPdNothing;
+    if (lane < 2 * C::NG) dma16(rs, sv, to + C::ROWS + w * C::SC);
+    slot_in = slot_in + 1 == C::NS ? 0 : slot_in + 1;
+    tokens |= (uint64_t)nv << (8 * (C::NS - 2));
+  };
+#pragma unroll
+  for (int i = 0; i < C::NS - 1; ++i) {
+    tokens >>= 8;
+    issue();
+  }
+
+  // transpose reads: lane i of a group of 16 gives the row of token 16 (i / 4) + 4 G + i % 4
+  const int offT = piece_at<C::SUB>(l16 >> 2) + (4 * G + (l16 & 3)) * C::RS * 16;
+  const int offA = piece_at<C::SUB>(w) + l16 * C::RS * 16 + 8 * G;
+  const bf16x8 minus24 = as_bf16x8(u32x4{0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u});
+  constexpr int NQ = C::NL + (SHARED ? 1 : 0);
+  u32x4 q[2 * NQ];
+  float start[NQ];  // -24 sum q of each run
+  f32x4 o[C::NB], os[2];
+  float m_run = 0.f, l_part = 0.f;
+  int slot = 0, par = 0, from = 0;
+  bool first = true;
+  const int g0 = w * C::NB / 4;  // the run of the wave's first column block
+
+  while (true) {
+    if (first) {
+      const int h = use.hg * 16 + l16;
+      const bf16* ql = p.q_lat + use.b * p.q_lat_sb + (int64_t)h * p.q_lat_sh;
+      const bf16* qp = p.q_rope + use.b * p.q_rope_sb + (int64_t)h * p.q_rope_sh;
+#pragma unroll
+      for (int i = 0; i < 2 * NQ; ++i) {
+        const int c = 64 * (i >> 1) + 16 * G + 8 * (i & 1);
+        q[i] = u32x4{0u, 0u, 0u, 0u};
+        if (h < p.H) q[i] = order8(i < 2 * C::NL ? ldg16(ql + c) : ldg16(qp + c - DL));
+      }
+#pragma unroll
+      for (int g = 0; g < NQ; ++g) {
+        f32x4 d = mfma16(minus24, as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
+        start[g] = mfma16(minus24, as_bf16x8(q[2 * g + 1]), d)[0];
+      }
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      os[0] = os[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (!SHARED) {
+        if (tid < 128) {
+          const int hj = min(use.hg * 16 + (tid >> 3), p.H - 1);
+          const u32x4 v = ldg16(p.q_rope + use.b * p.q_rope_sb + (int64_t)hj * p.q_rope_sh + 8 * (tid & 7));
+          float z = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z += lo_bf16(v[e]) + hi_bf16(v[e]);
+          for (int x = 4; x; x >>= 1) z += wave_shfl_xor(z, x);
+          sts16(qs + tid * 16, order8(v));
+          if ((tid & 7) == 0) qstart[tid >> 3] = -24.f * z;
+        }
+        pd_barrier();
+      }
+      m_run = -INFINITY;
+      l_part = 0.f;
+      from = use.tile;
+      first = false;
+    }
+    wait_loads<(C::NS - 2) * C::ND>();  // the wave's own piece of this tile
+    const unsigned char* buf = lds + slot * C::SLOT;
+    unsigned char* sc = lds + slot * C::SLOT + C::ROWS;
+    const int nv = (int)(tokens & 255);
+    tokens >>= 8;
+    if (nv < 16) {  // scales behind the sequence's end may be anything: 0, so that a p of 0 stays 0
+      for (int i = lane; i < C::NG * 16; i += 64)
+        if ((i & 15) >= nv) reinterpret_cast<unsigned short*>(sc + w * C::SC)[i] = 0;
+    }
+    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) {
+      const u32x2 c = lds8(buf + offA + 32 * g);
+      f32x4 d = mfma16(codes8(c[0]), as_bf16x8(q[2 * g]), f32x4{start[g], start[g], start[g], start[g]});
+      d = mfma16(codes8(c[1]), as_bf16x8(q[2 * g + 1]), d);
+      const f32x4 k = floats4(lds8(sc + w * C::SC + 32 * g + 8 * G));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(k[r], d[r], s[r]);
+    }
+    if constexpr (!SHARED) {
+      const int nh = min(16, p.H - use.hg * 16);
+#pragma unroll 2
+      for (int j = 0; j < nh; ++j) {  // head j's own run, its query in every column
+        const u32x2 c = lds8(buf + offA + 32 * (C::NL + j));
+        const float z = qstart[j];
+        f32x4 d = mfma16(codes8(c[0]), as_bf16x8(lds16(qs + j * 128 + 32 * G)), f32x4{z, z, z, z});
+        d = mfma16(codes8(c[1]), as_bf16x8(lds16(qs + j * 128 + 32 * G + 16)), d);
+        const f32x4 k = floats4(lds8(sc + w * C::SC + 32 * (C::NL + j) + 8 * G));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = l16 == j ? __builtin_fmaf(k[r], d[r], s[r]) : s[r];
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] = 4 * G + r < nv ? s[r] * p.scale_log2 : -INFINITY;
+      top = fmaxf(top, s[r]);
+    }
+    top = xor32_max(xor16_max(top));
+    auto weights = [&]() {
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+      f32x4 e;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) e[r] = fast_exp2(s[r] - m_use);
+      px[(par * 4 + w) * 64 + lane] = e;
+      return (e[0] + e[1]) + (e[2] + e[3]);
+    };
+    float sum = weights();
+    if (G == 0) mx[(par * 4 + w) * 16 + l16] = top;
+    pd_barrier();  // every wave's p and piece of the tile, and every wave done with the last one's slot
+    issue();
+    float t4 = fmaxf(fmaxf(mx[par * 64 + l16], mx[par * 64 + 16 + l16]), fmaxf(mx[par * 64 + 32 + l16], mx[par * 64 + 48 + l16]));
+    if (__any(t4 > m_run + kPdRescale)) {  // the same in every wave
+      const float m_new = fmaxf(m_run, t4), alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_part *= alpha;
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) o[i] *= alpha;
+      os[0] *= alpha;
+      os[1] *= alpha;
+      sum = weights();
+      pd_barrier();
+    }
+    l_part += sum;
+    f32x4 pv[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) pv[t] = px[(par * 4 + t) * 64 + lane];
+    par ^= 1;
+    bf16x8 pb[2];
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i) {
+      const int nb = w * C::NB + i, g = nb >> 2;
+      if (i == 0 || (nb & 3) == 0) {  // the run's scales into p
+        f32x4 e[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) e[t] = pv[t] * floats4(lds8(sc + t * C::SC + 32 * g + 8 * G));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          pb[t] = as_bf16x8(u32x4{pack_bf16x2(e[2 * t][0], e[2 * t + 1][0]), pack_bf16x2(e[2 * t][1], e[2 * t + 1][1]),
+                                  pack_bf16x2(e[2 * t][2], e[2 * t + 1][2]), pack_bf16x2(e[2 * t][3], e[2 * t + 1][3])});
+        if (g == g0) {
+          os[0] = mfma16(minus24, pb[0], os[0]);
+          os[0] = mfma16(minus24, pb[1], os[0]);
+        } else {
+          os[1] = mfma16(minus24, pb[0], os[1]);
+          os[1] = mfma16(minus24, pb[1], os[1]);
+        }
+      }
+      const i32x2 c = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(buf + offT + 8 * nb));
+      o[i] = mfma16(codes8((uint32_t)c[0]), pb[0], o[i]);
+      o[i] = mfma16(codes8((uint32_t)c[1]), pb[1], o[i]);
+    }
+    slot = slot + 1 == C::NS ? 0 : slot + 1;
+
+    const int b = use.b, hg = use.hg, n = use.n, tile = use.tile;
+    use.next(p);
+    if (tile + 1 == n || use.left == 0) {
+      const PdOut<DL, 64> out = {from == 0 && tile + 1 == n, 2 * (int)blockIdx.x + (from == 0 ? 1 : 0)};
+      const float mine = xor32_sum(xor16_sum(l_part));
+      if (G == 0) lx[w * 16 + l16] = mine;
+      pd_barrier();
+      const float l = (lx[l16] + lx[16 + l16]) + (lx[32 + l16] + lx[48 + l16]), inv = l == 0.f ? 0.f : 1.f / l;
+      const int h = hg * 16 + l16;
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) {
+        const int nb = w * C::NB + i;
+        out.columns(p, b, h, l16, 16 * nb + 4 * G, o[i] + ((nb >> 2) == g0 ? os[0] : os[1]), inv);
+      }
+      if (w == 0 && G == 0) out.sums(p, b, h, l16, m_run, l);
+      first = true;
+      if (use.left == 0) break;
+    }
+  }
+  wait_loads<0>();
+}
+
+// ------------------------------------------------------------------------------------------------ parts
+
+// One workgroup a head of a sequence: nothing where one run finished it, zeros for a sequence without tokens, else the sum of the
+// runs' parts, 2^(m - M) of each.
+template <int DL, int TT>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedDecodeParams p) {
+  constexpr int COLS = DL / 4, PARTS = 256 / COLS;  // threads of a part; parts at a time
+  __shared__ f32x4 o_s[PARTS][COLS];
+  const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H, hg = h >> 4, l16 = h & 15;
+  const int tid = threadIdx.x, lane = tid & 63;
+  int64_t total = 0, begin = 0;
+  int n = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    int nl;
+    const int64_t upto = pd_scan<TT>(p, b0, lane, nl);
+    if (b >= b0 && b < b0 + 64) {
+      n = __builtin_amdgcn_readlane(nl, b - b0);
+      begin = (total + lane_value(upto, b - b0) - n) * p.n_hg + (int64_t)hg * n;
+    }
+    total += lane_value(upto, 63);
+  }
+  total *= p.n_hg;
+  const int64_t row = (int64_t)b * p.H + h;
+  if (n == 0) {
+    if (tid < COLS) stg8(p.ctx + row * DL + 4 * tid, u32x2{0u, 0u});
+    if (tid == 0) p.lse[row] = -INFINITY;
+    return;
+  }
+  const int64_t each = (total + p.runs - 1) / p.runs;
+  const int run0 = (int)(begin / each), S = (int)((begin + n - 1) / each) - run0 + 1;
+  if (S == 1) return;
+  auto ml = [&](int s) { return p.part_ml + ((int64_t)(2 * (run0 + s) + (s == 0 ? 1 : 0)) * 16 + l16) * 2; };
+  float M = -INFINITY;
+  for (int s = lane; s < S; s += 64) M = fmaxf(M, ml(s)[0]);
+  for (int x = 32; x; x >>= 1) M = fmaxf(M, wave_shfl_xor(M, x));
+  const float Mu = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  for (int s = lane; s < S; s += 64) L += ml(s)[1] * fast_exp2(ml(s)[0] - Mu);
+  for (int x = 32; x; x >>= 1) L += wave_shfl_xor(L, x);
+  const int part = tid / COLS, col = tid - part * COLS;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = part; s < S && part < PARTS; s += PARTS) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p.part_o + ((int64_t)(2 * (run0 + s) + (s == 0 ? 1 : 0)) * 16 + l16) * DL + 4 * col);
+    o += v * fast_exp2(ml(s)[0] - Mu);
+  }
+  if (part < PARTS) o_s[part][col] = o;
+  __syncthreads();
+  if (part == 0) {
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) o += o_s[i][col];
+    o *= L == 0.f ? 0.f : 1.f / L;
+    stg8(p.ctx + row * DL + 4 * col, u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])});
+    if (col == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + fast_log2(L)) * kLn2;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+// Runs: a workgroup for each place that the card has (LDS bounds them), no more than there can be tiles.
+template <class C>
+int runs_of(int64_t B, int64_t n_hg, int64_t capacity) {
+  const int64_t places = 256 * std::max(1, std::min(2, 160 * 1024 / C::LDS));
+  const int64_t tiles = (capacity + C::TT - 1) / C::TT;
+  return (int)std::max<int64_t>(1, tiles >= places ? places : std::min(places, B * n_hg * tiles));
+}
+
+template <int DL, bool SHARED>
+int decode_launch(PagedDecodeParams& p, const char* op, hipStream_t st) {
+  if (p.c.scales)
+    paged_decode4_kernel<DL, SHARED><<<dim3(p.runs), 256, 0, st>>>(p);
+  else
+    paged_decode16_kernel<DL, SHARED><<<dim3(p.runs), 256, 0, st>>>(p);
+  MLA_TRY(launch_status(op));
+  const dim3 grid((unsigned)(p.B * p.H));
+  if (p.c.scales)
+    paged_merge_kernel<DL, 64><<<grid, 256, 0, st>>>(p);
+  else
+    paged_merge_kernel<DL, 16><<<grid, 256, 0, st>>>(p);
+  return launch_status(op);
+}
+
+template <int DL, bool SHARED>
+int decode_runs(const mla_paged_decode_args& a) {
+  const int64_t n_hg = (a.H + 15) / 16, capacity = a.cache.table_pages * a.cache.page_size;
+  return a.cache.scales ? runs_of<Pd4<DL, SHARED>>(a.B, n_hg, capacity) : runs_of<Pd16<DL, SHARED>>(a.B, n_hg, capacity);
+}
+
+template <class F>
+int by_layout(int64_t DL, bool shared, F&& f) {
+  switch (DL) {
+    case 64: return shared ? f.template operator()<64, true>() : f.template operator()<64, false>();
+    case 128: return shared ? f.template operator()<128, true>() : f.template operator()<128, false>();
+    case 256: return shared ? f.template operator()<256, true>() : f.template operator()<256, false>();
+    case 384: return shared ? f.template operator()<384, true>() : f.template operator()<384, false>();
+    default: return shared ? f.template operator()<512, true>() : f.template operator()<512, false>();
+  }
+}
+struct RunsOf {
+  const mla_paged_decode_args& a;
+  template <int DL, bool SHARED>
+  int operator()() { return decode_runs<DL, SHARED>(a); }
+};
+struct LaunchOf {
+  PagedDecodeParams& p;
+  const char* op;
+  hipStream_t st;
+  template <int DL, bool SHARED>
+  int operator()() { return decode_launch<DL, SHARED>(p, op, st); }
+};
+
+int decode_check(const mla_paged_decode_args* a, const char* op, PagedDecodeParams& p) {
+  MLA_CHECK(a, MLA_ERR_INVALID_ARG, "%s: null args", op);
+  MLA_CHECK(a->B >= 0 && a->B < (1 << 20) && a->H >= 1 && a->H <= 1024, MLA_ERR_INVALID_ARG, "%s: B %lld or H %lld is out of range", op,
+            (long long)a->B, (long long)a->H);
+  MLA_TRY(paged_setup(a->cache, op, a->B, p.c));
+  MLA_CHECK(a->cache.table_pages * a->cache.page_size < (1ll << 28), MLA_ERR_INVALID_ARG, "%s: table_pages %lld is out of range", op,
+            (long long)a->cache.table_pages);
+  MLA_CHECK(a->cache.n_k_rope_heads == 1 || a->cache.n_k_rope_heads == a->H, MLA_ERR_INVALID_ARG,
+            "%s: n_k_rope_heads must be 1 or H (%lld)", op, (long long)a->H);
+  return MLA_OK;
+}
+size_t parts_bytes(int runs, int64_t DL) { return (size_t)2 * runs * 16 * ((size_t)DL + 2) * 4; }
 
 }  // namespace mla
 
 using namespace mla;
 
 extern "C" size_t mla_paged_decode_workspace_bytes(const mla_paged_decode_args* a) {
-  return 0;
+  PagedDecodeParams p;
+  if (decode_check(a, "mla_paged_decode_workspace_bytes", p) != MLA_OK || a->B == 0) return 0;
+  RunsOf f{*a};
+  return parts_bytes(by_layout(a->cache.d_latent, a->cache.n_k_rope_heads == 1, f), a->cache.d_latent);
 }
 
 extern "C" int mla_paged_decode(const mla_paged_decode_args* a, void* stream) {
   const char* op = "mla_paged_decode";
-  MLA_CHECK(a, MLA_ERR_INVALID_ARG, "%s: null args", op);
-  MLA_CHECK(a->B >= 0 && a->B < (1 << 20) && a->H >= 1 && a->H <= 1024, MLA_ERR_INVALID_ARG, "%s: B %lld or H %lld is out of range", op,
-            (long long)a->B, (long long)a->H);
   PagedDecodeParams p;
-  MLA_TRY(paged_setup(a->cache, op, a->B, p.c));
-  MLA_CHECK(a->cache.n_k_rope_heads == 1 || a->cache.n_k_rope_heads == a->H, MLA_ERR_INVALID_ARG,
-            "%s: n_k_rope_heads must be 1 or H (%lld)", op, (long long)a->H);
+  MLA_TRY(decode_check(a, op, p));
   MLA_TRY(check_scale(op, a->scale));
   if (a->B == 0) return MLA_OK;
   MLA_CHECK(a->q_lat && a->q_rope && a->seq_lens && a->ctx && a->lse, MLA_ERR_INVALID_ARG, "%s: null pointer", op);
@@ -95,23 +809,29 @@ extern "C" int mla_paged_decode(const mla_paged_decode_args* a, void* stream) {
             MLA_ERR_INVALID_ARG, "%s: a pointer is not aligned", op);
   const int64_t st[] = {a->q_lat_sb, a->q_lat_sh, a->q_rope_sb, a->q_rope_sh};
   for (int64_t s : st) MLA_CHECK(s >= 0 && (s & 7) == 0, MLA_ERR_INVALID_ARG, "%s: strides must be non-negative multiples of 8", op);
+  const size_t need = mla_paged_decode_workspace_bytes(a);
+  MLA_CHECK(a->workspace && ((uintptr_t)a->workspace & 255) == 0 && a->workspace_bytes >= need, MLA_ERR_WORKSPACE,
+            "%s: needs %zu bytes of 256-byte aligned workspace", op, need);
+  MLA_CHECK(a->B * a->H < (1ll << 31), MLA_ERR_INVALID_ARG, "%s: too many heads", op);
   p.q_lat = (const bf16*)a->q_lat;
   p.q_rope = (const bf16*)a->q_rope;
   p.seq_lens = a->seq_lens;
   p.ctx = (bf16*)a->ctx;
   p.lse = a->lse;
+  p.B = (int)a->B;
   p.H = (int)a->H;
-  p.Hr = (int)a->cache.n_k_rope_heads;
-  p.DL = (int)a->cache.d_latent;
+  p.n_hg = (int)((a->H + 15) / 16);
+  p.pieces = p.c.size / 16;
+  p.piece_magic = p.pieces == 1 ? 0 : (uint32_t)(((1ull << 32) + p.pieces - 1) / p.pieces);
   p.q_lat_sb = a->q_lat_sb;
   p.q_lat_sh = a->q_lat_sh;
   p.q_rope_sb = a->q_rope_sb;
   p.q_rope_sh = a->q_rope_sh;
   p.scale_log2 = a->scale * kLog2e;
-  const dim3 grid((unsigned)(a->B * a->H));
-  if (p.c.scales)
-    paged_decode_kernel<true><<<grid, 256, 0, (hipStream_t)stream>>>(p);
-  else
-    paged_decode_kernel<false><<<grid, 256, 0, (hipStream_t)stream>>>(p);
-  return launch_status(op);
+  RunsOf runs{*a};
+  p.runs = by_layout(a->cache.d_latent, a->cache.n_k_rope_heads == 1, runs);
+  p.part_o = (float*)a->workspace;
+  p.part_ml = p.part_o + (size_t)2 * p.runs * 16 * a->cache.d_latent;
+  LaunchOf launch{p, op, (hipStream_t)stream};
+  return by_layout(a->cache.d_latent, a->cache.n_k_rope_heads == 1, launch);
 }
