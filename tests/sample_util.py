@@ -3,7 +3,8 @@ import numpy as np
 
 
 def draw(x, u, temperature, top_k, top_p, min_p):
-    """(token, logprob, room): ``room``: how far in weight the nearest border of the choice is (of 1 the largest weight)."""
+    """(token, logprob, room): ``room``: how far the nearest border of the choice is, in what a sum of weights (or a weight) may be off:
+    2^-39 of itself and 2^-45 a weight."""
     x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
     top = x.max()
     if top == -np.inf:
@@ -18,12 +19,12 @@ def draw(x, u, temperature, top_k, top_p, min_p):
     if top_p < 1:
         c = np.cumsum(w[order])
         before, target = c - w[order], np.float64(top_p) * c[-1]
-        room = min(room, np.abs(before[1:] - target).min(initial=np.inf))
+        room = min(room, np.abs(before[1:] - target).min(initial=np.inf) / (c[-1] * 2.0 ** -39 + len(x) * 2.0 ** -45))
         order = order[:max(1, int((before < target).sum()))]
-    room = min(room, np.abs(w[order] - min_p).min()) if 0 < min_p < 1 else room
+    room = min(room, np.abs(w[order] - min_p).min() / (min_p * 2.0 ** -39)) if 0 < min_p < 1 else room
     order = np.sort(order[w[order] >= min(min_p, 1.0)])
     c = np.cumsum(w[order])
     aim = np.float64(u) * c[-1]
-    room = min(room, np.abs(c[:-1] - aim).min(initial=np.inf), aim if aim else np.inf)
+    room = min(room, np.abs(c[:-1] - aim).min(initial=np.inf) / (c[-1] * 2.0 ** -39 + len(x) * 2.0 ** -45))
     i = min(int((c <= aim).sum()), len(order) - 1)
     return int(order[i]), float(np.log(w[order[i]] / c[-1])), room
