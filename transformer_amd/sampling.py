@@ -6,16 +6,16 @@ GPU.  The random numbers are an input: the same ones give the same tokens.  Ther
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
 
-from . import _lib, kernels
-from .kernels import _eager_call, _op
-from .linear_ops import _launch
+from . import kernels
+from .host_calls import Entry, plain
+from .kernels import _op
 
+_entry = Entry("mla_sample", "8P3q3f2i4x", "SampleArgs")
 MAX_VOCAB = 1 << 19
 _SETTINGS = ("temperature", "top_k", "top_p", "min_p")
 
@@ -25,31 +25,35 @@ def _sample(logits: Tensor, u: Tensor, temperature: float, top_k: int, top_p: fl
             temperature_rows: Optional[Tensor], top_k_rows: Optional[Tensor], top_p_rows: Optional[Tensor],
             min_p_rows: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
     op = "mla_mi355x::sample_tokens"
-    rows = (temperature_rows, top_k_rows, top_p_rows, min_p_rows)
-    if logits.dim() != 2 or not 1 <= logits.size(1) <= MAX_VOCAB or u.shape != logits.shape[:1]:
+    if logits.dim() != 2 or u.dim() != 1 or not 1 <= logits.size(1) <= MAX_VOCAB or u.size(0) != logits.size(0):
         raise ValueError(f"{op}: expected logits [B, V], V up to {MAX_VOCAB}, and u [B]; got {tuple(logits.shape)}, {tuple(u.shape)}")
-    if logits.dtype not in (torch.bfloat16, torch.float32) or u.dtype != torch.float32:
+    bf16 = logits.dtype is torch.bfloat16
+    if not (bf16 or logits.dtype is torch.float32) or u.dtype is not torch.float32:
         raise TypeError(f"{op}: logits must be bfloat16 or float32 and u float32, got {logits.dtype}, {u.dtype}")
-    B, V = logits.shape
-    for name, t in zip(_SETTINGS, rows):
-        want = torch.int32 if name == "top_k" else torch.float32
-        if t is not None and (t.dtype != want or t.shape != (B,)):
-            raise ValueError(f"{op}: {name} of rows must be {want} [{B}], got {t.dtype} {tuple(t.shape)}")
-    dev = logits.get_device()
+    (B, V), dev = logits.shape, logits.get_device()
+    rows, at = [temperature_rows, top_k_rows, top_p_rows, min_p_rows], [0, 0, 0, 0]
+    for k, t in enumerate(rows):
+        if t is None:
+            continue
+        if t.dtype is not (torch.int32 if k == 1 else torch.float32) or t.dim() != 1 or t.size(0) != B:
+            raise ValueError(f"{op}: {_SETTINGS[k]} of rows must be {'int32' if k == 1 else 'float32'} [{B}], got {t.dtype} {tuple(t.shape)}")
+        if not t.is_contiguous():
+            rows[k] = t = t.contiguous()
+        at[k] = t.data_ptr()
     for t in (logits, u, *rows):
-        if t is not None and (not t.is_cuda or t.get_device() != dev):
+        if t is not None and (dev < 0 or t.get_device() != dev):
             kernels._require_gpu(op, t)
             raise ValueError(f"{op}: all tensors must be on one device, got {t.device} and {logits.device}")
-    if logits.stride(1) != 1 and V > 1 or logits.stride(0) < 0:
+    stride, inner = logits.stride()
+    if (inner != 1 and V > 1) or stride < 0:
         logits = logits.contiguous()
-    u, *rows = [None if t is None else t.contiguous() for t in (u, *rows)]
-    tokens = torch.empty(B, dtype=torch.int64, device=logits.device)
-    logprobs = torch.empty(B, dtype=torch.float32, device=logits.device)
+        stride = V
+    u = u if u.is_contiguous() else u.contiguous()
+    tokens = logits.new_empty(B, dtype=torch.int64)
+    logprobs = u.new_empty(B)
     if B:
-        args = _lib.SampleArgs(logits.data_ptr(), u.data_ptr(), *(None if t is None else t.data_ptr() for t in rows),
-                               tokens.data_ptr(), logprobs.data_ptr(), B, V, logits.stride(0), temperature, top_p, min_p, top_k,
-                               kernels._dt_code(logits))
-        _launch("mla_sample", args, logits, op)
+        _entry(op, dev, logits.data_ptr(), u.data_ptr(), *at, tokens.data_ptr(), logprobs.data_ptr(), B, V, stride, temperature, top_p,
+               min_p, top_k, 0 if bf16 else 1)  # MLA_DTYPE_*
     return tokens, logprobs
 
 
@@ -59,7 +63,7 @@ def _(logits, u, temperature, top_k, top_p, min_p, temperature_rows, top_k_rows,
     return logits.new_empty(B, dtype=torch.int64), logits.new_empty(B, dtype=torch.float32)
 
 
-_call = _eager_call("sample_tokens")
+_ops, _run = torch.ops.mla_mi355x, kernels._BODIES["sample_tokens"]
 
 
 def sample_tokens(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, top_k: Union[int, Tensor] = 0,
@@ -72,14 +76,19 @@ def sample_tokens(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] =
     sum; its logprob is that of the distribution drawn from.  Of equal logits the lower index counts as the larger.  Temperature 0
     (or less) takes the largest.  A NaN counts as -inf; a row without a logit above -inf gives token -1 and logprob -inf.  Each
     setting is a number or a tensor ``[B]`` on the device (fp32; ``top_k`` int32)."""
-    one = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}
-    given, rows = dict(zip(_SETTINGS, (temperature, top_k, top_p, min_p))), {}
-    for name, v in given.items():
-        if isinstance(v, Tensor):
-            rows[name], given[name] = v, one[name]
-        elif isinstance(v, bool) or (name == "top_k" and not isinstance(v, int)) or math.isnan(v):
-            raise ValueError(f"sample_tokens: {name} must be {'a whole number' if name == 'top_k' else 'a number'}, got {v!r}")
-    if not -(1 << 31) <= given["top_k"] < 1 << 31:
-        raise ValueError(f"sample_tokens: top_k {given['top_k']} is out of range")
-    return _call(logits, u, float(given["temperature"]), given["top_k"], float(given["top_p"]), float(given["min_p"]),
-                 rows.get("temperature"), rows.get("top_k"), rows.get("top_p"), rows.get("min_p"))
+    rows = [None, None, None, None]
+    if isinstance(temperature, Tensor):
+        rows[0], temperature = temperature, 1.0
+    if isinstance(top_k, Tensor):
+        rows[1], top_k = top_k, 0
+    if isinstance(top_p, Tensor):
+        rows[2], top_p = top_p, 1.0
+    if isinstance(min_p, Tensor):
+        rows[3], min_p = min_p, 0.0
+    if type(top_k) is not int or not -(1 << 31) <= top_k < 1 << 31:
+        raise ValueError(f"sample_tokens: top_k must be a whole number of 32 bits, got {top_k!r}")
+    for name, v in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
+        if type(v) is bool or v != v:
+            raise ValueError(f"sample_tokens: {name} must be a number, got {v!r}")
+    run = _run if plain(logits, u, *rows) else _ops.sample_tokens
+    return run(logits, u, float(temperature), top_k, float(top_p), float(min_p), *rows)
