@@ -34,7 +34,7 @@ struct PagedDecodeParams {
   float* lse;
   float* part_o;   // [2 runs][16][DL]: slot 2 run for a unit that begins before the run, 2 run + 1 for one that ends after it
   float* part_ml;  // [2 runs][16][2]: m (log2) and l
-  int B, H, n_hg, runs;
+  int B, H, n_hg, runs;  // (runs * the places of one stays below 2^31)
   int pieces;          // 16-token pieces of a page
   uint32_t piece_magic;  // ceil(2^32 / pieces): the page of piece s < 2^24 is the high half of s times this (pieces > 1)
   int64_t q_lat_sb, q_lat_sh, q_rope_sb, q_rope_sh;
@@ -54,110 +54,114 @@ __device__ __forceinline__ void pd_barrier() { asm volatile("s_waitcnt lgkmcnt(0
 __device__ __forceinline__ int pd_len(const PagedDecodeParams& p, int b) {
   return min(max(p.seq_lens[b], 0), p.c.table_pages * p.c.size);
 }
+// the same for a b that is the same in all lanes, by a scalar load: a vector one would be waited for with all loads into the ring
+__device__ __forceinline__ int pd_len1(const PagedDecodeParams& p, int b) {
+  const auto* lens = (const __attribute__((address_space(4))) int32_t*)p.seq_lens;
+  return min(max(lens[b], 0), p.c.table_pages * p.c.size);
+}
 __device__ __forceinline__ int pd_page(const PagedDecodeParams& p, int piece) {
   return p.pieces == 1 ? piece : (int)__umulhi((uint32_t)piece, p.piece_magic);
 }
-__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
-  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
 
-// A place in the units' tiles: tile `tile` of the `n` of (b, hg), `left` tiles to go from here.
-template <int TT>
+// A place in the units' tiles: tile `tile` of the `n` of (b, hg), the workgroup's tiles going to `end` in the line of all.
+//
+// On that line a unit takes COST places before its tiles: what its beginning and end cost in tiles (queries, stores), so that a
+// workgroup whose run holds the ends of several gets fewer tiles.  All numbers stay below 2^31.
+template <class C>
 struct PdCursor {
-  int b, hg, tile, n, len;
-  int64_t left;
+  int b, hg, tile, n, len, left;  // left: of the run's line, from this tile on
 
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  // the next tile of the run, or left <= 0
   __device__ __forceinline__ void next(const PagedDecodeParams& p) {
     --left;
     if (++tile < n) return;
     tile = 0;
-    if (++hg < p.n_hg || left <= 0) return;
+    left -= C::COST;
+    if (left <= 0 || ++hg < p.n_hg) return;
     hg = 0;
     do {
-      len = pd_len(p, ++b);
-      n = (len + TT - 1) / TT;
+      len = pd_len1(p, ++b);
+      n = (len + C::TT - 1) / C::TT;
     } while (n == 0 && b + 1 < p.B);
   }
 };
 
-// The tiles of sequences up to and with lane's (64 b0 + lane); 64-bit sums, as every lane's n is below 2^28.
-template <int TT>
-__device__ __forceinline__ int64_t pd_scan(const PagedDecodeParams& p, int b0, int lane, int& n) {
+__device__ __forceinline__ int wave_scan(int v) {  // the lanes up to and with this one
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // lane 15 of rows 0 and 2 into the next ones
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31 into rows 2 and 3
+}
+// The places on the line of one unit of each of the sequences up to and with lane's (b0 + lane); n: its tiles.
+template <class C>
+__device__ __forceinline__ int pd_scan(const PagedDecodeParams& p, int b0, int lane, int& n) {
   const int b = b0 + lane;
-  n = b < p.B ? (pd_len(p, b) + TT - 1) / TT : 0;
-  int64_t s = n;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int64_t o = __shfl_up(s, m, 64);
-    s += lane >= m ? o : 0;
-  }
-  return s;
+  n = b < p.B ? (pd_len(p, b) + C::TT - 1) / C::TT : 0;
+  return wave_scan(n ? n + C::COST : 0);
 }
-// All units' tiles, as tiles a run: runs are of ceil(total / runs).
-template <int TT>
-__device__ __forceinline__ int64_t pd_run(const PagedDecodeParams& p, int lane) {
-  int64_t total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    int n;
-    total += lane_value(pd_scan<TT>(p, b0, lane, n), 63);
+// places a run
+__device__ __forceinline__ int pd_each(const PagedDecodeParams& p, int total, int least) {
+  return max((int)((uint32_t)(total + p.runs - 1) / (uint32_t)p.runs), least);
+}
+// The cursor of a run; left <= 0 where it has no tile.
+template <class C>
+__device__ __forceinline__ PdCursor<C> pd_begin(const PagedDecodeParams& p, int run, int lane) {
+  PdCursor<C> c = {0, 0, 0, 0, 0, 0};
+  int n, upto = pd_scan<C>(p, 0, lane, n), before = 0, total = __builtin_amdgcn_readlane(upto, 63);
+  for (int b0 = 64; b0 < p.B; b0 += 64) {
+    int nb;
+    total += __builtin_amdgcn_readlane(pd_scan<C>(p, b0, lane, nb), 63);
   }
   total *= p.n_hg;
-  return (total + p.runs - 1) / p.runs;
-}
-// The cursor of this workgroup's run; left = 0 where there is none.
-template <int TT>
-__device__ __forceinline__ PdCursor<TT> pd_begin(const PagedDecodeParams& p, int run, int lane) {
-  PdCursor<TT> c = {0, 0, 0, 0, 0, 0};
-  int n = 0;
-  int64_t upto = 0, before = 0, total = 0;
-  if (p.B <= 64) {
-    upto = pd_scan<TT>(p, 0, lane, n);
-    total = lane_value(upto, 63);
-  } else {
-    for (int b0 = 0; b0 < p.B; b0 += 64) total += lane_value(pd_scan<TT>(p, b0, lane, n), 63);
-  }
-  total *= p.n_hg;
-  const int64_t each = (total + p.runs - 1) / p.runs, from = run * each;
+  const int each = pd_each(p, total, C::LEAST), from = run * each;
   if (from >= total) return c;
-  for (int b0 = 0;; b0 += 64) {
-    if (p.B > 64) upto = pd_scan<TT>(p, b0, lane, n);
+  for (int b0 = 0;;) {
     const uint64_t past = __ballot((before + upto) * p.n_hg > from);
     if (past) {
       const int at = __builtin_ctzll(past);
       c.b = b0 + at;
       c.n = __builtin_amdgcn_readlane(n, at);
-      const int64_t in = from - (before + lane_value(upto, at) - c.n) * p.n_hg;
-      c.hg = (int)(in / c.n);
-      c.tile = (int)(in - (int64_t)c.hg * c.n);
+      const int unit = c.n + C::COST, in = from - (before + __builtin_amdgcn_readlane(upto, at) - unit) * p.n_hg;
+      c.hg = p.n_hg == 1 ? 0 : in / unit;
+      c.tile = in - c.hg * unit - C::COST;
       break;
     }
-    before += lane_value(upto, 63);
+    before += __builtin_amdgcn_readlane(upto, 63);
+    b0 += 64;
+    upto = pd_scan<C>(p, b0, lane, n);
   }
-  c.len = pd_len(p, c.b);
+  c.len = pd_len1(p, c.b);
   c.left = min(each, total - from);
+  if (c.tile < 0) {  // the run begins among the unit's first places
+    c.left += c.tile;
+    c.tile = 0;
+  }
   return c;
 }
 
 // The pages of a wave's next 64 tiles, one a lane: 16-token piece tile * PIECES + piece of each.
-template <int TT>
+template <class C>
 struct PdPages {
-  static constexpr int PIECES = TT / 16;
+  static constexpr int PIECES = C::TT / 16;
   int ids, first, b;
 
-  __device__ __forceinline__ int at(const PagedDecodeParams& p, const PdCursor<TT>& c, int piece, int lane) {
+  __device__ __forceinline__ int at(const PagedDecodeParams& p, const PdCursor<C>& c, int piece, int lane) {
     if (c.b != b || c.tile - first >= 64 || c.tile < first) {
       b = c.b;
       first = c.tile;
       const int sub = (first + lane) * PIECES + piece;
       ids = sub * 16 < c.len ? page_of(p.c, b, pd_page(p, sub)) : -1;
+      asm volatile("" : "+v"(ids));  // waited for here: at its use each time it would be with all loads into the ring
     }
     return __builtin_amdgcn_readlane(ids, c.tile - first);
   }
 };
 
 // Stores of a unit's 16 heads x 4 columns a lane: the result, or the run's part.
-template <int DL, int TT>
+template <int DL>
 struct PdOut {
   bool whole;
   int slot;
@@ -185,56 +189,53 @@ struct PdOut {
 // row (RS = 8 mod 16): the QK reads (16 tokens x one chunk) and the transpose reads (4 tokens x 2 chunks a 16 lanes) are free of bank
 // conflicts.  Keys of their own lie head by head, 16 tokens x 8 chunks, chunk c at c ^ (t / 2): in a ring one slot shorter, since only
 // the scores read them.
+//
+// Four waves compute and two load.  A load into LDS holds its wave up (about 90 cycles while all waves of the workgroup issue some),
+// which the computing waves do not have between two barriers; and theirs are the only vector loads that the compiler does not see, so it
+// may wait for the others (queries) as it likes.
 template <int DL, bool SHARED>
 struct Pd16 {
-  static constexpr int TT = 16;
+  static constexpr int TT = 16, COST = 3, LEAST = 5;
   static constexpr int NCH = DL / 8 + (SHARED ? 8 : 0), RS = NCH % 16 == 8 ? NCH : NCH + 8;
   static constexpr int NKS = NCH / 4, NKW = (NKS + 3) / 4;  // k-steps of the scores; of a wave
   static constexpr int NB = DL / 64;                        // column blocks of 16 a wave
   static constexpr int SLOT = 16 * RS * 16, ROPE = SHARED ? 0 : 16 * 2048, SX = 2 * 4096;
   static constexpr int LIMIT = 160 * 1024;
-  static constexpr int NS = SHARED ? std::min(8, (LIMIT - SX) / SLOT) : 4 * SLOT + 3 * ROPE + SX <= LIMIT ? 4 : 3;
+  static constexpr int NS = SHARED ? std::min(8, (LIMIT - SX - 64) / SLOT) : 4 * SLOT + 3 * ROPE + SX <= LIMIT ? 4 : 3;
   static constexpr int LDS = NS * SLOT + (NS - 1) * ROPE + SX;
-  static constexpr int NI = RS / 4 + (SHARED ? 0 : 32);  // loads of 1 KiB a tile
-  static constexpr int ND = (NI + 3) / 4;                // of waves 0 .. (NI - 1) % 4; one less of the others
-  static_assert((NS - 2) * ND < 63, "vmcnt");
+  static constexpr int NI = RS / 4 + (SHARED ? 0 : 32), ND = NI / 2;  // loads of 1 KiB a tile; of a loading wave
+  static constexpr int THREADS = 384;
+  static_assert(NI % 2 == 0 && (NS - 2) * ND <= 63, "vmcnt");
 };
 
 __device__ __forceinline__ int tok_swz16(int t) { return ((t >> 2) & 1) | (((t >> 3) & 1) << 1) | (((t >> 1) & 1) << 2); }
 
+// The loading waves: tile k + NS - 1 goes into the slot of tile k - 1 once every wave is done with that (the barrier of tile k), and
+// tile k + 1 has landed before that barrier.  Past the end they load nothing (descriptors of no bytes), so the counts stay the same.
 template <int DL, bool SHARED>
-__global__ __launch_bounds__(256, 1) void paged_decode16_kernel(PagedDecodeParams p) {
+__device__ __forceinline__ void paged_load16(const PagedDecodeParams& p, unsigned char* lds, PdCursor<Pd16<DL, SHARED>> load, int lw,
+                                             int lane, int tiles) {
   using C = Pd16<DL, SHARED>;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
-  unsigned char* ropes = lds + C::NS * C::SLOT;
-  f32x4* sx = reinterpret_cast<f32x4*>(ropes + (C::NS - 1) * C::ROPE);  // [2][4 waves][64]
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, G = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-  PdCursor<16> use = pd_begin<16>(p, blockIdx.x, lane), load = use;
-  if (use.left == 0) return;
-  PdPages<16> pages = {0, 0, -1};
-
-  // what a lane loads of a tile's row chunks: instruction i of the wave is piece w + 4 i of the slot
   constexpr int NR = C::RS / 4;  // row pieces; then 32 key pieces (head j / 2, tokens 8 (j % 2) ..)
-  uint32_t off[(NR + 3) / 4], roff[2];
+  PdPages<C> pages = {0, 0, -1};
+  uint32_t off[NR / 2], roff;
 #pragma unroll
-  for (int i = 0; i < (NR + 3) / 4; ++i) {
-    const int q = 64 * (w + 4 * i) + lane, row = q / C::RS, c = (q - row * C::RS) ^ tok_swz16(row);
+  for (int i = 0; i < NR / 2; ++i) {
+    const int q = 64 * (lw + 2 * i) + lane, row = q / C::RS, c = (q - row * C::RS) ^ tok_swz16(row);
     off[i] = c < C::NCH ? (uint32_t)(row * p.c.row_bytes + 16 * c) : kPdNothing;
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int t = 8 * i + (lane >> 3);
-    roff[i] = (uint32_t)(t * p.c.row_bytes + 2 * DL + 16 * ((lane & 7) ^ (t >> 1)));
+  {
+    const int t = 8 * lw + (lane >> 3);
+    roff = (uint32_t)(t * p.c.row_bytes + 2 * DL + 16 * ((lane & 7) ^ (t >> 1)));
   }
-  uint64_t tokens = 0;  // of the tiles in the ring, a byte each, the oldest lowest
-  int slot_in = 0, rope_in = 0;
+  uint32_t to = lds_addr(lds) + lw * 1024;
+  const uint32_t end = to + C::NS * C::SLOT;
+  uint32_t rto = lds_addr(lds) + C::NS * C::SLOT + lw * 1024;
+  const uint32_t rend = rto + (C::NS - 1) * C::ROPE;
   auto issue = [&]() {
-    int nv = 0;
+    int nv = 0, hg = 0;
     const unsigned char* base = p.c.pages;
-    int hg = 0;
-    if (load.left > 0) {
+    if (load.more()) {
       const int id = pages.at(p, load, 0, lane);
       if (id >= 0) {
         const int piece = load.tile - pd_page(p, load.tile) * p.pieces;
@@ -245,28 +246,53 @@ __global__ __launch_bounds__(256, 1) void paged_decode16_kernel(PagedDecodeParam
       load.next(p);
     }
     const buf_rsrc r = make_rsrc(base, (uint32_t)(nv * p.c.row_bytes));
-    const uint32_t to = lds_addr(lds) + slot_in * C::SLOT;
 #pragma unroll
-    for (int i = 0; i < (NR + 3) / 4; ++i)
-      if (w + 4 * i < NR) dma16(r, off[i], to + (w + 4 * i) * 1024);
+    for (int i = 0; i < NR / 2; ++i) dma16(r, off[i], to + i * 2048);
     if constexpr (!SHARED) {
-      const uint32_t rto = lds_addr(ropes) + rope_in * C::ROPE;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = ((w - NR) & 3) + 4 * i;  // so that the wave's pieces go on where its row pieces ended
-        const int h = hg * 16 + (j >> 1);
-        dma16(r, h < p.H ? (j & 1 ? roff[1] : roff[0]) + (uint32_t)h * 128 : kPdNothing, rto + j * 1024);
+      for (int i = 0; i < 16; ++i) {
+        const int h = hg * 16 + i;
+        dma16(r, h < p.H ? roff + (uint32_t)h * 128 : kPdNothing, rto + i * 2048);
       }
-      rope_in = rope_in + 1 == C::NS - 1 ? 0 : rope_in + 1;
+      rto = rto + C::ROPE == rend ? rend - (C::NS - 1) * C::ROPE : rto + C::ROPE;
     }
-    slot_in = slot_in + 1 == C::NS ? 0 : slot_in + 1;
-    tokens |= (uint64_t)nv << (8 * (C::NS - 2));
+    to = to + C::SLOT == end ? end - C::NS * C::SLOT : to + C::SLOT;
   };
-  const bool more_loads = w <= (C::NI - 1) % 4;  // ND loads a tile, or one less
-#pragma unroll
-  for (int i = 0; i < C::NS - 1; ++i) {
-    tokens >>= 8;
+#pragma unroll 1
+  for (int i = 0; i < C::NS - 1; ++i) issue();
+  wait_loads<(C::NS - 2) * C::ND>();
+  pd_barrier();
+#pragma unroll 1
+  for (; tiles > 0; --tiles) {
+    wait_loads<(C::NS - 3) * C::ND>();
+    pd_barrier();
     issue();
+  }
+  wait_loads<0>();  // (loads of nothing into the ring)
+}
+
+template <int DL, bool SHARED>
+__global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParams p) {
+  using C = Pd16<DL, SHARED>;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
+  unsigned char* ropes = lds + C::NS * C::SLOT;
+  f32x4* sx = reinterpret_cast<f32x4*>(ropes + (C::NS - 1) * C::ROPE);  // [2][4 waves][64]
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, G = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  PdCursor<C> use = pd_begin<C>(p, blockIdx.x, lane);
+  if (!use.more()) return;
+  if (w >= 4) {
+    int tiles = 0;
+    for (PdCursor<C> c = use; c.more();) {  // (whole units at a time)
+      const int k = min(c.n - c.tile, c.left);
+      tiles += k;
+      c.tile += k - 1;
+      c.left -= k - 1;
+      c.next(p);
+    }
+    paged_load16<DL, SHARED>(p, lds, use, w - 4, lane, tiles);
+    return;
   }
 
   const int swA = tok_swz16(l16);
@@ -275,18 +301,12 @@ __global__ __launch_bounds__(256, 1) void paged_decode16_kernel(PagedDecodeParam
   const int offB = rowB * C::RS * 16 + (((2 * w) ^ (swB & 6)) + ((((l16 & 3) >> 1) ^ swB) & 1)) * 16 + (l16 & 1) * 8;  // block w + 4 i: + 128 i
   const int offR = l16 * 128 + ((G ^ (l16 >> 1)) * 16);  // k-step 1: chunk 4 further, ^ 64
 
+  PdPages<C> pages = {0, 0, -1};  // (a tile without a page has no tokens)
   u32x4 q[C::NKW], qr[SHARED ? 1 : 8];
   f32x4 o[C::NB];
   float m_run = 0.f, l_part = 0.f;
-  int slot = 0, rope = 0, par = 0;
-  bool first = true;
-  int from = 0;
-
-  if (more_loads)
-    wait_loads<(C::NS - 2) * C::ND>();
-  else
-    wait_loads<(C::NS - 2) * (C::ND - 1)>();
-  pd_barrier();
+  int slot = 0, rope = 0, par = 0, from = 0;
+  bool first = true, started = false;
   while (true) {
     if (first) {  // a unit begins
       const int h = use.hg * 16 + l16;
@@ -311,19 +331,28 @@ __global__ __launch_bounds__(256, 1) void paged_decode16_kernel(PagedDecodeParam
       l_part = 0.f;
       from = use.tile;
       first = false;
+      if (!started) pd_barrier();  // the first tile has landed
+      started = true;
     }
+    const int nv = pages.at(p, use, 0, lane) < 0 ? 0 : min(16, use.len - use.tile * 16);
     const unsigned char* buf = lds + slot * C::SLOT;
     // the wave's part of S^T: S[token 4 G + r][head l16]
     f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 a[C::NKW];
 #pragma unroll
-    for (int i = 0; i < C::NKW; ++i)
-      if (w + 4 * i < C::NKS) s = mfma16(as_bf16x8(lds16(buf + offA + 256 * i)), as_bf16x8(q[i]), s);
+    for (int i = 0; i < C::NKS / 4; ++i) a[i] = lds16(buf + offA + 256 * i);
+    if (C::NKW > C::NKS / 4 && w < C::NKS % 4) {
+      a[C::NKW - 1] = lds16(buf + offA + 256 * (C::NKW - 1));
+      s = mfma16(as_bf16x8(a[C::NKW - 1]), as_bf16x8(q[C::NKW - 1]), s);
+    }
+#pragma unroll
+    for (int i = 0; i < C::NKS / 4; ++i) s = mfma16(as_bf16x8(a[i]), as_bf16x8(q[i]), s);
     if constexpr (!SHARED) {
-      const unsigned char* rb = ropes + rope * C::ROPE + 4 * w * 2048 + offR;
+      const unsigned char* rb = ropes + rope * C::ROPE + 4 * w * 2048;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f32x4 d = mfma16(as_bf16x8(lds16(rb + j * 2048)), as_bf16x8(qr[2 * j]), f32x4{0.f, 0.f, 0.f, 0.f});
-        d = mfma16(as_bf16x8(lds16(ropes + rope * C::ROPE + (4 * w + j) * 2048 + (offR ^ 64))), as_bf16x8(qr[2 * j + 1]), d);
+        f32x4 d = mfma16(as_bf16x8(lds16(rb + j * 2048 + offR)), as_bf16x8(qr[2 * j]), f32x4{0.f, 0.f, 0.f, 0.f});
+        d = mfma16(as_bf16x8(lds16(rb + j * 2048 + (offR ^ 64))), as_bf16x8(qr[2 * j + 1]), d);
         // (each head's own product: one chain over the heads would carry a head's infinities into the others)
         const bool mine = l16 == 4 * w + j;
 #pragma unroll
@@ -332,14 +361,7 @@ __global__ __launch_bounds__(256, 1) void paged_decode16_kernel(PagedDecodeParam
       rope = rope + 1 == C::NS - 1 ? 0 : rope + 1;
     }
     sx[(par * 4 + w) * 64 + lane] = s;
-    if (more_loads)
-      wait_loads<(C::NS - 3) * C::ND>();
-    else
-      wait_loads<(C::NS - 3) * (C::ND - 1)>();
     pd_barrier();  // every part of S, the next tile, and every wave done with the last one's slot
-    const int nv = (int)(tokens & 255);
-    tokens >>= 8;
-    issue();
 
     f32x4 x = sx[(par * 4) * 64 + lane];
     x += sx[(par * 4 + 1) * 64 + lane];
@@ -376,18 +398,17 @@ __global__ __launch_bounds__(256, 1) void paged_decode16_kernel(PagedDecodeParam
 
     const int b = use.b, hg = use.hg, n = use.n, tile = use.tile;
     use.next(p);
-    if (tile + 1 == n || use.left == 0) {
-      const PdOut<DL, 16> out = {from == 0 && tile + 1 == n, 2 * (int)blockIdx.x + (from == 0 ? 1 : 0)};
+    if (tile + 1 == n || !use.more()) {
+      const PdOut<DL> out = {from == 0 && tile + 1 == n, 2 * (int)blockIdx.x + (from == 0 ? 1 : 0)};
       const float l = xor32_sum(xor16_sum(l_part)), inv = l == 0.f ? 0.f : 1.f / l;
       const int h = hg * 16 + l16;
 #pragma unroll
       for (int i = 0; i < C::NB; ++i) out.columns(p, b, h, l16, 16 * (w + 4 * i) + 4 * G, o[i], inv);
       if (w == 0 && G == 0) out.sums(p, b, h, l16, m_run, l);
       first = true;
-      if (use.left == 0) break;
+      if (!use.more()) break;
     }
   }
-  wait_loads<0>();  // (loads of nothing into the ring)
 }
 
 // ------------------------------------------------------------------------------------------------ 4 bits
@@ -404,7 +425,7 @@ __global__ __launch_bounds__(256, 1) void paged_decode16_kernel(PagedDecodeParam
 // scores' reads.
 template <int DL, bool SHARED>
 struct Pd4 {
-  static constexpr int TT = 64;
+  static constexpr int TT = 64, COST = 1, LEAST = 2;
   static constexpr int NCH = DL / 32 + (SHARED ? 2 : 32), RS = NCH + 1;
   static constexpr int NL = DL / 64, NG = NL + (SHARED ? 1 : 16);  // runs of a row: the latent's; with the keys
   static constexpr int NB = DL / 64;                               // column blocks of 16 a wave
@@ -442,9 +463,9 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, G = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  PdCursor<64> use = pd_begin<64>(p, blockIdx.x, lane), load = use;
-  if (use.left == 0) return;
-  PdPages<64> pages = {0, 0, -1};
+  PdCursor<C> use = pd_begin<C>(p, blockIdx.x, lane), load = use;
+  if (!use.more()) return;
+  PdPages<C> pages = {0, 0, -1};
 
   uint32_t off[C::NR];
 #pragma unroll
@@ -459,7 +480,7 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
     int nv = 0, hg = 0;
     const unsigned char* base = p.c.pages;
     const bf16* sc = p.c.scales;
-    if (load.left > 0) {
+    if (load.more()) {
       const int id = pages.at(p, load, w, lane);
       const int sub = load.tile * 4 + w;
       if (id >= 0) {
@@ -522,6 +543,8 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
         q[i] = u32x4{0u, 0u, 0u, 0u};
         if (h < p.H) q[i] = order8(i < 2 * C::NL ? ldg16(ql + c) : ldg16(qp + c - DL));
       }
+#pragma unroll
+      for (int i = 0; i < 2 * NQ; ++i) asm volatile("" : "+v"(q[i]));  // (waited for here, as above)
 #pragma unroll
       for (int g = 0; g < NQ; ++g) {
         f32x4 d = mfma16(minus24, as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
@@ -644,8 +667,8 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
 
     const int b = use.b, hg = use.hg, n = use.n, tile = use.tile;
     use.next(p);
-    if (tile + 1 == n || use.left == 0) {
-      const PdOut<DL, 64> out = {from == 0 && tile + 1 == n, 2 * (int)blockIdx.x + (from == 0 ? 1 : 0)};
+    if (tile + 1 == n || !use.more()) {
+      const PdOut<DL> out = {from == 0 && tile + 1 == n, 2 * (int)blockIdx.x + (from == 0 ? 1 : 0)};
       const float mine = xor32_sum(xor16_sum(l_part));
       if (G == 0) lx[w * 16 + l16] = mine;
       pd_barrier();
@@ -658,7 +681,7 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
       }
       if (w == 0 && G == 0) out.sums(p, b, h, l16, m_run, l);
       first = true;
-      if (use.left == 0) break;
+      if (!use.more()) break;
     }
   }
   wait_loads<0>();
@@ -667,23 +690,22 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
 // ------------------------------------------------------------------------------------------------ parts
 
 // One workgroup a head of a sequence: nothing where one run finished it, zeros for a sequence without tokens, else the sum of the
-// runs' parts, 2^(m - M) of each.
-template <int DL, int TT>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedDecodeParams p) {
-  constexpr int COLS = DL / 4, PARTS = 256 / COLS;  // threads of a part; parts at a time
+// runs' parts, 2^(m - M) of each.  Latency: the lengths, then m, l and 8 parts a thread at once.
+template <int DL, class C>
+__global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
+  constexpr int COLS = DL / 4, PARTS = 512 / COLS;  // threads of a part; parts at a time
   __shared__ f32x4 o_s[PARTS][COLS];
   const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H, hg = h >> 4, l16 = h & 15;
   const int tid = threadIdx.x, lane = tid & 63;
-  int64_t total = 0, begin = 0;
-  int n = 0;
+  int total = 0, begin = 0, n = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     int nl;
-    const int64_t upto = pd_scan<TT>(p, b0, lane, nl);
+    const int upto = pd_scan<C>(p, b0, lane, nl);
     if (b >= b0 && b < b0 + 64) {
       n = __builtin_amdgcn_readlane(nl, b - b0);
-      begin = (total + lane_value(upto, b - b0) - n) * p.n_hg + (int64_t)hg * n;
+      begin = (total + __builtin_amdgcn_readlane(upto, b - b0) - (n + C::COST)) * p.n_hg + hg * (n + C::COST) + C::COST;
     }
-    total += lane_value(upto, 63);
+    total += __builtin_amdgcn_readlane(upto, 63);
   }
   total *= p.n_hg;
   const int64_t row = (int64_t)b * p.H + h;
@@ -692,24 +714,47 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedDecodeParams p) {
     if (tid == 0) p.lse[row] = -INFINITY;
     return;
   }
-  const int64_t each = (total + p.runs - 1) / p.runs;
-  const int run0 = (int)(begin / each), S = (int)((begin + n - 1) / each) - run0 + 1;
+  const int each = pd_each(p, total, C::LEAST), run0 = begin / each, S = (begin + n - 1) / each - run0 + 1;
   if (S == 1) return;
-  auto ml = [&](int s) { return p.part_ml + ((int64_t)(2 * (run0 + s) + (s == 0 ? 1 : 0)) * 16 + l16) * 2; };
-  float M = -INFINITY;
-  for (int s = lane; s < S; s += 64) M = fmaxf(M, ml(s)[0]);
-  for (int x = 32; x; x >>= 1) M = fmaxf(M, wave_shfl_xor(M, x));
-  const float Mu = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  for (int s = lane; s < S; s += 64) L += ml(s)[1] * fast_exp2(ml(s)[0] - Mu);
-  for (int x = 32; x; x >>= 1) L += wave_shfl_xor(L, x);
+  // the s-th part; s is cut to the last one
+  auto part_of = [&](int s) { return ((int64_t)2 * (run0 + min(s, S - 1)) + (s == 0 ? 1 : 0)) * 16 + l16; };
   const int part = tid / COLS, col = tid - part * COLS;
+  const bool in = part < PARTS;  // (COLS need not divide the workgroup)
+  float M = -INFINITY, L = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = part; s < S && part < PARTS; s += PARTS) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(p.part_o + ((int64_t)(2 * (run0 + s) + (s == 0 ? 1 : 0)) * 16 + l16) * DL + 4 * col);
-    o += v * fast_exp2(ml(s)[0] - Mu);
+  for (int s0 = 0; s0 < S; s0 += 8 * PARTS) {
+    f32x4 v[8];
+    float m[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t at = part_of(s0 + (in ? part : 0) + i * PARTS);
+      v[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * DL + 4 * (in ? col : 0));
+      m[i] = p.part_ml[2 * at];
+    }
+    static_assert(8 * PARTS <= 256, "");
+    float ms = -INFINITY, ls = 0.f, mk[4], lk[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int s = s0 + lane + 64 * k;
+      const bool is = lane + 64 * k < 8 * PARTS && s < S;
+      const int64_t at = part_of(s);
+      mk[k] = is ? p.part_ml[2 * at] : -INFINITY;
+      lk[k] = is ? p.part_ml[2 * at + 1] : 0.f;
+      ms = fmaxf(ms, mk[k]);
+    }
+    for (int x = 8; x; x >>= 1) ms = fmaxf(ms, wave_shfl_xor(ms, x));
+    ms = fmaxf(M, xor32_max(xor16_max(ms)));
+    const float mu = ms == -INFINITY ? 0.f : ms, a = fast_exp2(M - mu);  // (M = -inf: 0, and the sums are 0)
+    M = ms;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) ls += lk[k] * fast_exp2(mk[k] - mu);
+    for (int x = 8; x; x >>= 1) ls += wave_shfl_xor(ls, x);
+    L = L * a + xor32_sum(xor16_sum(ls));
+    o *= a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o += s0 + part + i * PARTS < S ? v[i] * fast_exp2(m[i] - mu) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (part < PARTS) o_s[part][col] = o;
+  if (in) o_s[part][col] = o;
   __syncthreads();
   if (part == 0) {
 #pragma unroll
@@ -726,8 +771,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedDecodeParams p) {
 template <class C>
 int runs_of(int64_t B, int64_t n_hg, int64_t capacity) {
   const int64_t places = 256 * std::max(1, std::min(2, 160 * 1024 / C::LDS));
-  const int64_t tiles = (capacity + C::TT - 1) / C::TT;
-  return (int)std::max<int64_t>(1, tiles >= places ? places : std::min(places, B * n_hg * tiles));
+  const int64_t line = B * n_hg * ((capacity + C::TT - 1) / C::TT + C::COST);  // (below 2^30)
+  return (int)std::max<int64_t>(1, std::min(places, (line + C::LEAST - 1) / C::LEAST));
 }
 
 template <int DL, bool SHARED>
@@ -735,13 +780,13 @@ int decode_launch(PagedDecodeParams& p, const char* op, hipStream_t st) {
   if (p.c.scales)
     paged_decode4_kernel<DL, SHARED><<<dim3(p.runs), 256, 0, st>>>(p);
   else
-    paged_decode16_kernel<DL, SHARED><<<dim3(p.runs), 256, 0, st>>>(p);
+    paged_decode16_kernel<DL, SHARED><<<dim3(p.runs), Pd16<DL, SHARED>::THREADS, 0, st>>>(p);
   MLA_TRY(launch_status(op));
   const dim3 grid((unsigned)(p.B * p.H));
   if (p.c.scales)
-    paged_merge_kernel<DL, 64><<<grid, 256, 0, st>>>(p);
+    paged_merge_kernel<DL, Pd4<DL, SHARED>><<<grid, 512, 0, st>>>(p);
   else
-    paged_merge_kernel<DL, 16><<<grid, 256, 0, st>>>(p);
+    paged_merge_kernel<DL, Pd16<DL, SHARED>><<<grid, 512, 0, st>>>(p);
   return launch_status(op);
 }
 
@@ -781,6 +826,8 @@ int decode_check(const mla_paged_decode_args* a, const char* op, PagedDecodePara
   MLA_TRY(paged_setup(a->cache, op, a->B, p.c));
   MLA_CHECK(a->cache.table_pages * a->cache.page_size < (1ll << 28), MLA_ERR_INVALID_ARG, "%s: table_pages %lld is out of range", op,
             (long long)a->cache.table_pages);
+  MLA_CHECK(a->B * ((a->H + 15) / 16) * (a->cache.table_pages * a->cache.page_size / 16 + 4) < (1ll << 30), MLA_ERR_INVALID_ARG,
+            "%s: B %lld sequences of %lld pages are too many", op, (long long)a->B, (long long)a->cache.table_pages);
   MLA_CHECK(a->cache.n_k_rope_heads == 1 || a->cache.n_k_rope_heads == a->H, MLA_ERR_INVALID_ARG,
             "%s: n_k_rope_heads must be 1 or H (%lld)", op, (long long)a->H);
   return MLA_OK;
