@@ -44,6 +44,12 @@ struct PagedDecodeParams {
 constexpr uint32_t kPdNothing = 0x40000000u;  // an offset past every descriptor: reads as zero
 constexpr float kPdRescale = 8.0f;  // growth of a head's running max (log2) that makes O be scaled again
 
+// a descriptor of values that are the same in all lanes, in scalar registers
+__device__ __forceinline__ buf_rsrc scalar_rsrc(const void* base, uint32_t nbytes) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)base);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uintptr_t)base >> 32));
+  return make_rsrc((const void*)((uintptr_t)hi << 32 | lo), __builtin_amdgcn_readfirstlane((int)nbytes));
+}
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
@@ -86,6 +92,20 @@ struct PdCursor {
     } while (n == 0 && b + 1 < p.B);
   }
 };
+
+// the tiles of a run
+template <class C>
+__device__ __forceinline__ int pd_tiles(const PagedDecodeParams& p, PdCursor<C> c) {
+  int tiles = 0;
+  while (c.more()) {  // whole units at a time
+    const int k = min(c.n - c.tile, c.left);
+    tiles += k;
+    c.tile += k - 1;
+    c.left -= k - 1;
+    c.next(p);
+  }
+  return tiles;
+}
 
 __device__ __forceinline__ int wave_scan(int v) {  // the lanes up to and with this one
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
@@ -245,7 +265,7 @@ __device__ __forceinline__ void paged_load16(const PagedDecodeParams& p, unsigne
       hg = load.hg;
       load.next(p);
     }
-    const buf_rsrc r = make_rsrc(base, (uint32_t)(nv * p.c.row_bytes));
+    const buf_rsrc r = scalar_rsrc(base, (uint32_t)(nv * p.c.row_bytes));
 #pragma unroll
     for (int i = 0; i < NR / 2; ++i) dma16(r, off[i], to + i * 2048);
     if constexpr (!SHARED) {
@@ -283,15 +303,7 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
   PdCursor<C> use = pd_begin<C>(p, blockIdx.x, lane);
   if (!use.more()) return;
   if (w >= 4) {
-    int tiles = 0;
-    for (PdCursor<C> c = use; c.more();) {  // (whole units at a time)
-      const int k = min(c.n - c.tile, c.left);
-      tiles += k;
-      c.tile += k - 1;
-      c.left -= k - 1;
-      c.next(p);
-    }
-    paged_load16<DL, SHARED>(p, lds, use, w - 4, lane, tiles);
+    paged_load16<DL, SHARED>(p, lds, use, w - 4, lane, pd_tiles(p, use));
     return;
   }
 
@@ -417,27 +429,35 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
 // code, which the matrix instructions take as they are.  With u = 16 + code a run of 64 adds scale (sum u q - 24 sum q) to a score:
 // -24 sum q is the accumulator's start, the scale a factor on the result, one a run and token.  For O the scale goes into p
 // before it is rounded to bf16, and -24 sum p' is an accumulator of its own, added at the end.  A code costs one VALU operation each
-// time, twice a token (scores, O).
+// time, twice a token (scores, O): with 530 a wave and tile of 64 tokens these bound the kernel nearly as much as the memory does.
 //
-// A wave scores its own 16 of the tile's 64 tokens, whose rows it loaded itself.  p goes through LDS in fp32; ds_read_b64_tr_b4 then
-// gives each lane one column's 16 tokens, those whose p the same lane's accumulator layout holds: token 16 t + 4 G + r for t, r < 4.
-// Rows of RS chunks, RS odd, and every second 16 rows 128 bytes further: 2-way bank conflicts in the transpose reads, none in the
-// scores' reads.
-template <int DL, bool SHARED>
+// So three kinds of waves work at once, a tile apart: two load tile i + NS - 2, four score tile i, four add up tile i - 1.  A scoring wave
+// takes 16 of the tile's tokens and leaves p relative to a running max of its own, with that max; an adding wave owns a quarter of the
+// latent's columns, brings the four to a common max and adds.  ds_read_b64_tr_b4 gives each lane one column's 16 tokens, those whose p
+// the lane reads as the scores' accumulators left them: token 16 t + 4 G + r for t, r < 4.
+//
+// A slot holds rows of RS chunks of 16 bytes, RS odd, every second 16 rows 128 bytes further (2-way bank conflicts in the transpose
+// reads, none in the scores' reads), then the runs' scales.  Keys of their own lie apart, [16 tokens' piece][head][token][32 bytes],
+// in a ring one slot shorter: only the scores read them.
+template <int DL, bool SHARED, int SLOTS>
 struct Pd4 {
   static constexpr int TT = 64, COST = 1, LEAST = 2;
-  static constexpr int NCH = DL / 32 + (SHARED ? 2 : 32), RS = NCH + 1;
+  static constexpr int NCH = DL / 32 + (SHARED ? 2 : 0), RS = NCH + 1;
   static constexpr int NL = DL / 64, NG = NL + (SHARED ? 1 : 16);  // runs of a row: the latent's; with the keys
   static constexpr int NB = DL / 64;                               // column blocks of 16 a wave
   static constexpr int SUB = 16 * RS * 16, ROWS = 4 * SUB + 256;
   static constexpr int SC = NG * 32;  // bytes of 16 tokens' scales
-  static constexpr int SLOT = ROWS + 4 * SC, SX = 2 * 4096 + 512 + 256 + (SHARED ? 0 : 16 * 128 + 64);
-  static constexpr int NS = 3 * SLOT + SX <= 160 * 1024 ? 3 : 2;
-  static constexpr int LDS = NS * SLOT + SX;
-  static constexpr int NR = (16 * RS + 63) / 64, ND = NR + 1;  // loads of a wave a tile
-  static_assert(LDS <= 160 * 1024 && ND < 63 && 2 * NG <= 64, "");
+  static constexpr int SLOT = ROWS + 4 * SC, SX = 2 * 4096 + 2 * 256 + 2 * 256 + (SHARED ? 0 : 1024), LIMIT = 160 * 1024;
+  static constexpr int NS = SLOTS;
+  // heads with keys of their own that SLOTS slots leave room for
+  static constexpr int HEADS = SHARED ? 16 : std::min(16, (LIMIT - SX - NS * SLOT) / (NS - 1) / 2048 / 2 * 2);
+  static constexpr int ROPE = SHARED ? 0 : HEADS * 2048;
+  static constexpr int LDS = NS * SLOT + (NS - 1) * ROPE + SX;
+  static constexpr int NR = (16 * RS + 63) / 64, ND = 2 * (NR + 1 + (SHARED ? 0 : 8));  // loads of 16 rows; of a loading wave a tile
+  static constexpr int THREADS = 640;
+  static_assert(LDS <= LIMIT && (NS - 2) * ND <= 63 && 2 * NG <= 64 && NS >= 3, "");
 };
-// where 16-token piece t of a slot begins: pieces 1 and 3 lie 128 bytes off the others
+// where 16-token piece t of a slot begins: pieces 1 and 2 lie 128 bytes off the others
 template <int SUB>
 __device__ __forceinline__ int piece_at(int t) { return t * SUB + (((t + 1) >> 1) << 7); }
 
@@ -450,88 +470,95 @@ __device__ __forceinline__ u32x4 order8(u32x4 v) {
   return u32x4{pack_lo16(v[0], v[2]), pack_hi16(v[0], v[2]), pack_lo16(v[1], v[3]), pack_hi16(v[1], v[3])};
 }
 __device__ __forceinline__ f32x4 floats4(u32x2 v) { return f32x4{lo_bf16(v[0]), hi_bf16(v[0]), lo_bf16(v[1]), hi_bf16(v[1])}; }
+__device__ __forceinline__ bf16x8 minus24() { return as_bf16x8(u32x4{0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u}); }
 
-template <int DL, bool SHARED>
-__global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(PagedDecodeParams p) {
-  using C = Pd4<DL, SHARED>;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
-  f32x4* px = reinterpret_cast<f32x4*>(lds + C::NS * C::SLOT);         // [2][4 waves][64]
-  float* mx = reinterpret_cast<float*>(lds + C::NS * C::SLOT + 8192);  // [2][4][16]
-  float* lx = mx + 128;                                                // [4][16]
-  float* qstart = lx + 64;                                             // [16], keys of their own: -24 sum q of each head
-  unsigned char* qs = reinterpret_cast<unsigned char*>(qstart + 16);   // [16][128], their queries in codes8's order
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, G = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-  PdCursor<C> use = pd_begin<C>(p, blockIdx.x, lane), load = use;
-  if (!use.more()) return;
-  PdPages<C> pages = {0, 0, -1};
-
+// The loading waves, 32 tokens of a tile each: tile i + NS - 2 goes into the slot of tile i - 2 after the barrier before which tile i has
+// landed and tile i - 2 was added up.  Past the end they load nothing, so the counts stay the same.
+template <class C, bool SHARED>
+__device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned char* lds, PdCursor<C> load, int lw, int lane, int tiles) {
+  PdPages<C> pages = {0, 0, -1};  // of both pieces, one lane each
   uint32_t off[C::NR];
 #pragma unroll
   for (int i = 0; i < C::NR; ++i) {
     const int q = 64 * i + lane, row = q / C::RS, c = q - row * C::RS;
     off[i] = c < C::NCH ? (uint32_t)(row * p.c.row_bytes + 16 * c) : kPdNothing;
   }
-  const int key_chunk = DL / 32;  // keys of their own: chunks and runs of head group hg
-  uint64_t tokens = 0;            // of the wave's piece of the tiles in the ring
-  int slot_in = 0;
+  const uint32_t koff = (uint32_t)((lane & 31) / 2 * p.c.row_bytes + 16 * C::NL * 2 + 32 * (lane >> 5) + 16 * (lane & 1));
+  PdPages<C> second = {0, 0, -1};
+  const uint32_t base = lds_addr(lds), keys = base + C::NS * C::SLOT, dump = keys + (C::NS - 1) * C::ROPE + C::SX - 1024;
+  int slot = 0, kslot = 0;
   auto issue = [&]() {
-    int nv = 0, hg = 0;
-    const unsigned char* base = p.c.pages;
-    const bf16* sc = p.c.scales;
-    if (load.more()) {
-      const int id = pages.at(p, load, w, lane);
-      const int sub = load.tile * 4 + w;
-      if (id >= 0) {
+    const bool more = load.more();
+    const int ids[2] = {more ? pages.at(p, load, 2 * lw, lane) : -1, more ? second.at(p, load, 2 * lw + 1, lane) : -1};
+    const int hg = load.hg;
+    const uint32_t to = base + slot * C::SLOT;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int t = 2 * lw + k, sub = load.tile * 4 + t;
+      int nv = 0;
+      const unsigned char* rows = p.c.pages;
+      const bf16* sc = p.c.scales;
+      if (ids[k] >= 0) {
         const int piece = sub - pd_page(p, sub) * p.pieces;
-        base += id * p.c.page_stride + (int64_t)piece * 16 * p.c.row_bytes;
-        sc += id * p.c.scale_stride + piece * 16;
+        rows += ids[k] * p.c.page_stride + (int64_t)piece * 16 * p.c.row_bytes;
+        sc += ids[k] * p.c.scale_stride + piece * 16;
         nv = max(0, min(16, load.len - sub * 16));
       }
-      hg = load.hg;
-      load.next(p);
-    }
-    const buf_rsrc r = make_rsrc(base, (uint32_t)(nv * p.c.row_bytes));
-    const uint32_t to = lds_addr(lds) + slot_in * C::SLOT;
-    const uint32_t rows_to = to + piece_at<C::SUB>(w);
+      const buf_rsrc r = scalar_rsrc(rows, (uint32_t)(nv * p.c.row_bytes));
+      const uint32_t rows_to = to + piece_at<C::SUB>(t);
 #pragma unroll
-    for (int i = 0; i < C::NR; ++i) {
-      uint32_t v = off[i];
+      for (int i = 0; i < C::NR; ++i)
+        if (64 * i + lane < 16 * C::RS) dma16(r, off[i], rows_to + i * 1024);
+      const buf_rsrc rs = scalar_rsrc(sc, nv ? (uint32_t)((p.c.groups - 1) * p.c.size + 16) * 2 : 0u);
+      int g = lane >> 1;
+      if (!SHARED && g >= C::NL) g += 16 * hg;
+      const uint32_t sv = g < p.c.groups ? (uint32_t)(g * p.c.size * 2 + 16 * (lane & 1)) : kPdNothing;
+      if (lane < 2 * C::NG) dma16(rs, sv, to + C::ROWS + t * C::SC);
       if constexpr (!SHARED) {
-        const int q = 64 * i + lane, c = q - q / C::RS * C::RS;
-        const bool key = c >= key_chunk && c < C::NCH;
-        v = key && c - key_chunk + 32 * hg >= 2 * p.H ? kPdNothing : key ? v + 512 * hg : v;
-      }
-      if (64 * i + lane < 16 * C::RS) dma16(r, v, rows_to + i * 1024);
-    }
-    const buf_rsrc rs = make_rsrc(sc, nv ? (uint32_t)((p.c.groups - 1) * p.c.size + 16) * 2 : 0u);
-    int g = lane >> 1;
-    if (!SHARED && g >= C::NL) g += 16 * hg;
-    const uint32_t sv = g < p.c.groups ? (uint32_t)(g * p.c.size * 2 + 16 * (lane & 1)) : kPdNothing;
-    if (lane < 2 * C::NG) dma16(rs, sv, to + C::ROWS + w * C::SC);
-    slot_in = slot_in + 1 == C::NS ? 0 : slot_in + 1;
-    tokens |= (uint64_t)nv << (8 * (C::NS - 2));
-  };
 #pragma unroll
-  for (int i = 0; i < C::NS - 1; ++i) {
-    tokens >>= 8;
+        for (int j = 0; j < 16; j += 2) {  // two heads; past the slot's heads nothing, into bytes that nobody reads
+          const int h = hg * 16 + j;
+          const uint32_t v = h + (lane >> 5) < p.H ? koff + (uint32_t)h * 32 : kPdNothing;
+          dma16(r, j < C::HEADS ? v : kPdNothing, j < C::HEADS ? keys + kslot * C::ROPE + t * C::HEADS * 512 + j * 512 : dump);
+        }
+      }
+    }
+    if (more) load.next(p);
+    slot = slot + 1 == C::NS ? 0 : slot + 1;
+    kslot = kslot + 1 == C::NS - 1 ? 0 : kslot + 1;
+  };
+#pragma unroll 1
+  for (int i = 0; i < C::NS - 2; ++i) issue();
+#pragma unroll 1
+  for (int i = 0; i < tiles; ++i) {
+    wait_loads<(C::NS - 3) * C::ND>();
+    pd_barrier();
     issue();
   }
+  pd_barrier();
+  wait_loads<0>();  // (loads of nothing into the ring)
+}
 
-  // transpose reads: lane i of a group of 16 gives the row of token 16 (i / 4) + 4 G + i % 4
-  const int offT = piece_at<C::SUB>(l16 >> 2) + (4 * G + (l16 & 3)) * C::RS * 16;
+// p and the max and sum it is relative to, from the scoring waves to the adding ones; two tiles' worth
+struct Pd4Shared {
+  f32x4* p;  // [2][4 waves][64]
+  float* m;  // [2][4][16]
+  float* l;  // [2][4][16]: at a unit's end
+};
+
+template <class C, int DL, bool SHARED>
+__device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigned char* lds, const Pd4Shared& x, PdCursor<C> use, int w,
+                                             int lane) {
+  const int l16 = lane & 15, G = lane >> 4;
   const int offA = piece_at<C::SUB>(w) + l16 * C::RS * 16 + 8 * G;
-  const bf16x8 minus24 = as_bf16x8(u32x4{0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u});
-  constexpr int NQ = C::NL + (SHARED ? 1 : 0);
+  PdPages<C> pages = {0, 0, -1};
+  constexpr int NQ = C::NL + 1;  // the latent's runs, and the key: shared, or this lane's head's
   u32x4 q[2 * NQ];
   float start[NQ];  // -24 sum q of each run
-  f32x4 o[C::NB], os[2];
   float m_run = 0.f, l_part = 0.f;
-  int slot = 0, par = 0, from = 0;
+  int slot = 0, kslot = 0, par = 0;
   bool first = true;
-  const int g0 = w * C::NB / 4;  // the run of the wave's first column block
-
+#pragma unroll 1
   while (true) {
     if (first) {
       const int h = use.hg * 16 + l16;
@@ -544,64 +571,49 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
         if (h < p.H) q[i] = order8(i < 2 * C::NL ? ldg16(ql + c) : ldg16(qp + c - DL));
       }
 #pragma unroll
-      for (int i = 0; i < 2 * NQ; ++i) asm volatile("" : "+v"(q[i]));  // (waited for here, as above)
-#pragma unroll
       for (int g = 0; g < NQ; ++g) {
-        f32x4 d = mfma16(minus24, as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
-        start[g] = mfma16(minus24, as_bf16x8(q[2 * g + 1]), d)[0];
-      }
-#pragma unroll
-      for (int i = 0; i < C::NB; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      os[0] = os[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (!SHARED) {
-        if (tid < 128) {
-          const int hj = min(use.hg * 16 + (tid >> 3), p.H - 1);
-          const u32x4 v = ldg16(p.q_rope + use.b * p.q_rope_sb + (int64_t)hj * p.q_rope_sh + 8 * (tid & 7));
-          float z = 0.f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) z += lo_bf16(v[e]) + hi_bf16(v[e]);
-          for (int x = 4; x; x >>= 1) z += wave_shfl_xor(z, x);
-          sts16(qs + tid * 16, order8(v));
-          if ((tid & 7) == 0) qstart[tid >> 3] = -24.f * z;
-        }
-        pd_barrier();
+        f32x4 d = mfma16(minus24(), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
+        start[g] = mfma16(minus24(), as_bf16x8(q[2 * g + 1]), d)[0];
       }
       m_run = -INFINITY;
       l_part = 0.f;
-      from = use.tile;
       first = false;
     }
-    wait_loads<(C::NS - 2) * C::ND>();  // the wave's own piece of this tile
+    pd_barrier();  // the tile has landed, and the tile before the last is added up
     const unsigned char* buf = lds + slot * C::SLOT;
-    unsigned char* sc = lds + slot * C::SLOT + C::ROWS;
-    const int nv = (int)(tokens & 255);
-    tokens >>= 8;
+    unsigned char* sc = lds + slot * C::SLOT + C::ROWS + w * C::SC;
+    const int sub = use.tile * 4 + w, nv = pages.at(p, use, w, lane) < 0 ? 0 : max(0, min(16, use.len - sub * 16));
     if (nv < 16) {  // scales behind the sequence's end may be anything: 0, so that a p of 0 stays 0
       for (int i = lane; i < C::NG * 16; i += 64)
-        if ((i & 15) >= nv) reinterpret_cast<unsigned short*>(sc + w * C::SC)[i] = 0;
+        if ((i & 15) >= nv) reinterpret_cast<unsigned short*>(sc)[i] = 0;
     }
     f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int g = 0; g < NQ; ++g) {
+    for (int g = 0; g < C::NL + (SHARED ? 1 : 0); ++g) {
       const u32x2 c = lds8(buf + offA + 32 * g);
       f32x4 d = mfma16(codes8(c[0]), as_bf16x8(q[2 * g]), f32x4{start[g], start[g], start[g], start[g]});
       d = mfma16(codes8(c[1]), as_bf16x8(q[2 * g + 1]), d);
-      const f32x4 k = floats4(lds8(sc + w * C::SC + 32 * g + 8 * G));
+      const f32x4 k = floats4(lds8(sc + 32 * g + 8 * G));
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(k[r], d[r], s[r]);
     }
     if constexpr (!SHARED) {
-      const int nh = min(16, p.H - use.hg * 16);
-#pragma unroll 2
-      for (int j = 0; j < nh; ++j) {  // head j's own run, its query in every column
-        const u32x2 c = lds8(buf + offA + 32 * (C::NL + j));
-        const float z = qstart[j];
-        f32x4 d = mfma16(codes8(c[0]), as_bf16x8(lds16(qs + j * 128 + 32 * G)), f32x4{z, z, z, z});
-        d = mfma16(codes8(c[1]), as_bf16x8(lds16(qs + j * 128 + 32 * G + 16)), d);
-        const f32x4 k = floats4(lds8(sc + w * C::SC + 32 * (C::NL + j) + 8 * G));
+      // head j's keys with every head's query: lane l16 keeps its own.  The scale of its key comes last.
+      const unsigned char* kb = lds + C::NS * C::SLOT + kslot * C::ROPE + w * C::HEADS * 512 + l16 * 32 + 8 * G;
+      const float z = start[C::NL];
+      f32x4 e = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = l16 == j ? __builtin_fmaf(k[r], d[r], s[r]) : s[r];
+      for (int j = 0; j < C::HEADS; ++j) {
+        const u32x2 c = lds8(kb + j * 512);
+        f32x4 d = mfma16(codes8(c[0]), as_bf16x8(q[2 * C::NL]), f32x4{z, z, z, z});
+        d = mfma16(codes8(c[1]), as_bf16x8(q[2 * C::NL + 1]), d);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = l16 == j ? d[r] : e[r];
       }
+      const f32x4 k = floats4(lds8(sc + 32 * (C::NL + l16) + 8 * G));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(k[r], e[r], s[r]);
+      kslot = kslot + 1 == C::NS - 1 ? 0 : kslot + 1;
     }
     float top = -INFINITY;
 #pragma unroll
@@ -610,35 +622,78 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
       top = fmaxf(top, s[r]);
     }
     top = xor32_max(xor16_max(top));
-    auto weights = [&]() {
-      const float m_use = m_run == -INFINITY ? 0.f : m_run;
-      f32x4 e;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) e[r] = fast_exp2(s[r] - m_use);
-      px[(par * 4 + w) * 64 + lane] = e;
-      return (e[0] + e[1]) + (e[2] + e[3]);
-    };
-    float sum = weights();
-    if (G == 0) mx[(par * 4 + w) * 16 + l16] = top;
-    pd_barrier();  // every wave's p and piece of the tile, and every wave done with the last one's slot
-    issue();
-    float t4 = fmaxf(fmaxf(mx[par * 64 + l16], mx[par * 64 + 16 + l16]), fmaxf(mx[par * 64 + 32 + l16], mx[par * 64 + 48 + l16]));
-    if (__any(t4 > m_run + kPdRescale)) {  // the same in every wave
-      const float m_new = fmaxf(m_run, t4), alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+    if (__any(top > m_run + kPdRescale)) {
+      const float m_new = fmaxf(m_run, top);
+      l_part *= m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
       m_run = m_new;
-      l_part *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] = fast_exp2(s[r] - m_use);
+      l_part += s[r];
+    }
+    x.p[(par * 4 + w) * 64 + lane] = s;
+    if (G == 0) x.m[(par * 4 + w) * 16 + l16] = m_run;
+    const bool last = use.tile + 1 == use.n || use.left == 1;
+    if (last) {
+      const float l = xor32_sum(xor16_sum(l_part));
+      if (G == 0) x.l[(par * 4 + w) * 16 + l16] = l;
+    }
+    par ^= 1;
+    slot = slot + 1 == C::NS ? 0 : slot + 1;
+    first = last;
+    use.next(p);
+    if (!use.more()) break;
+  }
+  pd_barrier();
+}
+
+template <class C, int DL>
+__device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const unsigned char* lds, const Pd4Shared& x, PdCursor<C> use, int w,
+                                           int lane) {
+  const int l16 = lane & 15, G = lane >> 4;
+  // transpose reads: lane i of a group of 16 gives the row of token 16 (i / 4) + 4 G + i % 4
+  const int offT = piece_at<C::SUB>(l16 >> 2) + (4 * G + (l16 & 3)) * C::RS * 16;
+  const int g0 = w * C::NB / 4;  // the run of the wave's first column block
+  f32x4 o[C::NB], os[2];
+  float M = 0.f;
+  int slot = 0, par = 0, from = 0;
+  bool first = true;
+  pd_barrier();
+#pragma unroll 1
+  while (true) {
+    if (first) {
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      os[0] = os[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      M = -INFINITY;
+      from = use.tile;
+    }
+    pd_barrier();  // the tile is scored
+    const unsigned char* buf = lds + slot * C::SLOT;
+    const unsigned char* sc = buf + C::ROWS;
+    float m[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) m[t] = x.m[(par * 4 + t) * 16 + l16];
+    f32x4 pv[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) pv[t] = x.p[(par * 4 + t) * 64 + lane];
+    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    if (__any(top > M + kPdRescale)) {
+      const float m_new = fmaxf(M, top), alpha = m_new == -INFINITY ? 1.f : fast_exp2(M - m_new);
+      M = m_new;
 #pragma unroll
       for (int i = 0; i < C::NB; ++i) o[i] *= alpha;
       os[0] *= alpha;
       os[1] *= alpha;
-      sum = weights();
-      pd_barrier();
     }
-    l_part += sum;
-    f32x4 pv[4];
+    const float M_use = M == -INFINITY ? 0.f : M;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) pv[t] = px[(par * 4 + t) * 64 + lane];
-    par ^= 1;
+    for (int t = 0; t < 4; ++t) {
+      m[t] = fast_exp2(m[t] - M_use);  // what brings the wave's p (and l) to the common max
+      pv[t] *= m[t];
+    }
     bf16x8 pb[2];
 #pragma unroll
     for (int i = 0; i < C::NB; ++i) {
@@ -652,11 +707,11 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
           pb[t] = as_bf16x8(u32x4{pack_bf16x2(e[2 * t][0], e[2 * t + 1][0]), pack_bf16x2(e[2 * t][1], e[2 * t + 1][1]),
                                   pack_bf16x2(e[2 * t][2], e[2 * t + 1][2]), pack_bf16x2(e[2 * t][3], e[2 * t + 1][3])});
         if (g == g0) {
-          os[0] = mfma16(minus24, pb[0], os[0]);
-          os[0] = mfma16(minus24, pb[1], os[0]);
+          os[0] = mfma16(minus24(), pb[0], os[0]);
+          os[0] = mfma16(minus24(), pb[1], os[0]);
         } else {
-          os[1] = mfma16(minus24, pb[0], os[1]);
-          os[1] = mfma16(minus24, pb[1], os[1]);
+          os[1] = mfma16(minus24(), pb[0], os[1]);
+          os[1] = mfma16(minus24(), pb[1], os[1]);
         }
       }
       const i32x2 c = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(buf + offT + 8 * nb));
@@ -664,27 +719,43 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void paged_decode4_kernel(Page
       o[i] = mfma16(codes8((uint32_t)c[1]), pb[1], o[i]);
     }
     slot = slot + 1 == C::NS ? 0 : slot + 1;
-
     const int b = use.b, hg = use.hg, n = use.n, tile = use.tile;
     use.next(p);
-    if (tile + 1 == n || !use.more()) {
+    first = tile + 1 == n || !use.more();
+    if (first) {
       const PdOut<DL> out = {from == 0 && tile + 1 == n, 2 * (int)blockIdx.x + (from == 0 ? 1 : 0)};
-      const float mine = xor32_sum(xor16_sum(l_part));
-      if (G == 0) lx[w * 16 + l16] = mine;
-      pd_barrier();
-      const float l = (lx[l16] + lx[16 + l16]) + (lx[32 + l16] + lx[48 + l16]), inv = l == 0.f ? 0.f : 1.f / l;
+      float l = 0.f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) l += x.l[(par * 4 + t) * 16 + l16] * m[t];
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       const int h = hg * 16 + l16;
 #pragma unroll
       for (int i = 0; i < C::NB; ++i) {
         const int nb = w * C::NB + i;
         out.columns(p, b, h, l16, 16 * nb + 4 * G, o[i] + ((nb >> 2) == g0 ? os[0] : os[1]), inv);
       }
-      if (w == 0 && G == 0) out.sums(p, b, h, l16, m_run, l);
-      first = true;
+      if (w == 0 && G == 0) out.sums(p, b, h, l16, M, l);
       if (!use.more()) break;
     }
+    par ^= 1;
   }
-  wait_loads<0>();
+}
+
+template <int DL, bool SHARED, int SLOTS>
+__global__ __launch_bounds__(640, 1) void paged_decode4_kernel(PagedDecodeParams p) {
+  using C = Pd4<DL, SHARED, SLOTS>;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
+  unsigned char* at = lds + C::NS * C::SLOT + (C::NS - 1) * C::ROPE;
+  const Pd4Shared x = {reinterpret_cast<f32x4*>(at), reinterpret_cast<float*>(at + 8192), reinterpret_cast<float*>(at + 8192 + 512)};
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const PdCursor<C> use = pd_begin<C>(p, blockIdx.x, lane);
+  if (!use.more()) return;
+  if (w < 4)
+    paged_score4<C, DL, SHARED>(p, lds, x, use, w, lane);
+  else if (w < 8)
+    paged_add4<C, DL>(p, lds, x, use, w - 4, lane);
+  else
+    paged_load4<C, SHARED>(p, lds, use, w - 8, lane, pd_tiles(p, use));
 }
 
 // ------------------------------------------------------------------------------------------------ parts
@@ -767,6 +838,12 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
 
 // ------------------------------------------------------------------------------------------------ host
 
+// Slots of the ring in 4 bits: as many as fit, 8 at most; with keys of their own 4, or 3 where 4 leave no room for the heads'.
+template <int DL>
+constexpr int slots4() {
+  using C = Pd4<DL, true, 3>;
+  return std::min(8, (C::LIMIT - C::SX) / C::SLOT);
+}
 // Runs: a workgroup for each place that the card has (LDS bounds them), no more than there can be tiles.
 template <class C>
 int runs_of(int64_t B, int64_t n_hg, int64_t capacity) {
@@ -774,49 +851,49 @@ int runs_of(int64_t B, int64_t n_hg, int64_t capacity) {
   const int64_t line = B * n_hg * ((capacity + C::TT - 1) / C::TT + C::COST);  // (below 2^30)
   return (int)std::max<int64_t>(1, std::min(places, (line + C::LEAST - 1) / C::LEAST));
 }
-
-template <int DL, bool SHARED>
-int decode_launch(PagedDecodeParams& p, const char* op, hipStream_t st) {
-  if (p.c.scales)
-    paged_decode4_kernel<DL, SHARED><<<dim3(p.runs), 256, 0, st>>>(p);
-  else
-    paged_decode16_kernel<DL, SHARED><<<dim3(p.runs), Pd16<DL, SHARED>::THREADS, 0, st>>>(p);
-  MLA_TRY(launch_status(op));
-  const dim3 grid((unsigned)(p.B * p.H));
-  if (p.c.scales)
-    paged_merge_kernel<DL, Pd4<DL, SHARED>><<<grid, 512, 0, st>>>(p);
-  else
-    paged_merge_kernel<DL, Pd16<DL, SHARED>><<<grid, 512, 0, st>>>(p);
-  return launch_status(op);
-}
-
-template <int DL, bool SHARED>
-int decode_runs(const mla_paged_decode_args& a) {
-  const int64_t n_hg = (a.H + 15) / 16, capacity = a.cache.table_pages * a.cache.page_size;
-  return a.cache.scales ? runs_of<Pd4<DL, SHARED>>(a.B, n_hg, capacity) : runs_of<Pd16<DL, SHARED>>(a.B, n_hg, capacity);
+// f.take<kernel's constants>() for the kernel that serves the layout
+template <int DL, bool SHARED, class F>
+auto by_kernel(const mla_paged_cache& c, int64_t H, F&& f) {
+  if (!c.scales) return f.template take<DL, SHARED, Pd16<DL, SHARED>>(paged_decode16_kernel<DL, SHARED>);
+  if constexpr (SHARED) {
+    constexpr int S = slots4<DL>();
+    return f.template take<DL, SHARED, Pd4<DL, true, S>>(paged_decode4_kernel<DL, true, S>);
+  } else {
+    if (std::min<int64_t>(H, 16) <= Pd4<DL, false, 4>::HEADS)
+      return f.template take<DL, SHARED, Pd4<DL, false, 4>>(paged_decode4_kernel<DL, false, 4>);
+    return f.template take<DL, SHARED, Pd4<DL, false, 3>>(paged_decode4_kernel<DL, false, 3>);
+  }
 }
 
 template <class F>
-int by_layout(int64_t DL, bool shared, F&& f) {
-  switch (DL) {
-    case 64: return shared ? f.template operator()<64, true>() : f.template operator()<64, false>();
-    case 128: return shared ? f.template operator()<128, true>() : f.template operator()<128, false>();
-    case 256: return shared ? f.template operator()<256, true>() : f.template operator()<256, false>();
-    case 384: return shared ? f.template operator()<384, true>() : f.template operator()<384, false>();
-    default: return shared ? f.template operator()<512, true>() : f.template operator()<512, false>();
+auto by_layout(const mla_paged_cache& c, int64_t H, F&& f) {
+  const bool shared = c.n_k_rope_heads == 1;
+  switch (c.d_latent) {
+    case 64: return shared ? by_kernel<64, true>(c, H, f) : by_kernel<64, false>(c, H, f);
+    case 128: return shared ? by_kernel<128, true>(c, H, f) : by_kernel<128, false>(c, H, f);
+    case 256: return shared ? by_kernel<256, true>(c, H, f) : by_kernel<256, false>(c, H, f);
+    case 384: return shared ? by_kernel<384, true>(c, H, f) : by_kernel<384, false>(c, H, f);
+    default: return shared ? by_kernel<512, true>(c, H, f) : by_kernel<512, false>(c, H, f);
   }
 }
 struct RunsOf {
   const mla_paged_decode_args& a;
-  template <int DL, bool SHARED>
-  int operator()() { return decode_runs<DL, SHARED>(a); }
+  template <int DL, bool SHARED, class C, class K>
+  int take(K) {
+    return runs_of<C>(a.B, (a.H + 15) / 16, a.cache.table_pages * a.cache.page_size);
+  }
 };
 struct LaunchOf {
   PagedDecodeParams& p;
   const char* op;
   hipStream_t st;
-  template <int DL, bool SHARED>
-  int operator()() { return decode_launch<DL, SHARED>(p, op, st); }
+  template <int DL, bool SHARED, class C, class K>
+  int take(K kernel) {
+    kernel<<<dim3(p.runs), C::THREADS, 0, st>>>(p);
+    MLA_TRY(launch_status(op));
+    paged_merge_kernel<DL, C><<<dim3((unsigned)p.B * p.H), 512, 0, st>>>(p);
+    return launch_status(op);
+  }
 };
 
 int decode_check(const mla_paged_decode_args* a, const char* op, PagedDecodeParams& p) {
@@ -841,8 +918,7 @@ using namespace mla;
 extern "C" size_t mla_paged_decode_workspace_bytes(const mla_paged_decode_args* a) {
   PagedDecodeParams p;
   if (decode_check(a, "mla_paged_decode_workspace_bytes", p) != MLA_OK || a->B == 0) return 0;
-  RunsOf f{*a};
-  return parts_bytes(by_layout(a->cache.d_latent, a->cache.n_k_rope_heads == 1, f), a->cache.d_latent);
+  return parts_bytes(by_layout(a->cache, a->H, RunsOf{*a}), a->cache.d_latent);
 }
 
 extern "C" int mla_paged_decode(const mla_paged_decode_args* a, void* stream) {
@@ -875,10 +951,8 @@ extern "C" int mla_paged_decode(const mla_paged_decode_args* a, void* stream) {
   p.q_rope_sb = a->q_rope_sb;
   p.q_rope_sh = a->q_rope_sh;
   p.scale_log2 = a->scale * kLog2e;
-  RunsOf runs{*a};
-  p.runs = by_layout(a->cache.d_latent, a->cache.n_k_rope_heads == 1, runs);
+  p.runs = by_layout(a->cache, a->H, RunsOf{*a});
   p.part_o = (float*)a->workspace;
   p.part_ml = p.part_o + (size_t)2 * p.runs * 16 * a->cache.d_latent;
-  LaunchOf launch{p, op, (hipStream_t)stream};
-  return by_layout(a->cache.d_latent, a->cache.n_k_rope_heads == 1, launch);
+  return by_layout(a->cache, a->H, LaunchOf{p, op, (hipStream_t)stream});
 }
