@@ -461,9 +461,14 @@ struct Pd4 {
 template <int SUB>
 __device__ __forceinline__ int piece_at(int t) { return t * SUB + (((t + 1) >> 1) << 7); }
 
+// (w & 0x00780078) | 0x41804180 in one instruction: of two literals the compiler makes two
+__device__ __forceinline__ uint32_t two_codes(uint32_t w) {
+  uint32_t r;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(0x00780078u), "v"(0x41804180u));
+  return r;
+}
 __device__ __forceinline__ bf16x8 codes8(uint32_t w) {
-  const uint32_t m = 0x00780078u, k = 0x41804180u;
-  return as_bf16x8(u32x4{((w << 3) & m) | k, ((w >> 1) & m) | k, ((w >> 5) & m) | k, ((w >> 9) & m) | k});
+  return as_bf16x8(u32x4{two_codes(w << 3), two_codes(w >> 1), two_codes(w >> 5), two_codes(w >> 9)});
 }
 // 8 values in the order in which codes8 leaves the codes: 0 4 1 5 2 6 3 7
 __device__ __forceinline__ u32x4 order8(u32x4 v) {
@@ -554,8 +559,12 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
   PdPages<C> pages = {0, 0, -1};
   constexpr int NQ = C::NL + 1;  // the latent's runs, and the key: shared, or this lane's head's
   u32x4 q[2 * NQ];
-  float start[NQ];  // -24 sum q of each run
+  // The runs' -24 scale sum q come from one product: the tile's scales (rows: tokens) with -24 sum q in three bf16 pieces (24 bits) as
+  // its columns: K slots 8 G .. of group G < 3 are piece G of the latent's runs, of group 3 the pieces of the shared key's.
+  bf16x8 start;
+  f32x4 key_start;  // keys of their own: of this lane's head's, the start of its sums
   float m_run = 0.f, l_part = 0.f;
+  const int offS = ((l16 >> 2) & 3) * 32 + (l16 & 3) * 8;  // transpose read: row (run) i / 4, tokens 4 (i % 4) ..
   int slot = 0, kslot = 0, par = 0;
   bool first = true;
 #pragma unroll 1
@@ -570,10 +579,32 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
         q[i] = u32x4{0u, 0u, 0u, 0u};
         if (h < p.H) q[i] = order8(i < 2 * C::NL ? ldg16(ql + c) : ldg16(qp + c - DL));
       }
+      float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int g = 0; g < NQ; ++g) {
         f32x4 d = mfma16(minus24(), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
-        start[g] = mfma16(minus24(), as_bf16x8(q[2 * g + 1]), d)[0];
+        d = mfma16(minus24(), as_bf16x8(q[2 * g + 1]), d);
+        if (g < C::NL)
+          z[g] = d[0];
+        else
+          key_start = d;
+      }
+      if (!SHARED && G == 3) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = 0.f;
+      }
+      if (SHARED && G == 3) {
+        const bf16 hi = (bf16)key_start[0], mid = (bf16)(key_start[0] - (float)hi);
+        z[0] = (float)hi;
+        z[1] = (float)mid;
+        z[2] = key_start[0] - (float)hi - (float)mid;
+#pragma unroll
+        for (int e = 3; e < 8; ++e) z[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float hi = (float)(bf16)z[e], mid = (float)(bf16)(z[e] - hi);
+        start[e] = (bf16)(G == 0 || G == 3 ? z[e] : G == 1 ? z[e] - hi : z[e] - hi - mid);
       }
       m_run = -INFINITY;
       l_part = 0.f;
@@ -587,11 +618,20 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       for (int i = lane; i < C::NG * 16; i += 64)
         if ((i & 15) >= nv) reinterpret_cast<unsigned short*>(sc)[i] = 0;
     }
-    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 s;
+    {
+      // rows 0 .. 3 and 4 .. 7 of the runs (past the latent's the first again: their pieces are 0); group 3: the key's, four times
+      const int a0 = G == 3 && SHARED ? C::NL * 32 + (l16 & 3) * 8 : C::NL >= 4 ? offS : (l16 >> 2) < C::NL ? offS : (l16 & 3) * 8;
+      const int a1 = C::NL >= 8 || (C::NL > 4 && 4 + (l16 >> 2) < C::NL) ? offS + 128 : (l16 & 3) * 8;
+      const s16x4 r0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sc + a0));
+      const s16x4 r1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sc + a1));
+      const u32x2 w0 = __builtin_bit_cast(u32x2, r0), w1 = __builtin_bit_cast(u32x2, r1);
+      s = mfma16(as_bf16x8(u32x4{w0[0], w0[1], w1[0], w1[1]}), start, f32x4{0.f, 0.f, 0.f, 0.f});
+    }
 #pragma unroll
     for (int g = 0; g < C::NL + (SHARED ? 1 : 0); ++g) {
       const u32x2 c = lds8(buf + offA + 32 * g);
-      f32x4 d = mfma16(codes8(c[0]), as_bf16x8(q[2 * g]), f32x4{start[g], start[g], start[g], start[g]});
+      f32x4 d = mfma16(codes8(c[0]), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
       d = mfma16(codes8(c[1]), as_bf16x8(q[2 * g + 1]), d);
       const f32x4 k = floats4(lds8(sc + 32 * g + 8 * G));
 #pragma unroll
@@ -600,12 +640,11 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
     if constexpr (!SHARED) {
       // head j's keys with every head's query: lane l16 keeps its own.  The scale of its key comes last.
       const unsigned char* kb = lds + C::NS * C::SLOT + kslot * C::ROPE + w * C::HEADS * 512 + l16 * 32 + 8 * G;
-      const float z = start[C::NL];
       f32x4 e = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < C::HEADS; ++j) {
         const u32x2 c = lds8(kb + j * 512);
-        f32x4 d = mfma16(codes8(c[0]), as_bf16x8(q[2 * C::NL]), f32x4{z, z, z, z});
+        f32x4 d = mfma16(codes8(c[0]), as_bf16x8(q[2 * C::NL]), key_start);
         d = mfma16(codes8(c[1]), as_bf16x8(q[2 * C::NL + 1]), d);
 #pragma unroll
         for (int r = 0; r < 4; ++r) e[r] = l16 == j ? d[r] : e[r];
@@ -654,7 +693,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
                                            int lane) {
   const int l16 = lane & 15, G = lane >> 4;
   // transpose reads: lane i of a group of 16 gives the row of token 16 (i / 4) + 4 G + i % 4
-  const int offT = piece_at<C::SUB>(l16 >> 2) + (4 * G + (l16 & 3)) * C::RS * 16;
+  const int offT = piece_at<C::SUB>(l16 >> 2) + (4 * G + (l16 & 3)) * C::RS * 16 + 8 * w * C::NB;
   const int g0 = w * C::NB / 4;  // the run of the wave's first column block
   f32x4 o[C::NB], os[2];
   float M = 0.f;
@@ -714,7 +753,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
           os[1] = mfma16(minus24(), pb[1], os[1]);
         }
       }
-      const i32x2 c = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(buf + offT + 8 * nb));
+      const i32x2 c = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(buf + offT + 8 * i));
       o[i] = mfma16(codes8((uint32_t)c[0]), pb[0], o[i]);
       o[i] = mfma16(codes8((uint32_t)c[1]), pb[1], o[i]);
     }
