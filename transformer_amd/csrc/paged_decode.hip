@@ -16,6 +16,7 @@
 // behind a sequence's end reads as zero and never reaches a product.  The four waves share the scores through LDS and then own a
 // quarter of the latent's columns each, so no wave's O has to be merged with another's.  One barrier a tile.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.h"
 
@@ -44,12 +45,6 @@ struct PagedDecodeParams {
 constexpr uint32_t kPdNothing = 0x40000000u;  // an offset past every descriptor: reads as zero
 constexpr float kPdRescale = 8.0f;  // growth of a head's running max (log2) that makes O be scaled again
 
-// a descriptor of values that are the same in all lanes, in scalar registers
-__device__ __forceinline__ buf_rsrc scalar_rsrc(const void* base, uint32_t nbytes) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)base);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uintptr_t)base >> 32));
-  return make_rsrc((const void*)((uintptr_t)hi << 32 | lo), __builtin_amdgcn_readfirstlane((int)nbytes));
-}
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
@@ -93,20 +88,6 @@ struct PdCursor {
   }
 };
 
-// the tiles of a run
-template <class C>
-__device__ __forceinline__ int pd_tiles(const PagedDecodeParams& p, PdCursor<C> c) {
-  int tiles = 0;
-  while (c.more()) {  // whole units at a time
-    const int k = min(c.n - c.tile, c.left);
-    tiles += k;
-    c.tile += k - 1;
-    c.left -= k - 1;
-    c.next(p);
-  }
-  return tiles;
-}
-
 __device__ __forceinline__ int wave_scan(int v) {  // the lanes up to and with this one
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
@@ -117,9 +98,10 @@ __device__ __forceinline__ int wave_scan(int v) {  // the lanes up to and with t
 }
 // The places on the line of one unit of each of the sequences up to and with lane's (b0 + lane); n: its tiles.
 template <class C>
-__device__ __forceinline__ int pd_scan(const PagedDecodeParams& p, int b0, int lane, int& n) {
+__device__ __forceinline__ int pd_scan(const PagedDecodeParams& p, int b0, int lane, int& n, int& len) {
   const int b = b0 + lane;
-  n = b < p.B ? (pd_len(p, b) + C::TT - 1) / C::TT : 0;
+  len = b < p.B ? pd_len(p, b) : 0;
+  n = (len + C::TT - 1) / C::TT;
   return wave_scan(n ? n + C::COST : 0);
 }
 // places a run
@@ -130,10 +112,10 @@ __device__ __forceinline__ int pd_each(const PagedDecodeParams& p, int total, in
 template <class C>
 __device__ __forceinline__ PdCursor<C> pd_begin(const PagedDecodeParams& p, int run, int lane) {
   PdCursor<C> c = {0, 0, 0, 0, 0, 0};
-  int n, upto = pd_scan<C>(p, 0, lane, n), before = 0, total = __builtin_amdgcn_readlane(upto, 63);
+  int n, len, upto = pd_scan<C>(p, 0, lane, n, len), before = 0, total = __builtin_amdgcn_readlane(upto, 63);
   for (int b0 = 64; b0 < p.B; b0 += 64) {
-    int nb;
-    total += __builtin_amdgcn_readlane(pd_scan<C>(p, b0, lane, nb), 63);
+    int nb, lb;
+    total += __builtin_amdgcn_readlane(pd_scan<C>(p, b0, lane, nb, lb), 63);
   }
   total *= p.n_hg;
   const int each = pd_each(p, total, C::LEAST), from = run * each;
@@ -144,6 +126,7 @@ __device__ __forceinline__ PdCursor<C> pd_begin(const PagedDecodeParams& p, int 
       const int at = __builtin_ctzll(past);
       c.b = b0 + at;
       c.n = __builtin_amdgcn_readlane(n, at);
+      c.len = __builtin_amdgcn_readlane(len, at);
       const int unit = c.n + C::COST, in = from - (before + __builtin_amdgcn_readlane(upto, at) - unit) * p.n_hg;
       c.hg = p.n_hg == 1 ? 0 : in / unit;
       c.tile = in - c.hg * unit - C::COST;
@@ -151,9 +134,8 @@ __device__ __forceinline__ PdCursor<C> pd_begin(const PagedDecodeParams& p, int 
     }
     before += __builtin_amdgcn_readlane(upto, 63);
     b0 += 64;
-    upto = pd_scan<C>(p, b0, lane, n);
+    upto = pd_scan<C>(p, b0, lane, n, len);
   }
-  c.len = pd_len1(p, c.b);
   c.left = min(each, total - from);
   if (c.tile < 0) {  // the run begins among the unit's first places
     c.left += c.tile;
@@ -162,21 +144,40 @@ __device__ __forceinline__ PdCursor<C> pd_begin(const PagedDecodeParams& p, int 
   return c;
 }
 
-// The pages of a wave's next 64 tiles, one a lane: 16-token piece tile * PIECES + piece of each.
+// Where the 16-token piece `piece` of each of the next 64 tiles lies, a tile a lane, and how many of its tokens there are (none without
+// a page).  Looked up together: in scalar operations each tile's address was most of a loading wave's time.
 template <class C>
-struct PdPages {
-  static constexpr int PIECES = C::TT / 16;
-  int ids, first, b;
+struct PdPieces {
+  int first, b;
+  uint32_t rows_lo, rows_hi, scales_lo, scales_hi;
+  int tokens;
 
-  __device__ __forceinline__ int at(const PagedDecodeParams& p, const PdCursor<C>& c, int piece, int lane) {
+  // the lane of tile c.tile
+  __device__ __forceinline__ int lane_of(const PagedDecodeParams& p, const PdCursor<C>& c, int piece, int lane) {
     if (c.b != b || c.tile - first >= 64 || c.tile < first) {
       b = c.b;
       first = c.tile;
-      const int sub = (first + lane) * PIECES + piece;
-      ids = sub * 16 < c.len ? page_of(p.c, b, pd_page(p, sub)) : -1;
-      asm volatile("" : "+v"(ids));  // waited for here: at its use each time it would be with all loads into the ring
+      const int sub = (first + lane) * (C::TT / 16) + piece, page = pd_page(p, sub), in = sub - page * p.pieces;
+      const int id = sub * 16 < c.len ? page_of(p.c, b, page) : -1;
+      tokens = id < 0 ? 0 : min(16, c.len - sub * 16);
+      const uint64_t rows = (uint64_t)p.c.pages + max(id, 0) * p.c.page_stride + (int64_t)in * 16 * p.c.row_bytes;
+      const uint64_t scales = (uint64_t)p.c.scales + 2 * (max(id, 0) * p.c.scale_stride + in * 16);
+      rows_lo = (uint32_t)rows;
+      rows_hi = (uint32_t)(rows >> 32);
+      scales_lo = (uint32_t)scales;
+      scales_hi = (uint32_t)(scales >> 32);
+      asm volatile("" : "+v"(tokens));  // waited for here: at its use in each tile it would be with all loads into the ring
     }
-    return __builtin_amdgcn_readlane(ids, c.tile - first);
+    return c.tile - first;
+  }
+  __device__ __forceinline__ int tokens_of(int at) const { return __builtin_amdgcn_readlane(tokens, at); }
+  __device__ __forceinline__ buf_rsrc rows_of(int at, uint32_t nbytes) const {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)rows_lo, at), hi = __builtin_amdgcn_readlane((int)rows_hi, at);
+    return make_rsrc((const void*)((uint64_t)hi << 32 | lo), nbytes);
+  }
+  __device__ __forceinline__ buf_rsrc scales_of(int at, uint32_t nbytes) const {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)scales_lo, at), hi = __builtin_amdgcn_readlane((int)scales_hi, at);
+    return make_rsrc((const void*)((uint64_t)hi << 32 | lo), nbytes);
   }
 };
 
@@ -231,13 +232,15 @@ struct Pd16 {
 __device__ __forceinline__ int tok_swz16(int t) { return ((t >> 2) & 1) | (((t >> 3) & 1) << 1) | (((t >> 1) & 1) << 2); }
 
 // The loading waves: tile k + NS - 1 goes into the slot of tile k - 1 once every wave is done with that (the barrier of tile k), and
-// tile k + 1 has landed before that barrier.  Past the end they load nothing (descriptors of no bytes), so the counts stay the same.
+// tile k + 1 has landed before that barrier.  The first tiles go out two at a time, so that the first is not waited for behind a whole
+// ring.  Past the end nothing is loaded (descriptors of no bytes), so the counts stay the same.
 template <int DL, bool SHARED>
 __device__ __forceinline__ void paged_load16(const PagedDecodeParams& p, unsigned char* lds, PdCursor<Pd16<DL, SHARED>> load, int lw,
-                                             int lane, int tiles) {
+                                             int lane) {
   using C = Pd16<DL, SHARED>;
   constexpr int NR = C::RS / 4;  // row pieces; then 32 key pieces (head j / 2, tokens 8 (j % 2) ..)
-  PdPages<C> pages = {0, 0, -1};
+  PdPieces<C> pieces = {0, -1, 0, 0, 0, 0, 0};
+  PdCursor<C> use = load;
   uint32_t off[NR / 2], roff;
 #pragma unroll
   for (int i = 0; i < NR / 2; ++i) {
@@ -253,19 +256,14 @@ __device__ __forceinline__ void paged_load16(const PagedDecodeParams& p, unsigne
   uint32_t rto = lds_addr(lds) + C::NS * C::SLOT + lw * 1024;
   const uint32_t rend = rto + (C::NS - 1) * C::ROPE;
   auto issue = [&]() {
-    int nv = 0, hg = 0;
-    const unsigned char* base = p.c.pages;
+    int at = 0, nv = 0;
+    const int hg = load.hg;
     if (load.more()) {
-      const int id = pages.at(p, load, 0, lane);
-      if (id >= 0) {
-        const int piece = load.tile - pd_page(p, load.tile) * p.pieces;
-        base += id * p.c.page_stride + (int64_t)piece * 16 * p.c.row_bytes;
-        nv = min(16, load.len - load.tile * 16);
-      }
-      hg = load.hg;
+      at = pieces.lane_of(p, load, 0, lane);
+      nv = pieces.tokens_of(at);
       load.next(p);
     }
-    const buf_rsrc r = scalar_rsrc(base, (uint32_t)(nv * p.c.row_bytes));
+    const buf_rsrc r = pieces.rows_of(at, (uint32_t)(nv * p.c.row_bytes));
 #pragma unroll
     for (int i = 0; i < NR / 2; ++i) dma16(r, off[i], to + i * 2048);
     if constexpr (!SHARED) {
@@ -278,12 +276,27 @@ __device__ __forceinline__ void paged_load16(const PagedDecodeParams& p, unsigne
     }
     to = to + C::SLOT == end ? end - C::NS * C::SLOT : to + C::SLOT;
   };
-#pragma unroll 1
-  for (int i = 0; i < C::NS - 1; ++i) issue();
-  wait_loads<(C::NS - 2) * C::ND>();
+  issue();
+  issue();
+  wait_loads<C::ND>();
   pd_barrier();
+  constexpr int more = std::min(2, C::NS - 3), ramp = std::max(0, C::NS - 5);
+#pragma unroll
+  for (int i = 0; i < more; ++i) issue();
+  auto ramp_up = [&](auto k) {
+    if (!use.more()) return;
+    wait_loads<(k + 2) * C::ND>();
+    pd_barrier();
+    issue();
+    issue();
+    use.next(p);
+  };
+  if constexpr (ramp > 0) ramp_up(std::integral_constant<int, 0>{});
+  if constexpr (ramp > 1) ramp_up(std::integral_constant<int, 1>{});
+  if constexpr (ramp > 2) ramp_up(std::integral_constant<int, 2>{});
+  static_assert(ramp <= 3, "");
 #pragma unroll 1
-  for (; tiles > 0; --tiles) {
+  for (; use.more(); use.next(p)) {
     wait_loads<(C::NS - 3) * C::ND>();
     pd_barrier();
     issue();
@@ -303,7 +316,7 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
   PdCursor<C> use = pd_begin<C>(p, blockIdx.x, lane);
   if (!use.more()) return;
   if (w >= 4) {
-    paged_load16<DL, SHARED>(p, lds, use, w - 4, lane, pd_tiles(p, use));
+    paged_load16<DL, SHARED>(p, lds, use, w - 4, lane);
     return;
   }
 
@@ -313,7 +326,7 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
   const int offB = rowB * C::RS * 16 + (((2 * w) ^ (swB & 6)) + ((((l16 & 3) >> 1) ^ swB) & 1)) * 16 + (l16 & 1) * 8;  // block w + 4 i: + 128 i
   const int offR = l16 * 128 + ((G ^ (l16 >> 1)) * 16);  // k-step 1: chunk 4 further, ^ 64
 
-  PdPages<C> pages = {0, 0, -1};  // (a tile without a page has no tokens)
+  PdPieces<C> pieces = {0, -1, 0, 0, 0, 0, 0};
   u32x4 q[C::NKW], qr[SHARED ? 1 : 8];
   f32x4 o[C::NB];
   float m_run = 0.f, l_part = 0.f;
@@ -346,7 +359,7 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
       if (!started) pd_barrier();  // the first tile has landed
       started = true;
     }
-    const int nv = pages.at(p, use, 0, lane) < 0 ? 0 : min(16, use.len - use.tile * 16);
+    const int nv = pieces.tokens_of(pieces.lane_of(p, use, 0, lane));
     const unsigned char* buf = lds + slot * C::SLOT;
     // the wave's part of S^T: S[token 4 G + r][head l16]
     f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -478,46 +491,42 @@ __device__ __forceinline__ f32x4 floats4(u32x2 v) { return f32x4{lo_bf16(v[0]), 
 __device__ __forceinline__ bf16x8 minus24() { return as_bf16x8(u32x4{0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u}); }
 
 // The loading waves, 32 tokens of a tile each: tile i + NS - 2 goes into the slot of tile i - 2 after the barrier before which tile i has
-// landed and tile i - 2 was added up.  Past the end they load nothing, so the counts stay the same.
+// landed and tile i - 2 was added up.  The first tiles go out two at a time; past the end nothing is loaded, so the counts stay the same.
 template <class C, bool SHARED>
-__device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned char* lds, PdCursor<C> load, int lw, int lane, int tiles) {
-  PdPages<C> pages = {0, 0, -1};  // of both pieces, one lane each
+__device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned char* lds, PdCursor<C> load, int lw, int lane) {
+  PdPieces<C> pieces[2] = {{0, -1, 0, 0, 0, 0, 0}, {0, -1, 0, 0, 0, 0, 0}};
+  PdCursor<C> use = load;
   uint32_t off[C::NR];
 #pragma unroll
   for (int i = 0; i < C::NR; ++i) {
     const int q = 64 * i + lane, row = q / C::RS, c = q - row * C::RS;
     off[i] = c < C::NCH ? (uint32_t)(row * p.c.row_bytes + 16 * c) : kPdNothing;
   }
-  const uint32_t koff = (uint32_t)((lane & 31) / 2 * p.c.row_bytes + 16 * C::NL * 2 + 32 * (lane >> 5) + 16 * (lane & 1));
-  PdPages<C> second = {0, 0, -1};
+  const uint32_t koff = (uint32_t)((lane & 31) / 2 * p.c.row_bytes + 32 * C::NL + 32 * (lane >> 5) + 16 * (lane & 1));
   const uint32_t base = lds_addr(lds), keys = base + C::NS * C::SLOT, dump = keys + (C::NS - 1) * C::ROPE + C::SX - 1024;
+  const uint32_t scales_bytes = (uint32_t)((p.c.groups - 1) * p.c.size + 16) * 2;
   int slot = 0, kslot = 0;
   auto issue = [&]() {
     const bool more = load.more();
-    const int ids[2] = {more ? pages.at(p, load, 2 * lw, lane) : -1, more ? second.at(p, load, 2 * lw + 1, lane) : -1};
     const int hg = load.hg;
     const uint32_t to = base + slot * C::SLOT;
+    int g = lane >> 1;
+    if (!SHARED && g >= C::NL) g += 16 * hg;
+    const uint32_t sv = g < p.c.groups ? (uint32_t)(g * p.c.size * 2 + 16 * (lane & 1)) : kPdNothing;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int t = 2 * lw + k, sub = load.tile * 4 + t;
-      int nv = 0;
-      const unsigned char* rows = p.c.pages;
-      const bf16* sc = p.c.scales;
-      if (ids[k] >= 0) {
-        const int piece = sub - pd_page(p, sub) * p.pieces;
-        rows += ids[k] * p.c.page_stride + (int64_t)piece * 16 * p.c.row_bytes;
-        sc += ids[k] * p.c.scale_stride + piece * 16;
-        nv = max(0, min(16, load.len - sub * 16));
+      const int t = 2 * lw + k;
+      int at = 0, nv = 0;
+      if (more) {
+        at = pieces[k].lane_of(p, load, t, lane);
+        nv = pieces[k].tokens_of(at);
       }
-      const buf_rsrc r = scalar_rsrc(rows, (uint32_t)(nv * p.c.row_bytes));
+      const buf_rsrc r = pieces[k].rows_of(at, (uint32_t)(nv * p.c.row_bytes));
       const uint32_t rows_to = to + piece_at<C::SUB>(t);
 #pragma unroll
       for (int i = 0; i < C::NR; ++i)
         if (64 * i + lane < 16 * C::RS) dma16(r, off[i], rows_to + i * 1024);
-      const buf_rsrc rs = scalar_rsrc(sc, nv ? (uint32_t)((p.c.groups - 1) * p.c.size + 16) * 2 : 0u);
-      int g = lane >> 1;
-      if (!SHARED && g >= C::NL) g += 16 * hg;
-      const uint32_t sv = g < p.c.groups ? (uint32_t)(g * p.c.size * 2 + 16 * (lane & 1)) : kPdNothing;
+      const buf_rsrc rs = pieces[k].scales_of(at, nv ? scales_bytes : 0u);
       if (lane < 2 * C::NG) dma16(rs, sv, to + C::ROWS + t * C::SC);
       if constexpr (!SHARED) {
 #pragma unroll
@@ -532,10 +541,24 @@ __device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned
     slot = slot + 1 == C::NS ? 0 : slot + 1;
     kslot = kslot + 1 == C::NS - 1 ? 0 : kslot + 1;
   };
+  issue();
+  if constexpr (C::NS > 3) issue();
+  constexpr int ramp = std::max(0, C::NS - 4);
+  auto ramp_up = [&](auto k) {
+    if (!use.more()) return;
+    wait_loads<(k + 1) * C::ND>();
+    pd_barrier();
+    issue();
+    issue();
+    use.next(p);
+  };
+  if constexpr (ramp > 0) ramp_up(std::integral_constant<int, 0>{});
+  if constexpr (ramp > 1) ramp_up(std::integral_constant<int, 1>{});
+  if constexpr (ramp > 2) ramp_up(std::integral_constant<int, 2>{});
+  if constexpr (ramp > 3) ramp_up(std::integral_constant<int, 3>{});
+  static_assert(ramp <= 4, "");
 #pragma unroll 1
-  for (int i = 0; i < C::NS - 2; ++i) issue();
-#pragma unroll 1
-  for (int i = 0; i < tiles; ++i) {
+  for (; use.more(); use.next(p)) {
     wait_loads<(C::NS - 3) * C::ND>();
     pd_barrier();
     issue();
@@ -556,7 +579,7 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
                                              int lane) {
   const int l16 = lane & 15, G = lane >> 4;
   const int offA = piece_at<C::SUB>(w) + l16 * C::RS * 16 + 8 * G;
-  PdPages<C> pages = {0, 0, -1};
+  PdPieces<C> pieces = {0, -1, 0, 0, 0, 0, 0};
   constexpr int NQ = C::NL + 1;  // the latent's runs, and the key: shared, or this lane's head's
   u32x4 q[2 * NQ];
   // The runs' -24 scale sum q come from one product: the tile's scales (rows: tokens) with -24 sum q in three bf16 pieces (24 bits) as
@@ -613,7 +636,7 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
     pd_barrier();  // the tile has landed, and the tile before the last is added up
     const unsigned char* buf = lds + slot * C::SLOT;
     unsigned char* sc = lds + slot * C::SLOT + C::ROWS + w * C::SC;
-    const int sub = use.tile * 4 + w, nv = pages.at(p, use, w, lane) < 0 ? 0 : max(0, min(16, use.len - sub * 16));
+    const int nv = pieces.tokens_of(pieces.lane_of(p, use, w, lane));
     if (nv < 16) {  // scales behind the sequence's end may be anything: 0, so that a p of 0 stays 0
       for (int i = lane; i < C::NG * 16; i += 64)
         if ((i & 15) >= nv) reinterpret_cast<unsigned short*>(sc)[i] = 0;
@@ -794,7 +817,7 @@ __global__ __launch_bounds__(640, 1) void paged_decode4_kernel(PagedDecodeParams
   else if (w < 8)
     paged_add4<C, DL>(p, lds, x, use, w - 4, lane);
   else
-    paged_load4<C, SHARED>(p, lds, use, w - 8, lane, pd_tiles(p, use));
+    paged_load4<C, SHARED>(p, lds, use, w - 8, lane);
 }
 
 // ------------------------------------------------------------------------------------------------ parts
@@ -809,8 +832,8 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   int total = 0, begin = 0, n = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    int nl;
-    const int upto = pd_scan<C>(p, b0, lane, nl);
+    int nl, ll;
+    const int upto = pd_scan<C>(p, b0, lane, nl, ll);
     if (b >= b0 && b < b0 + 64) {
       n = __builtin_amdgcn_readlane(nl, b - b0);
       begin = (total + __builtin_amdgcn_readlane(upto, b - b0) - (n + C::COST)) * p.n_hg + hg * (n + C::COST) + C::COST;
@@ -826,8 +849,7 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
   }
   const int each = pd_each(p, total, C::LEAST), run0 = begin / each, S = (begin + n - 1) / each - run0 + 1;
   if (S == 1) return;
-  // the s-th part; s is cut to the last one
-  auto part_of = [&](int s) { return ((int64_t)2 * (run0 + min(s, S - 1)) + (s == 0 ? 1 : 0)) * 16 + l16; };
+  auto part_of = [&](int s) { return ((int64_t)2 * (run0 + s) + (s == 0 ? 1 : 0)) * 16 + l16; };
   const int part = tid / COLS, col = tid - part * COLS;
   const bool in = part < PARTS;  // (COLS need not divide the workgroup)
   float M = -INFINITY, L = 0.f;
@@ -837,9 +859,13 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
     float m[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int64_t at = part_of(s0 + (in ? part : 0) + i * PARTS);
-      v[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * DL + 4 * (in ? col : 0));
-      m[i] = p.part_ml[2 * at];
+      v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m[i] = -INFINITY;
+      if (in && s0 + part + i * PARTS < S) {
+        const int64_t at = part_of(s0 + part + i * PARTS);
+        v[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * DL + 4 * col);
+        m[i] = p.part_ml[2 * at];
+      }
     }
     static_assert(8 * PARTS <= 256, "");
     float ms = -INFINITY, ls = 0.f, mk[4], lk[4];
@@ -847,7 +873,7 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
     for (int k = 0; k < 4; ++k) {
       const int s = s0 + lane + 64 * k;
       const bool is = lane + 64 * k < 8 * PARTS && s < S;
-      const int64_t at = part_of(s);
+      const int64_t at = part_of(is ? s : 0);
       mk[k] = is ? p.part_ml[2 * at] : -INFINITY;
       lk[k] = is ? p.part_ml[2 * at + 1] : 0.f;
       ms = fmaxf(ms, mk[k]);
@@ -862,7 +888,7 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
     L = L * a + xor32_sum(xor16_sum(ls));
     o *= a;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o += s0 + part + i * PARTS < S ? v[i] * fast_exp2(m[i] - mu) : f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 8; ++i) o += v[i] * fast_exp2(m[i] - mu);
   }
   if (in) o_s[part][col] = o;
   __syncthreads();
