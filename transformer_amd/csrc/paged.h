@@ -4,11 +4,28 @@
 
 namespace mla {
 
+// Division of n < 2^31 by a number that is known at the launch: mul = ceil(2^(31 + l) / d) with 2^(l - 1) < d <= 2^l, so that n mul / 2^(31 + l)
+// is off by less than 1 / d.  (A 64-bit division is over a hundred instructions, more than all else that a thread of the appending and
+// reading kernels does.)
+struct Divisor {
+  uint32_t mul, d;
+  int shift;
+  Divisor() = default;
+  explicit Divisor(uint32_t by) : d(by) {
+    int l = 0;
+    while ((1u << l) < by) ++l;
+    mul = (uint32_t)((((uint64_t)1 << (31 + l)) + by - 1) / by);
+    shift = l - 1;
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+};
+
 struct PagedParams {
   unsigned char* pages;
   bf16* scales;  // null: 16 bits
   const int32_t* table;
   int64_t page_stride, scale_stride, table_stride;
+  Divisor by_size;
   int n_pages, size, table_pages, row_bytes, groups;  // row_bytes: of a row of a page; groups: runs of 64 values of a row
 };
 
@@ -58,6 +75,7 @@ inline int paged_setup(const mla_paged_cache& c, const char* op, int64_t B, Page
   p.table_stride = c.table_stride;
   p.n_pages = (int)c.n_pages;
   p.size = (int)c.page_size;
+  p.by_size = Divisor((uint32_t)c.page_size);
   p.table_pages = (int)c.table_pages;
   p.row_bytes = (int)row;
   p.groups = (int)(W / 64);
