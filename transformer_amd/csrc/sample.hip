@@ -1,5 +1,7 @@
 // Drawing one token for each row of logits: temperature, top-k, top-p, min-p and the draw from a given number (gfx950).
 #include <cmath>
+#include <cstddef>
+#include <type_traits>
 
 #include "mla_common.h"
 
@@ -36,6 +38,7 @@ __device__ __forceinline__ float sm_value(uint32_t key) {
 }
 
 typedef unsigned long long u64;
+#define SM_INLINE __attribute__((always_inline))  // a call would put what its lambda refers to into memory
 
 // 2^(44 + i / 32)
 __constant__ const double kSmTable[32] = {
@@ -51,21 +54,23 @@ __constant__ const double kSmTable[32] = {
 // degree 3 at the Chebyshev nodes: within 1.6e-13, in fp64 throughout (a token whose number falls that near a border could come out
 // as its neighbour).  The additions of 1.5 2^52 and 2^52 round to whole numbers and leave them in the low bits: fp64 additions and
 // products run at the full rate, conversions and exponent operations do not.
+constexpr u64 kSmBias = 0x433ull << 52;
 struct SmWeight {
   double w;  // in units of 2^-44, before the rounding
-  u64 whole;
+  u64 bits;  // kSmBias + the weight: sums of n of them less n kSmBias are the weights' (modulo 2^64)
+  __device__ u64 whole() const { return bits & 0xfffffffffffffull; }
 };
 __device__ __forceinline__ SmWeight sm_weight(double d, double per32, const double* table) {
   const double t = fma(d, per32, 6755399441055744.0), r = fma(d, per32, -(t - 6755399441055744.0));
-  const int n = (int)(unsigned)__double_as_longlong(t);
+  const unsigned n = (unsigned)__double_as_longlong(t);
   const double c = table[n & 31];
   double q = 9.172598566029335e-09;
   q = fma(q, r, 1.6938609067364198e-06);
   q = fma(q, r, 0.00023459619820112603);
   q = fma(q, r, 0.021660849392187844);
   const double e = fma(c * r, q, c);
-  const double w = __longlong_as_double(__double_as_longlong(e) + ((long long)(n >> 5) << 52));
-  return {w, (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull};
+  const double w = __hiloint2double(__double2hiint(e) + (int)((n & ~31u) << 15), __double2loint(e));
+  return {w, (u64)__double_as_longlong(w + 4503599627370496.0)};
 }
 
 // What the passes over a row share.
@@ -105,6 +110,11 @@ __device__ __forceinline__ u64 sm_lane(u64 v, int lane) {
   return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, lane);
 }
 __device__ __forceinline__ u64 sm_last(u64 v) { return sm_lane(v, 63); }
+// the lanes' sum, of numbers below 2^52: two pieces whose sums fit 32 bits
+__device__ __forceinline__ u64 sm_wave_sum(u64 v) {
+  const unsigned lo = sm_scan32<true>((unsigned)v & ((1u << 26) - 1)), hi = sm_scan32<true>((unsigned)(v >> 26));
+  return (unsigned)__builtin_amdgcn_readlane((int)lo, 63) + ((u64)(unsigned)__builtin_amdgcn_readlane((int)hi, 63) << 26);
+}
 // Sums of the threads up to and with this one, and of all; integers, so in any order.  `turn` says which half of `part` is free.
 __device__ __forceinline__ u64 sm_scan(u64 v, SmShared& s, int& turn, u64& total) {
   v = sm_wave_scan(v);
@@ -122,6 +132,48 @@ __device__ __forceinline__ u64 sm_sum(u64 v, SmShared& s, int& turn) {
   sm_scan(v, s, turn, total);
   return total;
 }
+// One step of a sorting network in a wave: lane t and lane t ^ J take the larger and the smaller of their values.  Nothing goes through
+// LDS: quads are permuted, halves of rows mirrored, rows rotated and exchanged.
+template <int CTRL>
+__device__ __forceinline__ u64 sm_moved(u64 v) {
+  return (u64)(unsigned)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xf, 0xf, false) << 32 |
+         (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, 0xf, 0xf, false);
+}
+template <int J>
+__device__ __forceinline__ u64 sm_step(u64 v, bool larger) {
+  u64 o;
+  if constexpr (J >= 16) {  // (which of the two is whose does not matter)
+    const auto lo = J == 32 ? __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false)
+                            : __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+    const auto hi = J == 32 ? __builtin_amdgcn_permlane32_swap((unsigned)(v >> 32), (unsigned)(v >> 32), false, false)
+                            : __builtin_amdgcn_permlane16_swap((unsigned)(v >> 32), (unsigned)(v >> 32), false, false);
+    v = (u64)hi[0] << 32 | lo[0];
+    o = (u64)hi[1] << 32 | lo[1];
+  } else if constexpr (J == 8) {
+    o = sm_moved<0x128>(v);  // row_ror 8
+  } else if constexpr (J == 4) {
+    o = sm_moved<0x141>(sm_moved<0x1b>(v));  // xor 3, then row_half_mirror: xor 7
+  } else {
+    o = sm_moved<J == 2 ? 0x4e : 0xb1>(v);
+  }
+  return larger == (v > o) ? v : o;
+}
+// the steps J, J / 2 .. 1 of the part that ends in runs of k
+template <int J>
+__device__ __forceinline__ u64 sm_steps(u64 v, int t, int k) {
+  v = sm_step<J>(v, ((t & J) == 0) == ((t & k) == 0));
+  if constexpr (J > 1) v = sm_steps<J / 2>(v, t, k);
+  return v;
+}
+// a wave's 64 values in order, the largest in lane 0 (in lane 63 where t has bit 6 set)
+__device__ __forceinline__ u64 sm_wave_sort(u64 v, int t) {
+  v = sm_steps<1>(v, t, 2);
+  v = sm_steps<2>(v, t, 4);
+  v = sm_steps<4>(v, t, 8);
+  v = sm_steps<8>(v, t, 16);
+  v = sm_steps<16>(v, t, 32);
+  return sm_steps<32>(v, t, 64);
+}
 // Sorts the list's n <= kSmList entries, the largest first; thread t gets the t-th (0 past the end).
 __device__ __forceinline__ u64 sm_sort(SmShared& s, int n) {
   const int t = threadIdx.x;
@@ -129,24 +181,22 @@ __device__ __forceinline__ u64 sm_sort(SmShared& s, int n) {
   u64 v = t < n ? s.order[t] : 0;
   int size = 64;  // (n <= kSmList: the threads past it only wait)
   while (size < n) size <<= 1;
-  for (int k = 2; k <= size; k <<= 1) {
-    for (int j = k >> 1; j; j >>= 1) {
-      u64 o;
-      if (j < 64) {
-        if ((t & ~63) >= size) continue;  // (whole waves)
-        o = __shfl_xor(v, j, 64);
-      } else {
-        __syncthreads();
-        if (t < kSmList) s.order[t] = v;
-        __syncthreads();
-        o = s.order[(t ^ j) & (kSmList - 1)];
-      }
-      const bool larger = ((t & j) == 0) == ((t & k) == 0);  // this place takes the larger of the two
-      v = larger == (v > o) ? v : o;
+  const bool in = (t & ~63) < size;  // (whole waves)
+  if (in) v = sm_wave_sort(v, t);
+#pragma unroll 1
+  for (int k = 128; k <= size; k <<= 1) {
+#pragma unroll 1
+    for (int j = k >> 1; j >= 64; j >>= 1) {
+      __syncthreads();
+      if (in) s.order[t] = v;
+      __syncthreads();
+      const u64 o = in ? s.order[t ^ j] : 0;
+      v = (((t & j) == 0) == ((t & k) == 0)) == (v > o) ? v : o;
     }
+    if (in) v = sm_steps<32>(v, t, k);
   }
   __syncthreads();
-  if (t < kSmList) s.order[t] = v;
+  if (in) s.order[t] = v;
   __syncthreads();
   return t < n ? v : 0;
 }
@@ -179,7 +229,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
   const int head = (int)((uintptr_t)row / sizeof(T) & 3);
   const int quads = CH > 0 ? CH : (V + head + 4 * kSmThreads - 1) / (4 * kSmThreads);
   bool all_or_nothing = false;
-  auto load = [&](int q) {
+  auto load = [&](int q) SM_INLINE {
     const int i0 = (q * kSmThreads + tid) * 4 - head;
     f32x4 v;
     if (i0 >= 0 && i0 + 4 <= V) {
@@ -201,7 +251,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
     }
     return v;
   };
-  auto at = [&](int q) {
+  auto at = [&](int q) SM_INLINE {
     if constexpr (CH > 0)
       return xs[q * kSmThreads + tid];
     else
@@ -209,7 +259,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
   };
   auto index = [&](int q, int e) { return (q * kSmThreads + tid) * 4 - head + e; };
   // f(value, index) of every logit of the thread
-  auto each = [&](auto&& f) {
+  auto each = [&](auto&& f) SM_INLINE {
 #pragma unroll 1
     for (int q = 0; q < quads; ++q) {
       const f32x4 v = at(q);
@@ -218,7 +268,9 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
     }
   };
 
+  auto top_of = [](f32x4 v) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
   float own = -INFINITY;
+  float quad_top[CH > 0 ? CH : 1];  // the largest of each of the thread's quads
   if constexpr (CH > 0) {
 #pragma unroll
     for (int q0 = 0; q0 < CH; q0 += 8) {
@@ -230,7 +282,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
       for (int q = 0; q < 8; ++q)
         if (q0 + q < CH) {
           xs[(q0 + q) * kSmThreads + tid] = v[q];
-          own = fmaxf(own, fmaxf(fmaxf(v[q][0], v[q][1]), fmaxf(v[q][2], v[q][3])));
+          own = fmaxf(own, quad_top[q0 + q] = top_of(v[q]));
         }
     }
   } else {
@@ -274,48 +326,83 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
     big = 0.f;
     own = own == INFINITY ? 0.f : -INFINITY;
     if constexpr (CH > 0) {
-#pragma unroll 1
+#pragma unroll
       for (int q = 0; q < CH; ++q) {
         f32x4& x = xs[q * kSmThreads + tid];
+        quad_top[q] = quad_top[q] == INFINITY ? 0.f : -INFINITY;
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
       }
     }
   }
-  const double xmax = (double)big, per32 = 46.16624130844683 / (double)temperature;  // 32 log2 e
+  const double xmax = (double)big, rate = 1.0 / (double)temperature, per32 = 46.16624130844683 * rate;  // 32 log2 e
   const double least_d = -33.0 * (double)temperature;                                // weighs nothing
   const double least = (double)min_p * kSmOne;
   const float bins_t = fminf((float)kSmPerNat / temperature, 1e30f);
-  auto weight = [&](float v) {
+  auto weight = [&](float v) SM_INLINE {
     SmWeight w = sm_weight(fmax((double)v - xmax, least_d), per32, s.table);
-    asm volatile("" : "+v"(w.whole));  // not put under the condition of its use: a branch for each logit, each waiting for the table
+    asm volatile("" : "+v"(w.bits));  // not put under the condition of its use: a branch for each logit, each waiting for the table
     return w;
   };
   // a logit's distance from the largest in bins; a bin is its whole part, the last one takes all beyond
   auto distance = [&](float v) { return (big - v) * bins_t; };
   auto bin_of = [&](float v) { return (int)fminf(distance(v), (float)(kSmBins - 1)); };
 
-  // what is kept: values above `cut`, and of those equal to it the ones below index `bound`; never a -inf
-  float cut = -kSmMost;
+  // what is kept: values of `cut` and more, from index `bound` on only larger ones; never a -inf
+  float cut = -kSmMost, above_cut = -kSmMost;
   int bound = V;
-  auto is_kept = [&](float v, int i) { return (v > cut) | ((v == cut) & (i < bound)); };
+  auto is_kept = [&](float v, int i) SM_INLINE {
+    const float least_here = i < bound ? +cut : +above_cut;
+    return v >= least_here;
+  };
+  // a quad with -inf for what is not; `bound` lies in few of them
+  auto kept_quad = [&](int q) SM_INLINE {
+    f32x4 v = at(q);
+    const int i0 = index(q, 0);
+    const float least_here = i0 < bound ? +cut : +above_cut;
+    if (__ballot((i0 < bound) & (bound < i0 + 4))) {
+#pragma unroll
+      for (int e = 1; e < 4; ++e) v[e] = is_kept(v[e], i0 + e) ? v[e] : -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = v[e] >= least_here ? v[e] : -INFINITY;
+    return v;
+  };
+  auto cut_at_key = [&](unsigned key) {
+    cut = sm_value(key);
+    above_cut = sm_value(key + 1);
+  };
   auto cut_at = [&](u64 last) {  // the last one kept
-    cut = sm_value((unsigned)(last >> 32));
+    cut_at_key((unsigned)(last >> 32));
     bound = (int)~(unsigned)last + 1;
   };
-  // lists the tokens that `f` says (s.n is 0 before); their number, which may be more than the list takes
-  auto list = [&](auto&& f) {
-    each([&](float v, int i) {
-      if (f(v, i)) {
-        const unsigned k = atomicAdd(&s.n, 1u);
-        if (k < kSmList) s.order[k] = (u64)sm_key(v) << 32 | ~(unsigned)i;
-      }
-    });
+  // lists the tokens that `f` says, of quads whose largest value `any` lets in (s.n is 0 before); their number, which may be more than
+  // the list takes
+  auto list = [&](auto&& any, auto&& f) SM_INLINE {
+    auto quad = [&](int q) SM_INLINE {
+      const f32x4 v = at(q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (f(v[e], index(q, e), 4 * q + e)) {
+          const unsigned k = atomicAdd(&s.n, 1u);
+          if (k < kSmList) s.order[k] = (u64)sm_key(v[e]) << 32 | ~(unsigned)index(q, e);
+        }
+    };
+    if constexpr (CH > 0) {
+      unsigned hot = 0;
+#pragma unroll
+      for (int q = 0; q < CH; ++q) hot |= (unsigned)any(quad_top[q]) << q;
+      for (; hot; hot &= hot - 1) quad(__ffs(hot) - 1);
+    } else {
+#pragma unroll 1
+      for (int q = 0; q < quads; ++q)
+        if (any(top_of(at(q)))) quad(q);
+    }
     __syncthreads();
     return (int)s.n;
   };
   // the bound that leaves the first r of the kept tokens equal to `cut`
-  auto bound_of = [&](u64 r) {
+  auto bound_of = [&](u64 r) SM_INLINE {
     int lo = 0;
 #pragma unroll 1
     for (int bit = kSmMaxV; bit; bit >>= 1) {
@@ -326,52 +413,24 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
     }
     return lo;
   };
-  // the bin at which the bins' numbers add up to `need`, and what lies above it, in s.found_bin (left alone if none) and s.above
-  auto find = [&](u64 n0, u64 n1, u64 need) {
-    u64 total;
-    const u64 before = sm_scan(n0 + n1, s, turn, total) - n0 - n1;
-    if (before < need && need <= before + n0 + n1) {
-      const bool second = before + n0 < need;
+  // the bin at which the bins' numbers add up to what `need` makes of their sum, and what lies above it, in s.found_bin (left alone if
+  // none) and s.above
+  auto find = [&](u64 n0, u64 n1, auto&& need) SM_INLINE {
+    u64 all;
+    const u64 before = sm_scan(n0 + n1, s, turn, all) - n0 - n1, n = need(all);
+    if (before < n && n <= before + n0 + n1) {
+      const bool second = before + n0 < n;
       s.found_bin = 2 * tid + second;
       s.above = before + (second ? n0 : 0);
     }
     __syncthreads();
   };
-  // One wave and a short list: its entries, two a lane, their weights, and of each its place and the weight before it, by a pass over
-  // the others.
-  u64 o[2], ow[2], before[2];
-  double owd[2];
-  int rank[2];
-  auto ranks = [&](int n) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int t = lane + 64 * k;
-      o[k] = t < n ? s.order[t] : 0;
-      const SmWeight x = weight(sm_value((unsigned)(o[k] >> 32)));
-      ow[k] = t < n ? x.whole : 0;
-      owd[k] = x.w;
-      s.mass[t] = ow[k];
-      rank[k] = 0;
-      before[k] = 0;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const u64 oj = s.order[j], wj = s.mass[j];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (k == 1 && n <= 64) continue;
-        rank[k] += oj > o[k];
-        before[k] += oj > o[k] ? wj : 0;
-      }
-    }
-  };
-
   // the draw: the first sum above `aim` is the token's.  Where it ends up is one thread's `hit`.
   auto aim_of = [&](u64 total) { return min((u64)((double)u * (double)total), total - 1); };
   bool hit = false;
   int token = 0;
   float value = 0.f;
+  double log_total = 0.0;
   u64 total = 0;
 
   int n_list = -1;  // a list of all that is kept, in order: thread t has entry t in `mine`
@@ -383,11 +442,12 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
       const int bin = bin_of(own);
       if (bin < kSmBins - 1) atomicAdd(&s.count[bin], 1u);
       __syncthreads();
-      find(s.count[2 * tid], s.count[2 * tid + 1], top_k);
+      find(s.count[2 * tid], s.count[2 * tid + 1], [&](u64) { return (u64)top_k; });
       if (s.found_bin < kSmBins) {
         const float end = (float)(s.found_bin + 1);
-        n_list = list([&](float v, int) { return distance(v) < end; });
-        in_one_wave = n_list <= 128;
+        auto near = [&](float v, int = 0, int = 0) { return distance(v) < end; };
+        n_list = list(near, near);
+        in_one_wave = n_list <= 64;
         if (n_list > kSmList) n_list = -1;
       }
     }
@@ -401,14 +461,15 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
         if (bin < kSmBins - 1) atomicAdd(&s.count[bin], 1u);
       });
       __syncthreads();
-      find(s.count[2 * tid], s.count[2 * tid + 1], top_k);
+      find(s.count[2 * tid], s.count[2 * tid + 1], [&](u64) { return (u64)top_k; });
       const int bin = s.found_bin;
       if (bin < kSmBins) {  // (else fewer than top_k weigh anything)
         const int above = (int)s.above, in = s.count[bin];
         const bool all = above + in <= kSmList;
         const float from = all ? 0.f : (float)bin, end = (float)(bin + 1);
         if (in <= kSmList) {
-          const int n = list([&](float v, int) { return (distance(v) >= from) & (distance(v) < end); });
+          const int n = list([&](float v) { return distance(v) < end; },
+                             [&](float v, int, int) { return (distance(v) >= from) & (distance(v) < end); });
           if (all) {
             n_list = n;
           } else {
@@ -426,14 +487,14 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
           u64 n = 0;
           each([&](float v, int) { n += sm_key(v) > t; });
           n = sm_sum(n, s, turn);
-          cut = sm_value(t);
+          cut_at_key(t);
           bound = bound_of(top_k - n);
         }
         if (n_list < 0 && top_k <= kSmList) {
           __syncthreads();
           if (tid == 0) s.n = 0;
           __syncthreads();
-          n_list = list([&](float v, int i) { return is_kept(v, i); });
+          n_list = list([&](float v) { return v >= cut; }, [&](float v, int i, int) { return is_kept(v, i); });
         }
       }
     }
@@ -444,50 +505,36 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
   }
 
   if (in_one_wave) {
+    // a lane an entry: in order for top_k and top_p, then by index (~index: the larger is the earlier) for the draw
     if (wave != 0) return;
-    ranks(n_list);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) ow[k] = rank[k] >= top_k ? 0 : ow[k];
+    mine = sm_wave_sort(lane < n_list ? s.order[lane] : 0, lane);
+    const SmWeight w = weight(sm_value((unsigned)(mine >> 32)));
+    u64 whole = lane < min(n_list, top_k) ? w.whole() : 0;
     if (top_p < 1.f) {
-      const u64 target = (u64)ceil((double)top_p * (double)sm_last(sm_wave_scan(ow[0] + ow[1])));
-#pragma unroll
-      for (int k = 0; k < 2; ++k) ow[k] = rank[k] > 0 && before[k] >= target ? 0 : ow[k];
+      const u64 upto = sm_wave_scan(whole), target = (u64)ceil((double)top_p * (double)sm_last(upto));
+      whole = lane > 0 && upto - whole >= target ? 0 : whole;
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      ow[k] = owd[k] < least ? 0 : ow[k];
-      s.mass[lane + 64 * k] = ow[k];
-      before[k] = 0;
-    }
-    total = sm_last(sm_wave_scan(ow[0] + ow[1]));
-    const u64 aim = aim_of(total);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 4
-    for (int j = 0; j < n_list; ++j) {
-      const unsigned ij = (unsigned)s.order[j];
-      const u64 wj = s.mass[j];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (k == 0 || n_list > 64) before[k] += ij > (unsigned)o[k] ? wj : 0;  // (~index: the larger is the earlier)
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (before[k] <= aim && aim < before[k] + ow[k]) {
-        hit = true;
-        token = (int)~(unsigned)o[k];
-        value = sm_value((unsigned)(o[k] >> 32));
-      }
+    whole = w.w < least ? 0 : whole;
+    total = sm_last(sm_wave_scan(whole));
+    log_total = log((double)total / kSmOne);
+    const u64 aim = aim_of(total), by_index = sm_wave_sort(mine << 32 | (unsigned)lane, lane);
+    const int from = (int)(unsigned)by_index;
+    whole = (u64)(unsigned)__shfl((int)(whole >> 32), from, 64) << 32 | (unsigned)__shfl((int)(unsigned)whole, from, 64);
+    const u64 upto = sm_wave_scan(whole);
+    hit = aim < upto && upto - whole <= aim;
+    token = (int)~(unsigned)(by_index >> 32);
+    value = sm_value((unsigned)__shfl((int)(mine >> 32), from, 64));
   } else if (n_list >= 0) {
     value = sm_value((unsigned)(mine >> 32));
     token = (int)~(unsigned)mine;
-    SmWeight w = weight(value);
-    if (tid >= n_list) w = {0.0, 0};
+    const SmWeight w = weight(value);
+    u64 whole = tid < n_list ? w.whole() : 0;
     if (top_p < 1.f) {
-      const u64 upto = sm_scan(w.whole, s, turn, total);
+      const u64 upto = sm_scan(whole, s, turn, total);
       const u64 target = (u64)ceil((double)top_p * (double)total);
-      if (tid > 0 && upto - w.whole >= target) w.whole = 0;
+      if (tid > 0 && upto - whole >= target) whole = 0;
     }
-    if (w.w < least) w.whole = 0;
+    if (w.w < least) whole = 0;
     // the vocabulary in kSmThreads runs, of which the list's tokens fill a few
     int shift = 0;
     while ((V - 1) >> shift >= kSmThreads) ++shift;
@@ -495,7 +542,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
     s.mass[tid] = 0;
     if (tid == 0) s.n = 0;
     __syncthreads();
-    if (w.whole) atomicAdd(&s.mass[token >> shift], w.whole);
+    if (whole) atomicAdd(&s.mass[token >> shift], whole);
     __syncthreads();
     const u64 run = s.mass[tid], upto = sm_scan(run, s, turn, total);
     const u64 aim = aim_of(total);
@@ -504,59 +551,74 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
       s.above = upto - run;
     }
     __syncthreads();
-    const bool in = w.whole && (unsigned)(token >> shift) == s.at;
+    const bool in = whole && (unsigned)(token >> shift) == s.at;
     if (in) {
       const unsigned k = atomicAdd(&s.n, 1u);
       s.order[k] = (u64)token;
-      s.mass[k] = w.whole;
+      s.mass[k] = whole;
     }
     __syncthreads();
     if (in) {
       u64 sum = s.above;
       for (unsigned k = 0; k < s.n; ++k) sum += (int)s.order[k] < token ? s.mass[k] : 0;
-      hit = sum <= aim && aim < sum + w.whole;
+      hit = sum <= aim && aim < sum + whole;
     }
   } else {
     // The whole row: its weights by bin for top_p, and again (there are no registers for 32 of them a thread) for the draw.
+    unsigned above_bits = 0, in_bits = 0;  // (CH > 0) the thread's logits, a bit each: what lies above top_p's bin, and in it
     if (top_p < 1.f) {
       __syncthreads();
       s.mass[tid] = s.mass[tid + kSmThreads] = 0;
       if (tid == 0) s.n = 0, s.found_bin = kSmBins;
-      u64 own_sum = 0;
       __syncthreads();
-      each([&](float v, int i) {
-        u64 w = weight(v).whole;
-        w = is_kept(v, i) ? w : 0;
-        own_sum += w;
-        if (w) atomicAdd(&s.mass[bin_of(v)], w);
-      });
-      const u64 sum = sm_sum(own_sum, s, turn);
-      const u64 target = max((u64)ceil((double)top_p * (double)sum), (u64)1);
-      find(s.mass[2 * tid], s.mass[2 * tid + 1], target);
+#pragma unroll 1
+      for (int q = 0; q < quads; ++q) {
+        const f32x4 v = kept_quad(q);
+        u64 whole[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) whole[e] = weight(v[e]).whole();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float d = distance(v[e]);
+          if (d < (float)(kSmBins - 1)) atomicAdd(&s.mass[(int)d], whole[e]);
+        }
+      }
+      __syncthreads();
+      u64 target;
+      find(s.mass[2 * tid], s.mass[2 * tid + 1], [&](u64 sum) { return target = max((u64)ceil((double)top_p * (double)sum), (u64)1); });
       const float from = (float)s.found_bin, end = (float)(s.found_bin + 1);
       const u64 above = s.above;
-      const int n = list([&](float v, int i) { return (distance(v) >= from) & (distance(v) < end) & is_kept(v, i); });
-      if (n <= 128) {
+      const int n = list([&](float v) { return distance(v) < end; },
+                         [&](float v, int i, int j) {
+                           const float d = distance(v);
+                           const bool k = (d < end) & is_kept(v, i), in = k & (d >= from);
+                           if (CH > 0) {
+                             above_bits |= (unsigned)(k & !in) << (j & 31);
+                             in_bits |= (unsigned)in << (j & 31);
+                           }
+                           return in;
+                         });
+      if (n <= 64) {
         if (wave == 0) {
-          ranks(n);
+          mine = sm_wave_sort(lane < n ? s.order[lane] : 0, lane);
+          const SmWeight x = weight(sm_value((unsigned)(mine >> 32)));
+          const u64 whole = lane < n ? x.whole() : 0, upto = above + sm_wave_scan(whole);
           // the last with less than the target before it: with its own weight it is reached
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            if (before[k] + above < target && before[k] + above + ow[k] >= target) s.order[kSmList - 1] = o[k];
+          if (upto - whole < target && upto >= target) s.order[kSmList - 1] = mine;
         }
         __syncthreads();
         cut_at(s.order[kSmList - 1]);
       } else if (n <= kSmList) {
         mine = sm_sort(s, n);
-        const u64 w = weight(sm_value((unsigned)(mine >> 32))).whole, mw = tid < n ? w : 0;
+        const u64 w = weight(sm_value((unsigned)(mine >> 32))).whole(), mw = tid < n ? w : 0;
         const u64 ahead = sm_scan(mw, s, turn, total) - mw + above;
         const u64 last = sm_sum(tid < n && ahead < target, s, turn);
         cut_at(s.order[last - 1]);
       } else {
-        auto mass_above = [&](unsigned t) {
+        auto mass_above = [&](unsigned t) SM_INLINE {
           u64 m = 0;
           each([&](float v, int i) {
-            const u64 w = weight(v).whole;
+            const u64 w = weight(v).whole();
             m += (sm_key(v) > t) & is_kept(v, i) ? w : 0;
           });
           return sm_sum(m, s, turn);
@@ -565,31 +627,71 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
 #pragma unroll 1
         for (unsigned bit = 1u << 31; bit; bit >>= 1)
           if (mass_above(t + bit - 1) >= target) t += bit;
-        const u64 ahead = mass_above(t), w = weight(sm_value(t)).whole;
+        const u64 ahead = mass_above(t), w = weight(sm_value(t)).whole();
         if (sm_value(t) > cut) {
-          cut = sm_value(t);
+          cut_at_key(t);
           bound = V;
         }
         bound = bound_of(w ? (target - ahead + w - 1) / w : V);
       }
     }
 
-    // the draw: runs of 256 indices, a wave's quad each
-    auto final_weight = [&](float v, int i) -> u64 {
-      const SmWeight w = weight(v);
-      return is_kept(v, i) & !(w.w < least) ? w.whole : 0;
+    // The draw: runs of 256 indices, a wave's quad each.  Where the row is kept in LDS and few of it are left, their indices are listed
+    // (where the counts and the list were) and only they are weighed again.
+    // the weights of a quad and kSmBias each, and their sum
+    u64 w[4];
+    auto quad_weights = [&](int q) SM_INLINE {
+      const f32x4 v = kept_quad(q);
+      SmWeight x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = (x[e] = weight(v[e])).bits;
+      if (least > 0) {
+        asm volatile("");  // (a branch: most rows have none)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = x[e].w < least ? kSmBias : w[e];
+      }
+      return w[0] + w[1] + w[2] + w[3] - 4 * kSmBias;
     };
     __syncthreads();
     for (int i = tid; i < kSmRuns; i += kSmThreads) s.mass[i] = 0;
     __syncthreads();
+    bool few = false;
+    if constexpr (CH > 0) {
+      unsigned short* at_of = reinterpret_cast<unsigned short*>(s.count);  // (places in xs)
+      constexpr unsigned kFew = (sizeof(s.count) + sizeof(s.order)) / 2;
+      static_assert(offsetof(SmShared, order) == offsetof(SmShared, count) + sizeof(s.count) && CH <= 8, "");
+      u64 n_kept = kFew + 1;
+      if (top_p < 1.f) {
+        unsigned kept = above_bits;
+        for (unsigned m = in_bits; m; m &= m - 1) {
+          const int j = __ffs(m) - 1, i = index(j >> 2, j & 3);
+          if (is_kept(reinterpret_cast<const float*>(xs)[i + head], i)) kept |= m & -m;
+        }
+        const unsigned n = __popc(kept);
+        unsigned k = (unsigned)sm_scan(n, s, turn, n_kept) - n;
+        if (n_kept <= kFew)
+          for (; kept; kept &= kept - 1) {
+            const int j = __ffs(kept) - 1;
+            at_of[k++] = (unsigned short)(((j >> 2) * kSmThreads + tid) * 4 + (j & 3));
+          }
+        __syncthreads();
+      }
+      few = n_kept <= kFew;
+      if (few) {
 #pragma unroll 1
-    for (int q = 0; q < quads; ++q) {
-      const f32x4 v = at(q);
-      u64 m = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) m += final_weight(v[e], index(q, e));
-      m = sm_last(sm_wave_scan(m));
-      if (lane == 0) s.mass[q * kSmWaves + wave] = m;
+        for (unsigned k = tid; k < n_kept; k += kSmThreads) {
+          const unsigned i = at_of[k];
+          const SmWeight w = weight(reinterpret_cast<const float*>(xs)[i]);
+          if (!(w.w < least) && w.whole()) atomicAdd(&s.mass[i / 256], w.whole());
+        }
+      }
+    }
+    if (!few) {
+#pragma unroll 1
+      for (int q = 0; q < quads; ++q) {
+        const u64 m = sm_wave_sum(quad_weights(q));
+        if (lane == 0) s.mass[q * kSmWaves + wave] = m;
+      }
     }
     __syncthreads();
     constexpr int PER = (kSmRuns + kSmThreads - 1) / kSmThreads;
@@ -610,23 +712,22 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
     if ((int)s.at % kSmWaves != wave) return;
     const int q = s.at / kSmWaves;
     const f32x4 v = at(q);
-    u64 w[4], m = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m += w[e] = final_weight(v[e], index(q, e));
+    const u64 m = quad_weights(q);
     ahead = s.above + sm_wave_scan(m) - m;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (ahead <= aim && aim < ahead + w[e]) {
+      const u64 we = w[e] - kSmBias;
+      if (ahead <= aim && aim < ahead + we) {
         hit = true;
         token = index(q, e);
         value = v[e];
       }
-      ahead += w[e];
+      ahead += we;
     }
   }
   if (hit) {
     a.tokens[b] = token;
-    a.logprobs[b] = (float)(((double)value - xmax) / (double)temperature - log((double)total / kSmOne));
+    a.logprobs[b] = (float)(((double)value - xmax) * rate - (in_one_wave ? log_total : log((double)total / kSmOne)));
   }
 }
 
