@@ -127,6 +127,18 @@ __device__ __forceinline__ u64 sm_scan(u64 v, SmShared& s, int& turn, u64& total
   total = sm_lane(p, kSmWaves - 1);
   return v + (w ? sm_lane(p, w - 1) : 0);
 }
+// the same of counts: 32 bits
+__device__ __forceinline__ unsigned sm_scan_count(unsigned v, SmShared& s, int& turn, unsigned& total) {
+  v = sm_scan32<true>(v);
+  u64* part = s.part[turn];
+  turn ^= 1;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if ((threadIdx.x & 63) == 63) part[w] = v;
+  __syncthreads();
+  const unsigned p = sm_scan32<false>((unsigned)part[threadIdx.x & (kSmWaves - 1)]);
+  total = (unsigned)__builtin_amdgcn_readlane((int)p, kSmWaves - 1);
+  return v + (w ? (unsigned)__builtin_amdgcn_readlane((int)p, w - 1) : 0);
+}
 __device__ __forceinline__ u64 sm_sum(u64 v, SmShared& s, int& turn) {
   u64 total;
   sm_scan(v, s, turn, total);
@@ -290,7 +302,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
   }
   if (tid < 32) s.table[tid] = kSmTable[tid];
   s.count[tid] = s.count[tid + kSmThreads] = 0;
-  if (tid == 0) s.n = 0, s.found_bin = kSmBins;
+  if (tid == 0) s.found_bin = kSmBins;
   float big = own;
 #pragma unroll
   for (int m = 8; m; m >>= 1) big = fmaxf(big, wave_shfl_xor(big, m));
@@ -376,30 +388,49 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
     cut_at_key((unsigned)(last >> 32));
     bound = (int)~(unsigned)last + 1;
   };
-  // lists the tokens that `f` says, of quads whose largest value `any` lets in (s.n is 0 before); their number, which may be more than
-  // the list takes
+  // g(j, k) of the thread's logits whose bits are set in `bits` (bit j: place j & 3 of quad j / 4), the k-th of all threads'; their number
+  auto number = [&](unsigned bits, unsigned most, auto&& g) SM_INLINE {
+    unsigned n;
+    unsigned k = sm_scan_count(__popc(bits), s, turn, n) - __popc(bits);
+    for (; bits && k < most; bits &= bits - 1) g(__ffs(bits) - 1, k++);
+    __syncthreads();
+    return n;
+  };
+  auto place = [&](int j) { return ((j >> 2) * kSmThreads + tid) * 4 + (j & 3); };  // of logit j in xs: its index + head
+  auto entry = [&](float v, int i) { return (u64)sm_key(v) << 32 | ~(unsigned)i; };
+  // lists the tokens that `f` says, of quads whose largest value `any` lets in; their number, which may be more than the list takes.
+  // f gets the value, the index and the thread's number for it.
   auto list = [&](auto&& any, auto&& f) SM_INLINE {
-    auto quad = [&](int q) SM_INLINE {
-      const f32x4 v = at(q);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (f(v[e], index(q, e), 4 * q + e)) {
-          const unsigned k = atomicAdd(&s.n, 1u);
-          if (k < kSmList) s.order[k] = (u64)sm_key(v[e]) << 32 | ~(unsigned)index(q, e);
-        }
-    };
     if constexpr (CH > 0) {
-      unsigned hot = 0;
+      unsigned hot = 0, bits = 0;
 #pragma unroll
       for (int q = 0; q < CH; ++q) hot |= (unsigned)any(quad_top[q]) << q;
-      for (; hot; hot &= hot - 1) quad(__ffs(hot) - 1);
+      for (; hot; hot &= hot - 1) {
+        const int q = __ffs(hot) - 1;
+        const f32x4 v = at(q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bits |= (unsigned)f(v[e], index(q, e), 4 * q + e) << (4 * q + e);
+      }
+      return (int)number(bits, kSmList,
+                         [&](int j, unsigned k) { s.order[k] = entry(reinterpret_cast<const float*>(xs)[place(j)], place(j) - head); });
     } else {
+      if (tid == 0) s.n = 0;
+      __syncthreads();
 #pragma unroll 1
-      for (int q = 0; q < quads; ++q)
-        if (any(top_of(at(q)))) quad(q);
+      for (int q = 0; q < quads; ++q) {
+        const f32x4 v = at(q);
+        if (any(top_of(v))) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (f(v[e], index(q, e), 0)) {
+              const unsigned k = atomicAdd(&s.n, 1u);
+              if (k < kSmList) s.order[k] = entry(v[e], index(q, e));
+            }
+        }
+      }
+      __syncthreads();
+      return (int)s.n;
     }
-    __syncthreads();
-    return (int)s.n;
   };
   // the bound that leaves the first r of the kept tokens equal to `cut`
   auto bound_of = [&](u64 r) SM_INLINE {
@@ -454,7 +485,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
     if (n_list < 0) {
       __syncthreads();
       s.count[tid] = s.count[tid + kSmThreads] = 0;
-      if (tid == 0) s.n = 0, s.found_bin = kSmBins;
+      if (tid == 0) s.found_bin = kSmBins;
       __syncthreads();
       each([&](float v, int) {
         const int bin = bin_of(v);
@@ -491,8 +522,6 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
           bound = bound_of(top_k - n);
         }
         if (n_list < 0 && top_k <= kSmList) {
-          __syncthreads();
-          if (tid == 0) s.n = 0;
           __syncthreads();
           n_list = list([&](float v) { return v >= cut; }, [&](float v, int i, int) { return is_kept(v, i); });
         }
@@ -569,7 +598,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
     if (top_p < 1.f) {
       __syncthreads();
       s.mass[tid] = s.mass[tid + kSmThreads] = 0;
-      if (tid == 0) s.n = 0, s.found_bin = kSmBins;
+      if (tid == 0) s.found_bin = kSmBins;
       __syncthreads();
 #pragma unroll 1
       for (int q = 0; q < quads; ++q) {
@@ -593,8 +622,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
                            const float d = distance(v);
                            const bool k = (d < end) & is_kept(v, i), in = k & (d >= from);
                            if (CH > 0) {
-                             above_bits |= (unsigned)(k & !in) << (j & 31);
-                             in_bits |= (unsigned)in << (j & 31);
+                             above_bits |= (unsigned)(k & !in) << j;
+                             in_bits |= (unsigned)in << j;
                            }
                            return in;
                          });
@@ -660,21 +689,14 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
       unsigned short* at_of = reinterpret_cast<unsigned short*>(s.count);  // (places in xs)
       constexpr unsigned kFew = (sizeof(s.count) + sizeof(s.order)) / 2;
       static_assert(offsetof(SmShared, order) == offsetof(SmShared, count) + sizeof(s.count) && CH <= 8, "");
-      u64 n_kept = kFew + 1;
+      unsigned n_kept = kFew + 1;
       if (top_p < 1.f) {
         unsigned kept = above_bits;
         for (unsigned m = in_bits; m; m &= m - 1) {
-          const int j = __ffs(m) - 1, i = index(j >> 2, j & 3);
-          if (is_kept(reinterpret_cast<const float*>(xs)[i + head], i)) kept |= m & -m;
+          const int i = place(__ffs(m) - 1);
+          if (is_kept(reinterpret_cast<const float*>(xs)[i], i - head)) kept |= m & -m;
         }
-        const unsigned n = __popc(kept);
-        unsigned k = (unsigned)sm_scan(n, s, turn, n_kept) - n;
-        if (n_kept <= kFew)
-          for (; kept; kept &= kept - 1) {
-            const int j = __ffs(kept) - 1;
-            at_of[k++] = (unsigned short)(((j >> 2) * kSmThreads + tid) * 4 + (j & 3));
-          }
-        __syncthreads();
+        n_kept = number(kept, kFew, [&](int j, unsigned k) { at_of[k] = (unsigned short)place(j); });
       }
       few = n_kept <= kFew;
       if (few) {
