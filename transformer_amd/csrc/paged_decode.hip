@@ -466,8 +466,8 @@ struct Pd4 {
   static constexpr int HEADS = SHARED ? 16 : std::min(16, (LIMIT - SX - NS * SLOT) / (NS - 1) / 2048 / 2 * 2);
   static constexpr int ROPE = SHARED ? 0 : HEADS * 2048;
   static constexpr int LDS = NS * SLOT + (NS - 1) * ROPE + SX;
-  static constexpr int NR = (16 * RS + 63) / 64, ND = 2 * (NR + 1 + (SHARED ? 0 : 8));  // loads of 16 rows; of a loading wave a tile
-  static constexpr int THREADS = 640;
+  static constexpr int NR = (16 * RS + 63) / 64, ND = NR + 1 + (SHARED ? 0 : 8);  // loads of 16 rows; of a loading wave a tile
+  static constexpr int THREADS = 768;
   static_assert(LDS <= LIMIT && (NS - 2) * ND <= 63 && 2 * NG <= 64 && NS >= 3, "");
 };
 // where 16-token piece t of a slot begins: pieces 1 and 2 lie 128 bytes off the others
@@ -490,11 +490,11 @@ __device__ __forceinline__ u32x4 order8(u32x4 v) {
 __device__ __forceinline__ f32x4 floats4(u32x2 v) { return f32x4{lo_bf16(v[0]), hi_bf16(v[0]), lo_bf16(v[1]), hi_bf16(v[1])}; }
 __device__ __forceinline__ bf16x8 minus24() { return as_bf16x8(u32x4{0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u}); }
 
-// The loading waves, 32 tokens of a tile each: tile i + NS - 2 goes into the slot of tile i - 2 after the barrier before which tile i has
+// The loading waves, 16 tokens of a tile each: tile i + NS - 2 goes into the slot of tile i - 2 after the barrier before which tile i has
 // landed and tile i - 2 was added up.  The first tiles go out two at a time; past the end nothing is loaded, so the counts stay the same.
 template <class C, bool SHARED>
 __device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned char* lds, PdCursor<C> load, int lw, int lane) {
-  PdPieces<C> pieces[2] = {{0, -1, 0, 0, 0, 0, 0}, {0, -1, 0, 0, 0, 0, 0}};
+  PdPieces<C> pieces = {0, -1, 0, 0, 0, 0, 0};
   PdCursor<C> use = load;
   uint32_t off[C::NR];
 #pragma unroll
@@ -513,28 +513,24 @@ __device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned
     int g = lane >> 1;
     if (!SHARED && g >= C::NL) g += 16 * hg;
     const uint32_t sv = g < p.c.groups ? (uint32_t)(g * p.c.size * 2 + 16 * (lane & 1)) : kPdNothing;
+    int at = 0, nv = 0;
+    if (more) {
+      at = pieces.lane_of(p, load, lw, lane);
+      nv = pieces.tokens_of(at);
+    }
+    const buf_rsrc r = pieces.rows_of(at, (uint32_t)(nv * p.c.row_bytes));
+    const uint32_t rows_to = to + piece_at<C::SUB>(lw);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int t = 2 * lw + k;
-      int at = 0, nv = 0;
-      if (more) {
-        at = pieces[k].lane_of(p, load, t, lane);
-        nv = pieces[k].tokens_of(at);
-      }
-      const buf_rsrc r = pieces[k].rows_of(at, (uint32_t)(nv * p.c.row_bytes));
-      const uint32_t rows_to = to + piece_at<C::SUB>(t);
+    for (int i = 0; i < C::NR; ++i)
+      if (64 * i + lane < 16 * C::RS) dma16(r, off[i], rows_to + i * 1024);
+    const buf_rsrc rs = pieces.scales_of(at, nv ? scales_bytes : 0u);
+    if (lane < 2 * C::NG) dma16(rs, sv, to + C::ROWS + lw * C::SC);
+    if constexpr (!SHARED) {
 #pragma unroll
-      for (int i = 0; i < C::NR; ++i)
-        if (64 * i + lane < 16 * C::RS) dma16(r, off[i], rows_to + i * 1024);
-      const buf_rsrc rs = pieces[k].scales_of(at, nv ? scales_bytes : 0u);
-      if (lane < 2 * C::NG) dma16(rs, sv, to + C::ROWS + t * C::SC);
-      if constexpr (!SHARED) {
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {  // two heads; past the slot's heads nothing, into bytes that nobody reads
-          const int h = hg * 16 + j;
-          const uint32_t v = h + (lane >> 5) < p.H ? koff + (uint32_t)h * 32 : kPdNothing;
-          dma16(r, j < C::HEADS ? v : kPdNothing, j < C::HEADS ? keys + kslot * C::ROPE + t * C::HEADS * 512 + j * 512 : dump);
-        }
+      for (int j = 0; j < 16; j += 2) {  // two heads; past the slot's heads nothing, into bytes that nobody reads
+        const int h = hg * 16 + j;
+        const uint32_t v = h + (lane >> 5) < p.H ? koff + (uint32_t)h * 32 : kPdNothing;
+        dma16(r, j < C::HEADS ? v : kPdNothing, j < C::HEADS ? keys + kslot * C::ROPE + lw * C::HEADS * 512 + j * 512 : dump);
       }
     }
     if (more) load.next(p);
@@ -804,7 +800,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
 }
 
 template <int DL, bool SHARED, int SLOTS>
-__global__ __launch_bounds__(640, 1) void paged_decode4_kernel(PagedDecodeParams p) {
+__global__ __launch_bounds__(768, 1) void paged_decode4_kernel(PagedDecodeParams p) {
   using C = Pd4<DL, SHARED, SLOTS>;
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
   unsigned char* at = lds + C::NS * C::SLOT + (C::NS - 1) * C::ROPE;
