@@ -457,7 +457,7 @@ struct Pd4 {
   static constexpr int TT = 64, COST = 1, LEAST = 2;
   static constexpr int NCH = DL / 32 + (SHARED ? 2 : 0), RS = NCH + 1;
   static constexpr int NL = DL / 64, NG = NL + (SHARED ? 1 : 16);  // runs of a row: the latent's; with the keys
-  static constexpr int NB = DL / 64;                               // column blocks of 16 a wave
+  static constexpr int NA = SHARED ? NL : 4, NB = DL / 16 / NA;    // adding waves; column blocks of 16 of one
   static constexpr int SUB = 16 * RS * 16, ROWS = 4 * SUB + 256;
   static constexpr int SC = NG * 32;  // bytes of 16 tokens' scales
   static constexpr int SLOT = ROWS + 4 * SC, SX = 2 * 4096 + 2 * 256 + 2 * 256 + (SHARED ? 0 : 1024), LIMIT = 160 * 1024;
@@ -467,28 +467,31 @@ struct Pd4 {
   static constexpr int ROPE = SHARED ? 0 : HEADS * 2048;
   static constexpr int LDS = NS * SLOT + (NS - 1) * ROPE + SX;
   static constexpr int NR = (16 * RS + 63) / 64, ND = NR + 1 + (SHARED ? 0 : 8);  // loads of 16 rows; of a loading wave a tile
-  static constexpr int THREADS = 768;
+  static constexpr int THREADS = 64 * (8 + NA);
   static_assert(LDS <= LIMIT && (NS - 2) * ND <= 63 && 2 * NG <= 64 && NS >= 3, "");
 };
 // where 16-token piece t of a slot begins: pieces 1 and 2 lie 128 bytes off the others
 template <int SUB>
 __device__ __forceinline__ int piece_at(int t) { return t * SUB + (((t + 1) >> 1) << 7); }
 
-// (w & 0x00780078) | 0x41804180 in one instruction: of two literals the compiler makes two
+// (w & MASK) | BASE in one instruction: of two literals the compiler makes two
+template <uint32_t MASK, uint32_t BASE>
 __device__ __forceinline__ uint32_t two_codes(uint32_t w) {
   uint32_t r;
-  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(0x00780078u), "v"(0x41804180u));
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(MASK), "v"(BASE));
   return r;
 }
 __device__ __forceinline__ bf16x8 codes8(uint32_t w) {
-  return as_bf16x8(u32x4{two_codes(w << 3), two_codes(w >> 1), two_codes(w >> 5), two_codes(w >> 9)});
+  constexpr uint32_t M = 0x00780078, B = 0x41804180;
+  return as_bf16x8(u32x4{two_codes<0x000f000f, 0x43004300>(w), two_codes<M, B>(w >> 1), two_codes<M, B>(w >> 5), two_codes<M, B>(w >> 9)});
 }
 // 8 values in the order in which codes8 leaves the codes: 0 4 1 5 2 6 3 7
 __device__ __forceinline__ u32x4 order8(u32x4 v) {
   return u32x4{pack_lo16(v[0], v[2]), pack_hi16(v[0], v[2]), pack_lo16(v[1], v[3]), pack_hi16(v[1], v[3])};
 }
 __device__ __forceinline__ f32x4 floats4(u32x2 v) { return f32x4{lo_bf16(v[0]), hi_bf16(v[0]), lo_bf16(v[1]), hi_bf16(v[1])}; }
-__device__ __forceinline__ bf16x8 minus24() { return as_bf16x8(u32x4{0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u}); }
+// what takes 128 + code and 16 + code back to code - 8
+__device__ __forceinline__ bf16x8 offsets8() { return as_bf16x8(u32x4{0xc308c308u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u}); }
 
 // The loading waves, 16 tokens of a tile each: tile i + NS - 2 goes into the slot of tile i - 2 after the barrier before which tile i has
 // landed and tile i - 2 was added up.  The first tiles go out two at a time; past the end nothing is loaded, so the counts stay the same.
@@ -601,8 +604,8 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int g = 0; g < NQ; ++g) {
-        f32x4 d = mfma16(minus24(), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
-        d = mfma16(minus24(), as_bf16x8(q[2 * g + 1]), d);
+        f32x4 d = mfma16(offsets8(), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
+        d = mfma16(offsets8(), as_bf16x8(q[2 * g + 1]), d);
         if (g < C::NL)
           z[g] = d[0];
         else
@@ -765,11 +768,11 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
           pb[t] = as_bf16x8(u32x4{pack_bf16x2(e[2 * t][0], e[2 * t + 1][0]), pack_bf16x2(e[2 * t][1], e[2 * t + 1][1]),
                                   pack_bf16x2(e[2 * t][2], e[2 * t + 1][2]), pack_bf16x2(e[2 * t][3], e[2 * t + 1][3])});
         if (g == g0) {
-          os[0] = mfma16(minus24(), pb[0], os[0]);
-          os[0] = mfma16(minus24(), pb[1], os[0]);
+          os[0] = mfma16(offsets8(), pb[0], os[0]);
+          os[0] = mfma16(offsets8(), pb[1], os[0]);
         } else {
-          os[1] = mfma16(minus24(), pb[0], os[1]);
-          os[1] = mfma16(minus24(), pb[1], os[1]);
+          os[1] = mfma16(offsets8(), pb[0], os[1]);
+          os[1] = mfma16(offsets8(), pb[1], os[1]);
         }
       }
       const i32x2 c = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(buf + offT + 8 * i));
@@ -800,7 +803,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
 }
 
 template <int DL, bool SHARED, int SLOTS>
-__global__ __launch_bounds__(768, 1) void paged_decode4_kernel(PagedDecodeParams p) {
+__global__ __launch_bounds__((Pd4<DL, SHARED, SLOTS>::THREADS), 1) void paged_decode4_kernel(PagedDecodeParams p) {
   using C = Pd4<DL, SHARED, SLOTS>;
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
   unsigned char* at = lds + C::NS * C::SLOT + (C::NS - 1) * C::ROPE;
@@ -810,10 +813,10 @@ __global__ __launch_bounds__(768, 1) void paged_decode4_kernel(PagedDecodeParams
   if (!use.more()) return;
   if (w < 4)
     paged_score4<C, DL, SHARED>(p, lds, x, use, w, lane);
-  else if (w < 8)
+  else if (w < 4 + C::NA)
     paged_add4<C, DL>(p, lds, x, use, w - 4, lane);
   else
-    paged_load4<C, SHARED>(p, lds, use, w - 8, lane);
+    paged_load4<C, SHARED>(p, lds, use, w - 4 - C::NA, lane);
 }
 
 // ------------------------------------------------------------------------------------------------ parts
