@@ -474,18 +474,20 @@ struct Pd4 {
 template <int SUB>
 __device__ __forceinline__ int piece_at(int t) { return t * SUB + (((t + 1) >> 1) << 7); }
 
-// (w & MASK) | BASE in one instruction: of two literals the compiler makes two
-template <uint32_t MASK, uint32_t BASE>
-__device__ __forceinline__ uint32_t two_codes(uint32_t w) {
-  uint32_t r;
-  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(MASK), "v"(BASE));
-  return r;
-}
-__device__ __forceinline__ bf16x8 codes8(uint32_t w) {
-  constexpr uint32_t M = 0x00780078, B = 0x41804180;
-  return as_bf16x8(u32x4{two_codes<0x000f000f, 0x43004300>(w), two_codes<M, B>(w >> 1), two_codes<M, B>(w >> 5), two_codes<M, B>(w >> 9)});
-}
-// 8 values in the order in which codes8 leaves the codes: 0 4 1 5 2 6 3 7
+// The masks and bases, as numbers that the compiler does not know: (w & mask) | base is then one instruction, of two literals it makes two.
+// (Not the instruction itself in assembly: what it writes may be a matrix instruction's accumulator until just before, and the compiler
+// waits for that only before instructions of its own.)
+struct Pd4Codes {
+  uint32_t mask0 = 0x000f000fu, mask1 = 0x00780078u, base0 = 0x43004300u, base1 = 0x41804180u;
+  __device__ __forceinline__ Pd4Codes() {
+    asm("" : "+s"(mask0), "+s"(mask1));
+    asm("" : "+v"(base0), "+v"(base1));
+  }
+  __device__ __forceinline__ bf16x8 of(uint32_t w) const {
+    return as_bf16x8(u32x4{(w & mask0) | base0, ((w >> 1) & mask1) | base1, ((w >> 5) & mask1) | base1, ((w >> 9) & mask1) | base1});
+  }
+};
+// 8 values in the order in which Pd4Codes leaves the codes: 0 4 1 5 2 6 3 7
 __device__ __forceinline__ u32x4 order8(u32x4 v) {
   return u32x4{pack_lo16(v[0], v[2]), pack_hi16(v[0], v[2]), pack_lo16(v[1], v[3]), pack_hi16(v[1], v[3])};
 }
@@ -587,6 +589,7 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
   f32x4 key_start;  // keys of their own: of this lane's head's, the start of its sums
   float m_run = 0.f, l_part = 0.f;
   const int offS = ((l16 >> 2) & 3) * 32 + (l16 & 3) * 8;  // transpose read: row (run) i / 4, tokens 4 (i % 4) ..
+  const Pd4Codes codes;
   int slot = 0, kslot = 0, par = 0;
   bool first = true;
 #pragma unroll 1
@@ -653,8 +656,8 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
 #pragma unroll
     for (int g = 0; g < C::NL + (SHARED ? 1 : 0); ++g) {
       const u32x2 c = lds8(buf + offA + 32 * g);
-      f32x4 d = mfma16(codes8(c[0]), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
-      d = mfma16(codes8(c[1]), as_bf16x8(q[2 * g + 1]), d);
+      f32x4 d = mfma16(codes.of(c[0]), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
+      d = mfma16(codes.of(c[1]), as_bf16x8(q[2 * g + 1]), d);
       const f32x4 k = floats4(lds8(sc + 32 * g + 8 * G));
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(k[r], d[r], s[r]);
@@ -666,8 +669,8 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
 #pragma unroll
       for (int j = 0; j < C::HEADS; ++j) {
         const u32x2 c = lds8(kb + j * 512);
-        f32x4 d = mfma16(codes8(c[0]), as_bf16x8(q[2 * C::NL]), key_start);
-        d = mfma16(codes8(c[1]), as_bf16x8(q[2 * C::NL + 1]), d);
+        f32x4 d = mfma16(codes.of(c[0]), as_bf16x8(q[2 * C::NL]), key_start);
+        d = mfma16(codes.of(c[1]), as_bf16x8(q[2 * C::NL + 1]), d);
 #pragma unroll
         for (int r = 0; r < 4; ++r) e[r] = l16 == j ? d[r] : e[r];
       }
@@ -718,6 +721,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
   const int offT = piece_at<C::SUB>(l16 >> 2) + (4 * G + (l16 & 3)) * C::RS * 16 + 8 * w * C::NB;
   const int g0 = w * C::NB / 4;  // the run of the wave's first column block
   f32x4 o[C::NB], os[2];
+  const Pd4Codes codes;
   float M = 0.f;
   int slot = 0, par = 0, from = 0;
   bool first = true;
@@ -731,15 +735,24 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
       M = -INFINITY;
       from = use.tile;
     }
-    pd_barrier();  // the tile is scored
     const unsigned char* buf = lds + slot * C::SLOT;
     const unsigned char* sc = buf + C::ROWS;
+    i32x2 c[C::NB];  // (the tile landed a barrier ago)
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i) c[i] = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(buf + offT + 8 * i));
+    pd_barrier();  // the tile is scored
     float m[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) m[t] = x.m[(par * 4 + t) * 16 + l16];
     f32x4 pv[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) pv[t] = x.p[(par * 4 + t) * 64 + lane];
+    constexpr int NG = C::NB > 4 ? 2 : 1;  // runs that the wave's columns can touch
+    u32x2 k[NG][4];
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) k[g][t] = lds8(sc + t * C::SC + 32 * min(g0 + g, C::NL - 1) + 8 * G);
     const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     if (__any(top > M + kPdRescale)) {
       const float m_new = fmaxf(M, top), alpha = m_new == -INFINITY ? 1.f : fast_exp2(M - m_new);
@@ -762,7 +775,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
       if (i == 0 || (nb & 3) == 0) {  // the run's scales into p
         f32x4 e[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) e[t] = pv[t] * floats4(lds8(sc + t * C::SC + 32 * g + 8 * G));
+        for (int t = 0; t < 4; ++t) e[t] = pv[t] * floats4(k[g == g0 ? 0 : 1][t]);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           pb[t] = as_bf16x8(u32x4{pack_bf16x2(e[2 * t][0], e[2 * t + 1][0]), pack_bf16x2(e[2 * t][1], e[2 * t + 1][1]),
@@ -775,9 +788,8 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
           os[1] = mfma16(offsets8(), pb[1], os[1]);
         }
       }
-      const i32x2 c = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(buf + offT + 8 * i));
-      o[i] = mfma16(codes8((uint32_t)c[0]), pb[0], o[i]);
-      o[i] = mfma16(codes8((uint32_t)c[1]), pb[1], o[i]);
+      o[i] = mfma16(codes.of((uint32_t)c[i][0]), pb[0], o[i]);
+      o[i] = mfma16(codes.of((uint32_t)c[i][1]), pb[1], o[i]);
     }
     slot = slot + 1 == C::NS ? 0 : slot + 1;
     const int b = use.b, hg = use.hg, n = use.n, tile = use.tile;
