@@ -935,9 +935,11 @@ auto by_kernel(const mla_paged_cache& c, int64_t H, F&& f) {
     constexpr int S = slots4<DL>();
     return f.template take<DL, SHARED, Pd4<DL, true, S>>(paged_decode4_kernel<DL, true, S>);
   } else {
-    if (std::min<int64_t>(H, 16) <= Pd4<DL, false, 4>::HEADS)
-      return f.template take<DL, SHARED, Pd4<DL, false, 4>>(paged_decode4_kernel<DL, false, 4>);
-    return f.template take<DL, SHARED, Pd4<DL, false, 3>>(paged_decode4_kernel<DL, false, 3>);
+    if constexpr (Pd4<DL, false, 4>::HEADS < 16) {
+      if (std::min<int64_t>(H, 16) > Pd4<DL, false, 4>::HEADS)
+        return f.template take<DL, SHARED, Pd4<DL, false, 3>>(paged_decode4_kernel<DL, false, 3>);
+    }
+    return f.template take<DL, SHARED, Pd4<DL, false, 4>>(paged_decode4_kernel<DL, false, 4>);
   }
 }
 
