@@ -649,7 +649,8 @@ typedef struct {
  *   c_new[b][t]               -> the row of p
  * A token with p < 0, p >= table_rows or p >= table_pages * page_size is skipped, its q_out zero.  qk bf16 [B, T, H + Hr, 64]
  * (qk_stride), c_new bf16 [B, T, d_latent] (c_new_sb, c_new_st), q_out bf16 [B, T, H, 64] contiguous; cos, sin bf16
- * [table_rows, 32]; pointers 16-byte aligned, strides multiples of 8.
+ * [table_rows, 32]; pointers 16-byte aligned, strides multiples of 8.  H and Hr up to 1024; B T (H + Hr) and B T d_latent / 32 below
+ * 2^29.
  */
 typedef struct {
   mla_paged_cache cache;
@@ -668,7 +669,7 @@ int mla_paged_append(const mla_paged_append_args* a, void* stream);
 
 /* The rows of positions starts[b] + t, t < counts[b] (starts NULL: 0; counts NULL: T), out of their pages:
  *   latent bf16 [B, T, d_latent], k_rope bf16 [B, Hr, T, 64], contiguous, 16-byte aligned; zeros for the other t, for positions
- *   that do not exist and where there is no page.  4-bit values are rounded to bf16 once.
+ *   that do not exist and where there is no page.  4-bit values are rounded to bf16 once.  B T W below 2^34.
  */
 typedef struct {
   mla_paged_cache cache;
@@ -684,6 +685,7 @@ int mla_paged_read(const mla_paged_read_args* a, void* stream);
  * recorded call follows the lengths).  A sequence with none gets ctx = 0, lse = -inf.
  *   q_lat bf16 [B, H, d_latent] (q_lat_sb, q_lat_sh), q_rope bf16 [B, H, 64] (q_rope_sb, q_rope_sh), n_k_rope_heads 1 or H
  *   ctx bf16 [B, H, d_latent] contiguous, lse fp32 [B, H] contiguous, natural log
+ * B below 2^20, H up to 1024, C = table_pages * page_size below 2^28, B ceil(H / 16) (C / 16 + 4) below 2^30.
  * The sequences' tiles are divided evenly over the workgroups whatever their lengths; a sequence that spans several leaves fp32
  * partials in the workspace, which a second kernel on the same stream adds in order: results repeat bit for bit.  Needs
  * mla_paged_decode_workspace_bytes() bytes of 256-byte aligned device memory of this call's own; what they hold does not matter.

@@ -177,6 +177,14 @@ def test_inputs_that_ask_for_gradients():
             ctx.float().sum().backward()
     assert q.grad is None
     check_cache(m.dev, before)
+    # what was saved for a backward pass and is appended to since is noticed there
+    pages = m.dev[0]
+    x = torch.ones_like(pages, requires_grad=True)
+    y = (x * pages).float().sum()
+    with torch.no_grad():
+        T.paged_append(m.qk_d[:2][:, None], m.c_d[:2][:, None], *m.dev, m.cos_d, m.sin_d, m.table, i32([20, 3]))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
 
 
 @pytest.mark.parametrize("bits", [16, 4])

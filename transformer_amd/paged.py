@@ -220,7 +220,9 @@ def _paged_decode(q_lat: Tensor, q_rope: Tensor, pages: Tensor, scales: Optional
         if nbytes is None:
             if len(_workspaces) > 4096:
                 _workspaces.clear()
-            nbytes = _workspaces[key] = _decode_bytes(op, dev, *cache, 0, 0, 0, 0, 0, 0, 0, B, H, 0, 0, 0, 0, 0.0)
+            nbytes = _decode_bytes(op, dev, *cache, 0, 0, 0, 0, 0, 0, 0, B, H, 0, 0, 0, 0, 0.0)
+            if nbytes:  # (0: arguments that the call will refuse)
+                _workspaces[key] = nbytes
         ws = q_lat.new_empty(nbytes, dtype=_U8)
         _decode_entry(op, dev, *cache, q_lat.data_ptr(), q_rope.data_ptr(), seq_lens.data_ptr(), ctx.data_ptr(), lse.data_ptr(),
                       ws.data_ptr(), nbytes, B, H, l0, l1, r0, r1, scale)
@@ -233,6 +235,7 @@ def _(q_lat, q_rope, pages, scales, block_table, seq_lens, scale):
 
 
 _ops = torch.ops.mla_mi355x
+_increment_version = torch._C._increment_version
 _append, _read, _decode = (kernels._BODIES[n] for n in ("paged_append", "paged_read", "paged_decode"))
 
 
@@ -245,8 +248,11 @@ def paged_append(qk: Tensor, c_new: Tensor, pages: Tensor, scales: Optional[Tens
     d_latent]`` written to their rows in ``pages`` (and ``scales``).  Returns the rotated q heads ``[B, T, H, 64]``, zeros for the
     other t.  A position without a page is not written; one outside the tables is skipped, its q heads zero.  Two tokens of a call
     must not go to the same place."""
-    run = _append if plain(qk, c_new, pages, scales, cos, sin, block_table, starts, counts) else _ops.paged_append
-    return run(qk, c_new, pages, scales, cos, sin, block_table, starts, counts)
+    if not plain(qk, c_new, pages, scales, cos, sin, block_table, starts, counts):
+        return _ops.paged_append(qk, c_new, pages, scales, cos, sin, block_table, starts, counts)
+    q_rope = _append(qk, c_new, pages, scales, cos, sin, block_table, starts, counts)
+    _increment_version([pages] if scales is None else [pages, scales])  # as the dispatcher does for what an operator writes
+    return q_rope
 
 
 def paged_read(pages: Tensor, scales: Optional[Tensor], block_table: Tensor, d_latent: int, T: int, starts: Optional[Tensor] = None,
