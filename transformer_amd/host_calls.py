@@ -18,21 +18,17 @@ _Parameter = torch.nn.Parameter
 
 
 def plain(first: Tensor, *others) -> bool:
-    """Whether a call with these tensors (or Nones) needs nothing of the dispatcher, as ``kernels.dispatcher_needed`` asks; of the
-    devices only the first's is looked at, since the operators compare all of them."""
+    """Whether a call with these tensors (or Nones) needs nothing of the dispatcher, as ``kernels.dispatcher_needed`` asks, and all are
+    on one GPU: the operator's body then need not look at that again."""
     if _compiling() or _dispatch_modes() > 0 or _tracing() is not None or _transform() is not None:
         return False
     if type(first) is not Tensor or not first.is_cuda:
         return False
-    if _grad_mode():
-        if first.requires_grad:
-            return False
-        for t in others:
-            if t is not None and (t.requires_grad or (type(t) is not Tensor and type(t) is not _Parameter)):
-                return False
-        return True
+    dev, grad = first.get_device(), _grad_mode()
+    if grad and first.requires_grad:
+        return False
     for t in others:
-        if t is not None and type(t) is not Tensor and type(t) is not _Parameter:
+        if t is not None and (t.get_device() != dev or (type(t) is not Tensor and type(t) is not _Parameter) or (grad and t.requires_grad)):
             return False
     return True
 

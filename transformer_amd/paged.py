@@ -74,8 +74,9 @@ def _refuse_cache(op, pages, scales, table, B, d_latent) -> None:
 
 def _cache(op: str, pages: Tensor, scales: Optional[Tensor], table: Tensor, B: int, d_latent: int):
     """(the fields of mla_paged_cache, Hr, what they point to) of a cache and a block table for B sequences."""
-    if pages.dim() != 3:
+    if pages.dim() != 3 or table.dim() != 2:
         _refuse_cache(op, pages, scales, table, B, d_latent)
+    rows, P = table.shape
     (n, size, cols), (p0, p1, p2), at = pages.shape, pages.stride(), pages.data_ptr()
     if scales is None:
         W, p0, s0, sat = cols, 2 * p0, 0, 0
@@ -88,11 +89,10 @@ def _cache(op: str, pages: Tensor, scales: Optional[Tensor], table: Tensor, B: i
             ok = s2 == 1 and s1 == size and not sat & 15 and (n == 1 or not s0 & 7)
     Hr, rest = divmod(W - d_latent, ROPE_DIM)
     ok = ok and d_latent in SUPPORTED_LATENT and Hr > 0 and not rest and not size & 15 and 16 <= size <= 4096 \
-        and table.dtype is _I32 and table.dim() == 2 and table.size(0) == B \
+        and table.dtype is _I32 and rows == B \
         and (n == 0 or (p2 == 1 and p1 == cols and not at & 15 and (n == 1 or not p0 & 15)))
     if not ok:
         _refuse_cache(op, pages, scales, table, B, d_latent)
-    P = table.size(1)
     t0, t1 = table.stride()
     if P > 1 and (t1 != 1 or t0 < 0):
         table = table.contiguous()
@@ -100,7 +100,8 @@ def _cache(op: str, pages: Tensor, scales: Optional[Tensor], table: Tensor, B: i
     return (at, sat, table.data_ptr(), n, size, p0, s0, P, t0, d_latent, Hr), Hr, table
 
 
-def _on_device(op: str, dev: int, like: Tensor, *tensors: Optional[Tensor]) -> None:
+def _on_device(op: str, like: Tensor, *tensors: Optional[Tensor]) -> None:
+    dev = like.get_device()
     if dev < 0:
         kernels._require_gpu(op, like)
     for t in tensors:
@@ -110,7 +111,7 @@ def _on_device(op: str, dev: int, like: Tensor, *tensors: Optional[Tensor]) -> N
 
 
 def _ints(op: str, name: str, t: Tensor, B: int) -> Tensor:
-    if t.dtype is not _I32 or t.dim() != 1 or t.size(0) != B:
+    if t.dtype is not _I32 or t.shape != (B,):
         raise ValueError(f"{op}: {name} must be int32 [{B}], got {t.dtype} {tuple(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -137,9 +138,12 @@ def _rope_table(t: Tensor) -> Tensor:
 @_op("paged_append", mutates_args=("pages", "scales"))
 def _paged_append(qk: Tensor, c_new: Tensor, pages: Tensor, scales: Optional[Tensor], cos: Tensor, sin: Tensor,
                   block_table: Tensor, starts: Tensor, counts: Optional[Tensor]) -> Tensor:
+    _on_device("mla_mi355x::paged_append", qk, c_new, pages, scales, cos, sin, block_table, starts, counts)
+    return _append(qk, c_new, pages, scales, cos, sin, block_table, starts, counts)
+
+
+def _append(qk, c_new, pages, scales, cos, sin, block_table, starts, counts):
     op = "mla_mi355x::paged_append"
-    dev = qk.get_device()
-    _on_device(op, dev, qk, c_new, pages, scales, cos, sin, block_table, starts, counts)
     if not qk.dtype is c_new.dtype is cos.dtype is sin.dtype is _BF16:
         kernels._bf16(op, qk=qk, c_new=c_new, cos=cos, sin=sin)
     if qk.dim() != 4 or c_new.dim() != 3 or qk.size(3) != ROPE_DIM or c_new.shape[:2] != qk.shape[:2]:
@@ -157,7 +161,7 @@ def _paged_append(qk: Tensor, c_new: Tensor, pages: Tensor, scales: Optional[Ten
     cos, sin = _rope_table(cos), _rope_table(sin)
     q_out = qk.new_empty((B, T, heads - Hr, ROPE_DIM))
     if B and T:
-        _append_entry(op, dev, *cache, qk.data_ptr(), c_new.data_ptr(), q_out.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        _append_entry(op, qk.get_device(), *cache, qk.data_ptr(), c_new.data_ptr(), q_out.data_ptr(), cos.data_ptr(), sin.data_ptr(),
                       starts.data_ptr(), 0 if counts is None else counts.data_ptr(), B, T, heads - Hr, cos.size(0), q0, q1, q2, c0, c1)
     return q_out
 
@@ -171,9 +175,12 @@ def _(qk, c_new, pages, scales, cos, sin, block_table, starts, counts):
 @_op("paged_read", mutates_args=())
 def _paged_read(pages: Tensor, scales: Optional[Tensor], block_table: Tensor, d_latent: int, T: int, starts: Optional[Tensor],
                 counts: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    _on_device("mla_mi355x::paged_read", pages, scales, block_table, starts, counts)
+    return _read(pages, scales, block_table, d_latent, T, starts, counts)
+
+
+def _read(pages, scales, block_table, d_latent, T, starts, counts):
     op = "mla_mi355x::paged_read"
-    dev = pages.get_device()
-    _on_device(op, dev, pages, scales, block_table, starts, counts)
     B = block_table.size(0) if block_table.dim() else 0
     if T < 0:
         raise ValueError(f"{op}: T must not be negative, got {T}")
@@ -183,7 +190,7 @@ def _paged_read(pages: Tensor, scales: Optional[Tensor], block_table: Tensor, d_
     latent = pages.new_empty((B, T, d_latent), dtype=_BF16)
     k_rope = pages.new_empty((B, Hr, T, ROPE_DIM), dtype=_BF16)
     if B and T:
-        _read_entry(op, dev, *cache, latent.data_ptr(), k_rope.data_ptr(), 0 if starts is None else starts.data_ptr(),
+        _read_entry(op, pages.get_device(), *cache, latent.data_ptr(), k_rope.data_ptr(), 0 if starts is None else starts.data_ptr(),
                     0 if counts is None else counts.data_ptr(), B, T)
     return latent, k_rope
 
@@ -198,9 +205,13 @@ def _(pages, scales, block_table, d_latent, T, starts, counts):
 @_op("paged_decode", mutates_args=())
 def _paged_decode(q_lat: Tensor, q_rope: Tensor, pages: Tensor, scales: Optional[Tensor], block_table: Tensor, seq_lens: Tensor,
                   scale: float) -> Tuple[Tensor, Tensor]:
+    _on_device("mla_mi355x::paged_decode", q_lat, q_rope, pages, scales, block_table, seq_lens)
+    return _decode(q_lat, q_rope, pages, scales, block_table, seq_lens, scale)
+
+
+def _decode(q_lat, q_rope, pages, scales, block_table, seq_lens, scale):
     op = "mla_mi355x::paged_decode"
     dev = q_lat.get_device()
-    _on_device(op, dev, q_lat, q_rope, pages, scales, block_table, seq_lens)
     if not q_lat.dtype is q_rope.dtype is _BF16:
         kernels._bf16(op, q_lat=q_lat, q_rope=q_rope)
     if q_lat.dim() != 3 or q_rope.shape != (*q_lat.shape[:2], ROPE_DIM):
@@ -236,7 +247,6 @@ def _(q_lat, q_rope, pages, scales, block_table, seq_lens, scale):
 
 _ops = torch.ops.mla_mi355x
 _increment_version = torch._C._increment_version
-_append, _read, _decode = (kernels._BODIES[n] for n in ("paged_append", "paged_read", "paged_decode"))
 
 
 # ----------------------------------------------------------------- public functions

@@ -25,6 +25,15 @@ def _sample(logits: Tensor, u: Tensor, temperature: float, top_k: int, top_p: fl
             temperature_rows: Optional[Tensor], top_k_rows: Optional[Tensor], top_p_rows: Optional[Tensor],
             min_p_rows: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
     op = "mla_mi355x::sample_tokens"
+    for t in (logits, u, temperature_rows, top_k_rows, top_p_rows, min_p_rows):
+        if t is not None and (logits.get_device() < 0 or t.get_device() != logits.get_device()):
+            kernels._require_gpu(op, t)
+            raise ValueError(f"{op}: all tensors must be on one device, got {t.device} and {logits.device}")
+    return _draw(logits, u, temperature, top_k, top_p, min_p, temperature_rows, top_k_rows, top_p_rows, min_p_rows)
+
+
+def _draw(logits, u, temperature, top_k, top_p, min_p, temperature_rows, top_k_rows, top_p_rows, min_p_rows):
+    op = "mla_mi355x::sample_tokens"
     if logits.dim() != 2 or u.dim() != 1 or not 1 <= logits.size(1) <= MAX_VOCAB or u.size(0) != logits.size(0):
         raise ValueError(f"{op}: expected logits [B, V], V up to {MAX_VOCAB}, and u [B]; got {tuple(logits.shape)}, {tuple(u.shape)}")
     bf16 = logits.dtype is torch.bfloat16
@@ -40,10 +49,6 @@ def _sample(logits: Tensor, u: Tensor, temperature: float, top_k: int, top_p: fl
         if not t.is_contiguous():
             rows[k] = t = t.contiguous()
         at[k] = t.data_ptr()
-    for t in (logits, u, *rows):
-        if t is not None and (dev < 0 or t.get_device() != dev):
-            kernels._require_gpu(op, t)
-            raise ValueError(f"{op}: all tensors must be on one device, got {t.device} and {logits.device}")
     stride, inner = logits.stride()
     if (inner != 1 and V > 1) or stride < 0:
         logits = logits.contiguous()
@@ -63,7 +68,7 @@ def _(logits, u, temperature, top_k, top_p, min_p, temperature_rows, top_k_rows,
     return logits.new_empty(B, dtype=torch.int64), logits.new_empty(B, dtype=torch.float32)
 
 
-_ops, _run = torch.ops.mla_mi355x, kernels._BODIES["sample_tokens"]
+_ops = torch.ops.mla_mi355x
 
 
 def sample_tokens(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, top_k: Union[int, Tensor] = 0,
@@ -90,5 +95,5 @@ def sample_tokens(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] =
     for name, v in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
         if type(v) is bool or v != v:
             raise ValueError(f"sample_tokens: {name} must be a number, got {v!r}")
-    run = _run if plain(logits, u, *rows) else _ops.sample_tokens
+    run = _draw if plain(logits, u, *rows) else _ops.sample_tokens
     return run(logits, u, float(temperature), top_k, float(top_p), float(min_p), *rows)
