@@ -1,4 +1,9 @@
 // Appending to a paged latent cache with the rotation on the way, and reading rows back out of pages (gfx950).
+//
+// Both move each value once, 16 bytes a thread and access.  Measured (kernel trace; a copy in HBM reaches 4.7 TB/s): 8 prompts' chunks of up
+// to 2048 tokens, 8450 in all, into 4-bit pages 16.6 us (63 MB, 3.8 TB/s; VALU busy 84 % of the time, most of it the quotients); 32000
+// rows of 1280 values out of 16-bit pages, 20300 of them tokens, 20.5 (134 MB; 28 where all of it comes from and goes to HBM: a copy's
+// rate).  Few rows are bound by the launch: one token 2.1, 64 tokens into 4 bits 6.1 (start, page and store one after the other).
 #include "paged.h"
 #include "rope_append.h"
 
@@ -23,8 +28,11 @@ __device__ __forceinline__ int append_position(const PagedAppendParams& a, uint3
   return (int)t < count && p >= 0 && p < a.limit ? (int)p : -1;
 }
 
+// y1 = x1 c - x2 s, y2 = x1 s + x2 c, each rounded to bf16 once, and to 4 bits from that, so that both caches hold what the rotation gave.
+//
 // Blocks [0, ceil(vectors / 256)): 4 threads a head vector, each 8 + 8 of its values (x[i] with x[i + 32]).  The others: a thread
-// for 8 values of a latent row, so 8 neighbouring threads hold a run.
+// for 8 values of a latent row, so 8 neighbouring threads hold a run and its largest magnitude takes three exchanges.  One launch for
+// both: a token's latency is the launch.
 template <bool FOUR>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams a) {
   const uint32_t rope_blocks = (a.vectors + 255) / 256;

@@ -2,8 +2,17 @@
 //
 //   s_j = (q_lat . c_j + q_rope . k_j) scale,   ctx = softmax(s) c,   lse = logsumexp(s)
 //
-// over the rows [c | k] of a sequence's pages, each read once for the 16 heads of a head group.  HBM bound: 1152 bytes a token in 16
-// bits (d_latent 512, one rotated key), 306 in 4.
+// over the rows [c | k] of a sequence's pages, each read once for the 16 heads of a head group: 1152 bytes a token in 16 bits
+// (d_latent 512, one rotated key), 306 in 4, for 35 KFLOP.  16 bits are bound by memory and by what a workgroup takes to begin and end,
+// 4 bits by the instructions that unpack.
+//
+// Measured (kernel trace; a stream that only reads reaches 6.0 TB/s), this kernel and the merge of the parts:
+//   16 bits, 32 sequences up to 4096, 85 MB        21.8 + 4.4 us  (3.9 TB/s, 3.2 with the merge)
+//   16 bits, one of 701 tokens, 14 keys            8.7 + 3.9
+//   4 bits, 64 up to 16384, 179 MB                 67.7 + 6.2  (2.6 TB/s; VALU busy 64 % of the time)
+//   4 bits, 64 up to 4000 with 14 keys, 87 MB      30.4 + 6.1  (2.9 TB/s)
+//   4 bits, one of 3001                            10.6 + 4.0
+// About 6 us of each are the launch, the lengths, the page look-ups and the first tile's way from memory.
 //
 // Work.  A unit is a sequence and head group, a tile 16 tokens of it (16 bits) or 64 (4 bits).  The tiles of all units in a row are
 // cut into equal runs, one a workgroup, whatever the sequences' lengths: every workgroup adds the lengths up and finds its place
@@ -13,8 +22,8 @@
 //
 // A workgroup's tiles come through a ring of LDS slots by direct-to-LDS loads, which run on across its units.  16 tokens never
 // straddle a page, so a buffer descriptor of the tokens that exist (none, where the entry is no page) bounds each load: what lies
-// behind a sequence's end reads as zero and never reaches a product.  The four waves share the scores through LDS and then own a
-// quarter of the latent's columns each, so no wave's O has to be merged with another's.  One barrier a tile.
+// behind a sequence's end reads as zero and never reaches a product.  Waves share the scores through LDS and each then owns some of
+// the latent's columns, so no wave's O has to be merged with another's.  One barrier a tile.
 #include <algorithm>
 #include <type_traits>
 
@@ -67,7 +76,8 @@ __device__ __forceinline__ int pd_page(const PagedDecodeParams& p, int piece) {
 // A place in the units' tiles: tile `tile` of the `n` of (b, hg), the workgroup's tiles going to `end` in the line of all.
 //
 // On that line a unit takes COST places before its tiles: what its beginning and end cost in tiles (queries, stores), so that a
-// workgroup whose run holds the ends of several gets fewer tiles.  All numbers stay below 2^31.
+// workgroup whose run holds the ends of several gets fewer tiles.  A run has LEAST places at least: one sequence is not cut so finely
+// that the parts take longer than the tiles.  All numbers stay below 2^31.
 template <class C>
 struct PdCursor {
   int b, hg, tile, n, len, left;  // left: of the run's line, from this tile on
@@ -213,7 +223,8 @@ struct PdOut {
 //
 // Four waves compute and two load.  A load into LDS holds its wave up (about 90 cycles while all waves of the workgroup issue some),
 // which the computing waves do not have between two barriers; and theirs are the only vector loads that the compiler does not see, so it
-// may wait for the others (queries) as it likes.
+// may wait for the others (queries) as it likes.  (All four waves loading and computing: 32.4 us for the 85 MB, with these 23.6.)
+// Keys of heads' own take 3 or 4 slots, whatever fits.
 template <int DL, bool SHARED>
 struct Pd16 {
   static constexpr int TT = 16, COST = 3, LEAST = 5;
@@ -439,15 +450,19 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
 // ------------------------------------------------------------------------------------------------ 4 bits
 
 // Codes are never turned into their values: (w >> s) & 0x00780078 | 0x41804180 makes two of a word's eight codes the bf16 numbers 16 +
-// code, which the matrix instructions take as they are.  With u = 16 + code a run of 64 adds scale (sum u q - 24 sum q) to a score:
-// -24 sum q is the accumulator's start, the scale a factor on the result, one a run and token.  For O the scale goes into p
-// before it is rounded to bf16, and -24 sum p' is an accumulator of its own, added at the end.  A code costs one VALU operation each
-// time, twice a token (scores, O): with 530 a wave and tile of 64 tokens these bound the kernel nearly as much as the memory does.
+// code, which the matrix instructions take as they are; w & 0x000f000f | 0x43004300 makes the first two 128 + code without a shift.  With
+// u = 16 + code a run of 64 adds scale (sum u q - 24 sum q) to a score (136 for the first two of eight): the second sum is the
+// accumulator's start, the scale a factor on the result, one a run and token.  For O the scale goes into p before p is rounded to bf16
+// (one rounding, as in 16 bits), and -24 sum p' is an accumulator of its own, added at the end; these sums are in fp32 and so large that
+// 2^-24 of them is 2^-17 of a code.  A code costs 7 / 8 of a VALU operation each time, twice a token (scores, O): with the scales' part
+// some 580 a SIMD and tile of 64 tokens, and these, not the memory, bound the kernel.
 //
-// So three kinds of waves work at once, a tile apart: two load tile i + NS - 2, four score tile i, four add up tile i - 1.  A scoring wave
-// takes 16 of the tile's tokens and leaves p relative to a running max of its own, with that max; an adding wave owns a quarter of the
-// latent's columns, brings the four to a common max and adds.  ds_read_b64_tr_b4 gives each lane one column's 16 tokens, those whose p
-// the lane reads as the scores' accumulators left them: token 16 t + 4 G + r for t, r < 4.
+// So three kinds of waves work at once, a tile apart: four load tile i + NS - 2, four score tile i, NA add up tile i - 1.  A scoring wave
+// takes 16 of the tile's tokens and leaves p relative to a running max of its own, with that max; an adding wave owns some of the
+// latent's columns (a run of 64 where there are registers for a wave each), brings the four to a common max and adds.
+// ds_read_b64_tr_b4 gives each lane one column's 16 tokens, those whose p the lane reads as the scores' accumulators left them: token
+// 16 t + 4 G + r for t, r < 4.  Waves that did all three one after the other took 60.0 us for 87 MB where these took 33.8.  Reading all of a
+// tile's codes ahead of their use takes longer (70 us for the 179 MB: more LDS reads at a time in the way of the arriving tiles).
 //
 // A slot holds rows of RS chunks of 16 bytes, RS odd, every second 16 rows 128 bytes further (2-way bank conflicts in the transpose
 // reads, none in the scores' reads), then the runs' scales.  Keys of their own lie apart, [16 tokens' piece][head][token][32 bytes],
@@ -834,7 +849,9 @@ __global__ __launch_bounds__((Pd4<DL, SHARED, SLOTS>::THREADS), 1) void paged_de
 // ------------------------------------------------------------------------------------------------ parts
 
 // One workgroup a head of a sequence: nothing where one run finished it, zeros for a sequence without tokens, else the sum of the
-// runs' parts, 2^(m - M) of each.  Latency: the lengths, then m, l and 8 parts a thread at once.
+// runs' parts, 2^(m - M) of each.  Latency: the lengths, then m, l and 8 parts a thread at once (3.9 us for one sequence, 6 for 64 of
+// 16 heads, of which a launch alone is 2).  The last run of a unit to end could add the parts instead; it would need counters that every
+// call finds cleared.
 template <int DL, class C>
 __global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
   constexpr int COLS = DL / 4, PARTS = 512 / COLS;  // threads of a part; parts at a time
@@ -914,7 +931,8 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
 
 // ------------------------------------------------------------------------------------------------ host
 
-// Slots of the ring in 4 bits: as many as fit, 8 at most; with keys of their own 4, or 3 where 4 leave no room for the heads'.
+// Slots of the ring in 4 bits: as many as fit, 8 at most; with keys of their own 4, or 3 where 4 leave no room for the heads' (more than 14
+// of d_latent 384, 10 of 512).
 template <int DL>
 constexpr int slots4() {
   using C = Pd4<DL, true, 3>;
