@@ -610,15 +610,16 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
 #pragma unroll 1
   while (true) {
     if (first) {
-      const int h = use.hg * 16 + l16;
+      const int h = min(use.hg * 16 + l16, p.H - 1);  // (past the last head the last again: under a condition each load would be waited for)
       const bf16* ql = p.q_lat + use.b * p.q_lat_sb + (int64_t)h * p.q_lat_sh;
       const bf16* qp = p.q_rope + use.b * p.q_rope_sb + (int64_t)h * p.q_rope_sh;
 #pragma unroll
       for (int i = 0; i < 2 * NQ; ++i) {
         const int c = 64 * (i >> 1) + 16 * G + 8 * (i & 1);
-        q[i] = u32x4{0u, 0u, 0u, 0u};
-        if (h < p.H) q[i] = order8(i < 2 * C::NL ? ldg16(ql + c) : ldg16(qp + c - DL));
+        q[i] = i < 2 * C::NL ? ldg16(ql + c) : ldg16(qp + c - DL);
       }
+#pragma unroll
+      for (int i = 0; i < 2 * NQ; ++i) q[i] = order8(q[i]);
       float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int g = 0; g < NQ; ++g) {
