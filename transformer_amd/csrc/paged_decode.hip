@@ -669,12 +669,15 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       const u32x2 w0 = __builtin_bit_cast(u32x2, r0), w1 = __builtin_bit_cast(u32x2, r1);
       s = mfma16(as_bf16x8(u32x4{w0[0], w0[1], w1[0], w1[1]}), start, f32x4{0.f, 0.f, 0.f, 0.f});
     }
+    u32x2 ahead = lds8(buf + offA);
 #pragma unroll
     for (int g = 0; g < C::NL + (SHARED ? 1 : 0); ++g) {
-      const u32x2 c = lds8(buf + offA + 32 * g);
+      const u32x2 c = ahead, kg = lds8(sc + 32 * g + 8 * G);
+      if (g + 1 < C::NL + (SHARED ? 1 : 0)) ahead = lds8(buf + offA + 32 * (g + 1));
+      asm volatile("" ::: "memory");  // (read here: left to itself the compiler reads and waits)
       f32x4 d = mfma16(codes.of(c[0]), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
       d = mfma16(codes.of(c[1]), as_bf16x8(q[2 * g + 1]), d);
-      const f32x4 k = floats4(lds8(sc + 32 * g + 8 * G));
+      const f32x4 k = floats4(kg);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(k[r], d[r], s[r]);
     }
@@ -682,15 +685,19 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       // head j's keys with every head's query: lane l16 keeps its own.  The scale of its key comes last.
       const unsigned char* kb = lds + C::NS * C::SLOT + kslot * C::ROPE + w * C::HEADS * 512 + l16 * 32 + 8 * G;
       f32x4 e = f32x4{0.f, 0.f, 0.f, 0.f};
+      ahead = lds8(kb);
+      const u32x2 ks = lds8(sc + 32 * (C::NL + l16) + 8 * G);
 #pragma unroll
       for (int j = 0; j < C::HEADS; ++j) {
-        const u32x2 c = lds8(kb + j * 512);
+        const u32x2 c = ahead;
+        if (j + 1 < C::HEADS) ahead = lds8(kb + (j + 1) * 512);
+        asm volatile("" ::: "memory");
         f32x4 d = mfma16(codes.of(c[0]), as_bf16x8(q[2 * C::NL]), key_start);
         d = mfma16(codes.of(c[1]), as_bf16x8(q[2 * C::NL + 1]), d);
 #pragma unroll
         for (int r = 0; r < 4; ++r) e[r] = l16 == j ? d[r] : e[r];
       }
-      const f32x4 k = floats4(lds8(sc + 32 * (C::NL + l16) + 8 * G));
+      const f32x4 k = floats4(ks);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(k[r], e[r], s[r]);
       kslot = kslot + 1 == C::NS - 1 ? 0 : kslot + 1;
