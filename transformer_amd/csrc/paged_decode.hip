@@ -649,9 +649,16 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       }
       m_run = -INFINITY;
       l_part = 0.f;
-      first = false;
     }
     pd_barrier();  // the tile has landed, and the tile before the last is added up
+    if (!first) {  // the largest of the four waves' maxima from now on, so that the adding waves find one for all (mostly it is)
+      const float* m = x.m + (par ^ 1) * 64 + l16;
+      const float top = fmaxf(fmaxf(m[0], m[16]), fmaxf(m[32], m[48]));
+      if (__any(top > m_run)) {
+        l_part *= top > m_run ? fast_exp2(m_run - top) : 1.f;
+        m_run = fmaxf(m_run, top);
+      }
+    }
     const unsigned char* buf = lds + slot * C::SLOT;
     unsigned char* sc = lds + slot * C::SLOT + C::ROWS + w * C::SC;
     const int nv = pieces.tokens_of(pieces.lane_of(p, use, w, lane));
@@ -669,12 +676,20 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       const u32x2 w0 = __builtin_bit_cast(u32x2, r0), w1 = __builtin_bit_cast(u32x2, r1);
       s = mfma16(as_bf16x8(u32x4{w0[0], w0[1], w1[0], w1[1]}), start, f32x4{0.f, 0.f, 0.f, 0.f});
     }
-    u32x2 ahead = lds8(buf + offA);
+    constexpr int RUNS = C::NL + (SHARED ? 1 : 0), AHEAD = 2;
+    u32x2 codes_of[AHEAD + 1], scales_of[AHEAD + 1];
+    auto read = [&](int g) {
+      if (g >= RUNS) return;
+      codes_of[g % (AHEAD + 1)] = lds8(buf + offA + 32 * g);
+      scales_of[g % (AHEAD + 1)] = lds8(sc + 32 * g + 8 * G);
+    };
 #pragma unroll
-    for (int g = 0; g < C::NL + (SHARED ? 1 : 0); ++g) {
-      const u32x2 c = ahead, kg = lds8(sc + 32 * g + 8 * G);
-      if (g + 1 < C::NL + (SHARED ? 1 : 0)) ahead = lds8(buf + offA + 32 * (g + 1));
+    for (int g = 0; g < AHEAD; ++g) read(g);
+#pragma unroll
+    for (int g = 0; g < RUNS; ++g) {
+      read(g + AHEAD);
       asm volatile("" ::: "memory");  // (read here: left to itself the compiler reads and waits)
+      const u32x2 c = codes_of[g % (AHEAD + 1)], kg = scales_of[g % (AHEAD + 1)];
       f32x4 d = mfma16(codes.of(c[0]), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
       d = mfma16(codes.of(c[1]), as_bf16x8(q[2 * g + 1]), d);
       const f32x4 k = floats4(kg);
@@ -685,7 +700,7 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       // head j's keys with every head's query: lane l16 keeps its own.  The scale of its key comes last.
       const unsigned char* kb = lds + C::NS * C::SLOT + kslot * C::ROPE + w * C::HEADS * 512 + l16 * 32 + 8 * G;
       f32x4 e = f32x4{0.f, 0.f, 0.f, 0.f};
-      ahead = lds8(kb);
+      u32x2 ahead = lds8(kb);
       const u32x2 ks = lds8(sc + 32 * (C::NL + l16) + 8 * G);
 #pragma unroll
       for (int j = 0; j < C::HEADS; ++j) {
@@ -777,7 +792,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
 #pragma unroll
       for (int t = 0; t < 4; ++t) k[g][t] = lds8(sc + t * C::SC + 32 * min(g0 + g, C::NL - 1) + 8 * G);
     const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-    if (__any(top > M + kPdRescale)) {
+    if (__any(top > M)) {
       const float m_new = fmaxf(M, top), alpha = m_new == -INFINITY ? 1.f : fast_exp2(M - m_new);
       M = m_new;
 #pragma unroll
@@ -785,11 +800,15 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
       os[0] *= alpha;
       os[1] *= alpha;
     }
-    const float M_use = M == -INFINITY ? 0.f : M;
+    if (__any(fminf(fminf(m[0], m[1]), fminf(m[2], m[3])) != M)) {  // what brings a wave's p (and l) to the common max
+      const float M_use = M == -INFINITY ? 0.f : M;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      m[t] = fast_exp2(m[t] - M_use);  // what brings the wave's p (and l) to the common max
-      pv[t] *= m[t];
+      for (int t = 0; t < 4; ++t) {
+        m[t] = fast_exp2(m[t] - M_use);
+        pv[t] *= m[t];
+      }
+    } else {
+      m[0] = m[1] = m[2] = m[3] = 1.f;
     }
     bf16x8 pb[2];
 #pragma unroll
@@ -850,8 +869,10 @@ __global__ __launch_bounds__((Pd4<DL, SHARED, SLOTS>::THREADS), 1) void paged_de
     paged_score4<C, DL, SHARED>(p, lds, x, use, w, lane);
   else if (w < 4 + C::NA)
     paged_add4<C, DL>(p, lds, x, use, w - 4, lane);
-  else
+  else {
+    __builtin_amdgcn_s_setprio(3);  // (a load that goes out late delays all; 9.6 us for one sequence where it took 10.4)
     paged_load4<C, SHARED>(p, lds, use, w - 4 - C::NA, lane);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ parts
