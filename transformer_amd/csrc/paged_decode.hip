@@ -466,7 +466,8 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
 //
 // A slot holds rows of RS chunks of 16 bytes, RS odd, every second 16 rows 128 bytes further (2-way bank conflicts in the transpose
 // reads, none in the scores' reads), then the runs' scales.  Keys of their own lie apart, [16 tokens' piece][head][token][32 bytes],
-// in a ring one slot shorter: only the scores read them.
+// in a ring one slot shorter: only the scores read them.  With a shared key there is room for the scales in fp32 as well, which the loading
+// waves, who have time for it, write for all others; what lies behind the sequence's end gets 0, so that a p of 0 stays 0.
 template <int DL, bool SHARED, int SLOTS>
 struct Pd4 {
   static constexpr int TT = 64, COST = 1, LEAST = 2;
@@ -475,7 +476,8 @@ struct Pd4 {
   static constexpr int NA = SHARED ? NL : 4, NB = DL / 16 / NA;    // adding waves; column blocks of 16 of one
   static constexpr int SUB = 16 * RS * 16, ROWS = 4 * SUB + 256;
   static constexpr int SC = NG * 32;  // bytes of 16 tokens' scales
-  static constexpr int SLOT = ROWS + 4 * SC, SX = 2 * 4096 + 2 * 256 + 2 * 256 + (SHARED ? 0 : 1024), LIMIT = 160 * 1024;
+  static constexpr int SF = 4 * NG * 64;  // a tile's scales in fp32: [16 tokens' piece][run][token]; three tiles'
+  static constexpr int SLOT = ROWS + 4 * SC, SX = 2 * 4096 + 2 * 256 + 2 * 256 + (SHARED ? 3 * SF : 1024), LIMIT = 160 * 1024;
   static constexpr int NS = SLOTS;
   // heads with keys of their own that SLOTS slots leave room for
   static constexpr int HEADS = SHARED ? 16 : std::min(16, (LIMIT - SX - NS * SLOT) / (NS - 1) / 2048 / 2 * 2);
@@ -526,6 +528,7 @@ __device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned
   const uint32_t base = lds_addr(lds), keys = base + C::NS * C::SLOT, dump = keys + (C::NS - 1) * C::ROPE + C::SX - 1024;
   const uint32_t scales_bytes = (uint32_t)((p.c.groups - 1) * p.c.size + 16) * 2;
   int slot = 0, kslot = 0;
+  uint64_t slot_tokens = 0;  // 8 bits a slot
   auto issue = [&]() {
     const bool more = load.more();
     const int hg = load.hg;
@@ -554,8 +557,24 @@ __device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned
       }
     }
     if (more) load.next(p);
+    if (SHARED) slot_tokens = (slot_tokens & ~(0xffull << (8 * slot))) | (uint64_t)nv << (8 * slot);
     slot = slot + 1 == C::NS ? 0 : slot + 1;
     kslot = kslot + 1 == C::NS - 1 ? 0 : kslot + 1;
+  };
+  // the scales of the next tile to be scored, which has landed, in fp32
+  int sslot = 0, sbuf = 0;
+  auto scales_out = [&]() {
+    if constexpr (SHARED) {
+      const int nv = (int)(slot_tokens >> (8 * sslot)) & 0xff, t = 4 * (lane & 3);
+      if (lane < 4 * C::NG) {
+        f32x4 v = floats4(lds8(lds + sslot * C::SLOT + C::ROWS + lw * C::SC + 8 * lane));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = t + r < nv ? v[r] : 0.f;
+        *reinterpret_cast<f32x4*>(lds + C::NS * C::SLOT + C::SX - 3 * C::SF + sbuf * C::SF + lw * C::NG * 64 + 16 * lane) = v;
+      }
+      sslot = sslot + 1 == C::NS ? 0 : sslot + 1;
+      sbuf = sbuf == 2 ? 0 : sbuf + 1;
+    }
   };
   issue();
   if constexpr (C::NS > 3) issue();
@@ -563,6 +582,7 @@ __device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned
   auto ramp_up = [&](auto k) {
     if (!use.more()) return;
     wait_loads<(k + 1) * C::ND>();
+    scales_out();
     pd_barrier();
     issue();
     issue();
@@ -576,6 +596,7 @@ __device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned
 #pragma unroll 1
   for (; use.more(); use.next(p)) {
     wait_loads<(C::NS - 3) * C::ND>();
+    scales_out();
     pd_barrier();
     issue();
   }
@@ -588,6 +609,25 @@ struct Pd4Shared {
   f32x4* p;  // [2][4 waves][64]
   float* m;  // [2][4][16]
   float* l;  // [2][4][16]: at a unit's end
+  const unsigned char* scales;  // a shared key: [3] tiles' in fp32
+};
+
+// 4 tokens' scales of run g, in fp32 or bf16
+template <bool FP32>
+struct Pd4Scales {
+  typename std::conditional<FP32, u32x4, u32x2>::type v;
+  __device__ __forceinline__ void read(const unsigned char* at, int g) {
+    if constexpr (FP32)
+      v = lds16(at + 64 * g);
+    else
+      v = lds8(at + 32 * g);
+  }
+  __device__ __forceinline__ f32x4 floats() const {
+    if constexpr (FP32)
+      return __builtin_bit_cast(f32x4, v);
+    else
+      return floats4(v);
+  }
 };
 
 template <class C, int DL, bool SHARED>
@@ -605,7 +645,7 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
   float m_run = 0.f, l_part = 0.f;
   const int offS = ((l16 >> 2) & 3) * 32 + (l16 & 3) * 8;  // transpose read: row (run) i / 4, tokens 4 (i % 4) ..
   const Pd4Codes codes;
-  int slot = 0, kslot = 0, par = 0;
+  int slot = 0, kslot = 0, par = 0, sbuf = 0;
   bool first = true;
 #pragma unroll 1
   while (true) {
@@ -662,7 +702,7 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
     const unsigned char* buf = lds + slot * C::SLOT;
     unsigned char* sc = lds + slot * C::SLOT + C::ROWS + w * C::SC;
     const int nv = pieces.tokens_of(pieces.lane_of(p, use, w, lane));
-    if (nv < 16) {  // scales behind the sequence's end may be anything: 0, so that a p of 0 stays 0
+    if (!SHARED && nv < 16) {  // scales behind the sequence's end may be anything: 0, so that a p of 0 stays 0
       for (int i = lane; i < C::NG * 16; i += 64)
         if ((i & 15) >= nv) reinterpret_cast<unsigned short*>(sc)[i] = 0;
     }
@@ -676,12 +716,14 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       const u32x2 w0 = __builtin_bit_cast(u32x2, r0), w1 = __builtin_bit_cast(u32x2, r1);
       s = mfma16(as_bf16x8(u32x4{w0[0], w0[1], w1[0], w1[1]}), start, f32x4{0.f, 0.f, 0.f, 0.f});
     }
-    constexpr int RUNS = C::NL + (SHARED ? 1 : 0), AHEAD = 2;
-    u32x2 codes_of[AHEAD + 1], scales_of[AHEAD + 1];
+    constexpr int RUNS = C::NL + (SHARED ? 1 : 0), AHEAD = SHARED ? 1 : 2;
+    u32x2 codes_of[AHEAD + 1];
+    Pd4Scales<SHARED> scales_of[AHEAD + 1];
+    const unsigned char* scales = SHARED ? x.scales + sbuf * C::SF + w * C::NG * 64 + 16 * G : sc + 8 * G;
     auto read = [&](int g) {
       if (g >= RUNS) return;
       codes_of[g % (AHEAD + 1)] = lds8(buf + offA + 32 * g);
-      scales_of[g % (AHEAD + 1)] = lds8(sc + 32 * g + 8 * G);
+      scales_of[g % (AHEAD + 1)].read(scales, g);
     };
 #pragma unroll
     for (int g = 0; g < AHEAD; ++g) read(g);
@@ -689,13 +731,14 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
     for (int g = 0; g < RUNS; ++g) {
       read(g + AHEAD);
       asm volatile("" ::: "memory");  // (read here: left to itself the compiler reads and waits)
-      const u32x2 c = codes_of[g % (AHEAD + 1)], kg = scales_of[g % (AHEAD + 1)];
+      const u32x2 c = codes_of[g % (AHEAD + 1)];
+      const f32x4 k = scales_of[g % (AHEAD + 1)].floats();
       f32x4 d = mfma16(codes.of(c[0]), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
       d = mfma16(codes.of(c[1]), as_bf16x8(q[2 * g + 1]), d);
-      const f32x4 k = floats4(kg);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(k[r], d[r], s[r]);
     }
+    sbuf = sbuf == 2 ? 0 : sbuf + 1;
     if constexpr (!SHARED) {
       // head j's keys with every head's query: lane l16 keeps its own.  The scale of its key comes last.
       const unsigned char* kb = lds + C::NS * C::SLOT + kslot * C::ROPE + w * C::HEADS * 512 + l16 * 32 + 8 * G;
@@ -751,7 +794,7 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
   pd_barrier();
 }
 
-template <class C, int DL>
+template <class C, int DL, bool SHARED>
 __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const unsigned char* lds, const Pd4Shared& x, PdCursor<C> use, int w,
                                            int lane) {
   const int l16 = lane & 15, G = lane >> 4;
@@ -761,7 +804,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
   f32x4 o[C::NB], os[2];
   const Pd4Codes codes;
   float M = 0.f;
-  int slot = 0, par = 0, from = 0;
+  int slot = 0, par = 0, from = 0, sbuf = 0;
   bool first = true;
   pd_barrier();
 #pragma unroll 1
@@ -786,11 +829,13 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
 #pragma unroll
     for (int t = 0; t < 4; ++t) pv[t] = x.p[(par * 4 + t) * 64 + lane];
     constexpr int NG = C::NB > 4 ? 2 : 1;  // runs that the wave's columns can touch
-    u32x2 k[NG][4];
+    Pd4Scales<SHARED> k[NG][4];
+    const unsigned char* scales = SHARED ? x.scales + sbuf * C::SF + 16 * G : sc + 8 * G;
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) k[g][t] = lds8(sc + t * C::SC + 32 * min(g0 + g, C::NL - 1) + 8 * G);
+      for (int t = 0; t < 4; ++t) k[g][t].read(scales + t * (SHARED ? C::NG * 64 : C::SC), min(g0 + g, C::NL - 1));
+    sbuf = sbuf == 2 ? 0 : sbuf + 1;
     const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     if (__any(top > M)) {
       const float m_new = fmaxf(M, top), alpha = m_new == -INFINITY ? 1.f : fast_exp2(M - m_new);
@@ -817,7 +862,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
       if (i == 0 || (nb & 3) == 0) {  // the run's scales into p
         f32x4 e[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) e[t] = pv[t] * floats4(k[g == g0 ? 0 : 1][t]);
+        for (int t = 0; t < 4; ++t) e[t] = pv[t] * k[g == g0 ? 0 : 1][t].floats();
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           pb[t] = as_bf16x8(u32x4{pack_bf16x2(e[2 * t][0], e[2 * t + 1][0]), pack_bf16x2(e[2 * t][1], e[2 * t + 1][1]),
@@ -861,14 +906,14 @@ __global__ __launch_bounds__((Pd4<DL, SHARED, SLOTS>::THREADS), 1) void paged_de
   using C = Pd4<DL, SHARED, SLOTS>;
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
   unsigned char* at = lds + C::NS * C::SLOT + (C::NS - 1) * C::ROPE;
-  const Pd4Shared x = {reinterpret_cast<f32x4*>(at), reinterpret_cast<float*>(at + 8192), reinterpret_cast<float*>(at + 8192 + 512)};
+  const Pd4Shared x = {reinterpret_cast<f32x4*>(at), reinterpret_cast<float*>(at + 8192), reinterpret_cast<float*>(at + 8192 + 512), at + 8192 + 1024};
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const PdCursor<C> use = pd_begin<C>(p, blockIdx.x, lane);
   if (!use.more()) return;
   if (w < 4)
     paged_score4<C, DL, SHARED>(p, lds, x, use, w, lane);
   else if (w < 4 + C::NA)
-    paged_add4<C, DL>(p, lds, x, use, w - 4, lane);
+    paged_add4<C, DL, SHARED>(p, lds, x, use, w - 4, lane);
   else {
     __builtin_amdgcn_s_setprio(3);  // (a load that goes out late delays all; 9.6 us for one sequence where it took 10.4)
     paged_load4<C, SHARED>(p, lds, use, w - 4 - C::NA, lane);
