@@ -204,3 +204,47 @@ def test_every_layout(H, Hr, DL, bits):
     q = T.paged_append(qk.cuda(), c_new.cuda(), *dev, cos.cuda(), sin.cuda(), table, i32([5, 0, 40]))
     assert same_bits(q, U.append(cache, qk, c_new, cos, sin, [5, 0, 40], None))
     check_cache(dev, cache)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_many_short_sequences(bits):
+    """More sequences than workgroups, empty ones among them, several in a workgroup's run."""
+    lens = [(7 * b * b + 3 * b) % 90 if b % 11 else 0 for b in range(1500)]
+    g = torch.Generator().manual_seed(12)
+    cache = U.Cache(g, bits, 64, 1, 32, lens)
+    q_lat, q_rope = U.normal(g, 1500, 2, 64), U.normal(g, 1500, 2, 64)
+    got = T.paged_decode(q_lat.cuda(), q_rope.cuda(), *cache.dev(), cache.table.cuda(), i32(lens), SCALE)
+    check_decode(cache, q_lat, q_rope, lens, SCALE, got)
+
+
+def test_an_empty_cache_and_then_one_of_the_same_sizes():
+    q = torch.ones(2, 16, 512, dtype=torch.bfloat16, device="cuda")
+    for n in (0, 200):
+        pages, scales = T.new_paged_cache(n, 64, 512, bits=4)
+        table = torch.arange(200, dtype=torch.int32, device="cuda").view(2, 100)
+        ctx, lse = T.paged_decode(q, q[..., :64], pages, scales, table, i32([6400, 100]), SCALE)
+        assert not ctx.any()
+        if n:  # rows of zeros: every token weighs the same
+            want = torch.tensor([6400.0, 100.0]).log()[:, None].expand(2, 16)
+            torch.testing.assert_close(lse.cpu(), want, rtol=0, atol=2.0 ** -18)
+        else:
+            assert (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_longest_rows(dtype):
+    """2^19 logits, a row that begins off its alignment."""
+    V = 1 << 19
+    g = torch.Generator().manual_seed(13)
+    x = (torch.randn(2, V, generator=g) * 2).to(dtype)
+    wide = torch.zeros(2, V + 5, dtype=dtype)
+    wide[:, 3:V + 3] = x
+    u = torch.tensor([0.3, 0.999])
+    for settings in (dict(temperature=0.9), dict(top_k=3000, top_p=0.8), dict(temperature=1.5, top_p=0.99, min_p=0.001)):
+        token, logprob = T.sample_tokens(wide.cuda()[:, 3:V + 3], u.cuda(), **settings)
+        s = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0, **settings}
+        for b in range(2):
+            want, lp, room = sample_util.draw(x[b].float().numpy(), np.float32(u[b].item()), np.float32(s["temperature"]), s["top_k"],
+                                              np.float32(s["top_p"]), np.float32(s["min_p"]))
+            if room > 1:
+                assert int(token[b]) == want and abs(float(logprob[b]) - lp) <= 2.0 ** -22 * max(1.0, abs(lp))

@@ -226,7 +226,7 @@ def _decode(q_lat, q_rope, pages, scales, block_table, seq_lens, scale):
     ctx = q_lat.new_empty((B, H, DL))
     lse = q_lat.new_empty((B, H), dtype=_F32)
     if B and H:
-        key = (B, H, DL, Hr, cache[7], cache[4], scales is None)
+        key = (B, H, DL, Hr, cache[7], cache[4], cache[1] == 0)  # (no scales: an empty cache in 4 bits too)
         nbytes = _workspaces.get(key)
         if nbytes is None:
             if len(_workspaces) > 4096:
