@@ -124,8 +124,8 @@ def decode(cache, q_lat, q_rope, lens, scale):
     """float64 (ctx, lse) and the bounds of what bf16 and fp32 roundings can change of each.
 
     p is rounded to bf16 once (2^-8 of it), the result once (2^-8 of it).  A score is a sum of DL + 64 products in fp32; in 4 bits
-    each run of 64 may be a sum of products with 16 + code (two of eight: 128 + code), off which 24 (136) times the queries' sum is
-    taken, and the runs are added then: its error is at most 2^-24 (DL + 66) S, or 2^-24 (64 + DL / 64 + 6) S, with S the sum of the magnitudes added, which
+    each run of 64 may be a sum of products with 16 + code, off which 24 times the queries' sum is taken, and the runs are added
+    then: its error is at most 2^-24 (DL + 66) S, or 2^-24 (64 + DL / 64 + 6) S, with S the sum of the magnitudes added, which
     moves p by that much, and an exponential with the hardware's by 2^-22 (1 + the score's magnitude 2^-2 or so); sums over n
     tokens in fp32 add 2^-24 (n + 40) of the magnitudes added."""
     B, H, DL = q_lat.shape
@@ -146,14 +146,15 @@ def decode(cache, q_lat, q_rope, lens, scale):
         P = torch.softmax(x, 0)
         ctx[b] = P.T @ c
         ca, ka = c.abs(), k.abs()
-        if cache.bits == 4:  # values 0 and 4 of 8: 128 + code, at most 143, and 136; the others: 16 + code, at most 31, and 24
+        added = ca
+        if cache.bits == 4:  # in scores 16 + code, at most 31, and 24; in ctx at most 128 + code, 143, and 136
             s = cache.scales.transpose(1, 2)[page, slot].double().repeat_interleave(64, -1)
-            s = s * torch.tensor([279.0, 55, 55, 55] * (cache.W // 4), dtype=torch.float64)
-            ca, ka = s[:, :DL], s[:, DL:].unflatten(-1, (cache.Hr, 64)).expand(-1, H, 64)
+            ca, ka = 55 * s[:, :DL], (55 * s[:, DL:]).unflatten(-1, (cache.Hr, 64)).expand(-1, H, 64)
+            added = 279 * s[:, :DL]
         S = (ca @ ql.abs().T + (ka * qr.abs()).sum(-1)) * scale
         off = (2.0 ** -24 * (DL + 66 if cache.bits == 16 else DL // 64 + 70) * S + 2.0 ** -22 * (1 + x.abs() / 4)).amax(0)  # of a score, natural units
         A = P.T @ c.abs()
         n = len(at)
-        ctx_tol[b] = 2.0 ** -8 * (ctx[b].abs() + 1.01 * A) + 2.1 * off[:, None] * A + 2.0 ** -24 * (n + 40) * (P.T @ ca)
+        ctx_tol[b] = 2.0 ** -8 * (ctx[b].abs() + 1.01 * A) + 2.1 * off[:, None] * A + 2.0 ** -24 * (n + 40) * (P.T @ added)
         lse_tol[b] = off + 2.0 ** -24 * (n + 40) + 2.0 ** -22 * lse[b].abs()
     return ctx, lse, ctx_tol, lse_tol

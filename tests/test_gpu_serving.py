@@ -248,3 +248,20 @@ def test_the_longest_rows(dtype):
                                               np.float32(s["top_p"]), np.float32(s["min_p"]))
             if room > 1:
                 assert int(token[b]) == want and abs(float(logprob[b]) - lp) <= 2.0 ** -22 * max(1.0, abs(lp))
+
+
+@pytest.mark.parametrize("layout", ["baseline", "model"])
+def test_a_single_tokens_score_in_four_bits(layout):
+    """lse of one token is its score.  A run's sum of u q, u = 16 + code (24.4 root mean square) and queries of size 1, is sqrt(k) 24.4 after
+    k products; rounded after each of the 64, by 2^-24 / sqrt(12) of it, it is 2^-24 / sqrt(12) 24.4 sqrt(2080) = 1.9e-5 off.  The run's
+    share of the score is sqrt(64) 2.8 = 22 (code - 8 is 2.8: a scale is 0.36 of the values), so it is 8.6e-7 of that, as is the sum of
+    all runs.  With 24 sum q, of the same size and rounded to 24 bits, and a spread of a sixth over 16 heads, 1.5e-6 bounds it; with 128 in
+    place of 16 throughout it would be 4e-6."""
+    H, Hr, DL = LAYOUTS[layout]
+    g = torch.Generator().manual_seed(21)
+    cache = U.Cache(g, 4, DL, Hr, 16, [1] * 24)
+    q_lat, q_rope = U.normal(g, 24, H, DL), U.normal(g, 24, H, 64)
+    _, lse = T.paged_decode(q_lat.cuda(), q_rope.cuda(), *cache.dev(), cache.table.cuda(), i32([1] * 24), SCALE)
+    _, want, _, _ = U.decode(cache, q_lat, q_rope, [1] * 24, SCALE)
+    off = (lse.double().cpu() - want).norm() / want.norm()
+    assert float(off) <= 1.5e-6, float(off)

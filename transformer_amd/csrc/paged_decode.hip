@@ -450,12 +450,12 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
 // ------------------------------------------------------------------------------------------------ 4 bits
 
 // Codes are never turned into their values: (w >> s) & 0x00780078 | 0x41804180 makes two of a word's eight codes the bf16 numbers 16 +
-// code, which the matrix instructions take as they are; w & 0x000f000f | 0x43004300 makes the first two 128 + code without a shift.  With
-// u = 16 + code a run of 64 adds scale (sum u q - 24 sum q) to a score (136 for the first two of eight): the second sum is the
-// accumulator's start, the scale a factor on the result, one a run and token.  For O the scale goes into p before p is rounded to bf16
-// (one rounding, as in 16 bits), and -24 sum p' is an accumulator of its own, added at the end; these sums are in fp32 and so large that
-// 2^-24 of them is 2^-17 of a code.  A code costs 7 / 8 of a VALU operation each time, twice a token (scores, O): with the scales' part
-// some 580 a SIMD and tile of 64 tokens, and these, not the memory, bound the kernel.
+// code, which the matrix instructions take as they are.  With u = 16 + code a run of 64 adds scale (sum u q - 24 sum q) to a score: the
+// second sum is the accumulator's start, the scale a factor on the result, one a run and token.  For O the scale goes into p before p is
+// rounded to bf16 (one rounding, as in 16 bits), and -24 sum p' is an accumulator of its own, added at the end; there the first two codes of
+// eight are 128 + code, w & 0x000f000f | 0x43004300, without a shift.  (In the scores too that would put 1.6e-6 of a single token's lse out,
+// 0.6e-6 with 16: these sums are in fp32, and the smaller what cancels the better.)  A code costs about a VALU operation each time,
+// twice a token (scores, O); these and the scoring waves' way through a tile, not the memory, bound the kernel.
 //
 // So three kinds of waves work at once, a tile apart: four load tile i + NS - 2, four score tile i, NA add up tile i - 1.  A scoring wave
 // takes 16 of the tile's tokens and leaves p relative to a running max of its own, with that max; an adding wave owns some of the
@@ -500,7 +500,10 @@ struct Pd4Codes {
     asm("" : "+s"(mask0), "+s"(mask1));
     asm("" : "+v"(base0), "+v"(base1));
   }
-  __device__ __forceinline__ bf16x8 of(uint32_t w) const {
+  __device__ __forceinline__ bf16x8 near(uint32_t w) const {  // 16 + code
+    return as_bf16x8(u32x4{((w << 3) & mask1) | base1, ((w >> 1) & mask1) | base1, ((w >> 5) & mask1) | base1, ((w >> 9) & mask1) | base1});
+  }
+  __device__ __forceinline__ bf16x8 of(uint32_t w) const {  // the first two 128 + code: an operation fewer, sums of three times the size
     return as_bf16x8(u32x4{(w & mask0) | base0, ((w >> 1) & mask1) | base1, ((w >> 5) & mask1) | base1, ((w >> 9) & mask1) | base1});
   }
 };
@@ -509,7 +512,8 @@ __device__ __forceinline__ u32x4 order8(u32x4 v) {
   return u32x4{pack_lo16(v[0], v[2]), pack_hi16(v[0], v[2]), pack_lo16(v[1], v[3]), pack_hi16(v[1], v[3])};
 }
 __device__ __forceinline__ f32x4 floats4(u32x2 v) { return f32x4{lo_bf16(v[0]), hi_bf16(v[0]), lo_bf16(v[1]), hi_bf16(v[1])}; }
-// what takes 128 + code and 16 + code back to code - 8
+// what takes 16 + code, and 128 + code, back to code - 8
+__device__ __forceinline__ bf16x8 minus24() { return as_bf16x8(u32x4{0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u}); }
 __device__ __forceinline__ bf16x8 offsets8() { return as_bf16x8(u32x4{0xc308c308u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u}); }
 
 // The loading waves, 16 tokens of a tile each: tile i + NS - 2 goes into the slot of tile i - 2 after the barrier before which tile i has
@@ -663,8 +667,8 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int g = 0; g < NQ; ++g) {
-        f32x4 d = mfma16(offsets8(), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
-        d = mfma16(offsets8(), as_bf16x8(q[2 * g + 1]), d);
+        f32x4 d = mfma16(minus24(), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
+        d = mfma16(minus24(), as_bf16x8(q[2 * g + 1]), d);
         if (g < C::NL)
           z[g] = d[0];
         else
@@ -733,8 +737,8 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
       asm volatile("" ::: "memory");  // (read here: left to itself the compiler reads and waits)
       const u32x2 c = codes_of[g % (AHEAD + 1)];
       const f32x4 k = scales_of[g % (AHEAD + 1)].floats();
-      f32x4 d = mfma16(codes.of(c[0]), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
-      d = mfma16(codes.of(c[1]), as_bf16x8(q[2 * g + 1]), d);
+      f32x4 d = mfma16(codes.near(c[0]), as_bf16x8(q[2 * g]), f32x4{0.f, 0.f, 0.f, 0.f});
+      d = mfma16(codes.near(c[1]), as_bf16x8(q[2 * g + 1]), d);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(k[r], d[r], s[r]);
     }
@@ -750,8 +754,8 @@ __device__ __forceinline__ void paged_score4(const PagedDecodeParams& p, unsigne
         const u32x2 c = ahead;
         if (j + 1 < C::HEADS) ahead = lds8(kb + (j + 1) * 512);
         asm volatile("" ::: "memory");
-        f32x4 d = mfma16(codes.of(c[0]), as_bf16x8(q[2 * C::NL]), key_start);
-        d = mfma16(codes.of(c[1]), as_bf16x8(q[2 * C::NL + 1]), d);
+        f32x4 d = mfma16(codes.near(c[0]), as_bf16x8(q[2 * C::NL]), key_start);
+        d = mfma16(codes.near(c[1]), as_bf16x8(q[2 * C::NL + 1]), d);
 #pragma unroll
         for (int r = 0; r < 4; ++r) e[r] = l16 == j ? d[r] : e[r];
       }
