@@ -7,12 +7,12 @@
 // 4 bits by the instructions that unpack.
 //
 // Measured (kernel trace; a stream that only reads reaches 6.0 TB/s), this kernel and the merge of the parts:
-//   16 bits, 32 sequences up to 4096, 85 MB        21.8 + 4.4 us  (3.9 TB/s, 3.2 with the merge)
-//   16 bits, one of 701 tokens, 14 keys            8.7 + 3.9
-//   4 bits, 64 up to 16384, 179 MB                 67.7 + 6.2  (2.6 TB/s; VALU busy 64 % of the time)
-//   4 bits, 64 up to 4000 with 14 keys, 87 MB      30.4 + 6.1  (2.9 TB/s)
-//   4 bits, one of 3001                            10.6 + 4.0
-// About 6 us of each are the launch, the lengths, the page look-ups and the first tile's way from memory.
+//   16 bits, 32 sequences up to 4096, 85 MB        22.0 + 4.5 us  (3.9 TB/s, 3.2 with the merge)
+//   16 bits, one of 701 tokens, 14 keys            8.8 + 3.9
+//   4 bits, 64 up to 16384, 179 MB                 58.6 + 6.0  (3.1 TB/s; VALU busy 65 % of the time)
+//   4 bits, 64 up to 4000 with 14 keys, 87 MB      27.8 + 5.9  (3.1 TB/s)
+//   4 bits, one of 3001                            9.6 + 3.9
+// About 5 us of each are the launch, the lengths, the page look-ups and the first tile's way from memory.
 //
 // Work.  A unit is a sequence and head group, a tile 16 tokens of it (16 bits) or 64 (4 bits).  The tiles of all units in a row are
 // cut into equal runs, one a workgroup, whatever the sequences' lengths: every workgroup adds the lengths up and finds its place
@@ -461,8 +461,11 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
 // takes 16 of the tile's tokens and leaves p relative to a running max of its own, with that max; an adding wave owns some of the
 // latent's columns (a run of 64 where there are registers for a wave each), brings the four to a common max and adds.
 // ds_read_b64_tr_b4 gives each lane one column's 16 tokens, those whose p the lane reads as the scores' accumulators left them: token
-// 16 t + 4 G + r for t, r < 4.  Waves that did all three one after the other took 60.0 us for 87 MB where these took 33.8.  Reading all of a
-// tile's codes ahead of their use takes longer (70 us for the 179 MB: more LDS reads at a time in the way of the arriving tiles).
+// 16 t + 4 G + r for t, r < 4.  Waves that did all three one after the other took 60.0 us for 87 MB where these took 33.8.  The scoring waves
+// keep to one max (that of all four, a tile late), so that the adding ones seldom have anything to bring together.
+//
+// Not loading anything would save nothing of the 179 MB's time, not unpacking 15 %: what bounds a tile is a scoring wave's 3000 cycles for
+// it, with two adding waves and a loading one on its SIMD.  Reading the next codes ahead took 2 % off, reading them all ahead put 5 % on.
 //
 // A slot holds rows of RS chunks of 16 bytes, RS odd, every second 16 rows 128 bytes further (2-way bank conflicts in the transpose
 // reads, none in the scores' reads), then the runs' scales.  Keys of their own lie apart, [16 tokens' piece][head][token][32 bytes],
