@@ -12,8 +12,8 @@ from transformer_amd import build as B
 BUDGETS = {
     # file: [(kernel name regex, max VGPR + AGPR per lane, kernels)]
     "paged_append.hip": [(r"append", 128, 2), (r"read", 128, 2)],
-    # 6 waves of a workgroup; 12, or 16 with d_latent 512 and a shared key; 8
-    "paged_decode.hip": [(r"paged_decode16_kernel", 256, 10), (r"paged_decode4_kernelILi512ELb1E", 128, 1),
+    # 6 waves of a workgroup; 12, or 14 and 16 with a shared key and d_latent 384 and 512; 8
+    "paged_decode.hip": [(r"paged_decode16_kernel", 256, 10), (r"paged_decode4_kernelILi(384|512)ELb1E", 128, 2),
                          (r"paged_decode4_kernel", 168, 12), (r"paged_merge_kernel", 128, 22)],
     "sample.hip": [(r"sample_kernel", 128, 6)],
 }
