@@ -8,10 +8,10 @@
 //
 // Measured (kernel trace; a stream that only reads reaches 6.0 TB/s), this kernel and the merge of the parts:
 //   16 bits, 32 sequences up to 4096, 85 MB        22.0 + 4.5 us  (3.9 TB/s, 3.2 with the merge)
-//   16 bits, one of 701 tokens, 14 keys            8.8 + 3.9
-//   4 bits, 64 up to 16384, 179 MB                 58.6 + 6.0  (3.1 TB/s; VALU busy 65 % of the time)
-//   4 bits, 64 up to 4000 with 14 keys, 87 MB      27.8 + 5.9  (3.1 TB/s)
-//   4 bits, one of 3001                            9.6 + 3.9
+//   16 bits, one of 701 tokens, 14 keys            7.4 + 3.8
+//   4 bits, 64 up to 16384, 179 MB                 57.8 + 6.1  (3.1 TB/s; VALU busy 65 % of the time)
+//   4 bits, 64 up to 4000 with 14 keys, 87 MB      27.7 + 5.7  (3.1 TB/s)
+//   4 bits, one of 3001                            10.0 + 4.0
 // About 5 us of each are the launch, the lengths, the page look-ups and the first tile's way from memory.
 //
 // Work.  A unit is a sequence and head group, a tile 16 tokens of it (16 bits) or 64 (4 bits).  The tiles of all units in a row are
@@ -77,7 +77,8 @@ __device__ __forceinline__ int pd_page(const PagedDecodeParams& p, int piece) {
 //
 // On that line a unit takes COST places before its tiles: what its beginning and end cost in tiles (queries, stores), so that a
 // workgroup whose run holds the ends of several gets fewer tiles.  A run has LEAST places at least: one sequence is not cut so finely
-// that the parts take longer than the tiles.  All numbers stay below 2^31.
+// that the parts take longer than the tiles (one of 701 tokens in 16 bits: 7.4 + 3.8 us with 3, 9.1 + 3.9 with 5; one of 3001 in 4 bits:
+// 10.0 + 4.0 with 2, 9.1 + 4.9 with 1).  All numbers stay below 2^31.
 template <class C>
 struct PdCursor {
   int b, hg, tile, n, len, left;  // left: of the run's line, from this tile on
@@ -227,7 +228,7 @@ struct PdOut {
 // Keys of heads' own take 3 or 4 slots, whatever fits.
 template <int DL, bool SHARED>
 struct Pd16 {
-  static constexpr int TT = 16, COST = 3, LEAST = 5;
+  static constexpr int TT = 16, COST = 3, LEAST = 3;
   static constexpr int NCH = DL / 8 + (SHARED ? 8 : 0), RS = NCH % 16 == 8 ? NCH : NCH + 8;
   static constexpr int NKS = NCH / 4, NKW = (NKS + 3) / 4;  // k-steps of the scores; of a wave
   static constexpr int NB = DL / 64;                        // column blocks of 16 a wave
@@ -473,7 +474,7 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
 // waves, who have time for it, write for all others; what lies behind the sequence's end gets 0, so that a p of 0 stays 0.
 template <int DL, bool SHARED, int SLOTS>
 struct Pd4 {
-  static constexpr int TT = 64, COST = 1, LEAST = 2;
+  static constexpr int TT = 64, COST = 2, LEAST = 2;
   static constexpr int NCH = DL / 32 + (SHARED ? 2 : 0), RS = NCH + 1;
   static constexpr int NL = DL / 64, NG = NL + (SHARED ? 1 : 16);  // runs of a row: the latent's; with the keys
   static constexpr int NA = SHARED ? NL : 4, NB = DL / 16 / NA;    // adding waves; column blocks of 16 of one
