@@ -191,23 +191,32 @@ __device__ __forceinline__ void wait_vmem(int n) {
 // LDS reads nor models it as a register result: the kernel orders these loads itself
 // (s_waitcnt vmcnt + barrier before a stage is read).  M0 is set here and is not used by
 // any other instruction of the kernels that use it.
+//
+// The compiler sees to the wait states of its own instructions alone, so these loads bring theirs: one between the write
+// of M0 and a load into LDS, and five between a vector instruction's write of an SGPR (a descriptor formed with v_readlane,
+// or come back from a spill by one) and a vector memory instruction that reads it.  M0's write is one of them and s_nop n
+// is n + 1: VECTOR_DESC where a descriptor may be that young, else 0.  tests/test_wait_states.py looks for missing ones in
+// the kernels' assembly.  (VECTOR_DESC for all loads: 1 % off the prefill forward, 3 % off a feed-forward of 1999 rows.)
+constexpr int VECTOR_DESC = 3;
+template <int NOP = 0>
 __device__ __forceinline__ void dma16(buf_rsrc r, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r),
+               "i"(NOP)
                : "memory", "m0");
 }
 // the same with the non-temporal hint, for data read once (it should not displace lines that
 // other workgroups reuse)
 __device__ __forceinline__ void dma16_nt(buf_rsrc r, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(voff), "s"(r)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(voff), "s"(r)
                : "memory", "m0");
 }
 // The same with the LDS destination given as a base register plus a constant (M0 =
 // lds_base + LDS_OFF is formed here): the compiler then keeps one base per stage in an SGPR
 // rather than one M0 value per stage and load.
-template <int LDS_OFF>
+template <int LDS_OFF, int NOP = 0>
 __device__ __forceinline__ void dma16_at(buf_rsrc r, uint32_t voff, uint32_t lds_base) {
-  asm volatile("s_add_u32 m0, %0, %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_base), "v"(voff), "s"(r),
-               "i"(LDS_OFF)
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop %4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_base),
+               "v"(voff), "s"(r), "i"(LDS_OFF), "i"(NOP)
                : "memory", "m0", "scc");
 }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {

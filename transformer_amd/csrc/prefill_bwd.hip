@@ -475,16 +475,17 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdParams p) {
                         make_rsrc(do_b + (int64_t)q0 * do_st, rows_bytes(nv, do_st, 256)),
                         make_rsrc(ld_b + (int64_t)(live ? qb : 0) * 64, live ? 256u : 0u), st};
     };
+    // (a block's descriptors come back from spills)
     auto issue = [&](const BlockLoads& bl, int n) {
       const uint32_t vo = n == 0 ? vl0 : n == 1 ? vl1 : n == 2 ? vl2 : n == 3 ? vl3 : n == 4 ? vl4 : vl5;
       if (n < C::MK_QN) {
-        dma16(bl.rqn, vo, lds_addr(bl.st + 1024 * (w + 4 * n)));
+        dma16<VECTOR_DESC>(bl.rqn, vo, lds_addr(bl.st + 1024 * (w + 4 * n)));
       } else if (n < C::MK_QN + C::MK_QR) {
-        dma16(bl.rqr, vo, lds_addr(bl.st + C::OFF_QR + 1024 * (w + 4 * (n - C::MK_QN))));
+        dma16<VECTOR_DESC>(bl.rqr, vo, lds_addr(bl.st + C::OFF_QR + 1024 * (w + 4 * (n - C::MK_QN))));
       } else if (n < C::MK_QN + C::MK_QR + C::MK_DO) {
-        dma16(bl.rdo, vo, lds_addr(bl.st + C::OFF_DO + 1024 * (w + 4 * (n - C::MK_QN - C::MK_QR))));
+        dma16<VECTOR_DESC>(bl.rdo, vo, lds_addr(bl.st + C::OFF_DO + 1024 * (w + 4 * (n - C::MK_QN - C::MK_QR))));
       } else if (n < C::NL) {
-        if (w == 0) dma16(bl.rld, vo, lds_addr(bl.st + C::OFF_LD));
+        if (w == 0) dma16<VECTOR_DESC>(bl.rld, vo, lds_addr(bl.st + C::OFF_LD));
       }
     };
     const int loads = C::NL - 1 + (w == 0 ? 1 : 0);

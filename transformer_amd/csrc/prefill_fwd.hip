@@ -339,14 +339,15 @@ __global__ __launch_bounds__(64 * FWD_NW, QB == 1 ? 2 : 1) void prefill_fwd_kern
   // load n of the wave's tile loads, n a constant: its region, descriptor and LDS offset
   auto issue_c = [&](const TileLoads& tl, auto n_tag) {
     constexpr int n = decltype(n_tag)::value;
+    constexpr int NOP = PT ? VECTOR_DESC : 0;  // (descriptors a tile: some come back from spills)
     const uint32_t vo = n == 0 ? vl0 : n == 1 ? vl1 : n == 2 ? vl2 : n == 3 ? vl3 : n == 4 ? vl4 : vl5;
     if constexpr (n < MK_KN) {
-      if (w + C::NW * n < C::T_KN) dma16_at<1024 * C::NW * n>(tl.rkn, vo + tl.okn, tl.lb);
+      if (w + C::NW * n < C::T_KN) dma16_at<1024 * C::NW * n, NOP>(tl.rkn, vo + tl.okn, tl.lb);
     } else if constexpr (n < MK_KN + MK_KR) {
-      if (w + C::NW * (n - MK_KN) < C::T_KR) dma16_at<C::OFF_KR + 1024 * C::NW * (n - MK_KN)>(tl.rkr, vo + tl.okr, tl.lb);
+      if (w + C::NW * (n - MK_KN) < C::T_KR) dma16_at<C::OFF_KR + 1024 * C::NW * (n - MK_KN), NOP>(tl.rkr, vo + tl.okr, tl.lb);
     } else if constexpr (n < NL) {
       if (w + C::NW * (n - MK_KN - MK_KR) < C::T_V)
-        dma16_at<C::K_STAGE + 1024 * C::NW * (n - MK_KN - MK_KR)>(tl.rv, vo + tl.ov, tl.lb);
+        dma16_at<C::K_STAGE + 1024 * C::NW * (n - MK_KN - MK_KR), NOP>(tl.rv, vo + tl.ov, tl.lb);
     }
   };
   // the same for n known only after unrolling (the switch folds away)
