@@ -1,0 +1,54 @@
+"""Calls of the paged operators that a program makes and no other test does: layouts of one sequence, token or head."""
+import pytest
+import torch
+
+import transformer_amd as T
+from tests import paged_util as U
+from tests.test_gpu_paged import LAYOUTS, check_cache, check_decode, i32, same_bits
+
+pytestmark = pytest.mark.gpu
+
+
+def odd(t, dims):
+    """``t`` with strides 1, 3, 5 .. in its dimensions ``dims`` of size 1."""
+    st = list(t.stride())
+    for k, d in enumerate(dims):
+        assert t.size(d) == 1
+        st[d] = 2 * k + 1
+    return t.as_strided(t.shape, st)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_one_sequences_queries_as_a_product_leaves_them(bits):
+    H, Hr, DL = LAYOUTS["baseline"]
+    g = torch.Generator().manual_seed(3)
+    cache = U.Cache(g, bits, DL, Hr, 16, [70])
+    w, x = U.normal(g, H, DL, 64).cuda(), U.normal(g, H, 64, 1, std=0.1).cuda()
+    q_lat = torch.matmul(w, x).permute(2, 0, 1)  # [1, H, DL], strides (1, DL, 1)
+    assert q_lat.stride(0) % 8
+    q_rope = U.normal(g, 1, H, 64)
+    got = T.paged_decode(q_lat, odd(q_rope.cuda(), (0,)), *cache.dev(), cache.table.cuda(), i32([70]), 0.07)
+    check_decode(cache, q_lat.cpu(), q_rope, [70], 0.07, got)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("layout,B,T_,dims", [("one", 4, 1, (1,)), ("one", 1, 3, (0,)), ("one", 1, 1, (0, 1)), ("model", 1, 1, (1, 0))])
+def test_appended_rows_of_one_token_or_sequence(bits, layout, B, T_, dims):
+    H, Hr, DL = LAYOUTS[layout]
+    g = torch.Generator().manual_seed(4 + B)
+    cache = U.Cache(g, bits, DL, Hr, 16, [40] * B)
+    qk, c_new, starts = U.normal(g, B, T_, H + Hr, 64), U.normal(g, B, T_, DL), [5 * b for b in range(B)]
+    cos, sin = U.tables(64)
+    dev = cache.dev()
+    q = T.paged_append(odd(qk.cuda(), dims), odd(c_new.cuda(), dims), *dev, cos.cuda(), sin.cuda(), cache.table.cuda(), i32(starts))
+    assert same_bits(q, U.append(cache, qk, c_new, cos, sin, starts, None))
+    check_cache(dev, cache)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_one_head(bits):
+    g = torch.Generator().manual_seed(6)
+    cache = U.Cache(g, bits, 128, 1, 16, [33, 5])
+    q_lat, q_rope = U.normal(g, 2, 1, 128), U.normal(g, 2, 1, 64)
+    got = T.paged_decode(odd(q_lat.cuda(), (1,)), odd(q_rope.cuda(), (1,)), *cache.dev(), cache.table.cuda(), i32([33, 5]), 0.1)
+    check_decode(cache, q_lat, q_rope, [33, 5], 0.1, got)

@@ -117,7 +117,8 @@ def _ints(op: str, name: str, t: Tensor, B: int) -> Tensor:
 
 
 def _strided(t: Tensor):
-    """``t`` (or a copy) with unit inner stride, 16-byte aligned, other strides multiples of 8, and those strides."""
+    """``t`` (or a copy) with unit inner stride, 16-byte aligned, other strides multiples of 8, and those strides (0 for a dimension
+    of size 1, whose own may be any number)."""
     st = t.stride()
     if st[-1] == 1 and not t.data_ptr() & 15:
         for s in st[:-1]:
@@ -126,7 +127,7 @@ def _strided(t: Tensor):
         else:
             return t, st
     t = _aligned4(t, 8)
-    return t, t.stride()
+    return t, (*(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)), 1)
 
 
 def _rope_table(t: Tensor) -> Tensor:
