@@ -52,3 +52,18 @@ def test_one_head(bits):
     q_lat, q_rope = U.normal(g, 2, 1, 128), U.normal(g, 2, 1, 64)
     got = T.paged_decode(odd(q_lat.cuda(), (1,)), odd(q_rope.cuda(), (1,)), *cache.dev(), cache.table.cuda(), i32([33, 5]), 0.1)
     check_decode(cache, q_lat, q_rope, [33, 5], 0.1, got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,T_,heads,dims", [(1, 5, 3, (0,)), (4, 1, 3, (1,)), (2, 5, 1, (2,)), (1, 1, 1, (0, 1, 2))])
+def test_rotation_of_one_sequence_token_or_head(dtype, B, T_, heads, dims):
+    """The rotation that the append does, as an operator of its own."""
+    g = torch.Generator().manual_seed(8)
+    x = U.normal(g, B, T_, heads, 64).to(dtype).cuda()
+    cos, sin = (t.cuda() for t in U.tables(16))
+    ops = torch.ops.mla_mi355x
+    want = ops.rope(x, cos, sin, 2, False)
+    y = odd(x.clone(), dims)
+    assert torch.equal(ops.rope(y, cos, sin, 2, False), want)
+    ops.rope_(y, cos, sin, 2, False)
+    assert torch.equal(y, want)

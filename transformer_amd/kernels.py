@@ -99,8 +99,7 @@ def _rope_launch(x: Tensor, y: Tensor, cos: Tensor, sin: Tensor, pos_offset: int
     args = RopeArgs(
         x=x.data_ptr(), y=y.data_ptr(), cos=cos.data_ptr(), sin=sin.data_ptr(),
         B=x.size(0), T=x.size(1), n_heads=x.size(2), table_rows=cos.size(0), pos_offset=int(pos_offset),
-        x_stride=Strides(x.stride(0), x.stride(1), x.stride(2)),
-        y_stride=Strides(y.stride(0), y.stride(1), y.stride(2)),
+        x_stride=_st4(x), y_stride=_st4(y),
         dtype=_lib.MLA_DTYPE_BF16 if x.dtype == torch.bfloat16 else _lib.MLA_DTYPE_F32,
         inverse=1 if inverse else 0)
     _lib.check(_lib.entry("mla_rope")(ctypes.byref(args), _stream(x)), "mla_rope")
