@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from transformer_amd import paged
+from transformer_amd import _lib, paged
+from transformer_amd.host_calls import Entry
 
 
 def layouts():
@@ -36,3 +37,21 @@ def test_what_fits_is_not_copied():
     for shape, strides in (((1, 16, 512), (1, 512, 1)), ((2, 1, 17, 64), (2000, 3, 64, 1)), ((4, 16, 64), (0, 64, 1))):
         t = flat.as_strided(shape, strides)
         assert paged._strided(t)[0].data_ptr() == t.data_ptr()
+
+
+def test_an_entry_point_is_called_only_once_it_is_bound_whole(monkeypatch):
+    """Another thread's call looks at ``fn`` alone: it must not see a function whose argument types are not set yet (a stream's handle
+    would go out as a C int)."""
+    entry = Entry("mla_sample", "8P3q3f2i4x", "SampleArgs")
+    seen = []
+
+    class Function:
+        def __setattr__(self, name, value):
+            seen.append((name, entry.fn))
+            super().__setattr__(name, value)
+
+    monkeypatch.setattr(_lib, "entry", lambda name: None)
+    monkeypatch.setattr(_lib, "load", lambda: {"mla_sample": Function()})
+    entry._bind()
+    assert {name for name, _ in seen} == {"restype", "argtypes"}
+    assert all(fn is None for _, fn in seen) and isinstance(entry.fn, Function)

@@ -47,9 +47,10 @@ class Entry:
         _lib.entry(self.name)  # raises if the library is missing or lacks it
         if self.size != ctypes.sizeof(getattr(_lib, self.declared)):
             raise RuntimeError(f"{self.name}: packed arguments of {self.size} bytes do not match {self.declared}")
-        self.fn = _lib.load()[self.name]  # a handle of its own, with its own argument types
-        self.fn.restype = _lib.SIGNATURES[self.name][0]
-        self.fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p] if self.stream else [ctypes.c_char_p]
+        fn = _lib.load()[self.name]  # a handle of its own, with its own argument types
+        fn.restype = _lib.SIGNATURES[self.name][0]
+        fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p] if self.stream else [ctypes.c_char_p]
+        self.fn = fn  # last: another thread calls whatever it finds here
 
     def __call__(self, op: str, dev: int, *values):
         if self.fn is None:
