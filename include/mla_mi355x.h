@@ -688,7 +688,8 @@ int mla_paged_read(const mla_paged_read_args* a, void* stream);
  * B below 2^20, H up to 1024, C = table_pages * page_size below 2^28, B ceil(H / 16) (C / 16 + 4) below 2^30.
  * The sequences' tiles are divided evenly over the workgroups whatever their lengths; a sequence that spans several leaves fp32
  * partials in the workspace, which a second kernel on the same stream adds in order: results repeat bit for bit.  Needs
- * mla_paged_decode_workspace_bytes() bytes of 256-byte aligned device memory of this call's own; what they hold does not matter.
+ * mla_paged_decode_workspace_bytes() bytes of 256-byte aligned device memory of this call's own (up to 17 MB and 4 bytes a sequence
+ * and 16 heads); what they hold does not matter.
  */
 typedef struct {
   mla_paged_cache cache;

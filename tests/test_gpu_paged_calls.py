@@ -67,3 +67,39 @@ def test_rotation_of_one_sequence_token_or_head(dtype, B, T_, heads, dims):
     assert torch.equal(ops.rope(y, cos, sin, 2, False), want)
     ops.rope_(y, cos, sin, 2, False)
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("H,Hr", [(16, 1), (33, 1), (5, 5)])
+def test_as_many_sequences_as_the_entry_takes(bits, H, Hr):
+    """2^20 - 1 sequences of up to a page, most of them empty: more workgroups of heads than 2^32 threads hold in one dimension (H = 16 and
+    33), and the time of one look at all lengths, not of one a head."""
+    B, n = (1 << 20) - 1, 251
+    lens = [(b * 7) % 17 if b % 3 else 0 for b in range(n)]
+    g = torch.Generator().manual_seed(31)
+    cache = U.Cache(g, bits, 64, Hr, 16, lens)
+    q_lat, q_rope, dev, table = U.normal(g, n, H, 64), U.normal(g, n, H, 64), cache.dev(), cache.table.cuda()
+    some = T.paged_decode(q_lat.cuda(), q_rope.cuda(), *dev, table, i32(lens), 0.2)
+    check_decode(cache, q_lat, q_rope, lens, 0.2, some)
+    at = torch.arange(B, device="cuda") % n
+    ql, qr = q_lat.cuda()[at], q_rope.cuda()[at]
+    torch.cuda.synchronize()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    ctx, lse = T.paged_decode(ql, qr, *dev, table[at], i32(lens)[at], 0.2)
+    end.record()
+    torch.cuda.synchronize()
+    assert torch.equal(ctx, some[0][at]) and torch.equal(lse, some[1][at])  # (one tile each: in one run whatever the batch)
+    assert start.elapsed_time(end) < 2000, start.elapsed_time(end)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_sequences_cut_into_many_runs_beside_short_and_empty_ones(bits):
+    """Parts of one sequence in two runs and in many, heads in several groups."""
+    g = torch.Generator().manual_seed(32)
+    lens = [0, 6000, 1, 0, 64, 700, 0, 2500, 16, 0]
+    cache = U.Cache(g, bits, 64, 1, 64, lens)
+    for H in (3, 16, 40):
+        q_lat, q_rope = U.normal(g, len(lens), H, 64), U.normal(g, len(lens), H, 64)
+        got = T.paged_decode(q_lat.cuda(), q_rope.cuda(), *cache.dev(), cache.table.cuda(), i32(lens), 0.1)
+        check_decode(cache, q_lat, q_rope, lens, 0.1, got)

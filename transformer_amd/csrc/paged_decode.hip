@@ -44,6 +44,7 @@ struct PagedDecodeParams {
   float* lse;
   float* part_o;   // [2 runs][16][DL]: slot 2 run for a unit that begins before the run, 2 run + 1 for one that ends after it
   float* part_ml;  // [2 runs][16][2]: m (log2) and l
+  int32_t* units;  // [B][n_hg]: the run that a unit with tiles begins in, and in how many runs it lies << 16
   int B, H, n_hg, runs;  // (runs * the places of one stays below 2^31)
   int pieces;          // 16-token pieces of a page
   uint32_t piece_magic;  // ceil(2^32 / pieces): the page of piece s < 2^24 is the high half of s times this (pieces > 1)
@@ -82,6 +83,7 @@ __device__ __forceinline__ int pd_page(const PagedDecodeParams& p, int piece) {
 template <class C>
 struct PdCursor {
   int b, hg, tile, n, len, left;  // left: of the run's line, from this tile on
+  int each;                       // places a run
 
   __device__ __forceinline__ bool more() const { return left > 0; }
   // the next tile of the run, or left <= 0
@@ -115,21 +117,17 @@ __device__ __forceinline__ int pd_scan(const PagedDecodeParams& p, int b0, int l
   n = (len + C::TT - 1) / C::TT;
   return wave_scan(n ? n + C::COST : 0);
 }
-// places a run
-__device__ __forceinline__ int pd_each(const PagedDecodeParams& p, int total, int least) {
-  return max((int)((uint32_t)(total + p.runs - 1) / (uint32_t)p.runs), least);
-}
 // The cursor of a run; left <= 0 where it has no tile.
 template <class C>
 __device__ __forceinline__ PdCursor<C> pd_begin(const PagedDecodeParams& p, int run, int lane) {
-  PdCursor<C> c = {0, 0, 0, 0, 0, 0};
+  PdCursor<C> c = {0, 0, 0, 0, 0, 0, 0};
   int n, len, upto = pd_scan<C>(p, 0, lane, n, len), before = 0, total = __builtin_amdgcn_readlane(upto, 63);
   for (int b0 = 64; b0 < p.B; b0 += 64) {
     int nb, lb;
     total += __builtin_amdgcn_readlane(pd_scan<C>(p, b0, lane, nb, lb), 63);
   }
   total *= p.n_hg;
-  const int each = pd_each(p, total, C::LEAST), from = run * each;
+  const int each = max((int)((uint32_t)(total + p.runs - 1) / (uint32_t)p.runs), C::LEAST), from = run * each;
   if (from >= total) return c;
   for (int b0 = 0;;) {
     const uint64_t past = __ballot((before + upto) * p.n_hg > from);
@@ -147,6 +145,7 @@ __device__ __forceinline__ PdCursor<C> pd_begin(const PagedDecodeParams& p, int 
     b0 += 64;
     upto = pd_scan<C>(p, b0, lane, n, len);
   }
+  c.each = each;
   c.left = min(each, total - from);
   if (c.tile < 0) {  // the run begins among the unit's first places
     c.left += c.tile;
@@ -197,6 +196,13 @@ template <int DL>
 struct PdOut {
   bool whole;
   int slot;
+  int runs;  // that the unit lies in; 0 where it began before this one
+  // a unit of n tiles whose tiles from .. tile are the run's
+  template <class C>
+  __device__ __forceinline__ PdOut(const PdCursor<C>& c, int from, int tile, int n)
+      : whole(from == 0 && tile + 1 == n),
+        slot(2 * (int)blockIdx.x + (from == 0 ? 1 : 0)),
+        runs(from ? 0 : whole ? 1 : 1 + (int)((uint32_t)(n - tile - 2 + c.each) / (uint32_t)c.each)) {}
   __device__ __forceinline__ void columns(const PagedDecodeParams& p, int b, int h, int l16, int col, f32x4 o, float inv) const {
     if (!whole) {
       *reinterpret_cast<f32x4*>(p.part_o + ((int64_t)slot * 16 + l16) * DL + col) = o;
@@ -205,7 +211,8 @@ struct PdOut {
       stg8(p.ctx + ((int64_t)b * p.H + h) * DL + col, u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])});
     }
   }
-  __device__ __forceinline__ void sums(const PagedDecodeParams& p, int b, int h, int l16, float m, float l) const {
+  __device__ __forceinline__ void sums(const PagedDecodeParams& p, int b, int hg, int h, int l16, float m, float l) const {
+    if (l16 == 0 && runs) p.units[(int64_t)b * p.n_hg + hg] = (int)blockIdx.x | runs << 16;
     if (!whole) {
       p.part_ml[(slot * 16 + l16) * 2] = m;
       p.part_ml[(slot * 16 + l16) * 2 + 1] = l;
@@ -436,12 +443,12 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
     const int b = use.b, hg = use.hg, n = use.n, tile = use.tile;
     use.next(p);
     if (tile + 1 == n || !use.more()) {
-      const PdOut<DL> out = {from == 0 && tile + 1 == n, 2 * (int)blockIdx.x + (from == 0 ? 1 : 0)};
+      const PdOut<DL> out(use, from, tile, n);
       const float l = xor32_sum(xor16_sum(l_part)), inv = l == 0.f ? 0.f : 1.f / l;
       const int h = hg * 16 + l16;
 #pragma unroll
       for (int i = 0; i < C::NB; ++i) out.columns(p, b, h, l16, 16 * (w + 4 * i) + 4 * G, o[i], inv);
-      if (w == 0 && G == 0) out.sums(p, b, h, l16, m_run, l);
+      if (w == 0 && G == 0) out.sums(p, b, hg, h, l16, m_run, l);
       first = true;
       if (!use.more()) break;
     }
@@ -891,7 +898,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
     use.next(p);
     first = tile + 1 == n || !use.more();
     if (first) {
-      const PdOut<DL> out = {from == 0 && tile + 1 == n, 2 * (int)blockIdx.x + (from == 0 ? 1 : 0)};
+      const PdOut<DL> out(use, from, tile, n);
       float l = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) l += x.l[(par * 4 + t) * 16 + l16] * m[t];
@@ -902,7 +909,7 @@ __device__ __forceinline__ void paged_add4(const PagedDecodeParams& p, const uns
         const int nb = w * C::NB + i;
         out.columns(p, b, h, l16, 16 * nb + 4 * G, o[i] + ((nb >> 2) == g0 ? os[0] : os[1]), inv);
       }
-      if (w == 0 && G == 0) out.sums(p, b, h, l16, M, l);
+      if (w == 0 && G == 0) out.sums(p, b, hg, h, l16, M, l);
       if (!use.more()) break;
     }
     par ^= 1;
@@ -931,33 +938,22 @@ __global__ __launch_bounds__((Pd4<DL, SHARED, SLOTS>::THREADS), 1) void paged_de
 // ------------------------------------------------------------------------------------------------ parts
 
 // One workgroup a head of a sequence: nothing where one run finished it, zeros for a sequence without tokens, else the sum of the
-// runs' parts, 2^(m - M) of each.  Latency: the lengths, then m, l and 8 parts a thread at once (3.9 us for one sequence, 6 for 64 of
-// 16 heads, of which a launch alone is 2).  The last run of a unit to end could add the parts instead; it would need counters that every
-// call finds cleared.
-template <int DL, class C>
+// runs' parts, 2^(m - M) of each.  Which runs those are the first of them has left.  Latency: that, then m, l and 8 parts a thread at
+// once (3.9 us for one sequence, 6 for 64 of 16 heads, of which a launch alone is 2).  The last run of a unit to end could add the parts instead.
+template <int DL, class C>  // (C: the kernel whose parts they are, so that a trace tells)
 __global__ __launch_bounds__(512) void paged_merge_kernel(PagedDecodeParams p) {
   constexpr int COLS = DL / 4, PARTS = 512 / COLS;  // threads of a part; parts at a time
   __shared__ f32x4 o_s[PARTS][COLS];
-  const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H, hg = h >> 4, l16 = h & 15;
+  const int b = blockIdx.x, h = blockIdx.y, hg = h >> 4, l16 = h & 15;
   const int tid = threadIdx.x, lane = tid & 63;
-  int total = 0, begin = 0, n = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    int nl, ll;
-    const int upto = pd_scan<C>(p, b0, lane, nl, ll);
-    if (b >= b0 && b < b0 + 64) {
-      n = __builtin_amdgcn_readlane(nl, b - b0);
-      begin = (total + __builtin_amdgcn_readlane(upto, b - b0) - (n + C::COST)) * p.n_hg + hg * (n + C::COST) + C::COST;
-    }
-    total += __builtin_amdgcn_readlane(upto, 63);
-  }
-  total *= p.n_hg;
+  const int len = pd_len(p, b), unit = p.units[(int64_t)b * p.n_hg + hg];
   const int64_t row = (int64_t)b * p.H + h;
-  if (n == 0) {
+  if (len == 0) {  // (no run has it)
     if (tid < COLS) stg8(p.ctx + row * DL + 4 * tid, u32x2{0u, 0u});
     if (tid == 0) p.lse[row] = -INFINITY;
     return;
   }
-  const int each = pd_each(p, total, C::LEAST), run0 = begin / each, S = (begin + n - 1) / each - run0 + 1;
+  const int run0 = unit & 0xffff, S = unit >> 16;
   if (S == 1) return;
   auto part_of = [&](int s) { return ((int64_t)2 * (run0 + s) + (s == 0 ? 1 : 0)) * 16 + l16; };
   const int part = tid / COLS, col = tid - part * COLS;
@@ -1069,7 +1065,8 @@ struct LaunchOf {
   int take(K kernel) {
     kernel<<<dim3(p.runs), C::THREADS, 0, st>>>(p);
     MLA_TRY(launch_status(op));
-    paged_merge_kernel<DL, C><<<dim3((unsigned)p.B * p.H), 512, 0, st>>>(p);
+    // (heads in a dimension of their own: a grid has less than 2^32 threads along each)
+    paged_merge_kernel<DL, C><<<dim3((unsigned)p.B, (unsigned)p.H), 512, 0, st>>>(p);
     return launch_status(op);
   }
 };
@@ -1088,6 +1085,7 @@ int decode_check(const mla_paged_decode_args* a, const char* op, PagedDecodePara
   return MLA_OK;
 }
 size_t parts_bytes(int runs, int64_t DL) { return (size_t)2 * runs * 16 * ((size_t)DL + 2) * 4; }
+size_t units_bytes(const mla_paged_decode_args& a) { return (size_t)a.B * ((a.H + 15) / 16) * 4; }
 
 }  // namespace mla
 
@@ -1096,7 +1094,7 @@ using namespace mla;
 extern "C" size_t mla_paged_decode_workspace_bytes(const mla_paged_decode_args* a) {
   PagedDecodeParams p;
   if (decode_check(a, "mla_paged_decode_workspace_bytes", p) != MLA_OK || a->B == 0) return 0;
-  return parts_bytes(by_layout(a->cache, a->H, RunsOf{*a}), a->cache.d_latent);
+  return parts_bytes(by_layout(a->cache, a->H, RunsOf{*a}), a->cache.d_latent) + units_bytes(*a);
 }
 
 extern "C" int mla_paged_decode(const mla_paged_decode_args* a, void* stream) {
@@ -1113,7 +1111,6 @@ extern "C" int mla_paged_decode(const mla_paged_decode_args* a, void* stream) {
   const size_t need = mla_paged_decode_workspace_bytes(a);
   MLA_CHECK(a->workspace && ((uintptr_t)a->workspace & 255) == 0 && a->workspace_bytes >= need, MLA_ERR_WORKSPACE,
             "%s: needs %zu bytes of 256-byte aligned workspace", op, need);
-  MLA_CHECK(a->B * a->H < (1ll << 31), MLA_ERR_INVALID_ARG, "%s: too many heads", op);
   p.q_lat = (const bf16*)a->q_lat;
   p.q_rope = (const bf16*)a->q_rope;
   p.seq_lens = a->seq_lens;
@@ -1132,5 +1129,6 @@ extern "C" int mla_paged_decode(const mla_paged_decode_args* a, void* stream) {
   p.runs = by_layout(a->cache, a->H, RunsOf{*a});
   p.part_o = (float*)a->workspace;
   p.part_ml = p.part_o + (size_t)2 * p.runs * 16 * a->cache.d_latent;
+  p.units = (int32_t*)(p.part_ml + (size_t)2 * p.runs * 16 * 2);
   return by_layout(a->cache, a->H, LaunchOf{p, op, (hipStream_t)stream});
 }
