@@ -283,13 +283,14 @@ __device__ __forceinline__ void paged_load16(const PagedDecodeParams& p, unsigne
       load.next(p);
     }
     const buf_rsrc r = pieces.rows_of(at, (uint32_t)(nv * p.c.row_bytes));
+    dma16<VECTOR_DESC>(r, off[0], to);
 #pragma unroll
-    for (int i = 0; i < NR / 2; ++i) dma16<VECTOR_DESC>(r, off[i], to + i * 2048);
+    for (int i = 1; i < NR / 2; ++i) dma16(r, off[i], to + i * 2048);
     if constexpr (!SHARED) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int h = hg * 16 + i;
-        dma16<VECTOR_DESC>(r, h < p.H ? roff + (uint32_t)h * 128 : kPdNothing, rto + i * 2048);
+        dma16(r, h < p.H ? roff + (uint32_t)h * 128 : kPdNothing, rto + i * 2048);
       }
       rto = rto + C::ROPE == rend ? rend - (C::NS - 1) * C::ROPE : rto + C::ROPE;
     }
@@ -558,9 +559,10 @@ __device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned
     }
     const buf_rsrc r = pieces.rows_of(at, (uint32_t)(nv * p.c.row_bytes));
     const uint32_t rows_to = to + piece_at<C::SUB>(lw);
+    if (lane < 16 * C::RS) dma16<VECTOR_DESC>(r, off[0], rows_to);
 #pragma unroll
-    for (int i = 0; i < C::NR; ++i)
-      if (64 * i + lane < 16 * C::RS) dma16<VECTOR_DESC>(r, off[i], rows_to + i * 1024);
+    for (int i = 1; i < C::NR; ++i)
+      if (64 * i + lane < 16 * C::RS) dma16(r, off[i], rows_to + i * 1024);
     const buf_rsrc rs = pieces.scales_of(at, nv ? scales_bytes : 0u);
     if (lane < 2 * C::NG) dma16<VECTOR_DESC>(rs, sv, to + C::ROWS + lw * C::SC);
     if constexpr (!SHARED) {
@@ -568,7 +570,7 @@ __device__ __forceinline__ void paged_load4(const PagedDecodeParams& p, unsigned
       for (int j = 0; j < 16; j += 2) {  // two heads; past the slot's heads nothing, into bytes that nobody reads
         const int h = hg * 16 + j;
         const uint32_t v = h + (lane >> 5) < p.H ? koff + (uint32_t)h * 32 : kPdNothing;
-        dma16<VECTOR_DESC>(r, j < C::HEADS ? v : kPdNothing, j < C::HEADS ? keys + kslot * C::ROPE + lw * C::HEADS * 512 + j * 512 : dump);
+        dma16(r, j < C::HEADS ? v : kPdNothing, j < C::HEADS ? keys + kslot * C::ROPE + lw * C::HEADS * 512 + j * 512 : dump);
       }
     }
     if (more) load.next(p);
