@@ -708,7 +708,8 @@ size_t mla_paged_decode_workspace_bytes(const mla_paged_decode_args* a);
 int mla_paged_decode(const mla_paged_decode_args* a, void* stream);
 
 /* ------------------------------------------------------------ sampling --
- * One token for each row of logits [B, V] (bf16 or fp32, row stride `stride`, V up to 2^19) from the given u[b] in [0, 1):
+ * One token for each row of logits [B, V] (bf16 or fp32, row stride `stride`, V up to 2^19, B below 2^22) from the given u[b] in
+ * [0, 1):
  *   w_i = exp((x_i - max x) / temperature)     (a NaN counts as -inf; infinities share all the weight)
  *   K1 = the top_k largest x                   (top_k <= 0: all)
  *   K2 = the shortest run of K1, largest first, that holds top_p of its weight, one token at least  (top_p >= 1: all)

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 
 from transformer_amd import _lib
-from tests.test_paged_args import BASE, CACHE
+from tests.test_paged_args import BASE, CACHE, SAMPLE
 
 
 def decode_args(**change):
@@ -22,3 +22,11 @@ def test_the_workspace_goes_by_sizes(B, H, scales, d_latent):
     n = _lib.load().mla_paged_decode_workspace_bytes(ctypes.byref(a))
     units = 4 * B * ((H + 15) // 16)
     assert units < n <= 17_000_000 + units
+
+
+@pytest.mark.parametrize("B", [1 << 22, (1 << 31) - 1])
+def test_more_rows_than_a_launch_holds_are_refused(B):
+    """A row is a workgroup of 1024 threads, and a launch has less than 2^32."""
+    lib = _lib.load()
+    a = _lib.SampleArgs(**{**SAMPLE, "B": B})
+    assert lib.mla_sample(ctypes.byref(a), None) == _lib.MLA_ERR_INVALID_ARG and b"out of range" in lib.mla_last_error()

@@ -783,8 +783,8 @@ using namespace mla;
 extern "C" int mla_sample(const mla_sample_args* a, void* stream) {
   const char* op = "mla_sample";
   MLA_CHECK(a, MLA_ERR_INVALID_ARG, "%s: null args", op);
-  MLA_CHECK(a->B >= 0 && a->B < (1ll << 31) && a->V >= 1 && a->V <= kSmMaxV, MLA_ERR_INVALID_ARG,
-            "%s: B %lld or V %lld is out of range (1 .. 2^19 logits)", op, (long long)a->B, (long long)a->V);
+  MLA_CHECK(a->B >= 0 && a->B < (1ll << 32) / kSmThreads && a->V >= 1 && a->V <= kSmMaxV, MLA_ERR_INVALID_ARG,
+            "%s: B %lld or V %lld is out of range (fewer than 2^22 rows, 1 .. 2^19 logits)", op, (long long)a->B, (long long)a->V);
   MLA_CHECK(a->dtype == MLA_DTYPE_BF16 || a->dtype == MLA_DTYPE_F32, MLA_ERR_UNSUPPORTED, "%s: logits must be bf16 or fp32", op);
   if (a->B == 0) return MLA_OK;
   MLA_CHECK(a->logits && a->u && a->tokens && a->logprobs, MLA_ERR_INVALID_ARG, "%s: null pointer", op);
