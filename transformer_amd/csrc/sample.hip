@@ -242,7 +242,6 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
   int top_k = a.top_k_rows ? a.top_k_rows[b] : a.top_k;
   const float u = fminf(fmaxf(a.u[b], 0.f), 1.f);
   if (!(temperature > 0.f) || top_p <= 0.f) top_k = 1;  // the largest alone (a NaN too)
-  temperature = fminf(temperature, kSmMost);
   int turn = 0;
 
   // quad q of a thread: 4 logits from index (kSmThreads q + tid) 4 - head on, aligned as one; -inf for what is out of the row
@@ -355,17 +354,19 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
       }
     }
   }
-  const double xmax = (double)big, rate = 1.0 / (double)temperature, per32 = 46.16624130844683 * rate;  // 32 log2 e
-  const double least_d = -33.0 * (double)temperature;                                // weighs nothing
+  const double t = fmin((double)temperature, 1e300);  // (an infinite one: all weights of finite logits 1)
+  const double xmax = (double)big, rate = 1.0 / t, per32 = 46.16624130844683 * rate;  // 32 log2 e
+  const double least_d = -33.0 * t;                                                   // weighs nothing
   const double least = (double)min_p * kSmOne;
-  const float bins_t = fminf((float)kSmPerNat / temperature, 1e30f);
+  const float half_big = 0.5f * big, bins_t = 2.f * fminf((float)kSmPerNat / temperature, 1e30f);
   auto weight = [&](float v) SM_INLINE {
     SmWeight w = sm_weight(fmax((double)v - xmax, least_d), per32, s.table);
     asm volatile("" : "+v"(w.bits));  // not put under the condition of its use: a branch for each logit, each waiting for the table
     return w;
   };
-  // a logit's distance from the largest in bins; a bin is its whole part, the last one takes all beyond
-  auto distance = [&](float v) { return (big - v) * bins_t; };
+  // a logit's distance from the largest in bins; a bin is its whole part, the last one takes all beyond.  By halves: two logits can be
+  // further apart than fp32's largest number.  (A -inf at an infinite temperature is a NaN, which no comparison lets in.)
+  auto distance = [&](float v) { return fmaf(v, -0.5f, half_big) * bins_t; };
   auto bin_of = [&](float v) { return (int)fminf(distance(v), (float)(kSmBins - 1)); };
 
   // what is kept: values of `cut` and more, from index `bound` on only larger ones; never a -inf
