@@ -89,6 +89,16 @@ def check(x, u, settings, got, share=0.9):
     assert compared >= share * x.size(0), (compared, x.size(0), settings)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", LENGTHS)
+def test_special_rows(V, dtype):
+    g = torch.Generator().manual_seed(V)
+    x = torch.stack(list(special_rows(V, g).values())).to(dtype)
+    u = (torch.rand(x.size(0), generator=g) * 0.98 + 0.01)
+    for settings in SETTINGS:
+        check(x, u, settings, ask(x.cuda(), u.cuda(), settings))
+
+
 @pytest.mark.parametrize("V", [4099, 20003, 40000])
 def test_ties_across_a_border(V):
     """top_k and top_p end inside a run of equal logits, wherever it begins: the lower indices stay."""
@@ -146,3 +156,18 @@ def test_logits_as_far_apart_as_fp32_has_them(V):
     u = torch.tensor([0.3, 0.6, 0.9, 0.5])
     for settings in ((1e38, 0, 0.9, 0.0), (3e38, 5, 1.0, 0.0), (3e38, V - 2, 0.7, 0.0), (2e38, 0, 1.0, 0.1), (math.inf, 0, 0.9, 0.0)):
         check(x, u, settings, ask(x.cuda(), u.cuda(), settings), share=0.75)  # (u = 0.5 of an even number of equal weights: a border)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [700, 20003, 40000])
+def test_rows_of_the_lowest_value(V, dtype):
+    """A mask of the type's lowest value over everything, over all but a few, and with -inf beside it."""
+    low = torch.finfo(dtype).min
+    x = torch.full((4, V), low, dtype=dtype)
+    x[1, V // 2:] = -math.inf
+    x[2, 9] = 0.0
+    x[3, ::3] = math.nan
+    u = torch.tensor([0.71, 0.43, 0.9, 0.31])
+    for settings in ((1.0, 0, 0.55, 0.0), (0.5, 600, 0.9, 0.0), (1.0, 0, 1.0, 0.0), (1.0, 30, 1.0, 0.0), (1.0, V - 1, 0.37, 0.2),
+                     (math.inf, 0, 0.81, 0.0)):
+        check(x, u, settings, ask(x.cuda(), u.cuda(), settings), share=0.75)

@@ -369,8 +369,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleParams a) {
   auto distance = [&](float v) { return fmaf(v, -0.5f, half_big) * bins_t; };
   auto bin_of = [&](float v) { return (int)fminf(distance(v), (float)(kSmBins - 1)); };
 
-  // what is kept: values of `cut` and more, from index `bound` on only larger ones; never a -inf
-  float cut = -kSmMost, above_cut = -kSmMost;
+  // what is kept: values of `cut` and more, from index `bound` on only those of `above_cut`, the next value, and more; never a -inf
+  float cut = -kSmMost, above_cut = sm_value(sm_key(-kSmMost) + 1);
   int bound = V;
   auto is_kept = [&](float v, int i) SM_INLINE {
     const float least_here = i < bound ? +cut : +above_cut;
