@@ -1,5 +1,5 @@
 """Host side of the serving operators, whose kernels often take less time than a call of them: entry points that take their
-arguments' fields packed at once, and the question whether a call needs torch's dispatcher."""
+arguments' fields packed at once; and what asks, for them and in ``kernels``, whether a call needs torch's dispatcher."""
 from __future__ import annotations
 
 import ctypes
@@ -17,10 +17,15 @@ _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurre
 _Parameter = torch.nn.Parameter
 
 
+def watched() -> bool:
+    """Whether torch has to see every operator: tracing (torch.compile, torch.jit.trace), a dispatch mode, a functorch transform."""
+    return _compiling() or _dispatch_modes() > 0 or _tracing() is not None or _transform() is not None
+
+
 def plain(first: Tensor, *others) -> bool:
-    """Whether a call with these tensors (or Nones) needs nothing of the dispatcher, as ``kernels.dispatcher_needed`` asks, and all are
-    on one GPU: the operator's body then need not look at that again."""
-    if _compiling() or _dispatch_modes() > 0 or _tracing() is not None or _transform() is not None:
+    """Whether a call with these tensors (or Nones) needs nothing of the dispatcher (``kernels.dispatcher_needed`` is the same of any
+    arguments), and all are on one GPU: the operator's body then need not look at that again."""
+    if watched():
         return False
     if type(first) is not Tensor or not first.is_cuda:
         return False

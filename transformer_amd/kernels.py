@@ -20,6 +20,7 @@ from torch import Tensor
 
 from . import _lib
 from ._lib import DecodeArgs, PrefillBwdArgs, PrefillFwdArgs, RopeArgs, Strides
+from .host_calls import watched
 
 ROPE_DIM = 64
 SUPPORTED_NOPE = (64, 128)
@@ -1044,8 +1045,7 @@ def _(logits, targets, lse, g_vec, g_scale, v0):
 def _not_plain(args) -> bool:
     """Tracing (torch.compile, torch.jit.trace), a dispatch mode, a functorch transform, tensor subclasses, or tensors off
     the GPU."""
-    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 \
-            or torch._C._get_tracing_state() is not None or torch._C._functorch.peek_interpreter_stack() is not None:
+    if watched():
         return True
     for a in args:
         if isinstance(a, Tensor) and ((type(a) is not Tensor and type(a) is not torch.nn.Parameter) or not a.is_cuda):
