@@ -3,7 +3,8 @@
 // Both move each value once, 16 bytes a thread and access.  Measured (kernel trace; a copy in HBM reaches 4.7 TB/s): 8 prompts' chunks of up
 // to 2048 tokens, 8450 in all, into 4-bit pages 16.6 us (63 MB, 3.8 TB/s; VALU busy 84 % of the time, most of it the quotients); 32000
 // rows of 1280 values out of 16-bit pages, 20300 of them tokens, 20.5 (134 MB; 28 where all of it comes from and goes to HBM: a copy's
-// rate).  Few rows are bound by the launch: one token 2.1, 64 tokens into 4 bits 6.1 (start, page and store one after the other).
+// rate).  Few rows are bound by the launch and by start, page and store one after the other: one token 2.2, 64 tokens 3.1.  In 4 bits the
+// runs' exchanges and quotients stand in between: one token 3.0, 64 tokens 4.0 with 14 keys and 5.9 with one (why more is not known).
 #include "paged.h"
 #include "rope_append.h"
 

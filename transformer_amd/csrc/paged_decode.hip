@@ -7,11 +7,11 @@
 // 4 bits by the instructions that unpack.
 //
 // Measured (kernel trace; a stream that only reads reaches 6.0 TB/s), this kernel and the merge of the parts:
-//   16 bits, 32 sequences up to 4096, 85 MB        22.0 + 4.5 us  (3.9 TB/s, 3.2 with the merge)
-//   16 bits, one of 701 tokens, 14 keys            7.4 + 3.8
-//   4 bits, 64 up to 16384, 179 MB                 57.8 + 6.1  (3.1 TB/s; VALU busy 65 % of the time)
-//   4 bits, 64 up to 4000 with 14 keys, 87 MB      27.7 + 5.7  (3.1 TB/s)
-//   4 bits, one of 3001                            10.0 + 4.0
+//   16 bits, 32 sequences up to 4096, 85 MB        22.4 + 4.3 us  (3.8 TB/s, 3.2 with the merge)
+//   16 bits, one of 701 tokens, 14 keys            7.4 + 3.9
+//   4 bits, 64 up to 16384, 179 MB                 58.6 + 6.3  (3.1 TB/s; VALU busy 65 % of the time)
+//   4 bits, 64 up to 4000 with 14 keys, 87 MB      27.0 + 5.7  (3.2 TB/s)
+//   4 bits, one of 3001                            9.9 + 3.9
 // About 5 us of each are the launch, the lengths, the page look-ups and the first tile's way from memory.
 //
 // Work.  A unit is a sequence and head group, a tile 16 tokens of it (16 bits) or 64 (4 bits).  The tiles of all units in a row are
@@ -21,9 +21,11 @@
 // repeat bit for bit).
 //
 // A workgroup's tiles come through a ring of LDS slots by direct-to-LDS loads, which run on across its units.  16 tokens never
-// straddle a page, so a buffer descriptor of the tokens that exist (none, where the entry is no page) bounds each load: what lies
-// behind a sequence's end reads as zero and never reaches a product.  Waves share the scores through LDS and each then owns some of
-// the latent's columns, so no wave's O has to be merged with another's.  One barrier a tile.
+// straddle a page, so a buffer descriptor of the tokens that exist (none, where the entry is no page) bounds each load of rows: those
+// behind a sequence's end read as zero.  The scales of 4 bits are read for all 16 tokens, whatever stands behind the end: the sums of O
+// take zeros for those (the fp32 copies, or the scales in LDS, are cleared), and the scores, whose first product takes them as they are,
+// are masked by the number of tokens.  Waves share the scores through LDS and each then owns some of the latent's columns, so no wave's
+// O has to be merged with another's.  One barrier a tile.
 #include <algorithm>
 #include <type_traits>
 
@@ -473,7 +475,7 @@ __global__ __launch_bounds__(384, 1) void paged_decode16_kernel(PagedDecodeParam
 // 16 t + 4 G + r for t, r < 4.  Waves that did all three one after the other took 60.0 us for 87 MB where these took 33.8.  The scoring waves
 // keep to one max (that of all four, a tile late), so that the adding ones seldom have anything to bring together.
 //
-// Not loading anything would save nothing of the 179 MB's time, not unpacking 15 %: what bounds a tile is a scoring wave's 3000 cycles for
+// Not loading anything would save nothing of the 179 MB's time, not unpacking 11 %: what bounds a tile is a scoring wave's 3000 cycles for
 // it, with two adding waves and a loading one on its SIMD.  Reading the next codes ahead took 2 % off, reading them all ahead put 5 % on.
 //
 // A slot holds rows of RS chunks of 16 bytes, RS odd, every second 16 rows 128 bytes further (2-way bank conflicts in the transpose

@@ -13,7 +13,7 @@
 namespace mla {
 
 constexpr int kSmThreads = 1024;
-constexpr int kSmMaxV = 1 << 19;  // 2^19 weights of up to 2^44 add up below 2^63
+constexpr int kSmMaxV = 1 << 19;  // 2^19 weights of up to 2^44 add up to 2^63 at most: unsigned 64 bits hold it
 constexpr int kSmWaves = kSmThreads / 64;
 constexpr int kSmBins = 2048, kSmPerNat = 64;  // 32 nats: what lies lower weighs less than half of 2^-44
 constexpr int kSmRuns = kSmMaxV / 256 + kSmThreads / 64;
