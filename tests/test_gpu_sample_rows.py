@@ -171,3 +171,21 @@ def test_rows_of_the_lowest_value(V, dtype):
     for settings in ((1.0, 0, 0.55, 0.0), (0.5, 600, 0.9, 0.0), (1.0, 0, 1.0, 0.0), (1.0, 30, 1.0, 0.0), (1.0, V - 1, 0.37, 0.2),
                      (math.inf, 0, 0.81, 0.0)):
         check(x, u, settings, ask(x.cuda(), u.cuda(), settings), share=0.75)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [8188, 8189, 8190, 8192, 8193, 32764, 32765, 32767, 32768, 32769, 65537])
+@pytest.mark.parametrize("head", [0, 1, 2])
+def test_lengths_about_the_kernels_ends(V, head, dtype):
+    """Rows that begin in any place of a quad, where one kernel takes over from another; settings of each row's own."""
+    g = torch.Generator().manual_seed(V + head)
+    B = 6
+    wide = torch.full((B, V + 6), 77.0).to(dtype)  # (what is read of it would win)
+    x = (torch.randn(B, V, generator=g) * torch.tensor([0.05, 0.5, 1.0, 2.0, 4.0, 9.0])[:, None]).to(dtype)
+    wide[:, head:head + V] = x
+    u = torch.rand(B, generator=g)
+    t, k = torch.rand(B, generator=g) * 1.5 + 0.1, torch.tensor([0, 3, 64, 300, 513, 5000], dtype=torch.int32)[torch.randperm(B, generator=g)]
+    p, m = torch.rand(B, generator=g) * 0.6 + 0.4, torch.tensor([0.0, 0.0, 0.001, 0.02, 0.3, 1.0])[torch.randperm(B, generator=g)]
+    got = T.sample_tokens(wide.cuda()[:, head:head + V], u.cuda(), t.cuda(), k.cuda(), p.cuda(), m.cuda())
+    for b in range(B):
+        check(x[b:b + 1], u[b:b + 1], (float(t[b]), int(k[b]), float(p[b]), float(m[b])), (got[0][b:b + 1], got[1][b:b + 1]), share=1.0)
