@@ -73,13 +73,14 @@ _ops = torch.ops.mla_mi355x
 
 def sample_tokens(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, top_k: Union[int, Tensor] = 0,
                   top_p: Union[float, Tensor] = 1.0, min_p: Union[float, Tensor] = 0.0) -> Tuple[Tensor, Tensor]:
-    """``(tokens int64 [B], logprobs fp32 [B])`` drawn from ``logits [B, V]`` (bf16 or fp32) with ``u [B]`` fp32 in [0, 1).
+    """``(tokens int64 [B], logprobs fp32 [B])`` drawn from ``logits [B, V]`` (bf16 or fp32; B below 2^22, V up to 2^19) with ``u [B]``
+    fp32 in [0, 1).
 
     Weights are ``exp((x - max x) / temperature)``.  Of these are kept the ``top_k`` largest (0 or less: all), of those the shortest
     run, largest first, that holds ``top_p`` of their weight (1 or more: all), of those the ones of at least ``min_p`` of the
     largest.  The token is the first, in the order of the vocabulary, at which the kept weights add up to more than ``u`` of their
     sum; its logprob is that of the distribution drawn from.  Of equal logits the lower index counts as the larger.  Temperature 0
-    (or less) takes the largest.  A NaN counts as -inf; a row without a logit above -inf gives token -1 and logprob -inf.  Each
+    (or less) takes the largest, an infinite one weighs all finite logits alike.  A NaN counts as -inf; a row without a logit above -inf gives token -1 and logprob -inf.  Each
     setting is a number or a tensor ``[B]`` on the device (fp32; ``top_k`` int32)."""
     rows = [None, None, None, None]
     if isinstance(temperature, Tensor):
