@@ -79,9 +79,9 @@ def sample_tokens(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] =
     Weights are ``exp((x - max x) / temperature)``.  Of these are kept the ``top_k`` largest (0 or less: all), of those the shortest
     run, largest first, that holds ``top_p`` of their weight (1 or more: all), of those the ones of at least ``min_p`` of the
     largest.  The token is the first, in the order of the vocabulary, at which the kept weights add up to more than ``u`` of their
-    sum; its logprob is that of the distribution drawn from.  Of equal logits the lower index counts as the larger.  Temperature 0
-    (or less) takes the largest, an infinite one weighs all finite logits alike.  A NaN counts as -inf; a row without a logit above -inf gives token -1 and logprob -inf.  Each
-    setting is a number or a tensor ``[B]`` on the device (fp32; ``top_k`` int32)."""
+    sum; its logprob is that of the distribution drawn from.  Of equal logits the lower index counts as the larger.  Temperature 0 (or
+    less) takes the largest, an infinite one weighs all finite logits alike.  A NaN counts as -inf; a row without a logit above -inf
+    gives token -1 and logprob -inf.  Each setting is a number or a tensor ``[B]`` on the device (fp32; ``top_k`` int32)."""
     rows = [None, None, None, None]
     if isinstance(temperature, Tensor):
         rows[0], temperature = temperature, 1.0
